@@ -9,7 +9,7 @@ same pass in float64, written on its own.
 Kinds:
   ffn     y = (silu(x Wg^T) * (x Wu^T)) Wd^T, forward only (serving)
   train   the block's forward and its backward; keep says what lies between them:
-          "full" the 16-bit projections, "fp8" x and the projections in 8 bits
+          "full" the projections in FP32, "fp8" x and the projections in 8 bits
   pack    an activation to 8 bits and back
   scan    a = sigmoid(f), s_t = a_t s_(t-1) + (1 - a_t) v_t, y = s silu(z): outputs and the
           last state, from a first one
