@@ -1,4 +1,4 @@
-"""ctypes binding of libmorph_optim.so (the C ABI in include/morph_optim.h).
+"""ctypes binding of libmorph_optim.so (the C ABI in include/morph_optim.h and morph_layers.h).
 
 The shared library is built in-tree by morph_amd.build into morph_amd/lib/.
 It links the same HIP runtime soname torch carries (libamdhip64.so.7), so
@@ -23,7 +23,7 @@ ADAMW_TABLE_SETS, ADAMW_TABLE_NUMEL = 8, 1 << 30  # limits of morph_adamw_table_
 DTYPE_NONE, DTYPE_F32, DTYPE_F16, DTYPE_BF16 = -1, 0, 1, 2
 HP_DIVIDE_SCALE, HP_APPLY_CLIP, HP_APPLY_DECAY, HP_LERP_LARGE = 1, 2, 4, 8
 
-# Every symbol include/morph_optim.h declares.
+# Every symbol that include/morph_optim.h and include/morph_layers.h declare.
 EXPORTS = (
     "morph_abi_version", "morph_strerror", "morph_flag_clear", "morph_nonfinite_or",
     "morph_nonfinite_or_multi", "morph_adamw_fused", "morph_adamw_multi",
@@ -36,7 +36,11 @@ EXPORTS = (
     "morph_muon_prepare", "morph_muon_newton_schulz", "morph_muon_finish",
     "morph_muon_finish_range", "morph_muon_newton_schulz_finish",
     "morph_muon_newton_schulz_ahead", "morph_muon_newton_schulz_finish_rest", "morph_host_copy",
+    "morph_act_pack", "morph_act_unpack",
+    "morph_ffn_workspace_bytes", "morph_ffn_forward", "morph_ffn_backward",
+    "morph_scan_workspace_bytes", "morph_scan_forward", "morph_scan_backward",
 )
+SCAN_SPAN = 64  # MORPH_SCAN_SPAN
 GEMM_TILE_M, GEMM_TILE_N, GEMM_TILE_K = 256, 256, 64
 GEMM_SYMMETRIC = 1
 GEMM_Q_KN = 2
@@ -99,6 +103,26 @@ class MuonHP(ctypes.Structure):
     _fields_ = [(name, ctypes.c_float) for name in (
         "momentum_weight", "nesterov_weight", "a", "b", "c", "update_scale", "decay",
         "neg_lr")] + [("ns_steps", ctypes.c_int32), ("update_scale_transposed", ctypes.c_float)]
+
+
+class FfnBlock(ctypes.Structure):
+    """morph_ffn."""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "gate", "up", "down")] + [
+        (name, ctypes.c_int64) for name in ("rows", "d", "ff", "x_ld", "gate_ld", "up_ld", "down_ld")]
+
+
+class FfnSaved(ctypes.Structure):
+    """morph_ffn_saved."""
+    _fields_ = [("keep", ctypes.c_int32), ("reserved", ctypes.c_int32)] + [
+        (name, ctypes.c_void_p) for name in (
+            "gate", "up", "gate_exponents", "up_exponents", "x_codes", "x_exponents")]
+
+
+class ScanArgs(ctypes.Structure):
+    """morph_scan."""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("f", "v", "z", "s0")] + [
+        (name, ctypes.c_int64) for name in ("batch", "steps", "dim", "f_batch", "f_step", "v_batch",
+                                            "v_step", "z_batch", "z_step")]
 
 
 _lib = None
@@ -181,6 +205,15 @@ def _load():
                                                   ctypes.POINTER(MuonHP), vp, ctypes.c_size_t,
                                                   vp], i32),
         "morph_host_copy": ([vp, vp, ctypes.c_size_t, i32], i32),
+        "morph_act_pack": ([vp, i32, i64, i64, i64, vp, vp, vp], i32),
+        "morph_act_unpack": ([vp, vp, i64, i64, vp, i32, i64, vp], i32),
+        "morph_ffn_workspace_bytes": ([i64, i64, i64, i32, i32], ctypes.c_size_t),
+        "morph_ffn_forward": ([vp, i32, vp, vp, i64, vp, ctypes.c_size_t, vp], i32),
+        "morph_ffn_backward": ([vp, i32, vp, vp, i64, vp, vp, vp, vp, vp, ctypes.c_size_t, vp], i32),
+        "morph_scan_workspace_bytes": ([i64, i64, i64, i32, i32], ctypes.c_size_t),
+        "morph_scan_forward": ([vp, i32, vp, vp, vp, vp, ctypes.c_size_t, vp], i32),
+        "morph_scan_backward": ([vp, i32, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, ctypes.c_size_t,
+                                 vp], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(handle, name)

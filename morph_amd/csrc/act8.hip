@@ -1,0 +1,183 @@
+// Activation checkpoints in 8 bits (morph_layers.h): E4M3 codes with a power-of-two scale
+// per 32 consecutive values of a row.
+//
+// A power of two as scale keeps the division and the multiplication back exact, so a value
+// is rounded once, and one byte holds it; a floating code loses nothing by it but where a
+// group spans more than E4M3's 2^17.  32 values are what the feed-forward block's epilogue
+// holds of a row in one wave (ffn kernels), so the same groups are written there without a
+// pass of their own.
+//
+// Four lanes hold a group, eight values each: the maximum is a reduction within a quad
+// (two DPP steps), and a wave reads whole lines and writes 512 contiguous codes.
+#include <type_traits>
+
+#include "layers.h"
+
+namespace morph {
+namespace {
+
+constexpr int kGroup = MORPH_ACT_GROUP;
+constexpr int kThreads = 256;
+
+// Values c .. c + 7 of a row of `cols` (zeros behind its end); wide: the row's address and
+// stride allow 16-byte accesses.
+template <typename T>
+__device__ __forceinline__ void load8(const void* row, int64_t c, int64_t cols, bool wide,
+                                      float (&x)[8]) {
+  if constexpr (std::is_same_v<T, F32>) {
+    const float* p = static_cast<const float*>(row) + c;
+    if (wide && c + 8 <= cols) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = lo[k], x[4 + k] = hi[k];
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = c + k < cols ? p[k] : 0.0f;
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(row) + c;
+    if (wide && c + 8 <= cols) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[2 * k] = to_float<T>(v[k] & 0xFFFFu);
+        x[2 * k + 1] = to_float<T>(v[k] >> 16);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = c + k < cols ? to_float<T>(p[k]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(void* row, int64_t c, int64_t cols, bool wide,
+                                       const float (&x)[8]) {
+  if constexpr (std::is_same_v<T, F32>) {
+    float* p = static_cast<float*>(row) + c;
+    if (wide && c + 8 <= cols) {
+      *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      return;
+    }
+    for (int k = 0; k < 8; ++k)
+      if (c + k < cols) p[k] = x[k];
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(row) + c;
+    if (wide && c + 8 <= cols) {
+      u32x4 v;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = from_float<T>(x[2 * k]) | (from_float<T>(x[2 * k + 1]) << 16);
+      *reinterpret_cast<u32x4*>(p) = v;
+      return;
+    }
+    for (int k = 0; k < 8; ++k)
+      if (c + k < cols) p[k] = (uint16_t)from_float<T>(x[k]);
+  }
+}
+
+// Lane: eight values at 8 part of a group; groups are numbered through all rows, of which
+// each has `groups`.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void act_pack_kernel(const void* __restrict__ src, int64_t cols,
+                                                            int64_t ld, uint8_t* __restrict__ codes,
+                                                            uint8_t* __restrict__ exponents,
+                                                            int64_t groups, int64_t total, bool wide) {
+  const int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 2;
+  if (at >= total) return;  // whole quads leave together
+  const int part = threadIdx.x & 3;
+  const int64_t row = at / groups, c = (at - row * groups) * kGroup + 8 * part;
+  float x[8];
+  load8<T>(static_cast<const char*>(src) + row * ld * Fmt<T>::bytes, c, cols, wide, x);
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = max(m, finite_magnitude(x[k]));
+  const int e = act_exponent(quad_max(m));
+  const float inverse = act_inverse(e);
+  *reinterpret_cast<u32x2*>(codes + at * kGroup + 8 * part) =
+      u32x2{act_encode4(x[0], x[1], x[2], x[3], inverse), act_encode4(x[4], x[5], x[6], x[7], inverse)};
+  if (part == 0) exponents[at] = (uint8_t)e;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void act_unpack_kernel(const uint8_t* __restrict__ codes,
+                                                              const uint8_t* __restrict__ exponents,
+                                                              int64_t cols, void* __restrict__ dst,
+                                                              int64_t ld, int64_t groups, int64_t total,
+                                                              bool wide) {
+  const int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 2;
+  if (at >= total) return;
+  const int part = threadIdx.x & 3;
+  const int64_t row = at / groups, c = (at - row * groups) * kGroup + 8 * part;
+  const u32x2 w = *reinterpret_cast<const u32x2*>(codes + at * kGroup + 8 * part);
+  const float scale = act_scale(exponents[at]);
+  float lo[4], hi[4];
+  act_decode4(w.x, scale, lo);
+  act_decode4(w.y, scale, hi);
+  const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  store8<T>(static_cast<char*>(dst) + row * ld * Fmt<T>::bytes, c, cols, wide, x);
+}
+
+bool misaligned(const void* p, uintptr_t by) { return reinterpret_cast<uintptr_t>(p) % by != 0; }
+
+// MORPH_OK with the number of groups and workgroups, or the status to return.
+int act_shape(const void* values, int dtype, int64_t rows, int64_t cols, int64_t ld,
+              const uint8_t* codes, const uint8_t* exponents, int64_t& groups, int64_t& total,
+              int64_t& grid, bool& wide) {
+  if (rows < 0 || cols < 0 || ld < cols) return MORPH_EINVAL;
+  if (dtype != MORPH_DTYPE_F32 && dtype != MORPH_DTYPE_F16 && dtype != MORPH_DTYPE_BF16)
+    return MORPH_EDTYPE;
+  grid = 0;
+  if (rows == 0 || cols == 0) return MORPH_OK;
+  const int64_t size = dtype == MORPH_DTYPE_F32 ? 4 : 2;
+  if (values == nullptr || codes == nullptr || exponents == nullptr || misaligned(codes, 8) ||
+      misaligned(values, size))
+    return MORPH_EINVAL;
+  // the last element's byte offset and the grid
+  if (ld > (INT64_MAX >> 4) / rows) return MORPH_ERANGE;
+  groups = (cols + kGroup - 1) / kGroup;
+  total = rows * groups;
+  grid = (total + kThreads / 4 - 1) / (kThreads / 4);
+  if (grid > 0x7FFFFFFF) return MORPH_ERANGE;
+  wide = !misaligned(values, 16) && (rows == 1 || ld * size % 16 == 0);
+  return MORPH_OK;
+}
+
+}  // namespace
+}  // namespace morph
+
+using namespace morph;
+
+extern "C" int morph_act_pack(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld,
+                              uint8_t* codes, uint8_t* exponents, void* stream) {
+  int64_t groups, total, grid;
+  bool wide;
+  const int status = act_shape(src, dtype, rows, cols, ld, codes, exponents, groups, total, grid, wide);
+  if (status != MORPH_OK || grid == 0) return status;
+  const dim3 g((unsigned)grid), b(kThreads);
+  hipStream_t s = as_stream(stream);
+  if (dtype == MORPH_DTYPE_F32)
+    hipLaunchKernelGGL(act_pack_kernel<F32>, g, b, 0, s, src, cols, ld, codes, exponents, groups, total, wide);
+  else if (dtype == MORPH_DTYPE_F16)
+    hipLaunchKernelGGL(act_pack_kernel<F16>, g, b, 0, s, src, cols, ld, codes, exponents, groups, total, wide);
+  else
+    hipLaunchKernelGGL(act_pack_kernel<BF16>, g, b, 0, s, src, cols, ld, codes, exponents, groups, total, wide);
+  return launch_status();
+}
+
+extern "C" int morph_act_unpack(const uint8_t* codes, const uint8_t* exponents, int64_t rows,
+                                int64_t cols, void* dst, int dtype, int64_t ld, void* stream) {
+  int64_t groups, total, grid;
+  bool wide;
+  const int status = act_shape(dst, dtype, rows, cols, ld, codes, exponents, groups, total, grid, wide);
+  if (status != MORPH_OK || grid == 0) return status;
+  const dim3 g((unsigned)grid), b(kThreads);
+  hipStream_t s = as_stream(stream);
+  if (dtype == MORPH_DTYPE_F32)
+    hipLaunchKernelGGL(act_unpack_kernel<F32>, g, b, 0, s, codes, exponents, cols, dst, ld, groups, total, wide);
+  else if (dtype == MORPH_DTYPE_F16)
+    hipLaunchKernelGGL(act_unpack_kernel<F16>, g, b, 0, s, codes, exponents, cols, dst, ld, groups, total, wide);
+  else
+    hipLaunchKernelGGL(act_unpack_kernel<BF16>, g, b, 0, s, codes, exponents, cols, dst, ld, groups, total, wide);
+  return launch_status();
+}

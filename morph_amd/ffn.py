@@ -1,0 +1,181 @@
+"""The gated feed-forward block of a stage (SwiGLU: gate, up, down), forward and backward.
+
+    h = silu(x @ gate.T) * (x @ up.T),    y = h @ down.T
+
+with the weights as the streamed engine holds them, gate and up [ff, d], down [d, ff], in FP16
+or BF16 (the compute copies that FusedAdamW exports).  The kernels (csrc/ffn.hip) accumulate in
+FP32 and carry the gate in the products' epilogues.
+
+    y = gated_ffn(x, gate, up, down)                              # serving: from one token on
+    y, saved = gated_ffn_forward(x, gate, up, down, keep="fp8")   # training
+    dx, dgate, dup, ddown = gated_ffn_backward(dy, saved, gate, up, down)
+
+The weight gradients have the weights' type and shape, as StageGradients.accumulate takes them.
+GatedFFN is the block as a module whose parameters carry the engine's names (gate.weight, ...).
+"""
+import ctypes
+
+import torch
+
+from ._lib import FfnBlock, FfnSaved, check, lib
+from .activations import PackedActivation
+from .layers import (GROUP, HALF, address, as_rows, current_stream, dtype_code, require_gpu, row_stride,
+                     running_on)
+
+KEEP = {"none": 0, "full": 1, "fp8": 2}
+
+
+class SavedFFN:
+    """What a forward kept for its backward.  keep "full": x itself and both projections in
+    FP32 (gate, up: [rows, 32 G], zero behind ff); "fp8": x, gate and up as PackedActivation."""
+
+    __slots__ = ("keep", "x", "gate", "up", "shape", "ff", "dtype")
+
+    def __init__(self, keep, x, gate, up, shape, ff, dtype):
+        self.keep, self.x, self.gate, self.up = keep, x, gate, up
+        self.shape, self.ff, self.dtype = shape, ff, dtype
+
+    @property
+    def nbytes(self):
+        """Bytes held beyond x, or with "fp8" in all (x need not be kept beside it)."""
+        if self.keep == "fp8":
+            return self.x.nbytes + self.gate.nbytes + self.up.nbytes
+        return 4 * (self.gate.numel() + self.up.numel())
+
+
+def _weights(x, gate, up, down):
+    """The weights as rows, and ff; checked against x."""
+    require_gpu(x, "x", HALF)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("x must be [..., d] with d >= 1")
+    d, device = x.shape[-1], x.device
+    require_gpu(gate, "gate", (x.dtype,), None, device)
+    if gate.dim() != 2 or gate.shape[1] != d or gate.shape[0] == 0:
+        raise ValueError(f"gate has shape {tuple(gate.shape)}, expected [ff, {d}] with ff >= 1")
+    ff = gate.shape[0]
+    require_gpu(up, "up", (x.dtype,), (ff, d), device)
+    require_gpu(down, "down", (x.dtype,), (d, ff), device)
+    return as_rows(gate), as_rows(up), as_rows(down), ff
+
+
+def _block(x, gate, up, down, rows, d, ff):
+    return FfnBlock(address(x), address(gate), address(up), address(down), rows, d, ff,
+                    row_stride(x) if x is not None else d, row_stride(gate), row_stride(up), row_stride(down))
+
+
+def _descriptor(saved):
+    if saved.keep == "full":
+        return FfnSaved(KEEP["full"], 0, address(saved.gate), address(saved.up), None, None, None, None)
+    return FfnSaved(KEEP["fp8"], 0, address(saved.gate.codes), address(saved.up.codes),
+                    address(saved.gate.exponents), address(saved.up.exponents),
+                    address(saved.x.codes), address(saved.x.exponents))
+
+
+def _packed(rows, cols, shape, dtype, device):
+    groups = -(-cols // GROUP)
+    return PackedActivation(torch.empty((rows, groups * GROUP), dtype=torch.uint8, device=device),
+                            torch.empty((rows, groups), dtype=torch.uint8, device=device), shape, dtype)
+
+
+def _forward(x, gate, up, down, keep, stream):
+    gate, up, down, ff = _weights(x, gate, up, down)
+    d, device, dtype = x.shape[-1], x.device, x.dtype
+    rows = x.numel() // d
+    with running_on(device, stream, (x, gate, up, down)):
+        flat = as_rows(x.detach())
+        y = torch.empty(x.shape, dtype=dtype, device=device)
+        saved = None
+        if keep == "full":
+            wide = -(-ff // GROUP) * GROUP
+            kept = torch.empty((2, rows, wide), dtype=torch.float32, device=device)
+            saved = SavedFFN(keep, flat, kept[0], kept[1], x.shape, ff, dtype)
+        elif keep == "fp8":
+            saved = SavedFFN(keep, _packed(rows, d, x.shape, dtype, device),
+                             _packed(rows, ff, (rows, ff), dtype, device),
+                             _packed(rows, ff, (rows, ff), dtype, device), x.shape, ff, dtype)
+        if rows:
+            L = lib()
+            size = L.morph_ffn_workspace_bytes(rows, d, ff, KEEP[keep], 0)
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            check(L.morph_ffn_forward(ctypes.byref(_block(flat, gate, up, down, rows, d, ff)), dtype_code(dtype),
+                                      ctypes.byref(_descriptor(saved)) if saved is not None else None,
+                                      address(y), d, address(workspace), size, current_stream()))
+        return y, saved
+
+
+def gated_ffn(x, gate, up, down, stream=None):
+    """y [..., d] of x [..., d]; nothing is kept for a backward."""
+    return _forward(x, gate, up, down, "none", stream)[0]
+
+
+def gated_ffn_forward(x, gate, up, down, keep="full", stream=None):
+    """(y, saved).  keep "full" holds the projections in FP32, so the gradients carry only the
+    roundings of the matrix instructions' 16-bit operands (8 ff bytes a row, and x by reference:
+    it may not change before the backward); "fp8" holds x and both projections in 8 bits, about
+    d + 2 ff bytes a row, and the backward takes them for x and the projections."""
+    if keep not in ("full", "fp8"):
+        raise ValueError('keep must be "full" or "fp8"')
+    return _forward(x, gate, up, down, keep, stream)
+
+
+def gated_ffn_backward(dy, saved, gate, up, down, stream=None):
+    """(dx, dgate, dup, ddown) from the gradient of y and what the forward kept."""
+    if not isinstance(saved, SavedFFN):
+        raise TypeError("saved must come from gated_ffn_forward")
+    device = (saved.gate.codes if saved.keep == "fp8" else saved.gate).device
+    require_gpu(dy, "dy", (saved.dtype,), saved.shape, device)
+    gate, up, down, ff = _weights(dy, gate, up, down)
+    if ff != saved.ff:
+        raise ValueError(f"the weights have {ff} hidden units, the forward had {saved.ff}")
+    d, dtype = dy.shape[-1], dy.dtype
+    rows = dy.numel() // d
+    kept = ((saved.x, saved.gate, saved.up) if saved.keep == "full" else
+            tuple(t for p in (saved.x, saved.gate, saved.up) for t in (p.codes, p.exponents)))
+    with running_on(device, stream, (dy, gate, up, down, *kept)):
+        flat = as_rows(dy.detach())
+        dx = torch.empty(saved.shape, dtype=dtype, device=device)
+        dgate, dup = (torch.empty((ff, d), dtype=dtype, device=device) for _ in range(2))
+        ddown = torch.empty((d, ff), dtype=dtype, device=device)
+        L = lib()
+        size = L.morph_ffn_workspace_bytes(rows, d, ff, KEEP[saved.keep], 1)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        block = _block(saved.x if saved.keep == "full" else None, gate, up, down, rows, d, ff)
+        check(L.morph_ffn_backward(ctypes.byref(block), dtype_code(dtype), ctypes.byref(_descriptor(saved)),
+                                   address(flat), row_stride(flat), address(dx), address(dgate), address(dup),
+                                   address(ddown), address(workspace), size, current_stream()))
+        return dx, dgate, dup, ddown
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, keep):
+        y, saved = gated_ffn_forward(x, gate, up, down, keep)
+        ctx.saved = saved
+        # tensors that autograd should guard against changes in place
+        ctx.save_for_backward(gate, up, down, *((x,) if keep == "full" else ()))
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        gate, up, down = ctx.saved_tensors[:3]
+        return *gated_ffn_backward(dy, ctx.saved, gate, up, down), None
+
+
+class GatedFFN(torch.nn.Module):
+    """The block as a module: gate, up and down as bias-free Linear layers, so a state dict has
+    gate.weight, up.weight and down.weight.  keep: as gated_ffn_forward's."""
+
+    def __init__(self, d, ff, keep="full", device=None, dtype=torch.float16):
+        super().__init__()
+        if keep not in ("full", "fp8"):
+            raise ValueError('keep must be "full" or "fp8"')
+        self.gate = torch.nn.Linear(d, ff, bias=False, device=device, dtype=dtype)
+        self.up = torch.nn.Linear(d, ff, bias=False, device=device, dtype=dtype)
+        self.down = torch.nn.Linear(ff, d, bias=False, device=device, dtype=dtype)
+        self.keep = keep
+
+    def forward(self, x):
+        weights = self.gate.weight, self.up.weight, self.down.weight
+        if torch.is_grad_enabled() and (x.requires_grad or any(w.requires_grad for w in weights)):
+            return _GatedFFN.apply(x, *weights, self.keep)
+        return gated_ffn(x, *weights)
