@@ -8,9 +8,12 @@
 // g and u meet in one workgroup, so neither is written unless the backward needs it, and dh
 // never is.  Where 8-bit groups are kept they are made from the FP32 sums in the epilogue.
 //
-// ffn_any_kernel takes operands of any stride and alignment, any size: 64 x 64 tiles
-// through LDS, loaded element by element along whichever index is contiguous.
-#include "ffn.h"
+// The tiles of ffn_tiles.h take operands whose rows are 16-byte aligned and a multiple of 8
+// values long.  ffn_any_kernel takes operands of any stride and alignment, any size: 64 x 64
+// tiles through LDS, loaded element by element along whichever index is contiguous.
+#include <cmath>
+
+#include "ffn_tiles.h"
 
 namespace morph {
 namespace {
@@ -99,7 +102,7 @@ __global__ __launch_bounds__(kThreads) void ffn_any_kernel(const FfnProduct a) {
 }
 
 template <typename T>
-int launch_product(FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
+int launch_any(FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
   if (a.M == 0 || a.N == 0) return MORPH_OK;
   const int cols = e == FfnEpilogue::kGate ? kTile / 2 : kTile;
   const int64_t gx = (a.N + cols - 1) / cols, gy = (a.M + kTile - 1) / kTile;
@@ -113,11 +116,179 @@ int launch_product(FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
   return launch_status();
 }
 
-int product(int dtype, FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
-  return dtype == MORPH_DTYPE_F16 ? launch_product<F16>(e, a, s) : launch_product<BF16>(e, a, s);
+// ---- tiles ----------------------------------------------------------------------
+
+// Time of a launch of `tiles` tiles of edge ts over kt stages of K, in us: the constants of
+// the Newton-Schulz products' launches (gemm.hip), which run the same pipeline.
+double tiles_us(int ts, int64_t tiles, int64_t kt, double epilogue) {
+  const double q = (double)tiles / 256.0, n = std::ceil(q);
+  if (ts == 256) {
+    const double full = q / n;
+    return n * ((double)kt * (1.0 + 0.45 * full * full) + 8.5 + 4 * epilogue);
+  }
+  const double stage = n <= 1.0 ? 0.55 : n <= 2.0 ? 0.8 : n <= 8.0 ? 0.45 * n + 0.1 : 0.5 * n - 0.3;
+  return (double)kt * stage + n * (1.3 + epilogue) + 2.0;
 }
 
+// A product in the tiles' form.  `padded`: of an internal buffer, whose rows hold zeros up to
+// a multiple of 32.
+struct Side {
+  const void* p;
+  int64_t ld;
+  bool padded;
+};
+bool fits(const Side& s, int64_t width) {
+  return reinterpret_cast<uintptr_t>(s.p) % 16 == 0 && s.ld % 8 == 0 && s.ld <= (int64_t(1) << 22) &&
+         (width % 8 == 0 || s.padded);
+}
+
+struct Launch {
+  FfnTileArgs a{};
+  bool ok = true;
+  void add(const Side& p, const Side& q, int64_t p_width, int64_t q_width, int64_t M, int64_t N, void* c,
+           int64_t ldc) {
+    FfnTileProblem& o = a.p[a.count++];
+    o.P[0] = o.P[1] = static_cast<const uint16_t*>(p.p);
+    o.Q[0] = o.Q[1] = static_cast<const uint16_t*>(q.p);
+    o.ldp[0] = o.ldp[1] = p.ld, o.ldq[0] = o.ldq[1] = q.ld;
+    o.C = static_cast<uint16_t*>(c), o.ldc = ldc, o.M = (int32_t)M, o.N = (int32_t)N;
+    o.vector = reinterpret_cast<uintptr_t>(c) % 16 == 0 && ldc % 8 == 0;
+    ok = ok && fits(p, p_width) && fits(q, q_width);
+  }
+  // The tile edge for this K, and with it the outputs' tiles; split: 2 where a tile has half as
+  // many output columns (the gate's).
+  int choose(int64_t K, int split, double epilogue) {
+    a.K = (int32_t)K;
+    const int64_t kt = (K + 63) / 64;
+    auto tiles = [&](int ts) {
+      int64_t n = 0;
+      for (int i = 0; i < a.count; ++i) {
+        FfnTileProblem& o = a.p[i];
+        o.first = (int32_t)n;
+        o.tiles_m = (o.M + ts - 1) / ts, o.tiles_n = (o.N + ts / split - 1) / (ts / split);
+        n += (int64_t)o.tiles_m * o.tiles_n;
+      }
+      return n;
+    };
+    const int ts = tiles_us(256, tiles(256), kt, epilogue) <= tiles_us(128, tiles(128), kt, epilogue) ? 256 : 128;
+    const int64_t n = tiles(ts);
+    ok = ok && n <= (1 << 30);
+    a.total = (int32_t)n;
+    return ts;
+  }
+  unsigned grid() const { return (unsigned)((a.total + 7) / 8 * 8); }
+};
+
 int64_t whole_groups(int64_t n) { return (n + MORPH_ACT_GROUP - 1) / MORPH_ACT_GROUP * MORPH_ACT_GROUP; }
+
+int any(int dtype, FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
+  return dtype == MORPH_DTYPE_F16 ? launch_any<F16>(e, a, s) : launch_any<BF16>(e, a, s);
+}
+FfnOperand along(const Side& s) { return FfnOperand{static_cast<const uint16_t*>(s.p), s.ld, 1}; }
+FfnOperand across(const Side& s) { return FfnOperand{static_cast<const uint16_t*>(s.p), 1, s.ld}; }
+
+// h (row length ld) and what `saved` keeps, from x.
+int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int64_t rows, int64_t d, int64_t ff,
+                 const morph_ffn_saved* saved, uint16_t* h, int64_t ld, hipStream_t s) {
+  const int keep = saved ? saved->keep : MORPH_FFN_KEEP_NONE;
+  Launch l;
+  l.add(x, gate, d, d, rows, ff, h, ld);
+  l.ok = l.ok && fits(up, d);
+  l.a.p[0].Q[1] = static_cast<const uint16_t*>(up.p), l.a.p[0].ldq[1] = up.ld;
+  const int ts = l.choose(d, 2, keep == MORPH_FFN_KEEP_NONE ? 0.0 : 1.0);
+  if (keep != MORPH_FFN_KEEP_NONE)
+    l.a.g = saved->gate, l.a.u = saved->up, l.a.g_exponents = saved->gate_exponents,
+    l.a.u_exponents = saved->up_exponents;
+  if (l.ok) {
+    ffn_tile_gate(ts, dtype, keep, l.grid(), s, l.a);
+    return launch_status();
+  }
+  FfnProduct p{};
+  p.P[0] = along(x), p.Q[0] = along(gate), p.Q[1] = along(up);
+  p.M = rows, p.N = ff, p.K = d, p.segments = 1, p.keep = keep, p.C = h, p.ldc = ld;
+  p.g = l.a.g, p.u = l.a.u, p.g_exponents = l.a.g_exponents, p.u_exponents = l.a.u_exponents;
+  return any(dtype, FfnEpilogue::kGate, p, s);
+}
+
+// y = h down^T.
+int down_product(int dtype, const Side& h, const Side& down, int64_t rows, int64_t d, int64_t ff, void* y,
+                 int64_t y_ld, hipStream_t s) {
+  Launch l;
+  l.add(h, down, ff, ff, rows, d, y, y_ld);
+  const int ts = l.choose(ff, 1, 0.0);
+  if (l.ok) {
+    ffn_tile_rows(ts, dtype, l.grid(), s, l.a);
+    return launch_status();
+  }
+  FfnProduct p{};
+  p.P[0] = along(h), p.Q[0] = along(down);
+  p.M = rows, p.N = d, p.K = ff, p.segments = 1, p.C = static_cast<uint16_t*>(y), p.ldc = y_ld;
+  return any(dtype, FfnEpilogue::kStore, p, s);
+}
+
+// h, dg and du (row length ld) from dy and what was kept.
+int grad_product(int dtype, const Side& dy, const Side& down, int64_t rows, int64_t d, int64_t ff,
+                 const morph_ffn_saved* saved, uint16_t* h, uint16_t* dg, uint16_t* du, int64_t ld, hipStream_t s) {
+  Launch l;
+  l.add(dy, down, d, ff, rows, ff, h, ld);
+  const int ts = l.choose(d, 1, 3.0);
+  l.a.dg = dg, l.a.du = du, l.a.g = saved->gate, l.a.u = saved->up;
+  l.a.g_exponents = saved->gate_exponents, l.a.u_exponents = saved->up_exponents;
+  if (l.ok) {
+    ffn_tile_grad(ts, dtype, saved->keep, l.grid(), s, l.a);
+    return launch_status();
+  }
+  FfnProduct p{};
+  p.P[0] = along(dy), p.Q[0] = across(down);
+  p.M = rows, p.N = ff, p.K = d, p.segments = 1, p.keep = saved->keep, p.C = h, p.ldc = ld, p.dg = dg, p.du = du;
+  p.g = saved->gate, p.u = saved->up, p.g_exponents = saved->gate_exponents, p.u_exponents = saved->up_exponents;
+  return any(dtype, FfnEpilogue::kGateGrad, p, s);
+}
+
+// dx = dg gate + du up.
+int input_product(int dtype, const Side& dg, const Side& du, const Side& gate, const Side& up, int64_t rows,
+                  int64_t d, int64_t ff, void* dx, hipStream_t s) {
+  Launch l;
+  l.add(dg, gate, ff, d, rows, d, dx, d);
+  l.ok = l.ok && fits(up, d) && gate.ld == up.ld;  // one set of offsets for both segments
+  FfnTileProblem& o = l.a.p[0];
+  o.P[1] = static_cast<const uint16_t*>(du.p), o.Q[1] = static_cast<const uint16_t*>(up.p);
+  const int ts = l.choose(ff, 1, 0.0);
+  if (l.ok) {
+    ffn_tile_two(ts, dtype, l.grid(), s, l.a);
+    return launch_status();
+  }
+  FfnProduct p{};
+  p.P[0] = along(dg), p.Q[0] = across(gate), p.P[1] = along(du), p.Q[1] = across(up);
+  p.M = rows, p.N = d, p.K = ff, p.segments = 2, p.C = static_cast<uint16_t*>(dx), p.ldc = d;
+  return any(dtype, FfnEpilogue::kStore, p, s);
+}
+
+// The three weight gradients, in one launch where the tiles take them.
+int weight_products(int dtype, const Side& dg, const Side& du, const Side& x, const Side& dy, const Side& h,
+                    int64_t rows, int64_t d, int64_t ff, void* dgate, void* dup, void* ddown, hipStream_t s) {
+  struct {
+    const Side &p, &q;
+    int64_t M, N;
+    void* out;
+  } w[3] = {{dg, x, ff, d, dgate}, {du, x, ff, d, dup}, {dy, h, d, ff, ddown}};
+  Launch l;
+  for (auto& e : w) l.add(e.p, e.q, e.M, e.N, e.M, e.N, e.out, e.N);
+  const int ts = l.choose(rows, 1, 0.0);
+  if (l.ok && rows > 0) {
+    ffn_tile_weights(ts, dtype, l.grid(), s, l.a);
+    return launch_status();
+  }
+  for (auto& e : w) {
+    FfnProduct p{};
+    p.P[0] = across(e.p), p.Q[0] = across(e.q);
+    p.M = e.M, p.N = e.N, p.K = rows, p.segments = 1, p.C = static_cast<uint16_t*>(e.out), p.ldc = e.N;
+    const int status = any(dtype, FfnEpilogue::kStore, p, s);
+    if (status != MORPH_OK) return status;
+  }
+  return MORPH_OK;
+}
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Limits under which every offset fits 64 bits and every grid the hardware (65535 tiles of
@@ -175,29 +346,14 @@ extern "C" int morph_ffn_forward(const morph_ffn* a, int dtype, const morph_ffn_
   hipStream_t s = as_stream(stream);
   uint16_t* h = static_cast<uint16_t*>(workspace);
   const int64_t ld = whole_groups(a->ff);
-  auto rows16 = [](const void* p, int64_t ldp) {
-    return FfnOperand{static_cast<const uint16_t*>(p), ldp, 1};
-  };
   if (keep == MORPH_FFN_KEEP_ACT8) {
     status = morph_act_pack(a->x, dtype, a->rows, a->d, a->x_ld, saved->x_codes, saved->x_exponents, stream);
     if (status != MORPH_OK) return status;
   }
-  FfnProduct p{};
-  p.P[0] = rows16(a->x, a->x_ld);
-  p.Q[0] = rows16(a->gate, a->gate_ld);
-  p.Q[1] = rows16(a->up, a->up_ld);
-  p.M = a->rows, p.N = a->ff, p.K = a->d, p.segments = 1, p.keep = keep;
-  p.C = h, p.ldc = ld;
-  if (keep != MORPH_FFN_KEEP_NONE)
-    p.g = saved->gate, p.u = saved->up, p.g_exponents = saved->gate_exponents, p.u_exponents = saved->up_exponents;
-  status = product(dtype, FfnEpilogue::kGate, p, s);
+  status = gate_product(dtype, Side{a->x, a->x_ld, false}, Side{a->gate, a->gate_ld, false},
+                        Side{a->up, a->up_ld, false}, a->rows, a->d, a->ff, saved, h, ld, s);
   if (status != MORPH_OK) return status;
-  FfnProduct o{};
-  o.P[0] = rows16(h, ld);
-  o.Q[0] = rows16(a->down, a->down_ld);
-  o.M = a->rows, o.N = a->d, o.K = a->ff, o.segments = 1;
-  o.C = static_cast<uint16_t*>(y), o.ldc = y_ld;
-  return product(dtype, FfnEpilogue::kStore, o, s);
+  return down_product(dtype, Side{h, ld, true}, Side{a->down, a->down_ld, false}, a->rows, a->d, a->ff, y, y_ld, s);
 }
 
 extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn_saved* saved,
@@ -218,44 +374,19 @@ extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn
   const int64_t ld = whole_groups(a->ff);
   uint16_t* h = static_cast<uint16_t*>(workspace);
   uint16_t *dg = h + a->rows * ld, *du = dg + a->rows * ld, *xs = du + a->rows * ld;
-  const uint16_t* x = static_cast<const uint16_t*>(a->x);
-  int64_t x_ld = a->x_ld;
+  Side x{a->x, a->x_ld, false};
   if (saved->keep == MORPH_FFN_KEEP_ACT8 && a->rows > 0) {
-    x = xs, x_ld = whole_groups(a->d);
-    status = morph_act_unpack(saved->x_codes, saved->x_exponents, a->rows, a->d, xs, dtype, x_ld, stream);
+    x = Side{xs, whole_groups(a->d), true};
+    status = morph_act_unpack(saved->x_codes, saved->x_exponents, a->rows, a->d, xs, dtype, x.ld, stream);
     if (status != MORPH_OK) return status;
   }
-  auto along = [](const void* p, int64_t ldp) {  // the rows of a stored matrix, K along them
-    return FfnOperand{static_cast<const uint16_t*>(p), ldp, 1};
-  };
-  auto across = [](const void* p, int64_t ldp) {  // its columns, K across its rows
-    return FfnOperand{static_cast<const uint16_t*>(p), 1, ldp};
-  };
-  auto run = [&](FfnEpilogue e, const FfnProduct& p) {
-    if (status == MORPH_OK) status = product(dtype, e, p, s);
-  };
-  FfnProduct p{};
-  p.P[0] = along(dy, dy_ld), p.Q[0] = across(a->down, a->down_ld);
-  p.M = a->rows, p.N = a->ff, p.K = a->d, p.segments = 1, p.keep = saved->keep;
-  p.C = h, p.ldc = ld, p.dg = dg, p.du = du;
-  p.g = saved->gate, p.u = saved->up, p.g_exponents = saved->gate_exponents, p.u_exponents = saved->up_exponents;
-  run(FfnEpilogue::kGateGrad, p);
-
-  FfnProduct q{};
-  q.P[0] = along(dg, ld), q.Q[0] = across(a->gate, a->gate_ld);
-  q.P[1] = along(du, ld), q.Q[1] = across(a->up, a->up_ld);
-  q.M = a->rows, q.N = a->d, q.K = a->ff, q.segments = 2;
-  q.C = static_cast<uint16_t*>(dx), q.ldc = a->d;
-  run(FfnEpilogue::kStore, q);
-
-  auto weight = [&](FfnOperand left, int64_t m, FfnOperand right, int64_t n, void* out) {
-    FfnProduct w{};
-    w.P[0] = left, w.Q[0] = right, w.M = m, w.N = n, w.K = a->rows, w.segments = 1;
-    w.C = static_cast<uint16_t*>(out), w.ldc = n;
-    run(FfnEpilogue::kStore, w);
-  };
-  weight(across(dg, ld), a->ff, across(x, x_ld), a->d, dgate);
-  weight(across(du, ld), a->ff, across(x, x_ld), a->d, dup);
-  weight(across(dy, dy_ld), a->d, across(h, ld), a->ff, ddown);
+  const Side gate{a->gate, a->gate_ld, false}, up{a->up, a->up_ld, false}, down{a->down, a->down_ld, false};
+  const Side sh{h, ld, true}, sg{dg, ld, true}, su{du, ld, true}, sy{dy, dy_ld, false};
+  if (a->rows > 0) {
+    status = grad_product(dtype, sy, down, a->rows, a->d, a->ff, saved, h, dg, du, ld, s);
+    if (status == MORPH_OK) status = input_product(dtype, sg, su, gate, up, a->rows, a->d, a->ff, dx, s);
+  }
+  if (status == MORPH_OK)
+    status = weight_products(dtype, sg, su, x, sy, sh, a->rows, a->d, a->ff, dgate, dup, ddown, s);
   return status;
 }
