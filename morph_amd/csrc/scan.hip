@@ -1,9 +1,31 @@
 // Gated linear recurrence (morph_layers.h) and its backward pass: s_t = a_t s_(t-1) + (1 - a_t) v_t
 // along the steps of [batch, steps, dim], every channel on its own.
 //
-// A lane walks the steps of one channel.  The backward walks the spans of MORPH_SCAN_SPAN steps
-// from the last to the first and computes each span's states again from the one that the
-// forward kept.
+// The recurrence of a stretch of steps is s -> A s + S with A the product of its gates and S
+// its result from a zero state, and two stretches compose: (A2, S2) after (A1, S1) is
+// (A2 A1, A2 S1 + S2).  So a workgroup takes a tile of steps and 128 channels, a lane two
+// channels, a wave kSteps consecutive steps, all loaded at once; each wave finds its (A, S) in
+// registers, the waves' are joined through LDS, and the second pass over the registers starts from
+// the true state.  Every tensor is read and written once.
+//
+// Tiles of one channel group follow each other in time through memory, with the same sums
+// whatever their timing: kRun of them make a run.  A tile publishes its (A, S) before it waits for
+// anything; then it applies the (A, S) of the tiles before it in its run, in order, to the state
+// that the run begins with, which the last tile of the run before published.  (Taking
+// whichever is there, a predecessor's state or its (A, S), would round differently from call to
+// call.)  A published word is 64 bits, value and mark together, so no ordering between words
+// is needed.  Tiles are taken by ticket, earlier times first: what a tile waits for is always
+// running or done, so every wait ends (kSpins bounds it all the same).
+//
+// The forward applies every step's (A, S) from the tile's beginning to the state that enters
+// the tile, so the state behind a tile's last step is, bit for bit, the one that the next tile
+// begins with: where all gates are 1 the state stays as it is, across waves and tiles.
+//
+// The backward runs the tiles from the last to the first: r_t = w_t + a_(t+1) r_(t+1) is the same
+// recurrence in reversed time with the same A, and the states come again from the one that
+// the forward kept for each tile, in the same pass.
+//
+// A lane per channel that walks all steps (scan_walk_kernel) serves single steps.
 #include <type_traits>
 
 #include "layers.h"
@@ -12,6 +34,7 @@ namespace morph {
 namespace {
 
 constexpr int kSpan = MORPH_SCAN_SPAN;
+constexpr int kWalk = 1;  // steps up to which a lane walks them all
 
 template <typename T>
 __device__ __forceinline__ float load1(const void* p, int64_t i) {
@@ -93,6 +116,367 @@ __global__ __launch_bounds__(64) void scan_walk_back_kernel(morph_scan a, const 
   if (ds0) ds0[b * a.dim + c] = r;
 }
 
+// ---- tiles ----------------------------------------------------------------------
+
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kForwardSteps = 16;  // of a wave: 128 steps a tile
+constexpr int kBackwardSteps = 8;  // 64: the backward holds four values per step and channel
+constexpr int kSpins = 1 << 20;
+static_assert(kWaves * kBackwardSteps == kSpan, "a backward tile begins with a kept state");
+static_assert(kSpan % kForwardSteps == 0, "states are kept at a wave's first step");
+
+// kVec consecutive channels of one step as loaded: 16-bit pairs or singles, floats.
+template <typename T, int kVec>
+struct Raw {
+  typedef uint32_t type;
+};
+template <int kVec>
+struct Raw<F32, kVec> {
+  typedef float type __attribute__((ext_vector_type(kVec)));
+};
+template <typename T, int kVec>
+__device__ __forceinline__ typename Raw<T, kVec>::type load_raw(const void* p, int64_t i) {
+  if constexpr (std::is_same_v<T, F32>)
+    return *reinterpret_cast<const typename Raw<F32, kVec>::type*>(static_cast<const float*>(p) + i);
+  else if constexpr (kVec == 2)
+    return *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+  else
+    return static_cast<const uint16_t*>(p)[i];
+}
+template <typename T, int kVec>
+__device__ __forceinline__ float value(const typename Raw<T, kVec>::type& r, int k) {
+  if constexpr (std::is_same_v<T, F32>) return r[k];
+  else return to_float<T>(k ? r >> 16 : kVec == 2 ? r & 0xFFFFu : r);
+}
+template <typename T, int kVec>
+__device__ __forceinline__ void store_vec(void* p, int64_t i, const float (&x)[kVec]) {
+  if constexpr (std::is_same_v<T, F32>) {
+    typename Raw<F32, kVec>::type v;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) v[k] = x[k];
+    *reinterpret_cast<typename Raw<F32, kVec>::type*>(static_cast<float*>(p) + i) = v;
+  } else if constexpr (kVec == 2) {
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + i) = from_float<T>(x[0]) | (from_float<T>(x[1]) << 16);
+  } else {
+    static_cast<uint16_t*>(p)[i] = (uint16_t)from_float<T>(x[0]);
+  }
+}
+
+// A launch's tiles: `groups` = batch x channel groups, `tiles` steps' tiles of each.
+struct ScanGrid {
+  uint32_t* ticket;  // the workspace: tickets given out, then
+  uint64_t* parts;   // [tiles][groups][64 lanes][kVec]{A, S}
+  uint64_t* runs;    // [runs][groups][64 lanes][kVec]: the state that run 1, 2, ... begins with
+  int32_t tiles, groups, channel_groups;
+};
+constexpr int kRun = 16;  // tiles: two for each wave to fetch
+constexpr uint64_t kMark = uint64_t(1) << 32;
+
+__device__ __forceinline__ void publish(uint64_t* at, float x) {
+  __hip_atomic_store(at, kMark | __builtin_bit_cast(uint32_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// kCount words of this lane, once all of the wave's are published (NaN should that never be).
+template <int kCount>
+__device__ __forceinline__ void fetch(const uint64_t* at, float (&x)[kCount]) {
+  uint64_t w[kCount];
+  bool all = false;
+  for (int spin = 0; spin < kSpins && !all; ++spin) {
+    if (spin > 0) __builtin_amdgcn_s_sleep(1);
+    bool mine = true;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      w[i] = __hip_atomic_load(at + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      mine = mine && w[i] >= kMark;
+    }
+    all = __all(mine);
+  }
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) x[i] = all ? __builtin_bit_cast(float, (uint32_t)w[i]) : __builtin_nanf("");
+}
+
+// This workgroup's tile, in the order of the tickets, and its group.
+__device__ __forceinline__ int take_tile(const ScanGrid& g, int& group) {
+  int id = (int)blockIdx.x;
+  if (g.tiles > 1) {
+    __shared__ int mine;
+    if (threadIdx.x == 0)
+      mine = (int)__hip_atomic_fetch_add(g.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    id = mine;
+  }
+  id = __builtin_amdgcn_readfirstlane(id);
+  group = id % g.groups;
+  return id / g.groups;
+}
+
+// What enters the tile (carry) and the (A, S) of its steps before this wave; first: what enters
+// the first tile.  `order`: the wave's place in the direction of the walk.
+template <int kVec>
+__device__ __forceinline__ void enter_tile(const ScanGrid& g, int tile, int group, int order, int lane,
+                                           const float (&A)[kVec], const float (&S)[kVec], const float (&first)[kVec],
+                                           float (&wa)[kVec], float (&ws)[kVec], float (&carry)[kVec]) {
+  __shared__ float sa[kWaves][kVec][64], ss[kWaves][kVec][64];
+  __shared__ float pa[kRun][kVec][64], ps[kRun][kVec][64], begin[kVec][64];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) sa[order][k][lane] = A[k], ss[order][k][lane] = S[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) {
+    wa[k] = 1.0f, ws[k] = 0.0f;
+    for (int w = 0; w < order; ++w) {
+      ws[k] = __fmaf_rn(sa[w][k][lane], ws[k], ss[w][k][lane]);
+      wa[k] *= sa[w][k][lane];
+    }
+  }
+  // with this wave's: of the whole tile in the last one
+  float la[kVec], ls[kVec];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) ls[k] = __fmaf_rn(A[k], ws[k], S[k]), la[k] = wa[k] * A[k];
+
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) carry[k] = first[k];
+  const int run = tile / kRun, before = tile % kRun;
+  if (g.tiles > 1) {
+    const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
+    if (order == kWaves - 1 && before < kRun - 1 && tile + 1 < g.tiles) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        publish(g.parts + 2 * (tile * stride + mine + k), la[k]);
+        publish(g.parts + 2 * (tile * stride + mine + k) + 1, ls[k]);
+      }
+    }
+    for (int i = order; i < before; i += kWaves) {
+      float w[2 * kVec];
+      fetch<2 * kVec>(g.parts + 2 * (((int64_t)run * kRun + i) * stride + mine), w);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) pa[i][k][lane] = w[2 * k], ps[i][k][lane] = w[2 * k + 1];
+    }
+    if (run > 0 && order == kWaves - 1) {
+      float w[kVec];
+      fetch<kVec>(g.runs + run * stride + mine, w);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) begin[k][lane] = w[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      if (run > 0) carry[k] = begin[k][lane];
+      for (int i = 0; i < before; ++i) carry[k] = __fmaf_rn(pa[i][k][lane], carry[k], ps[i][k][lane]);
+    }
+    if (order == kWaves - 1 && before == kRun - 1 && tile + 1 < g.tiles) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+        publish(g.runs + (run + 1) * stride + mine + k, __fmaf_rn(la[k], carry[k], ls[k]));
+    }
+  }
+}
+
+template <typename T, int kVec, bool kGated>
+__global__ __launch_bounds__(kThreads) void scan_tile_kernel(const morph_scan a, const ScanGrid g,
+                                                             void* __restrict__ y, float* __restrict__ last,
+                                                             float* __restrict__ states) {
+  constexpr int L = kForwardSteps;
+  int group;
+  const int tile = take_tile(g, group);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t b = group / g.channel_groups;
+  const int64_t c0 = ((int64_t)(group % g.channel_groups) * 64 + lane) * kVec;
+  const bool active = c0 < a.dim;
+  const int64_t c = active ? c0 : 0;
+  const int64_t t0 = ((int64_t)tile * kWaves + wave) * L;
+  const int n = (int)(a.steps - t0 < L ? a.steps - t0 : L);  // <= 0: no steps
+
+  float A[kVec], S[kVec], pa[L][kVec], ps[L][kVec];  // (A, S) from the wave's first step on
+  typename Raw<T, kVec>::type z[L];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) A[k] = 1.0f, S[k] = 0.0f;
+  if (n > 0) {
+    typename Raw<T, kVec>::type f[L], v[L];
+    const int64_t pf = b * a.f_batch + t0 * a.f_step + c, pv = b * a.v_batch + t0 * a.v_step + c;
+    const int64_t pz = b * a.z_batch + t0 * a.z_step + c;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int j = i < n ? i : n - 1;
+      f[i] = load_raw<T, kVec>(a.f, pf + j * a.f_step);
+      v[i] = load_raw<T, kVec>(a.v, pv + j * a.v_step);
+    }
+    if constexpr (kGated) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) z[i] = load_raw<T, kVec>(a.z, pz + (i < n ? i : n - 1) * a.z_step);
+    }
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        const Sigmoid s = sigmoid(value<T, kVec>(f[i], k));
+        const float gate = i < n ? s.a : 1.0f;  // steps past the end pass the state on
+        const float in = i < n ? s.b * value<T, kVec>(v[i], k) : 0.0f;
+        ps[i][k] = S[k] = __fmaf_rn(gate, S[k], in);
+        pa[i][k] = A[k] *= gate;
+      }
+    }
+  }
+  float first[kVec], wa[kVec], ws[kVec], carry[kVec];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) first[k] = a.s0 ? a.s0[b * a.dim + c + k] : 0.0f;
+  enter_tile<kVec>(g, tile, group, wave, lane, A, S, first, wa, ws, carry);
+  if (!active) return;
+  if (n > 0) {
+    if (states && t0 % kSpan == 0) {
+      const int64_t spans = (a.steps + kSpan - 1) / kSpan;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+        states[(b * spans + t0 / kSpan) * a.dim + c + k] = __fmaf_rn(wa[k], carry[k], ws[k]);
+    }
+    const int64_t py = (b * a.steps + t0) * a.dim + c;
+    float s[kVec];
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      float out[kVec];
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        s[k] = out[k] = __fmaf_rn(wa[k] * pa[i][k], carry[k], __fmaf_rn(pa[i][k], ws[k], ps[i][k]));
+        if constexpr (kGated) {
+          const float q = value<T, kVec>(z[i], k);
+          out[k] *= q * sigmoid(q).a;
+        }
+      }
+      if (i < n) store_vec<T, kVec>(y, py + (int64_t)i * a.dim, out);
+    }
+    if (last && t0 + n == a.steps) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) last[b * a.dim + c + k] = s[k];
+    }
+  }
+}
+
+template <typename T, int kVec, bool kGated>
+__global__ __launch_bounds__(kThreads) void scan_tile_back_kernel(const morph_scan a, const ScanGrid g,
+                                                                  const float* __restrict__ states,
+                                                                  const void* __restrict__ dy, int64_t dy_batch,
+                                                                  int64_t dy_step, const float* __restrict__ dlast,
+                                                                  void* __restrict__ df, void* __restrict__ dv,
+                                                                  void* __restrict__ dz, float* __restrict__ ds0) {
+  constexpr int L = kBackwardSteps;
+  int group;
+  const int walked = take_tile(g, group);
+  const int tile = g.tiles - 1 - walked;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t b = group / g.channel_groups;
+  const int64_t c0 = ((int64_t)(group % g.channel_groups) * 64 + lane) * kVec;
+  const bool active = c0 < a.dim;
+  const int64_t c = active ? c0 : 0;
+  const int64_t t0 = ((int64_t)tile * kWaves + wave) * L;
+  const int n = (int)(a.steps - t0 < L ? a.steps - t0 : L);
+
+  // gate: a; pass: 1 - a; w: dy silu(z); q: what r is multiplied by for df, from the states
+  float gate[L][kVec], pass[L][kVec], w[L][kVec], x[L][kVec], slope[kGated ? L : 1][kVec];
+  float A[kVec], S[kVec], R[kVec], s[kVec], r[kVec];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) A[k] = 1.0f, S[k] = 0.0f, R[k] = 0.0f;
+  if (n > 0) {
+    typename Raw<T, kVec>::type rf[L], rv[L], rz[kGated ? L : 1], rd[L];
+    const int64_t pf = b * a.f_batch + t0 * a.f_step + c, pv = b * a.v_batch + t0 * a.v_step + c;
+    const int64_t pz = b * a.z_batch + t0 * a.z_step + c, pd = b * dy_batch + t0 * dy_step + c;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int j = i < n ? i : n - 1;
+      rf[i] = load_raw<T, kVec>(a.f, pf + j * a.f_step);
+      rv[i] = load_raw<T, kVec>(a.v, pv + j * a.v_step);
+      if constexpr (kGated) rz[i] = load_raw<T, kVec>(a.z, pz + j * a.z_step);
+      rd[i] = load_raw<T, kVec>(dy, pd + j * dy_step);
+    }
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        const Sigmoid q = sigmoid(value<T, kVec>(rf[i], k));
+        gate[i][k] = i < n ? q.a : 1.0f;
+        pass[i][k] = i < n ? q.b : 0.0f;
+        x[i][k] = i < n ? value<T, kVec>(rv[i], k) : 0.0f;
+        w[i][k] = i < n ? value<T, kVec>(rd[i], k) : 0.0f;
+        if constexpr (kGated) {
+          const float zv = i < n ? value<T, kVec>(rz[i], k) : 0.0f;
+          const Sigmoid h = sigmoid(zv);
+          slope[i][k] = w[i][k] * (h.a * __fmaf_rn(zv, h.b, 1.0f));
+          w[i][k] *= zv * h.a;
+        }
+        S[k] = __fmaf_rn(gate[i][k], S[k], pass[i][k] * x[i][k]);
+        A[k] *= gate[i][k];
+      }
+    }
+#pragma unroll
+    for (int i = L - 1; i >= 0; --i)
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) R[k] = gate[i][k] * (w[i][k] + R[k]);
+  }
+  // the state that enters each wave, from the one kept for the tile
+  {
+    __shared__ float sa[kWaves][kVec][64], ss[kWaves][kVec][64];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) sa[wave][k][lane] = A[k], ss[wave][k][lane] = S[k];
+    __syncthreads();
+    const int64_t spans = (a.steps + kSpan - 1) / kSpan;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      s[k] = states[(b * spans + tile) * a.dim + c + k];
+      for (int i = 0; i < wave; ++i) s[k] = __fmaf_rn(sa[i][k][lane], s[k], ss[i][k][lane]);
+    }
+  }
+  if (n > 0) {
+    const int64_t at = (b * a.steps + t0) * a.dim + c;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      float out[kVec];
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        const float prev = s[k], v = x[i][k];
+        s[k] = __fmaf_rn(gate[i][k], prev, pass[i][k] * v);
+        x[i][k] = (prev - v) * (gate[i][k] * pass[i][k]);
+        if constexpr (kGated) out[k] = slope[i][k] * s[k];
+      }
+      if constexpr (kGated)
+        if (i < n && active) store_vec<T, kVec>(dz, at + (int64_t)i * a.dim, out);
+    }
+  }
+  float first[kVec], wa[kVec], wr[kVec], carry[kVec];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) first[k] = dlast ? dlast[b * a.dim + c + k] : 0.0f;
+  enter_tile<kVec>(g, walked, group, kWaves - 1 - wave, lane, A, R, first, wa, wr, carry);
+  if (!active || n <= 0) return;
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) r[k] = __fmaf_rn(wa[k], carry[k], wr[k]);
+  const int64_t at = (b * a.steps + t0) * a.dim + c;
+#pragma unroll
+  for (int i = L - 1; i >= 0; --i) {
+    float of[kVec], ov[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      r[k] += w[i][k];
+      ov[k] = r[k] * pass[i][k];
+      of[k] = r[k] * x[i][k];
+      r[k] *= gate[i][k];
+    }
+    if (i < n) {
+      store_vec<T, kVec>(dv, at + (int64_t)i * a.dim, ov);
+      store_vec<T, kVec>(df, at + (int64_t)i * a.dim, of);
+    }
+  }
+  if (ds0 && t0 == 0) {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) ds0[b * a.dim + c + k] = r[k];
+  }
+}
+
+// Zeros: the tickets and marks of a launch.  (A kernel, not a memset: a captured memset node is
+// not replayed reliably.)
+__global__ __launch_bounds__(256) void scan_clear_kernel(u32x4* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = u32x4{0u, 0u, 0u, 0u};
+}
+
 bool float_type(int dtype) {
   return dtype == MORPH_DTYPE_F32 || dtype == MORPH_DTYPE_F16 || dtype == MORPH_DTYPE_BF16;
 }
@@ -106,50 +490,135 @@ int scan_check(const morph_scan* a, int dtype) {
   return MORPH_OK;
 }
 
+// ---- host -------------------------------------------------------------------------
+
+constexpr size_t kTicketBytes = 256;
+
+int64_t tiles_of(int64_t steps, bool backward) {
+  const int64_t span = kWaves * (backward ? kBackwardSteps : kForwardSteps);
+  return (steps + span - 1) / span;
+}
+// Words for either channel count per lane, channels rounded up to 128: two a tile, one a run.
+size_t scan_words(int64_t channels, int64_t tiles) {
+  return (size_t)channels * (size_t)(2 * tiles + (tiles + kRun - 1) / kRun);
+}
+size_t scan_workspace(int64_t batch, int64_t steps, int64_t dim, bool backward) {
+  const int64_t tiles = tiles_of(steps, backward);
+  if (batch <= 0 || dim <= 0 || tiles <= 1) return 0;
+  return kTicketBytes + 8 * scan_words(batch * ((dim + 127) / 128 * 128), tiles);
+}
+
+// Whether two channels a lane fit: even rows, and pairs aligned.
+bool pairs(const void* p, int64_t batch, int64_t step, int64_t size) {
+  return p == nullptr || (batch % 2 == 0 && step % 2 == 0 && reinterpret_cast<uintptr_t>(p) % (2 * size) == 0);
+}
+
+int scan_grid(const morph_scan* a, int kvec, bool backward, void* workspace, hipStream_t s, ScanGrid& g,
+              unsigned& grid) {
+  const int64_t groups_c = (a->dim + 64 * kvec - 1) / (64 * kvec), groups = groups_c * a->batch;
+  const int64_t tiles = tiles_of(a->steps, backward), total = tiles * groups;
+  if (total > 0x7FFFFFFF) return MORPH_ERANGE;
+  g.ticket = static_cast<uint32_t*>(workspace);
+  g.parts = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kTicketBytes);
+  g.runs = g.parts + 2 * total * 64 * kvec;
+  g.tiles = (int32_t)tiles, g.groups = (int32_t)groups, g.channel_groups = (int32_t)groups_c;
+  grid = (unsigned)total;
+  if (tiles > 1) {
+    const int64_t n = (int64_t)(kTicketBytes + 8 * scan_words(groups * 64 * kvec, tiles)) / 16;
+    hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
+                       static_cast<u32x4*>(workspace), n);
+  }
+  return MORPH_OK;
+}
+
+// A call's kernel by its types: F(T, two channels a lane, output gate).
+template <typename F>
+void by_form(int dtype, bool two, bool gated, F&& f) {
+  auto with = [&](auto type) {
+    if (two && gated) f(type, std::integral_constant<int, 2>{}, std::true_type{});
+    else if (two) f(type, std::integral_constant<int, 2>{}, std::false_type{});
+    else if (gated) f(type, std::integral_constant<int, 1>{}, std::true_type{});
+    else f(type, std::integral_constant<int, 1>{}, std::false_type{});
+  };
+  if (dtype == MORPH_DTYPE_F32) with(F32{});
+  else if (dtype == MORPH_DTYPE_F16) with(F16{});
+  else with(BF16{});
+}
+
 }  // namespace
 }  // namespace morph
 
 using namespace morph;
 
-extern "C" size_t morph_scan_workspace_bytes(int64_t, int64_t, int64_t, int, int) { return 0; }
+extern "C" size_t morph_scan_workspace_bytes(int64_t batch, int64_t steps, int64_t dim, int, int backward) {
+  return scan_workspace(batch, steps, dim, backward != 0);
+}
 
-extern "C" int morph_scan_forward(const morph_scan* scan, int dtype, void* y, float* last,
-                                  float* states, void*, size_t, void* stream) {
+extern "C" int morph_scan_forward(const morph_scan* scan, int dtype, void* y, float* last, float* states,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
   const int status = scan_check(scan, dtype);
   if (status != MORPH_OK) return status;
   if (scan->batch == 0 || scan->dim == 0) return MORPH_OK;
   if (scan->steps > 0 && y == nullptr) return MORPH_EINVAL;
-  const dim3 grid((unsigned)((scan->dim + 63) / 64), (unsigned)scan->batch);
+  const size_t need = scan_workspace(scan->batch, scan->steps, scan->dim, false);
+  if (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
+    return MORPH_EWORKSPACE;
   hipStream_t s = as_stream(stream);
-  if (dtype == MORPH_DTYPE_F32)
-    hipLaunchKernelGGL(scan_walk_kernel<F32>, grid, dim3(64), 0, s, *scan, y, last, states);
-  else if (dtype == MORPH_DTYPE_F16)
-    hipLaunchKernelGGL(scan_walk_kernel<F16>, grid, dim3(64), 0, s, *scan, y, last, states);
-  else
-    hipLaunchKernelGGL(scan_walk_kernel<BF16>, grid, dim3(64), 0, s, *scan, y, last, states);
+  const morph_scan a = *scan;
+  if (a.steps <= kWalk) {
+    const dim3 grid((unsigned)((a.dim + 63) / 64), (unsigned)a.batch);
+    by_form(dtype, false, false, [&](auto type, auto, auto) {
+      hipLaunchKernelGGL(scan_walk_kernel<decltype(type)>, grid, dim3(64), 0, s, a, y, last, states);
+    });
+    return launch_status();
+  }
+  const int64_t size = dtype == MORPH_DTYPE_F32 ? 4 : 2;
+  const bool two = a.dim % 2 == 0 && pairs(a.f, a.f_batch, a.f_step, size) && pairs(a.v, a.v_batch, a.v_step, size) &&
+                   pairs(a.z, a.z_batch, a.z_step, size) && pairs(y, 0, 0, size);
+  ScanGrid g;
+  unsigned grid;
+  const int shape = scan_grid(scan, two ? 2 : 1, false, workspace, s, g, grid);
+  if (shape != MORPH_OK) return shape;
+  by_form(dtype, two, a.z != nullptr, [&](auto type, auto vec, auto gated) {
+    hipLaunchKernelGGL((scan_tile_kernel<decltype(type), decltype(vec)::value, decltype(gated)::value>), dim3(grid),
+                       dim3(kThreads), 0, s, a, g, y, last, states);
+  });
   return launch_status();
 }
 
-extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const float* states,
-                                   const void* dy, int64_t dy_batch, int64_t dy_step,
-                                   const float* dlast, void* df, void* dv, void* dz, float* ds0,
-                                   void*, size_t, void* stream) {
+extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const float* states, const void* dy,
+                                   int64_t dy_batch, int64_t dy_step, const float* dlast, void* df, void* dv,
+                                   void* dz, float* ds0, void* workspace, size_t workspace_bytes, void* stream) {
   const int status = scan_check(scan, dtype);
   if (status != MORPH_OK) return status;
   if (scan->batch == 0 || scan->dim == 0) return MORPH_OK;
   if (scan->steps > 0 && (states == nullptr || dy == nullptr || df == nullptr || dv == nullptr ||
                           (scan->z != nullptr && dz == nullptr)))
     return MORPH_EINVAL;
-  const dim3 grid((unsigned)((scan->dim + 63) / 64), (unsigned)scan->batch);
+  const size_t need = scan_workspace(scan->batch, scan->steps, scan->dim, true);
+  if (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
+    return MORPH_EWORKSPACE;
   hipStream_t s = as_stream(stream);
-  if (dtype == MORPH_DTYPE_F32)
-    hipLaunchKernelGGL(scan_walk_back_kernel<F32>, grid, dim3(64), 0, s, *scan, states, dy, dy_batch,
-                       dy_step, dlast, df, dv, dz, ds0);
-  else if (dtype == MORPH_DTYPE_F16)
-    hipLaunchKernelGGL(scan_walk_back_kernel<F16>, grid, dim3(64), 0, s, *scan, states, dy, dy_batch,
-                       dy_step, dlast, df, dv, dz, ds0);
-  else
-    hipLaunchKernelGGL(scan_walk_back_kernel<BF16>, grid, dim3(64), 0, s, *scan, states, dy, dy_batch,
-                       dy_step, dlast, df, dv, dz, ds0);
+  const morph_scan a = *scan;
+  if (a.steps <= kWalk) {
+    const dim3 grid((unsigned)((a.dim + 63) / 64), (unsigned)a.batch);
+    by_form(dtype, false, false, [&](auto type, auto, auto) {
+      hipLaunchKernelGGL(scan_walk_back_kernel<decltype(type)>, grid, dim3(64), 0, s, a, states, dy, dy_batch, dy_step,
+                         dlast, df, dv, dz, ds0);
+    });
+    return launch_status();
+  }
+  const int64_t size = dtype == MORPH_DTYPE_F32 ? 4 : 2;
+  const bool two = a.dim % 2 == 0 && pairs(a.f, a.f_batch, a.f_step, size) && pairs(a.v, a.v_batch, a.v_step, size) &&
+                   pairs(a.z, a.z_batch, a.z_step, size) && pairs(dy, dy_batch, dy_step, size) &&
+                   pairs(df, 0, 0, size) && pairs(dv, 0, 0, size) && pairs(dz, 0, 0, size);
+  ScanGrid g;
+  unsigned grid;
+  const int shape = scan_grid(scan, two ? 2 : 1, true, workspace, s, g, grid);
+  if (shape != MORPH_OK) return shape;
+  by_form(dtype, two, a.z != nullptr, [&](auto type, auto vec, auto gated) {
+    hipLaunchKernelGGL((scan_tile_back_kernel<decltype(type), decltype(vec)::value, decltype(gated)::value>),
+                       dim3(grid), dim3(kThreads), 0, s, a, g, states, dy, dy_batch, dy_step, dlast, df, dv, dz, ds0);
+  });
   return launch_status();
 }
