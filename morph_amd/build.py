@@ -19,8 +19,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 SOURCES = ["abi.hip", "adamw.hip", "nonfinite.hip", "step.hip", "grads.hip", "convert.hip", "fp8.hip", "gemm.hip", "muon.hip", "muon_small.hip", "hostcopy.hip",
-           "act8.hip", "ffn.hip", "ffn_tiles_gate.hip", "ffn_tiles_grad.hip", "ffn_tiles_rows.hip",
-           "ffn_tiles_weights.hip", "scan.hip"]
+           "act8.hip", "ffn.hip", "ffn_rows.hip", "ffn_tiles_gate.hip", "ffn_tiles_grad.hip",
+           "ffn_tiles_rows.hip", "ffn_tiles_weights.hip", "scan.hip"]
 OUTPUT = PKG / "lib" / "libmorph_optim.so"
 HOSTPATH = PKG / "lib" / "_hostpath.so"  # Python extension over torch's C++ tensors (hostpath.cpp)
 ARCH = os.environ.get("MORPH_OFFLOAD_ARCH", "gfx950")

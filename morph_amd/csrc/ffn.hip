@@ -13,6 +13,7 @@
 // tiles through LDS, loaded element by element along whichever index is contiguous.
 #include <cmath>
 
+#include "ffn_rows.h"
 #include "ffn_tiles.h"
 
 namespace morph {
@@ -184,6 +185,7 @@ int64_t whole_groups(int64_t n) { return (n + MORPH_ACT_GROUP - 1) / MORPH_ACT_G
 int any(int dtype, FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
   return dtype == MORPH_DTYPE_F16 ? launch_any<F16>(e, a, s) : launch_any<BF16>(e, a, s);
 }
+const uint16_t* u16(const Side& s) { return static_cast<const uint16_t*>(s.p); }
 FfnOperand along(const Side& s) { return FfnOperand{static_cast<const uint16_t*>(s.p), s.ld, 1}; }
 FfnOperand across(const Side& s) { return FfnOperand{static_cast<const uint16_t*>(s.p), 1, s.ld}; }
 
@@ -191,6 +193,8 @@ FfnOperand across(const Side& s) { return FfnOperand{static_cast<const uint16_t*
 int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int64_t rows, int64_t d, int64_t ff,
                  const morph_ffn_saved* saved, uint16_t* h, int64_t ld, hipStream_t s) {
   const int keep = saved ? saved->keep : MORPH_FFN_KEEP_NONE;
+  if (rows <= kFewRows && keep == MORPH_FFN_KEEP_NONE)
+    return ffn_few_rows(dtype, true, u16(x), x.ld, u16(gate), gate.ld, u16(up), up.ld, rows, ff, d, h, ld, s);
   Launch l;
   l.add(x, gate, d, d, rows, ff, h, ld);
   l.ok = l.ok && fits(up, d);
@@ -213,6 +217,9 @@ int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int
 // y = h down^T.
 int down_product(int dtype, const Side& h, const Side& down, int64_t rows, int64_t d, int64_t ff, void* y,
                  int64_t y_ld, hipStream_t s) {
+  if (rows <= kFewRows)
+    return ffn_few_rows(dtype, false, u16(h), h.ld, u16(down), down.ld, nullptr, 0, rows, d, ff,
+                        static_cast<uint16_t*>(y), y_ld, s);
   Launch l;
   l.add(h, down, ff, ff, rows, d, y, y_ld);
   const int ts = l.choose(ff, 1, 0.0);

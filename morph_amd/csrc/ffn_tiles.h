@@ -474,6 +474,24 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     step(KT - 2, ps, std::integral_constant<int, 1>{});
     advance();
   }
+  // kGateGrad: what was kept of the first blocks is on its way under the last stage's MFMAs, and
+  // kAhead blocks ahead of its use from then on (a wait per block was 70 us of a 4096 x 6144 launch).
+  constexpr int kAhead = kE != FfnEpilogue::kGateGrad ? 1 : kKeep == MORPH_FFN_KEEP_FULL ? 3 : 4;
+  [[maybe_unused]] KeptBlock<kKeep> kg[kAhead], ku[kAhead] = {};
+  auto load_block = [&](int n) {
+    if constexpr (kE == FfnEpilogue::kGateGrad) {
+      const int row = row0 + wr + 32 * (n / kB) + fr, block = col0 + wc + 32 * (n % kB);
+      if (block >= o.ldc) return;
+      const int64_t at = (int64_t)min(row, o.M - 1) * o.ldc + block;
+      load_kept<kKeep>(kg[n % kAhead], g.g, g.g_exponents, at, fh);
+      load_kept<kKeep>(ku[n % kAhead], g.u, g.u_exponents, at, fh);
+    }
+  };
+  if constexpr (kE == FfnEpilogue::kGateGrad) {
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) load_block(n);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   step(KT - 1, ps, std::integral_constant<int, 2>{});
 
   // ---- epilogue: straight from the registers ------------------------------------
@@ -513,7 +531,7 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
 #pragma unroll
       for (int j = 0; j < kB / 2; ++j) {
         const int block = col0 + (wc + 64 * j) / 2;
-        if (block >= ldc) continue;  // rows of h are whole groups
+        if (block >= ldc) continue;  // rows of the buffers are whole groups
         float gv[16], uv[16], h[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -539,14 +557,12 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
 #pragma unroll
       for (int j = 0; j < kB; ++j) {
         const int block = col0 + wc + 32 * j;
-        if (block >= ldc) continue;
-        const int64_t at = (int64_t)(inside ? row : M - 1) * ldc + block;
-        KeptBlock<kKeep> kg, ku;
-        load_kept<kKeep>(kg, g.g, g.g_exponents, at, fh);
-        load_kept<kKeep>(ku, g.u, g.u_exponents, at, fh);
+        const int64_t at = (int64_t)row * ldc + block;
         float gv[16], uv[16], h[16];
-        kept_values<kKeep>(kg, gv);
-        kept_values<kKeep>(ku, uv);
+        kept_values<kKeep>(kg[(i * kB + j) % kAhead], gv);
+        kept_values<kKeep>(ku[(i * kB + j) % kAhead], uv);
+        if (i * kB + j + kAhead < kB * kB) load_block(i * kB + j + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const GateGrad d = ffn_gate_grad(acc[i][j][r], gv[r], uv[r]);
@@ -558,7 +574,7 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
         row_words<T>(h, w[0], w[1]);
         row_words<T>(gv, w[2], w[3]);
         row_words<T>(uv, w[4], w[5]);
-        if (inside) {
+        if (inside && block < ldc) {  // rows of the buffers are whole groups
           uint16_t* to[3] = {o.C, g.dg, g.du};
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
