@@ -89,13 +89,9 @@ __global__ __launch_bounds__(kThreads) void act_pack_kernel(const void* __restri
   const int64_t row = at / groups, c = (at - row * groups) * kGroup + 8 * part;
   float x[8];
   load8<T>(static_cast<const char*>(src) + row * ld * Fmt<T>::bytes, c, cols, wide, x);
-  uint32_t m = 0;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) m = max(m, finite_magnitude(x[k]));
-  const int e = act_exponent(quad_max(m));
-  const float inverse = act_inverse(e);
-  *reinterpret_cast<u32x2*>(codes + at * kGroup + 8 * part) =
-      u32x2{act_encode4(x[0], x[1], x[2], x[3], inverse), act_encode4(x[4], x[5], x[6], x[7], inverse)};
+  uint32_t w[2];
+  const int e = act_encode<8>(x, w, [](uint32_t m) { return quad_max(m); });
+  *reinterpret_cast<u32x2*>(codes + at * kGroup + 8 * part) = u32x2{w[0], w[1]};
   if (part == 0) exponents[at] = (uint8_t)e;
 }
 

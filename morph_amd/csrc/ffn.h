@@ -77,13 +77,9 @@ __device__ __forceinline__ void ffn_keep8(int keep, void* buffer, uint8_t* expon
     *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
     *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
   } else if (keep == MORPH_FFN_KEEP_ACT8) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, finite_magnitude(x[k]));
-    const int e = act_exponent(quad_max(m));
-    const float inverse = act_inverse(e);
-    *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(buffer) + at) =
-        u32x2{act_encode4(x[0], x[1], x[2], x[3], inverse), act_encode4(x[4], x[5], x[6], x[7], inverse)};
+    uint32_t w[2];
+    const int e = act_encode<8>(x, w, [](uint32_t m) { return quad_max(m); });
+    *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(buffer) + at) = u32x2{w[0], w[1]};
     if (at % MORPH_ACT_GROUP == 0) exponents[at / MORPH_ACT_GROUP] = (uint8_t)e;
   }
 }

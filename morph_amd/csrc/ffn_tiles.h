@@ -119,17 +119,12 @@ __device__ __forceinline__ void keep_block(const float (&x)[16], void* buffer, u
     for (int q = 0; q < 4; ++q)
       *reinterpret_cast<f32x4*>(p + 8 * q) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
   } else if constexpr (kKeep == MORPH_FFN_KEEP_ACT8) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) m = max(m, finite_magnitude(x[r]));
-    uint32_t a = m, b = m;  // the row's other half
-    swap_halves(a, b);
-    const int e = act_exponent(max(a, b));
-    const float inverse = act_inverse(e);
     uint32_t w[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      w[q] = act_encode4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3], inverse);
+    const int e = act_encode<16>(x, w, [](uint32_t m) {
+      uint32_t other = m;  // of the row's other half
+      swap_halves(m, other);
+      return max(m, other);
+    });
     swap_halves(w[0], w[2]);
     swap_halves(w[1], w[3]);
     if (!inside) return;
@@ -566,9 +561,12 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const GateGrad d = ffn_gate_grad(acc[i][j][r], gv[r], uv[r]);
-          // columns behind N are zero in every buffer; the sums there are not
-          const bool in = block + 8 * (r >> 2) + 4 * fh + (r & 3) < N;
-          h[r] = in ? d.h : 0.0f, gv[r] = in ? d.dg : 0.0f, uv[r] = in ? d.du : 0.0f;
+          h[r] = d.h, gv[r] = d.dg, uv[r] = d.du;
+        }
+        if (block + 32 > N) {  // columns behind N are zero in every buffer; the sums there are not
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (block + 8 * (r >> 2) + 4 * fh + (r & 3) >= N) h[r] = gv[r] = uv[r] = 0.0f;
         }
         u32x4 w[6];
         row_words<T>(h, w[0], w[1]);

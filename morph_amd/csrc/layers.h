@@ -20,10 +20,11 @@ __device__ __forceinline__ Sigmoid sigmoid(float x) {
 
 // ---- 8-bit activation groups (morph_layers.h) -------------------------------
 
-// |x| as an integer that orders like it, with 0 for inf and NaN: the group's scale comes
+// |x| as an integer that orders like it, and with 0 for inf and NaN: a group's scale comes
 // from its finite values.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
 __device__ __forceinline__ uint32_t finite_magnitude(float x) {
-  const uint32_t m = __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu;
+  const uint32_t m = magnitude(x);
   return m < 0x7F800000u ? m : 0u;
 }
 // The exponent byte of a group whose largest finite magnitude has these bits: with
@@ -41,16 +42,43 @@ __device__ __forceinline__ float act_inverse(int e) {  // 2^(127 - e), e <= 253
 }
 // Four codes of one word.  The multiplication is exact but where the product is subnormal,
 // far below half of the least code.  gfx950's conversion rounds to nearest even; what is
-// not finite gets the NaN code.
+// not finite gets the NaN code (kFinite: there is none).
+template <bool kFinite>
 __device__ __forceinline__ uint32_t act_encode4(float x0, float x1, float x2, float x3,
                                                 float inverse) {
   uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x0 * inverse, x1 * inverse, 0, false);
   w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x2 * inverse, x3 * inverse, (int)w, true);
-  const float x[4] = {x0, x1, x2, x3};
+  if constexpr (!kFinite) {
+    const float x[4] = {x0, x1, x2, x3};
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (nonfinite_f32_bits(__builtin_bit_cast(uint32_t, x[k]))) w = (w & ~(0xFFu << (8 * k))) | (0x7Fu << (8 * k));
+    for (int k = 0; k < 4; ++k)
+      if (nonfinite_f32_bits(__builtin_bit_cast(uint32_t, x[k]))) w = (w & ~(0xFFu << (8 * k))) | (0x7Fu << (8 * k));
+  }
   return w;
+}
+// The codes of kCount values of one lane and their group's exponent byte; most(m): the group's
+// maximum of its lanes' m.  One test of the whole wave takes the form for finite values.
+template <int kCount, typename Most>
+__device__ __forceinline__ int act_encode(const float (&x)[kCount], uint32_t (&w)[kCount / 4], Most&& most) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < kCount; ++k) m = max(m, magnitude(x[k]));
+  int e;
+  if (__any(m >= 0x7F800000u)) {
+    m = 0;
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) m = max(m, finite_magnitude(x[k]));
+    e = act_exponent(most(m));
+#pragma unroll
+    for (int k = 0; k < kCount; k += 4)
+      w[k / 4] = act_encode4<false>(x[k], x[k + 1], x[k + 2], x[k + 3], act_inverse(e));
+  } else {
+    e = act_exponent(most(m));
+#pragma unroll
+    for (int k = 0; k < kCount; k += 4)
+      w[k / 4] = act_encode4<true>(x[k], x[k + 1], x[k + 2], x[k + 3], act_inverse(e));
+  }
+  return e;
 }
 __device__ __forceinline__ void act_decode4(uint32_t w, float scale, float (&x)[4]) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
@@ -69,15 +97,20 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 }
 
 // ---- the gate of the feed-forward block --------------------------------------
-__device__ __forceinline__ float ffn_gate(float g, float u) { return g * sigmoid(g).a * u; }
+// Its sigmoid needs no small 1 - a: that is only added to, so a = 1 / (1 + e^-g) serves; e^-g
+// overflows to inf where a is 0.  (An epilogue holds 256 values a lane with no other wave to
+// fill in, so each instruction saved is microseconds a launch.)
+__device__ __forceinline__ float gate_sigmoid(float g) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
+}
+__device__ __forceinline__ float ffn_gate(float g, float u) { return g * gate_sigmoid(g) * u; }
 
 struct GateGrad {
   float h, dg, du;
 };
 __device__ __forceinline__ GateGrad ffn_gate_grad(float dh, float g, float u) {
-  const Sigmoid s = sigmoid(g);
-  const float act = g * s.a;
-  return GateGrad{act * u, dh * u * (s.a * __fmaf_rn(g, s.b, 1.0f)), dh * act};
+  const float a = gate_sigmoid(g), act = g * a;
+  return GateGrad{act * u, dh * u * __fmaf_rn(act, 1.0f - a, a), dh * act};
 }
 
 }  // namespace morph
