@@ -243,6 +243,20 @@ def hostpath():
     return _hostpath
 
 
+_layer_calls = None
+
+
+def layer_calls():
+    """The native path of the layer operators (hostlayers.cpp) over the library's entry points."""
+    global _layer_calls
+    if _layer_calls is None:
+        _layer_calls = hostpath().LayerCalls([entry_address(name) for name in (
+            "morph_act_pack", "morph_act_unpack", "morph_ffn_workspace_bytes", "morph_ffn_forward",
+            "morph_ffn_backward", "morph_scan_workspace_bytes", "morph_scan_forward",
+            "morph_scan_backward")])
+    return _layer_calls
+
+
 def entry_address(name):
     """The address of one of the library's entry points."""
     return ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value

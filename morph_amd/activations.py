@@ -11,8 +11,9 @@ scale it reaches the gradients, and the detector skips the step.
 """
 import torch
 
-from ._lib import check, lib
-from .layers import GROUP, address, as_rows, current_stream, dtype_code, require_gpu, row_stride, running_on
+from ._lib import check, layer_calls, lib
+from .layers import (GROUP, address, as_rows, current_stream, dtype_code, native, require_gpu, row_stride,
+                     running_on)
 
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -26,7 +27,7 @@ class PackedActivation:
 
     def __init__(self, codes, exponents, shape, dtype):
         self.codes, self.exponents = codes, exponents
-        self.shape, self.dtype = torch.Size(shape), dtype
+        self.shape, self.dtype = shape if type(shape) is torch.Size else torch.Size(shape), dtype
 
     @property
     def device(self):
@@ -45,6 +46,11 @@ class PackedActivation:
 def pack_activation(x, stream=None):
     """The 8-bit form of x ([..., cols], FP32, FP16 or BF16), scaled in groups along its last
     dimension."""
+    if stream is None:
+        made = layer_calls().pack(x)
+        if made is not None:
+            codes, exponents = native(made)
+            return PackedActivation(codes, exponents, x.shape, x.dtype)
     require_gpu(x, "x", FLOATS)
     if x.dim() == 0:
         raise ValueError("x must have at least one dimension")
@@ -68,6 +74,10 @@ def unpack_activation(packed, dtype=None, stream=None):
     dtype = packed.dtype if dtype is None else dtype
     if dtype not in FLOATS:
         raise TypeError(f"unsupported dtype {dtype}; expected float32, float16 or bfloat16")
+    if stream is None:
+        out = layer_calls().unpack(packed.codes, packed.exponents, packed.shape, dtype_code(dtype))
+        if out is not None:
+            return native(out)
     cols = packed.shape[-1]
     rows = packed.shape.numel() // cols if cols else 0
     groups = -(-cols // GROUP)

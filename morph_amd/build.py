@@ -22,7 +22,8 @@ SOURCES = ["abi.hip", "adamw.hip", "nonfinite.hip", "step.hip", "grads.hip", "co
            "act8.hip", "ffn.hip", "ffn_rows.hip", "ffn_tiles_gate.hip", "ffn_tiles_grad.hip",
            "ffn_tiles_rows.hip", "ffn_tiles_weights.hip", "scan.hip"]
 OUTPUT = PKG / "lib" / "libmorph_optim.so"
-HOSTPATH = PKG / "lib" / "_hostpath.so"  # Python extension over torch's C++ tensors (hostpath.cpp)
+HOSTPATH = PKG / "lib" / "_hostpath.so"  # Python extension over torch's C++ tensors
+HOST_SOURCES = ["hostpath.cpp", "hostlayers.cpp"]
 ARCH = os.environ.get("MORPH_OFFLOAD_ARCH", "gfx950")
 
 FLAGS = [
@@ -47,10 +48,11 @@ def build_hostpath(output=HOSTPATH):
     tmp = output.with_name(output.name + ".tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-isystem{p}" for p in cpp_extension.include_paths()],
+           "-D__HIP_PLATFORM_AMD__=1",  # torch's stream header includes HIP's
+           *[f"-isystem{p}" for p in [*cpp_extension.include_paths(), Path(hipcc()).parents[1] / "include"]],
            f"-isystem{sysconfig.get_paths()['include']}", "-o", str(tmp),
-           str(PKG / "csrc" / "hostpath.cpp"), f"-L{Path(torch.__file__).parent / 'lib'}",
-           "-lc10", "-ltorch_cpu", "-ltorch_python"]
+           *[str(PKG / "csrc" / s) for s in HOST_SOURCES], f"-L{Path(torch.__file__).parent / 'lib'}",
+           "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         sys.stderr.write(proc.stdout + proc.stderr)

@@ -12,34 +12,13 @@
 // list, a parameter or a moment that lies elsewhere, a gradient missing or new, another type,
 // device, size or layout, a tensor subclass, other export buffers); the caller then takes the
 // Python path, which rebuilds or raises.
-#include <ATen/TensorSubclassLikeUtils.h>
-#include <pybind11/pybind11.h>
-#include <pybind11/stl.h>
-#include <torch/csrc/autograd/python_variable.h>
+#include "hostpath.h"
 
 #include <vector>
 
 #include "../../include/morph_optim.h"
 
-namespace py = pybind11;
-
 namespace {
-
-// at::isTensorSubclassLike without its question for a dispatch mode, which match() asks once.
-bool plain(const at::Tensor& t) {
-  return (t.key_set() & at::kTensorSubclassLike).empty() && t.has_storage();
-}
-
-const at::Tensor* plain_tensor(PyObject* o) {
-  if (o == nullptr || !THPVariable_CheckExact(o)) return nullptr;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  return t.defined() && plain(t) ? &t : nullptr;
-}
-
-// Whether t is n contiguous elements of `type`.
-bool holds(const at::Tensor& t, at::ScalarType type, int64_t n) {
-  return t.numel() == n && t.scalar_type() == type && t.is_contiguous();
-}
 
 // Whether o is still the n floats at `address` that a descriptor points at.
 bool still_at(PyObject* o, const void* address, int64_t n) {
@@ -282,6 +261,7 @@ py::bytes places(const py::list& tensors) {
 }  // namespace
 
 PYBIND11_MODULE(_hostpath, m) {
+  bind_layers(m);
   m.def("places", &places);
   py::class_<StepPlan>(m, "StepPlan")
       .def(py::init<py::list, std::vector<int64_t>, uint64_t, int, int, uint64_t, uint64_t, uint64_t,

@@ -17,10 +17,10 @@ import ctypes
 
 import torch
 
-from ._lib import FfnBlock, FfnSaved, check, lib
+from ._lib import FfnBlock, FfnSaved, check, layer_calls, lib
 from .activations import PackedActivation
-from .layers import (GROUP, HALF, address, as_rows, current_stream, dtype_code, require_gpu, row_stride,
-                     running_on)
+from .layers import (GROUP, HALF, address, as_rows, current_stream, dtype_code, native, require_gpu,
+                     row_stride, running_on)
 
 KEEP = {"none": 0, "full": 1, "fp8": 2}
 
@@ -29,18 +29,35 @@ class SavedFFN:
     """What a forward kept for its backward.  keep "full": x itself and both projections in
     FP32 (gate, up: [rows, 32 G], zero behind ff); "fp8": x, gate and up as PackedActivation."""
 
-    __slots__ = ("keep", "x", "gate", "up", "shape", "ff", "dtype")
+    __slots__ = ("keep", "x", "projections", "packed", "shape", "ff", "dtype")
 
-    def __init__(self, keep, x, gate, up, shape, ff, dtype):
-        self.keep, self.x, self.gate, self.up = keep, x, gate, up
-        self.shape, self.ff, self.dtype = shape, ff, dtype
+    def __init__(self, keep, x, projections, packed, shape, ff, dtype):
+        self.keep, self.shape, self.ff, self.dtype = keep, shape, ff, dtype
+        self.x, self.projections, self.packed = x, projections, packed  # of one kind or the other
+
+    @property
+    def gate(self):
+        return self.packed[1] if self.keep == "fp8" else self.projections[0]
+
+    @property
+    def up(self):
+        return self.packed[2] if self.keep == "fp8" else self.projections[1]
+
+    def tensors(self):
+        if self.keep == "fp8":
+            return tuple(t for p in self.packed for t in (p.codes, p.exponents))
+        return self.x, self.projections
+
+    @property
+    def device(self):
+        return self.tensors()[1].device
 
     @property
     def nbytes(self):
         """Bytes held beyond x, or with "fp8" in all (x need not be kept beside it)."""
         if self.keep == "fp8":
-            return self.x.nbytes + self.gate.nbytes + self.up.nbytes
-        return 4 * (self.gate.numel() + self.up.numel())
+            return sum(p.nbytes for p in self.packed)
+        return 4 * self.projections.numel()
 
 
 def _weights(x, gate, up, down):
@@ -66,18 +83,30 @@ def _block(x, gate, up, down, rows, d, ff):
 def _descriptor(saved):
     if saved.keep == "full":
         return FfnSaved(KEEP["full"], 0, address(saved.gate), address(saved.up), None, None, None, None)
-    return FfnSaved(KEEP["fp8"], 0, address(saved.gate.codes), address(saved.up.codes),
-                    address(saved.gate.exponents), address(saved.up.exponents),
-                    address(saved.x.codes), address(saved.x.exponents))
+    x, gate, up = saved.packed
+    return FfnSaved(KEEP["fp8"], 0, address(gate.codes), address(up.codes), address(gate.exponents),
+                    address(up.exponents), address(x.codes), address(x.exponents))
 
 
-def _packed(rows, cols, shape, dtype, device):
-    groups = -(-cols // GROUP)
-    return PackedActivation(torch.empty((rows, groups * GROUP), dtype=torch.uint8, device=device),
-                            torch.empty((rows, groups), dtype=torch.uint8, device=device), shape, dtype)
+def _packings(tensors, shape, rows, ff, dtype):
+    """x, gate and up from their codes and exponents."""
+    return tuple(PackedActivation(tensors[2 * i], tensors[2 * i + 1], s, dtype)
+                 for i, s in enumerate((shape, (rows, ff), (rows, ff))))
 
 
 def _forward(x, gate, up, down, keep, stream):
+    if stream is None:
+        made = layer_calls().ffn_forward(x, gate, up, down, KEEP[keep])
+        if made is not None:
+            made = native(made)
+            if keep == "none":
+                return made, None
+            y, kept = made
+            ff = gate.shape[0]
+            if keep == "full":
+                return y, SavedFFN(keep, x.detach().view(-1, x.shape[-1]), kept[0], None, x.shape, ff, x.dtype)
+            packed = _packings(kept, x.shape, kept[0].shape[0], ff, x.dtype)
+            return y, SavedFFN(keep, packed[0], None, packed, x.shape, ff, x.dtype)
     gate, up, down, ff = _weights(x, gate, up, down)
     d, device, dtype = x.shape[-1], x.device, x.dtype
     rows = x.numel() // d
@@ -87,12 +116,12 @@ def _forward(x, gate, up, down, keep, stream):
         saved = None
         if keep == "full":
             wide = -(-ff // GROUP) * GROUP
-            kept = torch.empty((2, rows, wide), dtype=torch.float32, device=device)
-            saved = SavedFFN(keep, flat, kept[0], kept[1], x.shape, ff, dtype)
+            saved = SavedFFN(keep, flat, torch.empty((2, rows, wide), dtype=torch.float32, device=device), None,
+                             x.shape, ff, dtype)
         elif keep == "fp8":
-            saved = SavedFFN(keep, _packed(rows, d, x.shape, dtype, device),
-                             _packed(rows, ff, (rows, ff), dtype, device),
-                             _packed(rows, ff, (rows, ff), dtype, device), x.shape, ff, dtype)
+            packed = _packings([torch.empty((rows, -(-n // GROUP) * size), dtype=torch.uint8, device=device)
+                                for n in (d, ff, ff) for size in (GROUP, 1)], x.shape, rows, ff, dtype)
+            saved = SavedFFN(keep, packed[0], None, packed, x.shape, ff, dtype)
         if rows:
             L = lib()
             size = L.morph_ffn_workspace_bytes(rows, d, ff, KEEP[keep], 0)
@@ -122,16 +151,18 @@ def gated_ffn_backward(dy, saved, gate, up, down, stream=None):
     """(dx, dgate, dup, ddown) from the gradient of y and what the forward kept."""
     if not isinstance(saved, SavedFFN):
         raise TypeError("saved must come from gated_ffn_forward")
-    device = (saved.gate.codes if saved.keep == "fp8" else saved.gate).device
+    device = saved.device
     require_gpu(dy, "dy", (saved.dtype,), saved.shape, device)
+    if stream is None and isinstance(gate, torch.Tensor) and gate.shape[:1] == (saved.ff,):
+        made = layer_calls().ffn_backward(dy, saved.tensors(), gate, up, down, KEEP[saved.keep])
+        if made is not None:
+            return native(made)
     gate, up, down, ff = _weights(dy, gate, up, down)
     if ff != saved.ff:
         raise ValueError(f"the weights have {ff} hidden units, the forward had {saved.ff}")
     d, dtype = dy.shape[-1], dy.dtype
     rows = dy.numel() // d
-    kept = ((saved.x, saved.gate, saved.up) if saved.keep == "full" else
-            tuple(t for p in (saved.x, saved.gate, saved.up) for t in (p.codes, p.exponents)))
-    with running_on(device, stream, (dy, gate, up, down, *kept)):
+    with running_on(device, stream, (dy, gate, up, down, *saved.tensors())):
         flat = as_rows(dy.detach())
         dx = torch.empty(saved.shape, dtype=dtype, device=device)
         dgate, dup = (torch.empty((ff, d), dtype=dtype, device=device) for _ in range(2))

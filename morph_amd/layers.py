@@ -4,7 +4,7 @@ import ctypes
 
 import torch
 
-from ._lib import dtype_code
+from ._lib import check, dtype_code
 
 HALF = (torch.float16, torch.bfloat16)
 GROUP = 32  # values of a row that share a scale in the 8-bit form (MORPH_ACT_GROUP)
@@ -63,6 +63,13 @@ def running_on(device, stream, inputs=()):
     return _elsewhere(device, stream, inputs if stream is not None else ())
 
 
+def native(result):
+    """A result of LayerCalls (hostlayers.cpp); raises where it is a status of the library."""
+    if type(result) is int:
+        check(result)
+    return result
+
+
 def address(t):
     return t.data_ptr() if t is not None else None
 
@@ -70,6 +77,3 @@ def address(t):
 def current_stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
-
-__all__ = ["HALF", "GROUP", "require_gpu", "as_rows", "row_stride", "running_on", "address",
-           "current_stream", "dtype_code"]

@@ -14,8 +14,8 @@ import ctypes
 
 import torch
 
-from ._lib import SCAN_SPAN, ScanArgs, check, lib
-from .layers import address, current_stream, dtype_code, require_gpu, running_on
+from ._lib import SCAN_SPAN, ScanArgs, check, layer_calls, lib
+from .layers import address, current_stream, dtype_code, native, require_gpu, running_on
 
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -62,6 +62,15 @@ def _workspace(f, backward):
 
 
 def _forward(f, v, z, state, train, stream):
+    if stream is None:
+        made = layer_calls().scan_forward(f, v, z, state, train)
+        if made is not None:
+            if not train:
+                return native(made)
+            y, last, states = native(made)
+            return y, last, SavedScan(f.detach(), v.detach(), z.detach() if z is not None else None,
+                                      state.detach() if state is not None else None, states)
+    require_gpu(f, "f", FLOATS)
     with running_on(f.device, stream, (f, v, z, state)):
         f, v, z, state = _checked(f, v, z, state)
         batch, steps, dim = f.shape
@@ -79,13 +88,11 @@ def _forward(f, v, z, state, train, stream):
 
 def gated_scan(f, v, z=None, state=None, stream=None):
     """(y, state behind the last step); state: the one before the first (None: zeros)."""
-    require_gpu(f, "f", FLOATS)
     return _forward(f, v, z, state, False, stream)[:2]
 
 
 def gated_scan_forward(f, v, z=None, state=None, stream=None):
     """(y, last state, saved): gated_scan, with what the backward needs."""
-    require_gpu(f, "f", FLOATS)
     return _forward(f, v, z, state, True, stream)
 
 
@@ -95,6 +102,10 @@ def gated_scan_backward(dy, saved, dlast=None, stream=None):
     if not isinstance(saved, SavedScan):
         raise TypeError("saved must come from gated_scan_forward")
     f, v, z = saved.f, saved.v, saved.z
+    if stream is None:
+        made = layer_calls().scan_backward(dy, f, v, z, saved.state, saved.states, dlast)
+        if made is not None:
+            return native(made)
     require_gpu(dy, "dy", (f.dtype,), f.shape, f.device)
     if dlast is not None:
         require_gpu(dlast, "dlast", (torch.float32,), (f.shape[0], f.shape[2]), f.device)

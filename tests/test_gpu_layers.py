@@ -532,3 +532,68 @@ def test_scan_refuses():
                         ((f, saved, f[:1, 0]), ValueError)):
         with pytest.raises(error):
             gated_scan_backward(*args)
+
+
+# ---- the native path of the wrappers -------------------------------------------
+def test_native_path_equals_the_python_path(monkeypatch):
+    """Calls that hostlayers.cpp takes give what the Python path gives (taken here by naming
+    the stream), and calls that it does not take arrive there."""
+    from morph_amd import _lib, activations, ffn, recurrence
+    gen = torch.Generator().manual_seed(5)
+    weights = [w.to(DEV) for w in _weights(gen, 72, 200, torch.bfloat16)]
+    x, dy = (normal(gen, 3, 50, 72, dtype=torch.bfloat16).to(DEV) for _ in range(2))
+    s0, ds = (normal(gen, 3, 72).to(DEV) for _ in range(2))
+
+    def results(stream):
+        out = [gated_ffn(x, *weights, stream=stream)]
+        for keep in ("full", "fp8"):
+            y, saved = gated_ffn_forward(x, *weights, keep=keep, stream=stream)
+            out += [y, *saved.tensors(), *gated_ffn_backward(dy, saved, *weights, stream=stream)]
+            assert saved.shape == x.shape and saved.ff == 200 and saved.dtype == x.dtype and saved.nbytes > 0
+        packed = pack_activation(x, stream=stream)
+        assert packed.shape == x.shape and packed.dtype == x.dtype
+        out += [packed.codes, packed.exponents, unpack_activation(packed, stream=stream),
+                unpack_activation(packed, torch.float32, stream=stream)]
+        for z in (x, None):
+            for state in (s0, None):
+                out += gated_scan(x, dy, z, state, stream=stream)
+                y, last, saved = gated_scan_forward(x, dy, z, state, stream=stream)
+                out += [y, last, saved.states]
+                out += [t for t in gated_scan_backward(dy, saved, ds, stream=stream) if t is not None]
+        return out
+
+    class Counting:
+        def __init__(self):
+            self.calls, self.taken = 0, 0
+
+        def __getattr__(self, name):
+            def call(*args):
+                result = getattr(_lib.layer_calls(), name)(*args)
+                self.calls += 1
+                self.taken += result is not None
+                return result
+            return call
+    count = Counting()
+    for module in (activations, ffn, recurrence):
+        monkeypatch.setattr(module, "layer_calls", lambda: count)
+    native = results(None)
+    assert count.calls == count.taken == 20
+    python = results(torch.cuda.current_stream())
+    assert count.calls == 20
+    assert len(native) == len(python)
+    for a, b in zip(native, python):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+    count.taken = 0
+    gated_ffn(x.transpose(0, 1), *weights)                      # a layout that needs a copy
+    pack_activation(x[..., :30])
+    gated_scan(x[:, :0], x[:, :0])
+    assert count.taken == 0
+
+
+def test_native_path_under_autograd_keeps_no_graph():
+    x = torch.randn(4, 64, device=DEV, dtype=torch.float16, requires_grad=True)
+    weights = [torch.randn(s, device=DEV, dtype=torch.float16) for s in ((96, 64), (96, 64), (64, 96))]
+    y, saved = gated_ffn_forward(x, *weights)
+    assert not y.requires_grad and not saved.x.requires_grad
+    _, _, kept = gated_scan_forward(x[None], x[None])
+    assert not kept.f.requires_grad

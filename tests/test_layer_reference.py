@@ -142,3 +142,17 @@ def test_layer_struct_layouts_match_the_header(tmp_path, cls, ctype):
     out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(v) for v in out[:-2]] == [ctypes.sizeof(struct), *(getattr(struct, n).offset for n in fields)]
     assert [int(v) for v in out[-2:]] == [_lib.SCAN_SPAN, 32]
+
+
+@no_gpu_visible
+def test_wrappers_refuse_host_tensors():
+    """A CPU tensor raises the wrappers' own error, with or without a GPU in the machine."""
+    from morph_amd.activations import pack_activation
+    from morph_amd.ffn import gated_ffn
+    from morph_amd.recurrence import gated_scan
+    x = torch.zeros(4, 8, dtype=torch.float16)
+    for call in (lambda: pack_activation(x), lambda: gated_ffn(x, x, x, x.t()), lambda: gated_scan(x[None], x[None])):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+    with pytest.raises(TypeError):
+        pack_activation(None)
