@@ -9,7 +9,8 @@
 // never is.  Where 8-bit groups are kept they are made from the FP32 sums in the epilogue.
 //
 // The tiles of ffn_tiles.h take operands whose rows are 16-byte aligned and a multiple of 8
-// values long.  ffn_any_kernel takes operands of any stride and alignment, any size: 64 x 64
+// values long; operands of other widths are copied to such rows first (ffn_pad_kernel: a
+// read and a write of them beside the product's many reads).  ffn_any_kernel takes operands of any stride and alignment, any size: 64 x 64
 // tiles through LDS, loaded element by element along whichever index is contiguous.
 #include <cmath>
 
@@ -180,6 +181,61 @@ struct Launch {
   unsigned grid() const { return (unsigned)((a.total + 7) / 8 * 8); }
 };
 
+// Up to five matrices copied to rows of whole 16-byte chunks, zero behind their width.
+struct PadMatrix {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t rows, cols, src_ld, dst_ld, first;  // first: its first chunk of the launch
+};
+struct PadArgs {
+  PadMatrix m[5];
+  int64_t chunks;
+  int32_t count;
+};
+__global__ __launch_bounds__(kThreads) void ffn_pad_kernel(const PadArgs a) {
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (at >= a.chunks) return;
+  int i = 0;
+  while (i + 1 < a.count && at >= a.m[i + 1].first) ++i;
+  const PadMatrix& m = a.m[i];
+  const int64_t per_row = m.dst_ld / 8, row = (at - m.first) / per_row, c = (at - m.first - row * per_row) * 8;
+  const uint16_t* src = m.src + row * m.src_ld + c;
+  u32x4 v{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (c + k < m.cols) v[k >> 1] |= (uint32_t)src[k] << (16 * (k & 1));
+  *reinterpret_cast<u32x4*>(m.dst + row * m.dst_ld + c) = v;
+}
+
+int64_t padded_bytes(int64_t rows, int64_t cols) { return rows * ((cols + 7) / 8 * 8) * 2; }
+
+// Copies the sides whose width is no multiple of 8 into `room` (16-byte aligned, as much as
+// padded_bytes says of each) and points them there.
+struct Padding {
+  PadArgs a{};
+  char* room;
+  explicit Padding(void* p) : room(static_cast<char*>(p)) {}
+  void add(Side& s, int64_t rows, int64_t cols) {
+    if (cols % 8 == 0 || rows == 0) return;
+    PadMatrix& m = a.m[a.count++];
+    m = PadMatrix{static_cast<const uint16_t*>(s.p), reinterpret_cast<uint16_t*>(room), rows, cols, s.ld,
+                  (cols + 7) / 8 * 8, a.chunks};
+    a.chunks += rows * (m.dst_ld / 8);
+    room += padded_bytes(rows, cols);
+    s = Side{m.dst, m.dst_ld, true};
+  }
+  int launch(hipStream_t s) {
+    if (a.count == 0) return MORPH_OK;
+    const int64_t grid = (a.chunks + kThreads - 1) / kThreads;
+    if (grid > 0x7FFFFFFF) return MORPH_ERANGE;
+    hipLaunchKernelGGL(ffn_pad_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, a);
+    return launch_status();
+  }
+};
+
+// Whether a forward takes the few-rows kernels, which read any alignment.
+bool few_rows(int64_t rows, int keep) { return rows <= kFewRows && keep == MORPH_FFN_KEEP_NONE; }
+
 int64_t whole_groups(int64_t n) { return (n + MORPH_ACT_GROUP - 1) / MORPH_ACT_GROUP * MORPH_ACT_GROUP; }
 
 int any(int dtype, FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
@@ -193,7 +249,7 @@ FfnOperand across(const Side& s) { return FfnOperand{static_cast<const uint16_t*
 int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int64_t rows, int64_t d, int64_t ff,
                  const morph_ffn_saved* saved, uint16_t* h, int64_t ld, hipStream_t s) {
   const int keep = saved ? saved->keep : MORPH_FFN_KEEP_NONE;
-  if (rows <= kFewRows && keep == MORPH_FFN_KEEP_NONE)
+  if (few_rows(rows, keep))
     return ffn_few_rows(dtype, true, u16(x), x.ld, u16(gate), gate.ld, u16(up), up.ld, rows, ff, d, h, ld, s);
   Launch l;
   l.add(x, gate, d, d, rows, ff, h, ld);
@@ -216,8 +272,8 @@ int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int
 
 // y = h down^T.
 int down_product(int dtype, const Side& h, const Side& down, int64_t rows, int64_t d, int64_t ff, void* y,
-                 int64_t y_ld, hipStream_t s) {
-  if (rows <= kFewRows)
+                 int64_t y_ld, int keep, hipStream_t s) {
+  if (few_rows(rows, keep))
     return ffn_few_rows(dtype, false, u16(h), h.ld, u16(down), down.ld, nullptr, 0, rows, d, ff,
                         static_cast<uint16_t*>(y), y_ld, s);
   Launch l;
@@ -335,9 +391,14 @@ using namespace morph;
 
 extern "C" size_t morph_ffn_workspace_bytes(int64_t rows, int64_t d, int64_t ff, int keep, int backward) {
   if (rows <= 0 || d <= 0 || ff <= 0) return 0;
-  const size_t wide = 2 * (size_t)rows * (size_t)whole_groups(ff);  // h (and dg, du)
-  if (!backward) return wide;
-  return 3 * wide + (keep == MORPH_FFN_KEEP_ACT8 ? 2 * (size_t)rows * (size_t)whole_groups(d) : 0);
+  size_t bytes = 2 * (size_t)rows * (size_t)whole_groups(ff);  // h
+  if (backward) bytes *= 3;                                     // and dg, du
+  if (backward && keep == MORPH_FFN_KEEP_ACT8) bytes += 2 * (size_t)rows * (size_t)whole_groups(d);  // x
+  if (backward || !few_rows(rows, keep)) {  // copies of operands of odd widths
+    if (d % 8) bytes += (size_t)(padded_bytes(rows, d) * (backward ? 2 : 1) + 2 * padded_bytes(ff, d));
+    if (ff % 8) bytes += (size_t)padded_bytes(d, ff);
+  }
+  return bytes;
 }
 
 extern "C" int morph_ffn_forward(const morph_ffn* a, int dtype, const morph_ffn_saved* saved, void* y,
@@ -357,10 +418,20 @@ extern "C" int morph_ffn_forward(const morph_ffn* a, int dtype, const morph_ffn_
     status = morph_act_pack(a->x, dtype, a->rows, a->d, a->x_ld, saved->x_codes, saved->x_exponents, stream);
     if (status != MORPH_OK) return status;
   }
-  status = gate_product(dtype, Side{a->x, a->x_ld, false}, Side{a->gate, a->gate_ld, false},
-                        Side{a->up, a->up_ld, false}, a->rows, a->d, a->ff, saved, h, ld, s);
+  Side x{a->x, a->x_ld, false}, gate{a->gate, a->gate_ld, false}, up{a->up, a->up_ld, false};
+  Side down{a->down, a->down_ld, false};
+  if (!few_rows(a->rows, keep)) {
+    Padding pad(h + a->rows * ld);
+    pad.add(x, a->rows, a->d);
+    pad.add(gate, a->ff, a->d);
+    pad.add(up, a->ff, a->d);
+    pad.add(down, a->d, a->ff);
+    status = pad.launch(s);
+    if (status != MORPH_OK) return status;
+  }
+  status = gate_product(dtype, x, gate, up, a->rows, a->d, a->ff, saved, h, ld, s);
   if (status != MORPH_OK) return status;
-  return down_product(dtype, Side{h, ld, true}, Side{a->down, a->down_ld, false}, a->rows, a->d, a->ff, y, y_ld, s);
+  return down_product(dtype, Side{h, ld, true}, down, a->rows, a->d, a->ff, y, y_ld, keep, s);
 }
 
 extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn_saved* saved,
@@ -380,15 +451,27 @@ extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn
   hipStream_t s = as_stream(stream);
   const int64_t ld = whole_groups(a->ff);
   uint16_t* h = static_cast<uint16_t*>(workspace);
-  uint16_t *dg = h + a->rows * ld, *du = dg + a->rows * ld, *xs = du + a->rows * ld;
-  Side x{a->x, a->x_ld, false};
-  if (saved->keep == MORPH_FFN_KEEP_ACT8 && a->rows > 0) {
-    x = Side{xs, whole_groups(a->d), true};
-    status = morph_act_unpack(saved->x_codes, saved->x_exponents, a->rows, a->d, xs, dtype, x.ld, stream);
+  uint16_t *dg = h + a->rows * ld, *du = dg + a->rows * ld, *xs = du + a->rows * ld;  // xs: what else is needed
+  Side x{a->x, a->x_ld, false}, gate{a->gate, a->gate_ld, false}, up{a->up, a->up_ld, false};
+  Side down{a->down, a->down_ld, false}, sy{dy, dy_ld, false};
+  if (a->rows > 0) {
+    Padding pad(xs);
+    if (saved->keep == MORPH_FFN_KEEP_ACT8) {
+      x = Side{xs, whole_groups(a->d), true};
+      pad.room += 2 * a->rows * x.ld;
+      status = morph_act_unpack(saved->x_codes, saved->x_exponents, a->rows, a->d, xs, dtype, x.ld, stream);
+      if (status != MORPH_OK) return status;
+    } else {
+      pad.add(x, a->rows, a->d);
+    }
+    pad.add(sy, a->rows, a->d);
+    pad.add(gate, a->ff, a->d);
+    pad.add(up, a->ff, a->d);
+    pad.add(down, a->d, a->ff);
+    status = pad.launch(s);
     if (status != MORPH_OK) return status;
   }
-  const Side gate{a->gate, a->gate_ld, false}, up{a->up, a->up_ld, false}, down{a->down, a->down_ld, false};
-  const Side sh{h, ld, true}, sg{dg, ld, true}, su{du, ld, true}, sy{dy, dy_ld, false};
+  const Side sh{h, ld, true}, sg{dg, ld, true}, su{du, ld, true};
   if (a->rows > 0) {
     status = grad_product(dtype, sy, down, a->rows, a->d, a->ff, saved, h, dg, du, ld, s);
     if (status == MORPH_OK) status = input_product(dtype, sg, su, gate, up, a->rows, a->d, a->ff, dx, s);
