@@ -11,7 +11,6 @@ namespace morph {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // A matrix operand: element (row, k) of a product's P or Q at p[row * rs + k * ks], one of
 // the strides 1.  Rows run over M (P) or N (Q).
@@ -52,17 +51,6 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Two floats in one word, each rounded to nearest even (overflow to inf, as a conversion).
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, F16>) {
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
-  } else {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
-  }
-}
 template <typename T>
 __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
   return u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};

@@ -1,11 +1,26 @@
 // Device mathematics that the layer operators share.
 #pragma once
 
+#include <type_traits>
+
 #include "../../include/morph_layers.h"
 #include "common.h"
 
 namespace morph {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Two floats in one word, each rounded to nearest even (overflow to inf, as a conversion).
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, F16>) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  }
+}
 // sigmoid(x) and sigmoid(-x) from one exponential of -|x|, which neither overflows nor
 // cancels: both are accurate to a few ulp at either end, where 1 - sigmoid(x) would keep no
 // digit.  +-inf give exactly 1 and 0, NaN gives NaN.
@@ -16,6 +31,21 @@ __device__ __forceinline__ Sigmoid sigmoid(float x) {
   const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * __builtin_fabsf(x));
   const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
   return x < 0.0f ? Sigmoid{small, big} : Sigmoid{big, small};
+}
+
+// sigmoid(x) alone, where 1 - sigmoid(x) is not needed or only added to: e^-x overflows to inf
+// where it is 0.
+__device__ __forceinline__ float gate_sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
+}
+
+// silu(x) = x sigmoid(x) and its derivative.
+struct Silu {
+  float y, slope;
+};
+__device__ __forceinline__ Silu silu(float x) {
+  const float a = gate_sigmoid(x), y = x * a;
+  return Silu{y, __fmaf_rn(y, 1.0f - a, a)};
 }
 
 // ---- 8-bit activation groups (morph_layers.h) -------------------------------
@@ -97,20 +127,16 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 }
 
 // ---- the gate of the feed-forward block --------------------------------------
-// Its sigmoid needs no small 1 - a: that is only added to, so a = 1 / (1 + e^-g) serves; e^-g
-// overflows to inf where a is 0.  (An epilogue holds 256 values a lane with no other wave to
-// fill in, so each instruction saved is microseconds a launch.)
-__device__ __forceinline__ float gate_sigmoid(float g) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
-}
+// (An epilogue holds 256 values a lane with no other wave to fill in, so each instruction
+// saved is microseconds a launch.)
 __device__ __forceinline__ float ffn_gate(float g, float u) { return g * gate_sigmoid(g) * u; }
 
 struct GateGrad {
   float h, dg, du;
 };
 __device__ __forceinline__ GateGrad ffn_gate_grad(float dh, float g, float u) {
-  const float a = gate_sigmoid(g), act = g * a;
-  return GateGrad{act * u, dh * u * __fmaf_rn(act, 1.0f - a, a), dh * act};
+  const Silu s = silu(g);
+  return GateGrad{s.y * u, dh * u * s.slope, dh * s.y};
 }
 
 }  // namespace morph

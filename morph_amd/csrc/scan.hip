@@ -129,39 +129,43 @@ static_assert(kSpan % kForwardSteps == 0, "states are kept at a wave's first ste
 // kVec consecutive channels of one step as loaded: 16-bit pairs or singles, floats.
 template <typename T, int kVec>
 struct Raw {
-  typedef uint32_t type;
+  typedef std::conditional_t<kVec == 2, uint32_t, uint16_t> type;
 };
 template <int kVec>
 struct Raw<F32, kVec> {
   typedef float type __attribute__((ext_vector_type(kVec)));
 };
 template <typename T, int kVec>
-__device__ __forceinline__ typename Raw<T, kVec>::type load_raw(const void* p, int64_t i) {
-  if constexpr (std::is_same_v<T, F32>)
-    return *reinterpret_cast<const typename Raw<F32, kVec>::type*>(static_cast<const float*>(p) + i);
-  else if constexpr (kVec == 2)
-    return *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
-  else
-    return static_cast<const uint16_t*>(p)[i];
-}
-template <typename T, int kVec>
 __device__ __forceinline__ float value(const typename Raw<T, kVec>::type& r, int k) {
   if constexpr (std::is_same_v<T, F32>) return r[k];
-  else return to_float<T>(k ? r >> 16 : kVec == 2 ? r & 0xFFFFu : r);
+  else return to_float<T>(k ? (uint32_t)r >> 16 : r & 0xFFFFu);
 }
+
+// The tile's rows of one tensor: a wave-uniform address that advances by the step, and the
+// lane's offset in it.
 template <typename T, int kVec>
-__device__ __forceinline__ void store_vec(void* p, int64_t i, const float (&x)[kVec]) {
-  if constexpr (std::is_same_v<T, F32>) {
-    typename Raw<F32, kVec>::type v;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) v[k] = x[k];
-    *reinterpret_cast<typename Raw<F32, kVec>::type*>(static_cast<float*>(p) + i) = v;
-  } else if constexpr (kVec == 2) {
-    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + i) = from_float<T>(x[0]) | (from_float<T>(x[1]) << 16);
-  } else {
-    static_cast<uint16_t*>(p)[i] = (uint16_t)from_float<T>(x[0]);
+struct Rows {
+  typedef typename Raw<T, kVec>::type raw;
+  const char* at;
+  int64_t step;  // bytes
+  __device__ __forceinline__ Rows(const void* p, int64_t first, int64_t stride)
+      : at(static_cast<const char*>(p) + first * Fmt<T>::bytes), step(stride * Fmt<T>::bytes) {}
+  __device__ __forceinline__ raw load(int i, uint32_t lane) const {
+    return *reinterpret_cast<const raw*>(at + i * step + lane);
   }
-}
+  __device__ __forceinline__ void store(int i, uint32_t lane, const float (&x)[kVec]) const {
+    raw v;
+    if constexpr (std::is_same_v<T, F32>) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) v[k] = x[k];
+    } else if constexpr (kVec == 2) {
+      v = pack2<T>(x[0], x[1]);
+    } else {
+      v = (uint16_t)from_float<T>(x[0]);
+    }
+    *reinterpret_cast<raw*>(const_cast<char*>(at) + i * step + lane) = v;
+  }
+};
 
 // A launch's tiles: `groups` = batch x channel groups, `tiles` steps' tiles of each.
 struct ScanGrid {
@@ -273,64 +277,92 @@ __device__ __forceinline__ void enter_tile(const ScanGrid& g, int tile, int grou
   }
 }
 
+// A wave's place: its tile's group, channels and steps.
+template <typename T, int kVec>
+struct Place {
+  int64_t b, channel, c, t0;  // channel: the group's first; c: the lane's first
+  int n;                      // steps, <= 0: none
+  uint32_t lane;              // bytes
+  bool active;
+  __device__ __forceinline__ Place(const morph_scan& a, const ScanGrid& g, int tile, int group, int wave, int L) {
+    b = group / g.channel_groups;
+    channel = (int64_t)(group % g.channel_groups) * 64 * kVec;
+    const int l = threadIdx.x & 63;
+    active = channel + l * kVec < a.dim;
+    const int own = active ? l * kVec : 0;  // lanes past the end repeat the first and store nothing
+    c = channel + own;
+    lane = (uint32_t)own * Fmt<T>::bytes;
+    t0 = ((int64_t)tile * kWaves + wave) * L;
+    n = (int)(a.steps - t0 < L ? a.steps - t0 : L);
+  }
+};
+
+// Runs body(std::true_type) where the wave has all its steps, else body(std::false_type): the
+// tests for the sequence's end are in the second form only.
+template <typename F>
+__device__ __forceinline__ void whole_or_part(bool whole, F&& body) {
+  if (whole) body(std::true_type{});
+  else body(std::false_type{});
+}
+
 template <typename T, int kVec, bool kGated>
-__global__ __launch_bounds__(kThreads) void scan_tile_kernel(const morph_scan a, const ScanGrid g,
+__global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan a, const ScanGrid g,
                                                              void* __restrict__ y, float* __restrict__ last,
                                                              float* __restrict__ states) {
   constexpr int L = kForwardSteps;
+  typedef typename Raw<T, kVec>::type raw;
   int group;
   const int tile = take_tile(g, group);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t b = group / g.channel_groups;
-  const int64_t c0 = ((int64_t)(group % g.channel_groups) * 64 + lane) * kVec;
-  const bool active = c0 < a.dim;
-  const int64_t c = active ? c0 : 0;
-  const int64_t t0 = ((int64_t)tile * kWaves + wave) * L;
-  const int n = (int)(a.steps - t0 < L ? a.steps - t0 : L);  // <= 0: no steps
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place<T, kVec> p(a, g, tile, group, wave, L);
 
   float A[kVec], S[kVec], pa[L][kVec], ps[L][kVec];  // (A, S) from the wave's first step on
-  typename Raw<T, kVec>::type z[L];
+  raw z[kGated ? L : 1];
 #pragma unroll
   for (int k = 0; k < kVec; ++k) A[k] = 1.0f, S[k] = 0.0f;
-  if (n > 0) {
-    typename Raw<T, kVec>::type f[L], v[L];
-    const int64_t pf = b * a.f_batch + t0 * a.f_step + c, pv = b * a.v_batch + t0 * a.v_step + c;
-    const int64_t pz = b * a.z_batch + t0 * a.z_step + c;
+  const Rows<T, kVec> rf(a.f, p.b * a.f_batch + p.t0 * a.f_step + p.channel, a.f_step);
+  const Rows<T, kVec> rv(a.v, p.b * a.v_batch + p.t0 * a.v_step + p.channel, a.v_step);
+  const Rows<T, kVec> rz(a.z, p.b * a.z_batch + p.t0 * a.z_step + p.channel, a.z_step);
+  if (p.n > 0) {
+    whole_or_part(p.n == L, [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
+      raw f[L], v[L];
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int j = i < n ? i : n - 1;
-      f[i] = load_raw<T, kVec>(a.f, pf + j * a.f_step);
-      v[i] = load_raw<T, kVec>(a.v, pv + j * a.v_step);
-    }
-    if constexpr (kGated) {
-#pragma unroll
-      for (int i = 0; i < L; ++i) z[i] = load_raw<T, kVec>(a.z, pz + (i < n ? i : n - 1) * a.z_step);
-    }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const Sigmoid s = sigmoid(value<T, kVec>(f[i], k));
-        const float gate = i < n ? s.a : 1.0f;  // steps past the end pass the state on
-        const float in = i < n ? s.b * value<T, kVec>(v[i], k) : 0.0f;
-        ps[i][k] = S[k] = __fmaf_rn(gate, S[k], in);
-        pa[i][k] = A[k] *= gate;
+      for (int i = 0; i < L; ++i) {
+        const int j = kWhole || i < p.n ? i : p.n - 1;
+        f[i] = rf.load(j, p.lane);
+        v[i] = rv.load(j, p.lane);
       }
-    }
+      if constexpr (kGated) {
+#pragma unroll
+        for (int i = 0; i < L; ++i) z[i] = rz.load(kWhole || i < p.n ? i : p.n - 1, p.lane);
+      }
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          const Sigmoid s = sigmoid(value<T, kVec>(f[i], k));
+          float gate = s.a, in = s.b * value<T, kVec>(v[i], k);
+          if (!kWhole && i >= p.n) gate = 1.0f, in = 0.0f;  // steps past the end pass the state on
+          ps[i][k] = S[k] = __fmaf_rn(gate, S[k], in);
+          pa[i][k] = A[k] *= gate;
+        }
+      }
+    });
   }
   float first[kVec], wa[kVec], ws[kVec], carry[kVec];
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) first[k] = a.s0 ? a.s0[b * a.dim + c + k] : 0.0f;
-  enter_tile<kVec>(g, tile, group, wave, lane, A, S, first, wa, ws, carry);
-  if (!active) return;
-  if (n > 0) {
-    if (states && t0 % kSpan == 0) {
-      const int64_t spans = (a.steps + kSpan - 1) / kSpan;
+  for (int k = 0; k < kVec; ++k) first[k] = a.s0 ? a.s0[p.b * a.dim + p.c + k] : 0.0f;
+  enter_tile<kVec>(g, tile, group, wave, threadIdx.x & 63, A, S, first, wa, ws, carry);
+  if (!p.active || p.n <= 0) return;
+  if (states && p.t0 % kSpan == 0) {
+    const int64_t spans = (a.steps + kSpan - 1) / kSpan;
 #pragma unroll
-      for (int k = 0; k < kVec; ++k)
-        states[(b * spans + t0 / kSpan) * a.dim + c + k] = __fmaf_rn(wa[k], carry[k], ws[k]);
-    }
-    const int64_t py = (b * a.steps + t0) * a.dim + c;
+    for (int k = 0; k < kVec; ++k)
+      states[(p.b * spans + p.t0 / kSpan) * a.dim + p.c + k] = __fmaf_rn(wa[k], carry[k], ws[k]);
+  }
+  const Rows<T, kVec> ry(y, (p.b * a.steps + p.t0) * a.dim + p.channel, a.dim);
+  whole_or_part(p.n == L, [&](auto whole) {
     float s[kVec];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
@@ -340,73 +372,74 @@ __global__ __launch_bounds__(kThreads) void scan_tile_kernel(const morph_scan a,
         s[k] = out[k] = __fmaf_rn(wa[k] * pa[i][k], carry[k], __fmaf_rn(pa[i][k], ws[k], ps[i][k]));
         if constexpr (kGated) {
           const float q = value<T, kVec>(z[i], k);
-          out[k] *= q * sigmoid(q).a;
+          out[k] *= q * gate_sigmoid(q);
         }
       }
-      if (i < n) store_vec<T, kVec>(y, py + (int64_t)i * a.dim, out);
+      if (decltype(whole)::value || i < p.n) ry.store(i, p.lane, out);
     }
-    if (last && t0 + n == a.steps) {
+    if (last && p.t0 + p.n == a.steps) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) last[b * a.dim + c + k] = s[k];
+      for (int k = 0; k < kVec; ++k) last[p.b * a.dim + p.c + k] = s[k];
     }
-  }
+  });
 }
 
 template <typename T, int kVec, bool kGated>
-__global__ __launch_bounds__(kThreads) void scan_tile_back_kernel(const morph_scan a, const ScanGrid g,
+__global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph_scan a, const ScanGrid g,
                                                                   const float* __restrict__ states,
                                                                   const void* __restrict__ dy, int64_t dy_batch,
                                                                   int64_t dy_step, const float* __restrict__ dlast,
                                                                   void* __restrict__ df, void* __restrict__ dv,
                                                                   void* __restrict__ dz, float* __restrict__ ds0) {
   constexpr int L = kBackwardSteps;
+  typedef typename Raw<T, kVec>::type raw;
   int group;
   const int walked = take_tile(g, group);
   const int tile = g.tiles - 1 - walked;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t b = group / g.channel_groups;
-  const int64_t c0 = ((int64_t)(group % g.channel_groups) * 64 + lane) * kVec;
-  const bool active = c0 < a.dim;
-  const int64_t c = active ? c0 : 0;
-  const int64_t t0 = ((int64_t)tile * kWaves + wave) * L;
-  const int n = (int)(a.steps - t0 < L ? a.steps - t0 : L);
+  const Place<T, kVec> p(a, g, tile, group, wave, L);
 
-  // gate: a; pass: 1 - a; w: dy silu(z); q: what r is multiplied by for df, from the states
+  // gate: a; pass: 1 - a; w: dy silu(z); x: v, then what r is multiplied by for df
   float gate[L][kVec], pass[L][kVec], w[L][kVec], x[L][kVec], slope[kGated ? L : 1][kVec];
   float A[kVec], S[kVec], R[kVec], s[kVec], r[kVec];
 #pragma unroll
   for (int k = 0; k < kVec; ++k) A[k] = 1.0f, S[k] = 0.0f, R[k] = 0.0f;
-  if (n > 0) {
-    typename Raw<T, kVec>::type rf[L], rv[L], rz[kGated ? L : 1], rd[L];
-    const int64_t pf = b * a.f_batch + t0 * a.f_step + c, pv = b * a.v_batch + t0 * a.v_step + c;
-    const int64_t pz = b * a.z_batch + t0 * a.z_step + c, pd = b * dy_batch + t0 * dy_step + c;
+  const Rows<T, kVec> rf(a.f, p.b * a.f_batch + p.t0 * a.f_step + p.channel, a.f_step);
+  const Rows<T, kVec> rv(a.v, p.b * a.v_batch + p.t0 * a.v_step + p.channel, a.v_step);
+  const Rows<T, kVec> rz(a.z, p.b * a.z_batch + p.t0 * a.z_step + p.channel, a.z_step);
+  const Rows<T, kVec> rd(dy, p.b * dy_batch + p.t0 * dy_step + p.channel, dy_step);
+  if (p.n > 0) {
+    whole_or_part(p.n == L, [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
+      raw f[L], v[L], z[kGated ? L : 1], d[L];
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int j = i < n ? i : n - 1;
-      rf[i] = load_raw<T, kVec>(a.f, pf + j * a.f_step);
-      rv[i] = load_raw<T, kVec>(a.v, pv + j * a.v_step);
-      if constexpr (kGated) rz[i] = load_raw<T, kVec>(a.z, pz + j * a.z_step);
-      rd[i] = load_raw<T, kVec>(dy, pd + j * dy_step);
-    }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const Sigmoid q = sigmoid(value<T, kVec>(rf[i], k));
-        gate[i][k] = i < n ? q.a : 1.0f;
-        pass[i][k] = i < n ? q.b : 0.0f;
-        x[i][k] = i < n ? value<T, kVec>(rv[i], k) : 0.0f;
-        w[i][k] = i < n ? value<T, kVec>(rd[i], k) : 0.0f;
-        if constexpr (kGated) {
-          const float zv = i < n ? value<T, kVec>(rz[i], k) : 0.0f;
-          const Sigmoid h = sigmoid(zv);
-          slope[i][k] = w[i][k] * (h.a * __fmaf_rn(zv, h.b, 1.0f));
-          w[i][k] *= zv * h.a;
-        }
-        S[k] = __fmaf_rn(gate[i][k], S[k], pass[i][k] * x[i][k]);
-        A[k] *= gate[i][k];
+      for (int i = 0; i < L; ++i) {
+        const int j = kWhole || i < p.n ? i : p.n - 1;
+        f[i] = rf.load(j, p.lane);
+        v[i] = rv.load(j, p.lane);
+        if constexpr (kGated) z[i] = rz.load(j, p.lane);
+        d[i] = rd.load(j, p.lane);
       }
-    }
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const bool inside = kWhole || i < p.n;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          const Sigmoid q = sigmoid(value<T, kVec>(f[i], k));
+          gate[i][k] = inside ? q.a : 1.0f;
+          pass[i][k] = inside ? q.b : 0.0f;
+          x[i][k] = inside ? value<T, kVec>(v[i], k) : 0.0f;
+          w[i][k] = inside ? value<T, kVec>(d[i], k) : 0.0f;
+          if constexpr (kGated) {
+            const Silu h = silu(inside ? value<T, kVec>(z[i], k) : 0.0f);
+            slope[i][k] = w[i][k] * h.slope;
+            w[i][k] *= h.y;
+          }
+          S[k] = __fmaf_rn(gate[i][k], S[k], pass[i][k] * x[i][k]);
+          A[k] *= gate[i][k];
+        }
+      }
+    });
 #pragma unroll
     for (int i = L - 1; i >= 0; --i)
 #pragma unroll
@@ -421,52 +454,57 @@ __global__ __launch_bounds__(kThreads) void scan_tile_back_kernel(const morph_sc
     const int64_t spans = (a.steps + kSpan - 1) / kSpan;
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      s[k] = states[(b * spans + tile) * a.dim + c + k];
+      s[k] = states[(p.b * spans + tile) * a.dim + p.c + k];
       for (int i = 0; i < wave; ++i) s[k] = __fmaf_rn(sa[i][k][lane], s[k], ss[i][k][lane]);
     }
   }
-  if (n > 0) {
-    const int64_t at = (b * a.steps + t0) * a.dim + c;
+  const int64_t at = (p.b * a.steps + p.t0) * a.dim + p.channel;
+  if (p.n > 0) {
+    const Rows<T, kVec> oz(dz, at, a.dim);
+    whole_or_part(p.n == L, [&](auto whole) {
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      float out[kVec];
+      for (int i = 0; i < L; ++i) {
+        float out[kVec];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const float prev = s[k], v = x[i][k];
-        s[k] = __fmaf_rn(gate[i][k], prev, pass[i][k] * v);
-        x[i][k] = (prev - v) * (gate[i][k] * pass[i][k]);
-        if constexpr (kGated) out[k] = slope[i][k] * s[k];
+        for (int k = 0; k < kVec; ++k) {
+          const float prev = s[k], v = x[i][k];
+          s[k] = __fmaf_rn(gate[i][k], prev, pass[i][k] * v);
+          x[i][k] = (prev - v) * (gate[i][k] * pass[i][k]);
+          if constexpr (kGated) out[k] = slope[i][k] * s[k];
+        }
+        if constexpr (kGated)
+          if ((decltype(whole)::value || i < p.n) && p.active) oz.store(i, p.lane, out);
       }
-      if constexpr (kGated)
-        if (i < n && active) store_vec<T, kVec>(dz, at + (int64_t)i * a.dim, out);
-    }
+    });
   }
   float first[kVec], wa[kVec], wr[kVec], carry[kVec];
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) first[k] = dlast ? dlast[b * a.dim + c + k] : 0.0f;
+  for (int k = 0; k < kVec; ++k) first[k] = dlast ? dlast[p.b * a.dim + p.c + k] : 0.0f;
   enter_tile<kVec>(g, walked, group, kWaves - 1 - wave, lane, A, R, first, wa, wr, carry);
-  if (!active || n <= 0) return;
+  if (!p.active || p.n <= 0) return;
 #pragma unroll
   for (int k = 0; k < kVec; ++k) r[k] = __fmaf_rn(wa[k], carry[k], wr[k]);
-  const int64_t at = (b * a.steps + t0) * a.dim + c;
+  const Rows<T, kVec> of(df, at, a.dim), ov(dv, at, a.dim);
+  whole_or_part(p.n == L, [&](auto whole) {
 #pragma unroll
-  for (int i = L - 1; i >= 0; --i) {
-    float of[kVec], ov[kVec];
+    for (int i = L - 1; i >= 0; --i) {
+      float gf[kVec], gv[kVec];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      r[k] += w[i][k];
-      ov[k] = r[k] * pass[i][k];
-      of[k] = r[k] * x[i][k];
-      r[k] *= gate[i][k];
+      for (int k = 0; k < kVec; ++k) {
+        r[k] += w[i][k];
+        gv[k] = r[k] * pass[i][k];
+        gf[k] = r[k] * x[i][k];
+        r[k] *= gate[i][k];
+      }
+      if (decltype(whole)::value || i < p.n) {
+        ov.store(i, p.lane, gv);
+        of.store(i, p.lane, gf);
+      }
     }
-    if (i < n) {
-      store_vec<T, kVec>(dv, at + (int64_t)i * a.dim, ov);
-      store_vec<T, kVec>(df, at + (int64_t)i * a.dim, of);
-    }
-  }
-  if (ds0 && t0 == 0) {
+  });
+  if (ds0 && p.t0 == 0) {
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) ds0[b * a.dim + c + k] = r[k];
+    for (int k = 0; k < kVec; ++k) ds0[p.b * a.dim + p.c + k] = r[k];
   }
 }
 
