@@ -13,8 +13,8 @@
 // anything; then it applies the (A, S) of the tiles before it in its run, in order, to the state
 // that the run begins with, which the last tile of the run before published.  (Taking
 // whichever is there, a predecessor's state or its (A, S), would round differently from call to
-// call.)  A published word is 64 bits, value and mark together, so no ordering between words
-// is needed.  Tiles are taken by ticket, earlier times first: what a tile waits for is always
+// call.)  A published word is 64 bits and tells by itself whether it is there, so no ordering between
+// words is needed.  Tiles are taken by ticket, earlier times first: what a tile waits for is always
 // running or done, so every wait ends (kSpins bounds it all the same).
 //
 // The forward applies every step's (A, S) from the tile's beginning to the state that enters
@@ -123,6 +123,7 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kForwardSteps = 16;  // of a wave: 128 steps a tile
 constexpr int kBackwardSteps = 8;  // 64: the backward holds four values per step and channel
 constexpr int kSpins = 1 << 20;
+constexpr int kTicketBytes = 256;
 static_assert(kWaves * kBackwardSteps == kSpan, "a backward tile begins with a kept state");
 static_assert(kSpan % kForwardSteps == 0, "states are kept at a wave's first step");
 
@@ -170,34 +171,40 @@ struct Rows {
 // A launch's tiles: `groups` = batch x channel groups, `tiles` steps' tiles of each.
 struct ScanGrid {
   uint32_t* ticket;  // the workspace: tickets given out, then
-  uint64_t* parts;   // [tiles][groups][64 lanes][kVec]{A, S}
-  uint64_t* runs;    // [runs][groups][64 lanes][kVec]: the state that run 1, 2, ... begins with
+  uint64_t* parts;   // [tiles][groups][64 lanes][kVec]: A, S
+  uint64_t* runs;    // [runs][groups][64 lanes][kVec]: the state that run 1, 2, ... begins with, twice
   int32_t tiles, groups, channel_groups;
 };
-constexpr int kRun = 16;  // tiles: two for each wave to fetch
-constexpr uint64_t kMark = uint64_t(1) << 32;
+constexpr int kRun = 8;  // tiles: one for each wave to fetch
+static_assert(kRun <= kWaves, "the last wave, which fetches the run's first state, has no tile's words to fetch");
+constexpr uint64_t kNothing = ~uint64_t(0);  // a word that is not published yet
 
-__device__ __forceinline__ void publish(uint64_t* at, float x) {
-  __hip_atomic_store(at, kMark | __builtin_bit_cast(uint32_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Two floats as one word.  A pair of NaN that reads as kNothing is no result of arithmetic here
+// (the device's NaN has another payload), and would only be waited for until kSpins.
+__device__ __forceinline__ void publish(uint64_t* at, float x, float y) {
+  const uint64_t w = ((uint64_t)__builtin_bit_cast(uint32_t, y) << 32) | __builtin_bit_cast(uint32_t, x);
+  __hip_atomic_store(at, w == kNothing ? w ^ 1 : w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // kCount words of this lane, once all of the wave's are published (NaN should that never be).
 template <int kCount>
-__device__ __forceinline__ void fetch(const uint64_t* at, float (&x)[kCount]) {
+__device__ __forceinline__ void fetch(const uint64_t* at, float (&x)[kCount], float (&y)[kCount]) {
   uint64_t w[kCount];
   bool all = false;
   for (int spin = 0; spin < kSpins && !all; ++spin) {
-    if (spin > 0) __builtin_amdgcn_s_sleep(1);
     bool mine = true;
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
       w[i] = __hip_atomic_load(at + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      mine = mine && w[i] >= kMark;
+      mine = mine && w[i] != kNothing;
     }
     all = __all(mine);
   }
 #pragma unroll
-  for (int i = 0; i < kCount; ++i) x[i] = all ? __builtin_bit_cast(float, (uint32_t)w[i]) : __builtin_nanf("");
+  for (int i = 0; i < kCount; ++i) {
+    x[i] = all ? __builtin_bit_cast(float, (uint32_t)w[i]) : __builtin_nanf("");
+    y[i] = all ? __builtin_bit_cast(float, (uint32_t)(w[i] >> 32)) : __builtin_nanf("");
+  }
 }
 
 // This workgroup's tile, in the order of the tickets, and its group.
@@ -216,7 +223,7 @@ __device__ __forceinline__ int take_tile(const ScanGrid& g, int& group) {
 }
 
 // What enters the tile (carry) and the (A, S) of its steps before this wave; first: what enters
-// the first tile.  `order`: the wave's place in the direction of the walk.
+// the first tile, read in the first run.  `order`: the wave's place in the direction of the walk.
 template <int kVec>
 __device__ __forceinline__ void enter_tile(const ScanGrid& g, int tile, int group, int order, int lane,
                                            const float (&A)[kVec], const float (&S)[kVec], const float (&first)[kVec],
@@ -246,22 +253,18 @@ __device__ __forceinline__ void enter_tile(const ScanGrid& g, int tile, int grou
     const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
     if (order == kWaves - 1 && before < kRun - 1 && tile + 1 < g.tiles) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        publish(g.parts + 2 * (tile * stride + mine + k), la[k]);
-        publish(g.parts + 2 * (tile * stride + mine + k) + 1, ls[k]);
-      }
+      for (int k = 0; k < kVec; ++k) publish(g.parts + tile * stride + mine + k, la[k], ls[k]);
     }
-    for (int i = order; i < before; i += kWaves) {
-      float w[2 * kVec];
-      fetch<2 * kVec>(g.parts + 2 * (((int64_t)run * kRun + i) * stride + mine), w);
+    float x[kVec], y[kVec];
+    if (order < before) {
+      fetch<kVec>(g.parts + ((int64_t)run * kRun + order) * stride + mine, x, y);
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) pa[i][k][lane] = w[2 * k], ps[i][k][lane] = w[2 * k + 1];
+      for (int k = 0; k < kVec; ++k) pa[order][k][lane] = x[k], ps[order][k][lane] = y[k];
     }
     if (run > 0 && order == kWaves - 1) {
-      float w[kVec];
-      fetch<kVec>(g.runs + run * stride + mine, w);
+      fetch<kVec>(g.runs + run * stride + mine, x, y);
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) begin[k][lane] = w[k];
+      for (int k = 0; k < kVec; ++k) begin[k][lane] = x[k];
     }
     __syncthreads();
 #pragma unroll
@@ -271,8 +274,10 @@ __device__ __forceinline__ void enter_tile(const ScanGrid& g, int tile, int grou
     }
     if (order == kWaves - 1 && before == kRun - 1 && tile + 1 < g.tiles) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k)
-        publish(g.runs + (run + 1) * stride + mine + k, __fmaf_rn(la[k], carry[k], ls[k]));
+      for (int k = 0; k < kVec; ++k) {
+        const float next = __fmaf_rn(la[k], carry[k], ls[k]);
+        publish(g.runs + (run + 1) * stride + mine + k, next, next);
+      }
     }
   }
 }
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan
   }
   float first[kVec], wa[kVec], ws[kVec], carry[kVec];
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) first[k] = a.s0 ? a.s0[p.b * a.dim + p.c + k] : 0.0f;
+  for (int k = 0; k < kVec; ++k) first[k] = tile < kRun && a.s0 ? a.s0[p.b * a.dim + p.c + k] : 0.0f;
   enter_tile<kVec>(g, tile, group, wave, threadIdx.x & 63, A, S, first, wa, ws, carry);
   if (!p.active || p.n <= 0) return;
   if (states && p.t0 % kSpan == 0) {
@@ -407,6 +412,11 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
   const Rows<T, kVec> rf(a.f, p.b * a.f_batch + p.t0 * a.f_step + p.channel, a.f_step);
   const Rows<T, kVec> rv(a.v, p.b * a.v_batch + p.t0 * a.v_step + p.channel, a.v_step);
   const Rows<T, kVec> rz(a.z, p.b * a.z_batch + p.t0 * a.z_step + p.channel, a.z_step);
+  {
+    const int64_t spans = (a.steps + kSpan - 1) / kSpan;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) s[k] = states[(p.b * spans + tile) * a.dim + p.c + k];
+  }
   const Rows<T, kVec> rd(dy, p.b * dy_batch + p.t0 * dy_step + p.channel, dy_step);
   if (p.n > 0) {
     whole_or_part(p.n == L, [&](auto whole) {
@@ -451,10 +461,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
 #pragma unroll
     for (int k = 0; k < kVec; ++k) sa[wave][k][lane] = A[k], ss[wave][k][lane] = S[k];
     __syncthreads();
-    const int64_t spans = (a.steps + kSpan - 1) / kSpan;
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      s[k] = states[(p.b * spans + tile) * a.dim + p.c + k];
       for (int i = 0; i < wave; ++i) s[k] = __fmaf_rn(sa[i][k][lane], s[k], ss[i][k][lane]);
     }
   }
@@ -479,7 +487,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
   }
   float first[kVec], wa[kVec], wr[kVec], carry[kVec];
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) first[k] = dlast ? dlast[p.b * a.dim + p.c + k] : 0.0f;
+  for (int k = 0; k < kVec; ++k) first[k] = walked < kRun && dlast ? dlast[p.b * a.dim + p.c + k] : 0.0f;
   enter_tile<kVec>(g, walked, group, kWaves - 1 - wave, lane, A, R, first, wa, wr, carry);
   if (!p.active || p.n <= 0) return;
 #pragma unroll
@@ -508,11 +516,12 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
   }
 }
 
-// Zeros: the tickets and marks of a launch.  (A kernel, not a memset: a captured memset node is
+// The tickets (zero) and words (kNothing) of a launch.  (A kernel, not a memset: a captured memset node is
 // not replayed reliably.)
 __global__ __launch_bounds__(256) void scan_clear_kernel(u32x4* p, int64_t n) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = u32x4{0u, 0u, 0u, 0u};
+  const uint32_t x = i < kTicketBytes / 16 ? 0u : 0xFFFFFFFFu;
+  if (i < n) p[i] = u32x4{x, x, x, x};
 }
 
 bool float_type(int dtype) {
@@ -530,15 +539,13 @@ int scan_check(const morph_scan* a, int dtype) {
 
 // ---- host -------------------------------------------------------------------------
 
-constexpr size_t kTicketBytes = 256;
-
 int64_t tiles_of(int64_t steps, bool backward) {
   const int64_t span = kWaves * (backward ? kBackwardSteps : kForwardSteps);
   return (steps + span - 1) / span;
 }
-// Words for either channel count per lane, channels rounded up to 128: two a tile, one a run.
+// Words for either channel count per lane, channels rounded up to 128: one a tile, one a run.
 size_t scan_words(int64_t channels, int64_t tiles) {
-  return (size_t)channels * (size_t)(2 * tiles + (tiles + kRun - 1) / kRun);
+  return (size_t)channels * (size_t)(tiles + (tiles + kRun - 1) / kRun);
 }
 size_t scan_workspace(int64_t batch, int64_t steps, int64_t dim, bool backward) {
   const int64_t tiles = tiles_of(steps, backward);
@@ -558,7 +565,7 @@ int scan_grid(const morph_scan* a, int kvec, bool backward, void* workspace, hip
   if (total > 0x7FFFFFFF) return MORPH_ERANGE;
   g.ticket = static_cast<uint32_t*>(workspace);
   g.parts = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kTicketBytes);
-  g.runs = g.parts + 2 * total * 64 * kvec;
+  g.runs = g.parts + total * 64 * kvec;
   g.tiles = (int32_t)tiles, g.groups = (int32_t)groups, g.channel_groups = (int32_t)groups_c;
   grid = (unsigned)total;
   if (tiles > 1) {
