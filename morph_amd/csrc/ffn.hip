@@ -121,7 +121,12 @@ int launch_any(FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
 // ---- tiles ----------------------------------------------------------------------
 
 // Time of a launch of `tiles` tiles of edge ts over kt stages of K, in us: the constants of
-// the Newton-Schulz products' launches (gemm.hip), which run the same pipeline.
+// the Newton-Schulz products' launches (gemm.hip), which run the same pipeline, and what the
+// gate's epilogues add.  Measured, us with edges 64 / 128 / 256, rows x d x ff:
+//   gate (8 bits): 512 x 3072 x 6144 64 / 46 / 66, 2048: 284 / 164 / 154; 2048 x 768 x 2048 27 / 20 / 28;
+//   down: 128 x 3072 x 6144 28 / 52 / 100, 1024: 81 / 80 / 116, 4096: 261 / 181 / 134;
+//   gate's gradient (FP32 kept): 128 x 3072 x 6144 19 / 35 / 70, 1024: 79 / 59 / 89, 4096: 290 / 219 / 239;
+//   weights: 128 x 3072 x 6144 48 / 34 / 42, 1024: 183 / 125 / 122, 4096: 801 / 459 / 403.
 double tiles_us(int ts, int64_t tiles, int64_t kt, double epilogue) {
   const double q = (double)tiles / 256.0, n = std::ceil(q);
   if (ts == 256) {
@@ -294,7 +299,7 @@ int grad_product(int dtype, const Side& dy, const Side& down, int64_t rows, int6
                  const morph_ffn_saved* saved, uint16_t* h, uint16_t* dg, uint16_t* du, int64_t ld, hipStream_t s) {
   Launch l;
   l.add(dy, down, d, ff, rows, ff, h, ld);
-  const int ts = l.choose(d, 1, 3.0);
+  const int ts = l.choose(d, 1, 12.0);
   l.a.dg = dg, l.a.du = du, l.a.g = saved->gate, l.a.u = saved->up;
   l.a.g_exponents = saved->gate_exponents, l.a.u_exponents = saved->up_exponents;
   if (l.ok) {

@@ -8,8 +8,8 @@
 // transposing reads.
 //
 // Tiling and pipeline are the Newton-Schulz products' (gemm.hip, where the constants were
-// measured): a tile of 256 x 256 (or 128 x 128, two workgroups per CU, where those fill the
-// chip better), four waves with a quarter each as 32 x 32 x 16 MFMAs, K in stages of 64, a
+// measured): a tile of 256 x 256 (or 128 x 128, two workgroups per CU, or 64 x 64, three with a
+// pipeline of whole stages, where those fill the chip better), four waves with a quarter each as 32 x 32 x 16 MFMAs, K in stages of 64, a
 // ring of five LDS slots that hold the P or the Q of one stage, filled by direct loads
 // two stages ahead, two register sets of fragments; one barrier per stage.  Every 16-byte
 // chunk of an LDS row is stored XOR-swizzled, chosen by which chunk each lane fetches.
@@ -61,12 +61,12 @@ struct FfnTileArgs {
 
 template <int TS>
 struct FfnTile {
-  static_assert(TS == 256 || TS == 128, "tile edges");
+  static_assert(TS == 256 || TS == 128 || TS == 64, "tile edges");
   static constexpr int kDepth = 64;                  // K per stage: one 128-byte line per row
-  static constexpr int kSlots = 5;
+  static constexpr int kSlots = TS == 64 ? 6 : 5;    // of the LDS ring; 64: three whole stages
   static constexpr int kSubTile = TS * kDepth;       // 16-bit values per slot
-  static constexpr int kSmem = kSlots * kSubTile;    // 160 or 80 KiB
-  static constexpr int kPerCu = TS == 256 ? 1 : 2;   // workgroups per CU
+  static constexpr int kSmem = kSlots * kSubTile;    // 160, 80 or 48 KiB
+  static constexpr int kPerCu = TS == 256 ? 1 : TS == 128 ? 2 : 3;  // workgroups per CU
   static constexpr int kBlocks = TS / 64;            // 32-wide blocks per wave and dimension
   static constexpr int kLoads = TS / 32;             // load instructions per wave and slot
 };
@@ -263,7 +263,8 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
   // are the g and the u of the same columns.
   const int lrow = lane >> 3, lslot = lane & 7;
   auto swz = [](int r) { return (r ^ (r >> 3)) & 7; };
-  auto swz_cols = [](int r) { return 4 * (r & 3); };
+  // the 4 rows that a transposing read touches land on distinct banks (two rows fill them at 64)
+  auto swz_cols = [](int r) { return TS == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
   uint32_t offp[kLoads], offq[kLoads];
   uint32_t behind = 0;  // bit j: load j's chunk of a "rows" operand is past K in the last stage
 #pragma unroll
@@ -278,8 +279,10 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     if constexpr (kQCols) {
       offq[j] = (uint32_t)rk * (uint32_t)o.ldq[0] * 2u + ck * 16u;
     } else if constexpr (kDual) {
-      const bool up = TS == 256 ? j >= 4 : (wave & 1) != 0;
-      const int rt = TS == 256 ? wave * 32 + (j & 3) * 8 + lrow : (wave >> 1) * 32 + j * 8 + lrow;
+      const bool up = TS == 256 ? j >= 4 : TS == 128 ? (wave & 1) != 0 : wave >= 2;
+      const int rt = TS == 256   ? wave * 32 + (j & 3) * 8 + lrow
+                     : TS == 128 ? (wave >> 1) * 32 + j * 8 + lrow
+                                 : (wave & 1) * 16 + j * 8 + lrow;
       offq[j] = (uint32_t)rt * (uint32_t)(up ? o.ldq[1] : o.ldq[0]) * 2u + c * 16u;
     } else {
       offq[j] = (uint32_t)r * (uint32_t)o.ldq[0] * 2u + c * 16u;
@@ -293,7 +296,7 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     const bool last = s == KS - 1;
     Side side = q ? (second ? Q1 : Q0) : (second ? P1 : P0);
     if constexpr (kDual) {
-      if (q && (TS == 256 ? j >= 4 : (wave & 1) != 0)) side = Q1;
+      if (q && (TS == 256 ? j >= 4 : TS == 128 ? (wave & 1) != 0 : wave >= 2)) side = Q1;
     }
     const bool cols = q ? kQCols : kPCols;
     const uint16_t* base = side.base + (int64_t)s * side.step;
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
                           (cols ? (wave * 16 + j * (512 / TS)) * TS : (wave * (TS / 4) + j * 8) * BK);
     uint32_t off = q ? offq[j] : offp[j];
     if (!cols) off |= (behind << (31 - j)) & (last ? 0x80000000u : 0u);
-    if constexpr (kPCols || kQCols) {
+    if constexpr (kPCols || kQCols || TS == 64) {
       const uint64_t addr = reinterpret_cast<uint64_t>(uniform(base));
       const u32x4 rsrc = u32x4{(uint32_t)addr, (uint32_t)(addr >> 32) & 0xFFFFu,
                                (uint32_t)__builtin_amdgcn_readfirstlane((int)limit), 0x00020000u};
@@ -370,108 +373,9 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     }
   };
 
-  Frags f0, f1;
-  constexpr int kHalf = kLoads / 2;
-  constexpr int kPre = TS == 256 ? 2 : 1;  // MFMAs of the last sub-step before the barrier
-  // Behind MFMA n of a sub-step whose reads start after MFMA `first`.
-  auto reads_behind = [&](int n, int first, Frags& nxt, int rp, int rq, int kk) {
-    if constexpr (TS == 256) {
-      constexpr int kEach = kReads > 12 ? 2 : 1;
-#pragma unroll
-      for (int k = 0; k < kEach; ++k)
-        if (n >= first && (n - first) * kEach + k < kReads) read((n - first) * kEach + k, nxt, rp, rq, kk);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kReads; ++k)
-        if (k / (kReads / 2) == n - first) read(k, nxt, rp, rq, kk);
-    }
-  };
-  auto loads_behind = [&](int n, int first, bool lq, int ls_, int lstage, int j0) {
-    if constexpr (TS == 256) {
-      if (n >= first + 2 && n < first + 10 && (n & 1) == 0)
-        issue_load(lq, ls_, lstage, j0 + ((n - first - 2) >> 1));
-    } else if (n == first) {
-#pragma unroll
-      for (int j = 0; j < kHalf; ++j) issue_load(lq, ls_, lstage, j0 + j);
-    }
-  };
-  auto substep = [&](const Frags& cur, Frags& nxt, int rp, int rq, int kk, auto load, bool lq, int ls_,
-                     int lstage, int j0) {
-#pragma unroll
-    for (int n = 0; n < kMfmas; ++n) {
-      mfma(n, cur);
-      __builtin_amdgcn_sched_barrier(0);
-      reads_behind(n, 0, nxt, rp, rq, kk);
-      if constexpr (decltype(load)::value) loads_behind(n, 0, lq, ls_, lstage, j0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): next fragments in registers
-  };
-  // Step t computes stage t in four sub-steps, whose MFMAs run while the next sub-step's fragments
-  // are read.  kind: 0 with stages t + 1 and t + 2 to come, 1 the last but one, 2 the last.
-  auto step = [&](int t, int ps, auto kind) {
-    constexpr bool kNext = decltype(kind)::value < 2, kNext2 = decltype(kind)::value == 0;
-    const int qs = ps + 1 == kSlots ? 0 : ps + 1;
-    const int ps1 = qs + 1 == kSlots ? 0 : qs + 1;
-    const int qs1 = ps1 + 1 == kSlots ? 0 : ps1 + 1;
-    const int ps2 = qs1 + 1 == kSlots ? 0 : qs1 + 1;
-    const std::bool_constant<kNext> l1;
-    const std::bool_constant<kNext2> l2;
-    substep(f0, f1, ps, qs, 1, l1, true, qs1, t + 1, kHalf);   // Q of t + 1, second half
-    substep(f1, f0, ps, qs, 2, l2, false, ps2, t + 2, 0);      // P of t + 2, first half
-    substep(f0, f1, ps, qs, 3, l2, false, ps2, t + 2, kHalf);  // P of t + 2, second half
-#pragma unroll
-    for (int n = 0; n < kPre; ++n) mfma(n, f1);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (kNext) {
-      // all but P of t + 2 landed for this wave; the barrier publishes stage t + 1 and frees
-      // stage t's slots (every wave holds its last fragments)
-      __builtin_amdgcn_s_waitcnt(0x0F70 | (kNext2 ? kLoads : 0));
-      lds_barrier();
-    }
-#pragma unroll
-    for (int n = kPre; n < kMfmas; ++n) {
-      mfma(n, f1);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (kNext) {
-        reads_behind(n, kPre, f0, ps1, qs1, 0);
-        // Q of t + 2 into the freed P slot of t, first half
-        if constexpr (kNext2) loads_behind(n, TS == 256 ? 4 : kPre, true, ps, t + 2, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (kNext) __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-  };
-#pragma unroll
-  for (int j = 0; j < kLoads; ++j) issue_load(false, 0, 0, j);
-#pragma unroll
-  for (int j = 0; j < kLoads; ++j) issue_load(true, 1, 0, j);
-  if (KT > 1) {
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) issue_load(false, 2, 1, j);
-#pragma unroll
-    for (int j = 0; j < kHalf; ++j) issue_load(true, 3, 1, j);
-    __builtin_amdgcn_s_waitcnt(0x0F70 | (kLoads + kHalf));  // P and Q of stage 0 landed for this wave
-  } else {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  }
-  lds_barrier();
-#pragma unroll
-  for (int n = 0; n < kReads; ++n) read(n, f0, 0, 1, 0);
-  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-  int ps = 0;
-  auto advance = [&]() { ps = ps + 2 >= kSlots ? ps + 2 - kSlots : ps + 2; };
-  for (int t = 0; t + 2 < KT; ++t) {
-    step(t, ps, std::integral_constant<int, 0>{});
-    advance();
-  }
-  if (KT > 1) {
-    step(KT - 2, ps, std::integral_constant<int, 1>{});
-    advance();
-  }
   // kGateGrad: what was kept of the first blocks is on its way under the last stage's MFMAs, and
   // kAhead blocks ahead of its use from then on (a wait per block was 70 us of a 4096 x 6144 launch).
-  constexpr int kAhead = kE != FfnEpilogue::kGateGrad ? 1 : kKeep == MORPH_FFN_KEEP_FULL ? 3 : 4;
+  constexpr int kAhead = kE != FfnEpilogue::kGateGrad || TS == 64 ? 1 : kKeep == MORPH_FFN_KEEP_FULL ? 3 : 4;
   [[maybe_unused]] KeptBlock<kKeep> kg[kAhead], ku[kAhead] = {};
   auto load_block = [&](int n) {
     if constexpr (kE == FfnEpilogue::kGateGrad) {
@@ -482,16 +386,191 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
       load_kept<kKeep>(ku[n % kAhead], g.u, g.u_exponents, at, fh);
     }
   };
-  if constexpr (kE == FfnEpilogue::kGateGrad) {
+  auto load_ahead = [&]() {
+    if constexpr (kE == FfnEpilogue::kGateGrad) {
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) load_block(n);
-    __builtin_amdgcn_sched_barrier(0);
+      for (int n = 0; n < kAhead; ++n) load_block(n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if constexpr (TS == 64) {
+    // A ring of whole stages, and two register sets that hold all fragments of a stage each: step t
+    // waits until stage t + 1 has landed, the barrier publishes it and frees stage t's slots, and
+    // the reads of t + 1 and the loads of t + 3 run under stage t's MFMAs.
+    constexpr int kRing = kSlots / 2, kStageLoads = 2 * kLoads;
+    struct Stage {
+      Frags f[4];
+    };
+    auto load_stage = [&](int slot, int stage) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) issue_load(false, 2 * slot, stage, j);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) issue_load(true, 2 * slot + 1, stage, j);
+    };
+    auto read_stage = [&](Stage& st, int slot) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int n = 0; n < kReads; ++n) read(n, st.f[kk], 2 * slot, 2 * slot + 1, kk);
+    };
+    // this wave's loads of all but the youngest `pending` stages have landed
+    static_assert(kRing <= 3 && 2 * kStageLoads < 16, "the counts of wait_pending");
+    auto wait_pending = [&](int pending) {
+      if (pending <= 0) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      else if (pending == 1) __builtin_amdgcn_s_waitcnt(0x0F70 | kStageLoads);
+      else __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * kStageLoads));
+    };
+    Stage s0, s1;
+    int slot = 0;  // of stage t
+    auto step = [&](int t, const Stage& cur, Stage& nxt) {
+      const int nslot = slot + 1 == kRing ? 0 : slot + 1;
+      if (t + 1 < KT) {
+        wait_pending(min(kRing - 1, KT - 1 - t) - 1);
+        lds_barrier();
+        read_stage(nxt, nslot);
+        if (t + kRing < KT) load_stage(slot, t + kRing);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mfma(0, cur.f[kk]);
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): next fragments in registers
+      slot = nslot;
+    };
+#pragma unroll
+    for (int k = 0; k < kRing; ++k)
+      if (k < KT) load_stage(k, k);
+    wait_pending(min(kRing, KT) - 1);
+    lds_barrier();
+    read_stage(s0, 0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    for (int t = 0; t + 1 < KT; t += 2) {
+      step(t, s0, s1);
+      step(t + 1, s1, s0);
+    }
+    load_ahead();
+    if (KT & 1) step(KT - 1, s0, s1);
+  } else {
+    Frags f0, f1;
+    constexpr int kHalf = kLoads / 2;
+    constexpr int kPre = TS == 256 ? 2 : 1;  // MFMAs of the last sub-step before the barrier
+    // Behind MFMA n of a sub-step whose reads start after MFMA `first`.
+    auto reads_behind = [&](int n, int first, Frags& nxt, int rp, int rq, int kk) {
+      if constexpr (TS == 256) {
+        constexpr int kEach = kReads > 12 ? 2 : 1;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+          if (n >= first && (n - first) * kEach + k < kReads) read((n - first) * kEach + k, nxt, rp, rq, kk);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kReads; ++k)
+          if (k / (kReads / 2) == n - first) read(k, nxt, rp, rq, kk);
+      }
+    };
+    auto loads_behind = [&](int n, int first, bool lq, int ls_, int lstage, int j0) {
+      if constexpr (TS == 256) {
+        if (n >= first + 2 && n < first + 10 && (n & 1) == 0)
+          issue_load(lq, ls_, lstage, j0 + ((n - first - 2) >> 1));
+      } else if (n == first) {
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) issue_load(lq, ls_, lstage, j0 + j);
+      }
+    };
+    auto substep = [&](const Frags& cur, Frags& nxt, int rp, int rq, int kk, auto load, bool lq, int ls_,
+                       int lstage, int j0) {
+#pragma unroll
+      for (int n = 0; n < kMfmas; ++n) {
+        mfma(n, cur);
+        __builtin_amdgcn_sched_barrier(0);
+        reads_behind(n, 0, nxt, rp, rq, kk);
+        if constexpr (decltype(load)::value) loads_behind(n, 0, lq, ls_, lstage, j0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): next fragments in registers
+    };
+    // Step t computes stage t in four sub-steps, whose MFMAs run while the next sub-step's fragments
+    // are read.  kind: 0 with stages t + 1 and t + 2 to come, 1 the last but one, 2 the last.
+    auto step = [&](int t, int ps, auto kind) {
+      constexpr bool kNext = decltype(kind)::value < 2, kNext2 = decltype(kind)::value == 0;
+      const int qs = ps + 1 == kSlots ? 0 : ps + 1;
+      const int ps1 = qs + 1 == kSlots ? 0 : qs + 1;
+      const int qs1 = ps1 + 1 == kSlots ? 0 : ps1 + 1;
+      const int ps2 = qs1 + 1 == kSlots ? 0 : qs1 + 1;
+      const std::bool_constant<kNext> l1;
+      const std::bool_constant<kNext2> l2;
+      substep(f0, f1, ps, qs, 1, l1, true, qs1, t + 1, kHalf);   // Q of t + 1, second half
+      substep(f1, f0, ps, qs, 2, l2, false, ps2, t + 2, 0);      // P of t + 2, first half
+      substep(f0, f1, ps, qs, 3, l2, false, ps2, t + 2, kHalf);  // P of t + 2, second half
+#pragma unroll
+      for (int n = 0; n < kPre; ++n) mfma(n, f1);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kNext) {
+        // all but P of t + 2 landed for this wave; the barrier publishes stage t + 1 and frees
+        // stage t's slots (every wave holds its last fragments)
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (kNext2 ? kLoads : 0));
+        lds_barrier();
+      }
+#pragma unroll
+      for (int n = kPre; n < kMfmas; ++n) {
+        mfma(n, f1);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kNext) {
+          reads_behind(n, kPre, f0, ps1, qs1, 0);
+          // Q of t + 2 into the freed P slot of t, first half
+          if constexpr (kNext2) loads_behind(n, TS == 256 ? 4 : kPre, true, ps, t + 2, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (kNext) __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    };
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) issue_load(false, 0, 0, j);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) issue_load(true, 1, 0, j);
+    if (KT > 1) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) issue_load(false, 2, 1, j);
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j) issue_load(true, 3, 1, j);
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (kLoads + kHalf));  // P and Q of stage 0 landed for this wave
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    }
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < kReads; ++n) read(n, f0, 0, 1, 0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    int ps = 0;
+    auto advance = [&]() { ps = ps + 2 >= kSlots ? ps + 2 - kSlots : ps + 2; };
+    for (int t = 0; t + 2 < KT; ++t) {
+      step(t, ps, std::integral_constant<int, 0>{});
+      advance();
+    }
+    if (KT > 1) {
+      step(KT - 2, ps, std::integral_constant<int, 1>{});
+      advance();
+    }
+    load_ahead();
+    step(KT - 1, ps, std::integral_constant<int, 2>{});
   }
-  step(KT - 1, ps, std::integral_constant<int, 2>{});
 
   // ---- epilogue: straight from the registers ------------------------------------
   const int M = o.M, N = o.N;
   const int64_t ldc = o.ldc;
+  // h, and g and u as they are kept, of a 32 x 32 block
+  [[maybe_unused]] auto gate_block = [&](int row, int block, const float (&gv)[16], const float (&uv)[16],
+                                         const float (&h)[16]) {
+    const bool inside = row < M;
+    const int64_t at = (int64_t)row * ldc + block;
+    u32x4 lo, hi;
+    row_words<T>(h, lo, hi);
+    if (inside) {
+      *reinterpret_cast<u32x4*>(o.C + at + 16 * fh) = lo;
+      *reinterpret_cast<u32x4*>(o.C + at + 16 * fh + 8) = hi;
+    }
+    keep_block<kKeep>(gv, g.g, g.g_exponents, at, fh, inside);
+    keep_block<kKeep>(uv, g.u, g.u_exponents, at, fh, inside);
+  };
   if constexpr (kE == FfnEpilogue::kStore) {
 #pragma unroll
     for (int i = 0; i < kB; ++i) {
@@ -518,11 +597,29 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
         }
       }
     }
+  } else if constexpr (kE == FfnEpilogue::kGate && TS == 64) {
+    // waves 0 and 2 hold g of 32 rows each, 1 and 3 the u of the same: they meet through LDS
+    __syncthreads();  // every wave's fragment reads are done
+    f32x4* meet = reinterpret_cast<f32x4*>(smem) + (wave >> 1) * 256 + lane;
+    if (wave & 1) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        meet[64 * q] = f32x4{acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]};
+    }
+    __syncthreads();
+    if (wave & 1) return;
+    const int row = row0 + wr + fr;
+    float gv[16], uv[16], h[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      gv[r] = acc[0][0][r], uv[r] = meet[64 * (r >> 2)][r & 3];
+      h[r] = ffn_gate(gv[r], uv[r]);
+    }
+    gate_block(row, col0, gv, uv, h);
   } else if constexpr (kE == FfnEpilogue::kGate) {
 #pragma unroll
     for (int i = 0; i < kB; ++i) {
       const int row = row0 + wr + 32 * i + fr;
-      const bool inside = row < M;
 #pragma unroll
       for (int j = 0; j < kB / 2; ++j) {
         const int block = col0 + (wc + 64 * j) / 2;
@@ -533,15 +630,7 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
           gv[r] = acc[i][2 * j][r], uv[r] = acc[i][2 * j + 1][r];
           h[r] = ffn_gate(gv[r], uv[r]);
         }
-        const int64_t at = (int64_t)row * ldc + block;
-        u32x4 lo, hi;
-        row_words<T>(h, lo, hi);
-        if (inside) {
-          *reinterpret_cast<u32x4*>(o.C + at + 16 * fh) = lo;
-          *reinterpret_cast<u32x4*>(o.C + at + 16 * fh + 8) = hi;
-        }
-        keep_block<kKeep>(gv, g.g, g.g_exponents, at, fh, inside);
-        keep_block<kKeep>(uv, g.u, g.u_exponents, at, fh, inside);
+        gate_block(row, block, gv, uv, h);
       }
     }
   } else {
@@ -606,10 +695,12 @@ void launch_ffn_tiles(int ts, int dtype, unsigned grid, hipStream_t s, const Ffn
   const dim3 gd(grid), bd(kFfnThreads);
   if (dtype == MORPH_DTYPE_F16) {
     if (ts == 256) hipLaunchKernelGGL((ffn_tile_kernel<256, F16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-    else hipLaunchKernelGGL((ffn_tile_kernel<128, F16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
+    else if (ts == 128) hipLaunchKernelGGL((ffn_tile_kernel<128, F16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
+    else hipLaunchKernelGGL((ffn_tile_kernel<64, F16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
   } else {
     if (ts == 256) hipLaunchKernelGGL((ffn_tile_kernel<256, BF16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-    else hipLaunchKernelGGL((ffn_tile_kernel<128, BF16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
+    else if (ts == 128) hipLaunchKernelGGL((ffn_tile_kernel<128, BF16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
+    else hipLaunchKernelGGL((ffn_tile_kernel<64, BF16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
   }
 }
 
