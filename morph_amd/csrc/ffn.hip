@@ -12,6 +12,7 @@
 // values long; operands of other widths are copied to such rows first (ffn_pad_kernel: a
 // read and a write of them beside the product's many reads).  ffn_any_kernel takes operands of any stride and alignment, any size: 64 x 64
 // tiles through LDS, loaded element by element along whichever index is contiguous.
+#include <algorithm>
 #include <cmath>
 
 #include "ffn_rows.h"
@@ -133,6 +134,7 @@ double tiles_us(int ts, int64_t tiles, int64_t kt, double epilogue) {
     const double full = q / n;
     return n * ((double)kt * (1.0 + 0.45 * full * full) + 8.5 + 4 * epilogue);
   }
+  if (ts == 64) return (double)kt * std::max(0.22, 0.24 * q) + (0.2 + 0.1 * epilogue) * q + 3.0;
   const double stage = n <= 1.0 ? 0.55 : n <= 2.0 ? 0.8 : n <= 8.0 ? 0.45 * n + 0.1 : 0.5 * n - 0.3;
   return (double)kt * stage + n * (1.3 + epilogue) + 2.0;
 }
@@ -177,7 +179,12 @@ struct Launch {
       }
       return n;
     };
-    const int ts = tiles_us(256, tiles(256), kt, epilogue) <= tiles_us(128, tiles(128), kt, epilogue) ? 256 : 128;
+    int ts = 0;
+    double best = 0;
+    for (int edge = 256; edge >= 64; edge /= 2) {
+      const double us = tiles_us(edge, tiles(edge), kt, epilogue);
+      if (ts == 0 || us < best) ts = edge, best = us;
+    }
     const int64_t n = tiles(ts);
     ok = ok && n <= (1 << 30);
     a.total = (int32_t)n;
