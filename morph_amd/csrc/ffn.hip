@@ -121,22 +121,25 @@ int launch_any(FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
 
 // ---- tiles ----------------------------------------------------------------------
 
-// Time of a launch of `tiles` tiles of edge ts over kt stages of K, in us: the constants of
-// the Newton-Schulz products' launches (gemm.hip), which run the same pipeline, and what the
-// gate's epilogues add.  Measured, us with edges 64 / 128 / 256, rows x d x ff:
-//   gate (8 bits): 512 x 3072 x 6144 64 / 46 / 66, 2048: 284 / 164 / 154; 2048 x 768 x 2048 27 / 20 / 28;
-//   down: 128 x 3072 x 6144 28 / 52 / 100, 1024: 81 / 80 / 116, 4096: 261 / 181 / 134;
-//   gate's gradient (FP32 kept): 128 x 3072 x 6144 19 / 35 / 70, 1024: 79 / 59 / 89, 4096: 290 / 219 / 239;
-//   weights: 128 x 3072 x 6144 48 / 34 / 42, 1024: 183 / 125 / 122, 4096: 801 / 459 / 403.
-double tiles_us(int ts, int64_t tiles, int64_t kt, double epilogue) {
-  const double q = (double)tiles / 256.0, n = std::ceil(q);
-  if (ts == 256) {
-    const double full = q / n;
-    return n * ((double)kt * (1.0 + 0.45 * full * full) + 8.5 + 4 * epilogue);
+// Time of a launch of `tiles` tiles over kt stages of K, in us: the constants of the
+// Newton-Schulz products' launches (gemm.hip), which run the same pipeline, and what the
+// gate's epilogues add.  Measured, us with 64 x 64 / 128 x 128 / 256 x 128 / 256 x 256, rows x d x ff:
+//   gate: 512 x 3072 x 6144 64 / 49 / 44 / 68, 2048: 282 / 164 / 149 / 158, 4096 (FP32 kept): 557 / 377 / 316 / 270;
+//   down: 512 x 3072 x 6144 41 / 61 / 68 / 106, 2048: 150 / 108 / 89 / 120, 4096: 259 / 182 / 179 / 138;
+//   gate's gradient: 512 40 / 38 / 49 / 78, 2048: 139 / 98 / 112 / 104, 4096 (FP32 kept): 283 / 224 / 223 / 244;
+//   dx: 512 88 / 108 / 143 / 223, 2048: 282 / 197 / 173 / 247, 4096: 551 / 348 / 348 / 285;
+//   weights: 512 104 / 76 / 87 / 81, 2048: 360 / 234 / 237 / 219, 4096: 800 / 459 / 458 / 412.
+double tiles_us(FfnShape shape, int64_t tiles, int64_t kt, double epilogue) {
+  const double q = (double)tiles / 256.0, n = std::ceil(q), full = q / n;
+  switch (shape) {
+    case kTile256: return n * ((double)kt * (1.0 + 0.45 * full * full) + 8.5 + 4 * epilogue);
+    case kTile256x128: return n * ((double)kt * (0.65 + 0.2 * full * full) + 6.0 + 2 * epilogue);
+    case kTile128: {
+      const double stage = n <= 1.0 ? 0.55 : n <= 2.0 ? 0.8 : n <= 8.0 ? 0.45 * n + 0.1 : 0.5 * n - 0.3;
+      return (double)kt * stage + n * (1.3 + epilogue) + 2.0;
+    }
+    default: return (double)kt * std::max(0.22, 0.24 * q) + (0.2 + 0.1 * epilogue) * q + 3.0;
   }
-  if (ts == 64) return (double)kt * std::max(0.22, 0.24 * q) + (0.2 + 0.1 * epilogue) * q + 3.0;
-  const double stage = n <= 1.0 ? 0.55 : n <= 2.0 ? 0.8 : n <= 8.0 ? 0.45 * n + 0.1 : 0.5 * n - 0.3;
-  return (double)kt * stage + n * (1.3 + epilogue) + 2.0;
 }
 
 // A product in the tiles' form.  `padded`: of an internal buffer, whose rows hold zeros up to
@@ -164,31 +167,32 @@ struct Launch {
     o.vector = reinterpret_cast<uintptr_t>(c) % 16 == 0 && ldc % 8 == 0;
     ok = ok && fits(p, p_width) && fits(q, q_width);
   }
-  // The tile edge for this K, and with it the outputs' tiles; split: 2 where a tile has half as
+  // The tiles' shape for this K, and with it the outputs' tiles; split: 2 where a tile has half as
   // many output columns (the gate's).
-  int choose(int64_t K, int split, double epilogue) {
+  FfnShape choose(int64_t K, int split, double epilogue) {
     a.K = (int32_t)K;
     const int64_t kt = (K + 63) / 64;
-    auto tiles = [&](int ts) {
+    auto tiles = [&](int shape) {
+      const int tm = kFfnTileM[shape], tn = kFfnTileN[shape] / split;
       int64_t n = 0;
       for (int i = 0; i < a.count; ++i) {
         FfnTileProblem& o = a.p[i];
         o.first = (int32_t)n;
-        o.tiles_m = (o.M + ts - 1) / ts, o.tiles_n = (o.N + ts / split - 1) / (ts / split);
+        o.tiles_m = (o.M + tm - 1) / tm, o.tiles_n = (o.N + tn - 1) / tn;
         n += (int64_t)o.tiles_m * o.tiles_n;
       }
       return n;
     };
-    int ts = 0;
+    int shape = 0;
     double best = 0;
-    for (int edge = 256; edge >= 64; edge /= 2) {
-      const double us = tiles_us(edge, tiles(edge), kt, epilogue);
-      if (ts == 0 || us < best) ts = edge, best = us;
+    for (int i = 0; i < kFfnShapes; ++i) {
+      const double us = tiles_us((FfnShape)i, tiles(i), kt, epilogue);
+      if (i == 0 || us < best) shape = i, best = us;
     }
-    const int64_t n = tiles(ts);
+    const int64_t n = tiles(shape);
     ok = ok && n <= (1 << 30);
     a.total = (int32_t)n;
-    return ts;
+    return (FfnShape)shape;
   }
   unsigned grid() const { return (unsigned)((a.total + 7) / 8 * 8); }
 };
@@ -269,12 +273,12 @@ int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int
   l.add(x, gate, d, d, rows, ff, h, ld);
   l.ok = l.ok && fits(up, d);
   l.a.p[0].Q[1] = static_cast<const uint16_t*>(up.p), l.a.p[0].ldq[1] = up.ld;
-  const int ts = l.choose(d, 2, keep == MORPH_FFN_KEEP_NONE ? 0.0 : 1.0);
+  const FfnShape shape = l.choose(d, 2, keep == MORPH_FFN_KEEP_NONE ? 0.0 : 1.0);
   if (keep != MORPH_FFN_KEEP_NONE)
     l.a.g = saved->gate, l.a.u = saved->up, l.a.g_exponents = saved->gate_exponents,
     l.a.u_exponents = saved->up_exponents;
   if (l.ok) {
-    ffn_tile_gate(ts, dtype, keep, l.grid(), s, l.a);
+    ffn_tile_gate(shape, dtype, keep, l.grid(), s, l.a);
     return launch_status();
   }
   FfnProduct p{};
@@ -292,9 +296,9 @@ int down_product(int dtype, const Side& h, const Side& down, int64_t rows, int64
                         static_cast<uint16_t*>(y), y_ld, s);
   Launch l;
   l.add(h, down, ff, ff, rows, d, y, y_ld);
-  const int ts = l.choose(ff, 1, 0.0);
+  const FfnShape shape = l.choose(ff, 1, 0.0);
   if (l.ok) {
-    ffn_tile_rows(ts, dtype, l.grid(), s, l.a);
+    ffn_tile_rows(shape, dtype, l.grid(), s, l.a);
     return launch_status();
   }
   FfnProduct p{};
@@ -308,11 +312,11 @@ int grad_product(int dtype, const Side& dy, const Side& down, int64_t rows, int6
                  const morph_ffn_saved* saved, uint16_t* h, uint16_t* dg, uint16_t* du, int64_t ld, hipStream_t s) {
   Launch l;
   l.add(dy, down, d, ff, rows, ff, h, ld);
-  const int ts = l.choose(d, 1, 12.0);
+  const FfnShape shape = l.choose(d, 1, saved->keep == MORPH_FFN_KEEP_FULL ? 12.0 : 7.0);
   l.a.dg = dg, l.a.du = du, l.a.g = saved->gate, l.a.u = saved->up;
   l.a.g_exponents = saved->gate_exponents, l.a.u_exponents = saved->up_exponents;
   if (l.ok) {
-    ffn_tile_grad(ts, dtype, saved->keep, l.grid(), s, l.a);
+    ffn_tile_grad(shape, dtype, saved->keep, l.grid(), s, l.a);
     return launch_status();
   }
   FfnProduct p{};
@@ -330,9 +334,9 @@ int input_product(int dtype, const Side& dg, const Side& du, const Side& gate, c
   l.ok = l.ok && fits(up, d) && gate.ld == up.ld;  // one set of offsets for both segments
   FfnTileProblem& o = l.a.p[0];
   o.P[1] = static_cast<const uint16_t*>(du.p), o.Q[1] = static_cast<const uint16_t*>(up.p);
-  const int ts = l.choose(ff, 1, 0.0);
+  const FfnShape shape = l.choose(ff, 1, 0.0);
   if (l.ok) {
-    ffn_tile_two(ts, dtype, l.grid(), s, l.a);
+    ffn_tile_two(shape, dtype, l.grid(), s, l.a);
     return launch_status();
   }
   FfnProduct p{};
@@ -351,9 +355,9 @@ int weight_products(int dtype, const Side& dg, const Side& du, const Side& x, co
   } w[3] = {{dg, x, ff, d, dgate}, {du, x, ff, d, dup}, {dy, h, d, ff, ddown}};
   Launch l;
   for (auto& e : w) l.add(e.p, e.q, e.M, e.N, e.M, e.N, e.out, e.N);
-  const int ts = l.choose(rows, 1, 0.0);
+  const FfnShape shape = l.choose(rows, 1, 0.0);
   if (l.ok && rows > 0) {
-    ffn_tile_weights(ts, dtype, l.grid(), s, l.a);
+    ffn_tile_weights(shape, dtype, l.grid(), s, l.a);
     return launch_status();
   }
   for (auto& e : w) {

@@ -8,8 +8,8 @@
 // transposing reads.
 //
 // Tiling and pipeline are the Newton-Schulz products' (gemm.hip, where the constants were
-// measured): a tile of 256 x 256 (or 128 x 128, two workgroups per CU, or 64 x 64, three with a
-// pipeline of whole stages, where those fill the chip better), four waves with a quarter each as 32 x 32 x 16 MFMAs, K in stages of 64, a
+// measured): a tile of 256 x 256 (or 256 x 128, or 128 x 128 with two workgroups per CU, or 64 x 64,
+// three with a pipeline of whole stages, where those fill the chip better), four waves with a quarter each as 32 x 32 x 16 MFMAs, K in stages of 64, a
 // ring of five LDS slots that hold the P or the Q of one stage, filled by direct loads
 // two stages ahead, two register sets of fragments; one barrier per stage.  Every 16-byte
 // chunk of an LDS row is stored XOR-swizzled, chosen by which chunk each lane fetches.
@@ -59,16 +59,15 @@ struct FfnTileArgs {
   uint8_t *g_exponents, *u_exponents;
 };
 
-template <int TS>
+template <int TM, int TN>
 struct FfnTile {
-  static_assert(TS == 256 || TS == 128 || TS == 64, "tile edges");
+  static_assert((TM == 256 || TM == 128 || TM == 64) && (TN == TM || (TM == 256 && TN == 128)), "tile shapes");
   static constexpr int kDepth = 64;                  // K per stage: one 128-byte line per row
-  static constexpr int kSlots = TS == 64 ? 6 : 5;    // of the LDS ring; 64: three whole stages
-  static constexpr int kSubTile = TS * kDepth;       // 16-bit values per slot
-  static constexpr int kSmem = kSlots * kSubTile;    // 160, 80 or 48 KiB
-  static constexpr int kPerCu = TS == 256 ? 1 : TS == 128 ? 2 : 3;  // workgroups per CU
-  static constexpr int kBlocks = TS / 64;            // 32-wide blocks per wave and dimension
-  static constexpr int kLoads = TS / 32;             // load instructions per wave and slot
+  static constexpr int kSlots = TM == 64 ? 6 : 5;    // of the LDS ring; 64: three whole stages
+  static constexpr int kSlot = TM * kDepth;          // 16-bit values of a slot: the P or the Q of a stage
+  static constexpr int kSmem = kSlots * kSlot;       // 160, 80 or 48 KiB
+  static constexpr int kPerCu = TM == 256 ? 1 : TM == 128 ? 2 : 3;  // workgroups per CU
+  static constexpr int kBi = TM / 64, kBj = TN / 64;  // 32-wide blocks per wave and dimension
 };
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -178,10 +177,11 @@ __device__ __forceinline__ void kept_values(const KeptBlock<kKeep>& k, float (&x
 // ---- the tile -------------------------------------------------------------------
 
 // kPCols, kQCols: how P and Q are stored; kTwo: two segments of K; kKeep: what the gate keeps.
-template <int TS, typename T, bool kPCols, bool kQCols, bool kTwo, FfnEpilogue kE, int kKeep>
-__global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_kernel(const FfnTileArgs g) {
-  using C = FfnTile<TS>;
-  constexpr int BK = C::kDepth, kSlots = C::kSlots, kSubTile = C::kSubTile, kB = C::kBlocks, kLoads = C::kLoads;
+template <int TM, int TN, typename T, bool kPCols, bool kQCols, bool kTwo, FfnEpilogue kE, int kKeep>
+__global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_tile_kernel(const FfnTileArgs g) {
+  using C = FfnTile<TM, TN>;
+  constexpr int BK = C::kDepth, kSlots = C::kSlots, kSlot = C::kSlot, kBi = C::kBi, kBj = C::kBj;
+  constexpr int kLoadsP = TM / 32, kLoadsQ = TN / 32;  // load instructions per wave and slot
   constexpr bool kDual = kE == FfnEpilogue::kGate;
   static_assert(!(kDual && (kPCols || kQCols || kTwo)) && !(kPCols && kTwo), "forms in use");
   __shared__ __attribute__((aligned(16))) uint16_t smem[C::kSmem];
@@ -204,8 +204,8 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     tc = within / rows;
     tr = group * kGroupM + within % rows;
   }
-  constexpr int kCols = kDual ? TS / 2 : TS;  // output columns of a tile
-  const int row0 = tr * TS, col0 = tc * kCols;
+  constexpr int kCols = kDual ? TN / 2 : TN;  // output columns of a tile
+  const int row0 = tr * TM, col0 = tc * kCols;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -256,36 +256,39 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
   if constexpr (kTwo) P1 = side(o.P[1], o.ldp[1], false, row0, o.M, 0);
   if constexpr (kTwo || kDual) Q1 = side(o.Q[1], o.ldq[1], kQCols, col0, o.N, (o.N + 7) / 8 * 8);
 
-  // Loads.  "rows": wave w loads rows [w TS / 4, (w + 1) TS / 4) of a slot, 8 per instruction;
-  // lane l: row l / 8, LDS chunk l % 8, which holds the global chunk (l % 8) ^ swz(row).  "cols":
-  // 512 / TS of the stage's 64 rows of TS columns per instruction.  kGate: the LDS rows of Q
-  // alternate in blocks of 32 between gate and up, so that a wave's blocks 2j and 2j + 1
-  // are the g and the u of the same columns.
+  // Loads.  "rows": wave w loads a quarter of a slot's rows, 8 per instruction; lane l: row l / 8,
+  // LDS chunk l % 8, which holds the global chunk (l % 8) ^ swz(row).  "cols": 512 / width of the
+  // stage's 64 rows per instruction.  kGate: the LDS rows of Q alternate in blocks of 32 between
+  // gate and up, so that a wave's blocks 2j and 2j + 1 are the g and the u of the same
+  // columns (at 64: waves 0 and 2 hold the g, 1 and 3 the u).
   const int lrow = lane >> 3, lslot = lane & 7;
   auto swz = [](int r) { return (r ^ (r >> 3)) & 7; };
   // the 4 rows that a transposing read touches land on distinct banks (two rows fill them at 64)
-  auto swz_cols = [](int r) { return TS == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
-  uint32_t offp[kLoads], offq[kLoads];
-  uint32_t behind = 0;  // bit j: load j's chunk of a "rows" operand is past K in the last stage
-#pragma unroll
-  for (int j = 0; j < kLoads; ++j) {
-    const int r = wave * (TS / 4) + j * 8 + lrow;
+  auto swz_cols = [](int r, int width) { return width == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
+  auto is_up = [&](int j) { return TN == 256 ? j >= 4 : TN == 128 ? (wave & 1) != 0 : wave >= 2; };  // kGate
+  uint32_t offp[kLoadsP], offq[kLoadsQ];
+  uint32_t behindp = 0, behindq = 0;  // bit j: load j's chunk of a "rows" operand is past K in the last stage
+  auto offset = [&](int j, int width, bool cols, int64_t ld, uint32_t& behind, int tensor_row) {
+    if (cols) {
+      const int rk = wave * 16 + j * (512 / width) + lane / (width / 8);
+      return (uint32_t)rk * (uint32_t)ld * 2u + (uint32_t)((lane % (width / 8)) ^ swz_cols(rk, width)) * 16u;
+    }
+    const int r = wave * (width / 4) + j * 8 + lrow;
     const uint32_t c = (uint32_t)(lslot ^ swz(r));
-    const int rk = wave * 16 + j * (512 / TS) + lane / (TS / 8);
-    const uint32_t ck = (uint32_t)((lane % (TS / 8)) ^ swz_cols(rk));
     if ((int)c * 8 >= rest) behind |= 1u << j;
-    offp[j] = kPCols ? (uint32_t)rk * (uint32_t)o.ldp[0] * 2u + ck * 16u
-                     : (uint32_t)r * (uint32_t)o.ldp[0] * 2u + c * 16u;
-    if constexpr (kQCols) {
-      offq[j] = (uint32_t)rk * (uint32_t)o.ldq[0] * 2u + ck * 16u;
-    } else if constexpr (kDual) {
-      const bool up = TS == 256 ? j >= 4 : TS == 128 ? (wave & 1) != 0 : wave >= 2;
-      const int rt = TS == 256   ? wave * 32 + (j & 3) * 8 + lrow
-                     : TS == 128 ? (wave >> 1) * 32 + j * 8 + lrow
+    return (uint32_t)(tensor_row >= 0 ? tensor_row : r) * (uint32_t)ld * 2u + c * 16u;
+  };
+#pragma unroll
+  for (int j = 0; j < kLoadsP; ++j) offp[j] = offset(j, TM, kPCols, o.ldp[0], behindp, -1);
+#pragma unroll
+  for (int j = 0; j < kLoadsQ; ++j) {
+    if constexpr (kDual) {
+      const int rt = TN == 256   ? wave * 32 + (j & 3) * 8 + lrow
+                     : TN == 128 ? (wave >> 1) * 32 + j * 8 + lrow
                                  : (wave & 1) * 16 + j * 8 + lrow;
-      offq[j] = (uint32_t)rt * (uint32_t)(up ? o.ldq[1] : o.ldq[0]) * 2u + c * 16u;
+      offq[j] = offset(j, TN, false, is_up(j) ? o.ldq[1] : o.ldq[0], behindq, rt);
     } else {
-      offq[j] = (uint32_t)r * (uint32_t)o.ldq[0] * 2u + c * 16u;
+      offq[j] = offset(j, TN, kQCols, o.ldq[0], behindq, -1);
     }
   }
   // With a "cols" operand the load is inline assembly: the compiler then adds no waits of its
@@ -296,16 +299,17 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     const bool last = s == KS - 1;
     Side side = q ? (second ? Q1 : Q0) : (second ? P1 : P0);
     if constexpr (kDual) {
-      if (q && (TS == 256 ? j >= 4 : TS == 128 ? (wave & 1) != 0 : wave >= 2)) side = Q1;
+      if (q && is_up(j)) side = Q1;
     }
     const bool cols = q ? kQCols : kPCols;
+    const int width = q ? TN : TM;
     const uint16_t* base = side.base + (int64_t)s * side.step;
     const uint32_t limit = cols && last ? side.last : side.limit;
-    const uint16_t* dst = smem + slot * kSubTile +
-                          (cols ? (wave * 16 + j * (512 / TS)) * TS : (wave * (TS / 4) + j * 8) * BK);
-    uint32_t off = q ? offq[j] : offp[j];
-    if (!cols) off |= (behind << (31 - j)) & (last ? 0x80000000u : 0u);
-    if constexpr (kPCols || kQCols || TS == 64) {
+    const uint16_t* dst = smem + slot * kSlot +
+                          (cols ? (wave * 16 + j * (512 / width)) * width : (wave * (width / 4) + j * 8) * BK);
+    uint32_t off = q ? offq[q ? j : 0] : offp[j];
+    if (!cols) off |= ((q ? behindq : behindp) << (31 - j)) & (last ? 0x80000000u : 0u);
+    if constexpr (kPCols || kQCols || TM == 64) {
       const uint64_t addr = reinterpret_cast<uint64_t>(uniform(base));
       const u32x4 rsrc = u32x4{(uint32_t)addr, (uint32_t)(addr >> 32) & 0xFFFFu,
                                (uint32_t)__builtin_amdgcn_readfirstlane((int)limit), 0x00020000u};
@@ -323,24 +327,24 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     }
   };
 
-  const int wr = (wave >> 1) * (TS / 2), wc = (wave & 1) * (TS / 2);
+  const int wr = (wave >> 1) * (TM / 2), wc = (wave & 1) * (TN / 2);
   const int fr = lane & 31, fh = lane >> 5;
-  f32x16 acc[kB][kB];
+  f32x16 acc[kBi][kBj];
 #pragma unroll
-  for (int i = 0; i < kB; ++i)
+  for (int i = 0; i < kBi; ++i)
 #pragma unroll
-    for (int j = 0; j < kB; ++j) acc[i][j] = f32x16{};
+    for (int j = 0; j < kBj; ++j) acc[i][j] = f32x16{};
 
   auto frag = [&](const uint16_t* sub, int R, int c) {
     return *reinterpret_cast<const u32x4*>(sub + R * BK + ((c ^ swz(R)) * 8));
   };
   // Half h of a "cols" operand's fragment of rows n0 .. n0 + 31 at depth kk: in each group of 16
   // lanes the transposing read gives lane j, slot e, element j % 4 of source lane 4 e + j / 4.
-  auto frag_cols = [&](const uint16_t* sub, int n0, int kk, int h) {
+  auto frag_cols = [&](const uint16_t* sub, int width, int n0, int kk, int h) {
     const int j = lane & 15;
     const int row = kk * 16 + 8 * (lane >> 5) + 4 * h + (j >> 2);
     const int col = n0 + 16 * ((lane >> 4) & 1) + 4 * (j & 3);
-    const uint16_t* at = sub + row * TS + ((((col >> 3) ^ swz_cols(row)) << 3) | (col & 7));
+    const uint16_t* at = sub + row * width + ((((col >> 3) ^ swz_cols(row, width)) << 3) | (col & 7));
     typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
@@ -348,24 +352,28 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
   };
   auto lds_barrier = []() { asm volatile("s_barrier" ::: "memory"); };
   struct Frags {
-    u32x4 a[kB], q[kB];
+    u32x4 a[kBi], q[kBj];
   };
-  constexpr int kMfmas = kB * kB;
+  constexpr int kMfmas = kBi * kBj;  // per sub-step of 16 k
   auto mfma = [&](int n, const Frags& f) {
-    const int i = n / kB, j = n % kB;
+    const int i = n / kBj, j = n % kBj;
     acc[i][j] = mfma32<T>(f.q[j], f.a[i], acc[i][j]);
   };
-  constexpr int kPParts = kPCols ? 2 : 1, kQParts = kQCols ? 2 : 1, kParts = kPParts + kQParts;
-  constexpr int kReads = kB * kParts;
+  constexpr int kPParts = kPCols ? 2 : 1, kQParts = kQCols ? 2 : 1;
+  constexpr int kReads = kBi * kPParts + kBj * kQParts;
+  // Read n of a sub-step's fragments: P's and Q's in turn, then what is left of P's.
   auto read = [&](int n, Frags& f, int pslot, int qslot, int kk) {
-    const int i = n / kParts, part = n % kParts;
-    const bool q = part >= kPParts;
-    const int h = q ? part - kPParts : part;
-    const uint16_t* sub = smem + (q ? qslot : pslot) * kSubTile;
+    constexpr int kPair = kPParts + kQParts;
+    const bool paired = n < kBj * kPair;
+    const int m = paired ? n % kPair : (n - kBj * kPair) % kPParts;
+    const int i = paired ? n / kPair : kBj + (n - kBj * kPair) / kPParts;
+    const bool q = paired && m >= kPParts;
+    const int h = q ? m - kPParts : m;
+    const uint16_t* sub = smem + (q ? qslot : pslot) * kSlot;
     const int at = (q ? wc : wr) + i * 32;
-    u32x4& to = q ? f.q[i] : f.a[i];
+    u32x4& to = q ? f.q[q ? i : 0] : f.a[i];
     if (q ? kQCols : kPCols) {
-      const u32x2 half = frag_cols(sub, at, kk, h);
+      const u32x2 half = frag_cols(sub, q ? TN : TM, at, kk, h);
       if (h == 0) to.x = half.x, to.y = half.y;
       else to.z = half.x, to.w = half.y;
     } else {
@@ -375,11 +383,11 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
 
   // kGateGrad: what was kept of the first blocks is on its way under the last stage's MFMAs, and
   // kAhead blocks ahead of its use from then on (a wait per block was 70 us of a 4096 x 6144 launch).
-  constexpr int kAhead = kE != FfnEpilogue::kGateGrad || TS == 64 ? 1 : kKeep == MORPH_FFN_KEEP_FULL ? 3 : 4;
+  constexpr int kAhead = kE != FfnEpilogue::kGateGrad || TM == 64 ? 1 : kKeep == MORPH_FFN_KEEP_FULL ? 3 : 4;
   [[maybe_unused]] KeptBlock<kKeep> kg[kAhead], ku[kAhead] = {};
   auto load_block = [&](int n) {
     if constexpr (kE == FfnEpilogue::kGateGrad) {
-      const int row = row0 + wr + 32 * (n / kB) + fr, block = col0 + wc + 32 * (n % kB);
+      const int row = row0 + wr + 32 * (n / kBj) + fr, block = col0 + wc + 32 * (n % kBj);
       if (block >= o.ldc) return;
       const int64_t at = (int64_t)min(row, o.M - 1) * o.ldc + block;
       load_kept<kKeep>(kg[n % kAhead], g.g, g.g_exponents, at, fh);
@@ -394,19 +402,19 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     }
   };
 
-  if constexpr (TS == 64) {
+  if constexpr (TM == 64) {
     // A ring of whole stages, and two register sets that hold all fragments of a stage each: step t
     // waits until stage t + 1 has landed, the barrier publishes it and frees stage t's slots, and
     // the reads of t + 1 and the loads of t + 3 run under stage t's MFMAs.
-    constexpr int kRing = kSlots / 2, kStageLoads = 2 * kLoads;
+    constexpr int kRing = kSlots / 2, kStageLoads = kLoadsP + kLoadsQ;
     struct Stage {
       Frags f[4];
     };
     auto load_stage = [&](int slot, int stage) {
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) issue_load(false, 2 * slot, stage, j);
+      for (int j = 0; j < kLoadsP; ++j) issue_load(false, 2 * slot, stage, j);
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) issue_load(true, 2 * slot + 1, stage, j);
+      for (int j = 0; j < kLoadsQ; ++j) issue_load(true, 2 * slot + 1, stage, j);
     };
     auto read_stage = [&](Stage& st, int slot) {
 #pragma unroll
@@ -452,38 +460,37 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     if (KT & 1) step(KT - 1, s0, s1);
   } else {
     Frags f0, f1;
-    constexpr int kHalf = kLoads / 2;
-    constexpr int kPre = TS == 256 ? 2 : 1;  // MFMAs of the last sub-step before the barrier
-    // Behind MFMA n of a sub-step whose reads start after MFMA `first`.
+    constexpr int kHalfP = kLoadsP / 2, kHalfQ = kLoadsQ / 2;
+    constexpr int kPre = TM == 256 ? 2 : 1;  // MFMAs of the last sub-step before the barrier
+    // Behind MFMA n of a sub-step whose reads start after MFMA `first`: one or two reads at a
+    // time, at 128 x 128 half of them behind each of two MFMAs.
     auto reads_behind = [&](int n, int first, Frags& nxt, int rp, int rq, int kk) {
-      if constexpr (TS == 256) {
-        constexpr int kEach = kReads > 12 ? 2 : 1;
+      constexpr int kEach = TM == 256 ? (kReads + kMfmas - kPre - 1) / (kMfmas - kPre) : kReads / 2;
 #pragma unroll
-        for (int k = 0; k < kEach; ++k)
-          if (n >= first && (n - first) * kEach + k < kReads) read((n - first) * kEach + k, nxt, rp, rq, kk);
-      } else {
-#pragma unroll
-        for (int k = 0; k < kReads; ++k)
-          if (k / (kReads / 2) == n - first) read(k, nxt, rp, rq, kk);
-      }
+      for (int k = 0; k < kEach; ++k)
+        if (n >= first && (n - first) * kEach + k < kReads) read((n - first) * kEach + k, nxt, rp, rq, kk);
     };
-    auto loads_behind = [&](int n, int first, bool lq, int ls_, int lstage, int j0) {
-      if constexpr (TS == 256) {
-        if (n >= first + 2 && n < first + 10 && (n & 1) == 0)
-          issue_load(lq, ls_, lstage, j0 + ((n - first - 2) >> 1));
+    // Loads j0 on, half a slot's: one behind every other MFMA (256 x 256), every one (256 x 128),
+    // or all at once.
+    auto loads_behind = [&](int n, int first, bool lq, int ls_, int lstage, bool upper) {
+      const int half = lq ? kHalfQ : kHalfP, j0 = upper ? half : 0;
+      if constexpr (TM == 256) {
+        constexpr int kStep = TN == 256 ? 2 : 1;
+        const int l = (n - first - kStep) / kStep;
+        if (n >= first + kStep && (n - first) % kStep == 0 && l < half) issue_load(lq, ls_, lstage, j0 + l);
       } else if (n == first) {
 #pragma unroll
-        for (int j = 0; j < kHalf; ++j) issue_load(lq, ls_, lstage, j0 + j);
+        for (int j = 0; j < half; ++j) issue_load(lq, ls_, lstage, j0 + j);
       }
     };
     auto substep = [&](const Frags& cur, Frags& nxt, int rp, int rq, int kk, auto load, bool lq, int ls_,
-                       int lstage, int j0) {
+                       int lstage, bool upper) {
 #pragma unroll
       for (int n = 0; n < kMfmas; ++n) {
         mfma(n, cur);
         __builtin_amdgcn_sched_barrier(0);
         reads_behind(n, 0, nxt, rp, rq, kk);
-        if constexpr (decltype(load)::value) loads_behind(n, 0, lq, ls_, lstage, j0);
+        if constexpr (decltype(load)::value) loads_behind(n, 0, lq, ls_, lstage, upper);
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): next fragments in registers
@@ -498,16 +505,16 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
       const int ps2 = qs1 + 1 == kSlots ? 0 : qs1 + 1;
       const std::bool_constant<kNext> l1;
       const std::bool_constant<kNext2> l2;
-      substep(f0, f1, ps, qs, 1, l1, true, qs1, t + 1, kHalf);   // Q of t + 1, second half
-      substep(f1, f0, ps, qs, 2, l2, false, ps2, t + 2, 0);      // P of t + 2, first half
-      substep(f0, f1, ps, qs, 3, l2, false, ps2, t + 2, kHalf);  // P of t + 2, second half
+      substep(f0, f1, ps, qs, 1, l1, true, qs1, t + 1, true);    // Q of t + 1, second half
+      substep(f1, f0, ps, qs, 2, l2, false, ps2, t + 2, false);  // P of t + 2, first half
+      substep(f0, f1, ps, qs, 3, l2, false, ps2, t + 2, true);   // P of t + 2, second half
 #pragma unroll
       for (int n = 0; n < kPre; ++n) mfma(n, f1);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (kNext) {
         // all but P of t + 2 landed for this wave; the barrier publishes stage t + 1 and frees
         // stage t's slots (every wave holds its last fragments)
-        __builtin_amdgcn_s_waitcnt(0x0F70 | (kNext2 ? kLoads : 0));
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (kNext2 ? kLoadsP : 0));
         lds_barrier();
       }
 #pragma unroll
@@ -517,22 +524,22 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
         if constexpr (kNext) {
           reads_behind(n, kPre, f0, ps1, qs1, 0);
           // Q of t + 2 into the freed P slot of t, first half
-          if constexpr (kNext2) loads_behind(n, TS == 256 ? 4 : kPre, true, ps, t + 2, 0);
+          if constexpr (kNext2) loads_behind(n, TN == 256 ? 4 : kPre, true, ps, t + 2, false);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (kNext) __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     };
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) issue_load(false, 0, 0, j);
+    for (int j = 0; j < kLoadsP; ++j) issue_load(false, 0, 0, j);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) issue_load(true, 1, 0, j);
+    for (int j = 0; j < kLoadsQ; ++j) issue_load(true, 1, 0, j);
     if (KT > 1) {
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) issue_load(false, 2, 1, j);
+      for (int j = 0; j < kLoadsP; ++j) issue_load(false, 2, 1, j);
 #pragma unroll
-      for (int j = 0; j < kHalf; ++j) issue_load(true, 3, 1, j);
-      __builtin_amdgcn_s_waitcnt(0x0F70 | (kLoads + kHalf));  // P and Q of stage 0 landed for this wave
+      for (int j = 0; j < kHalfQ; ++j) issue_load(true, 3, 1, j);
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (kLoadsP + kHalfQ));  // P and Q of stage 0 landed for this wave
     } else {
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     }
@@ -573,10 +580,10 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
   };
   if constexpr (kE == FfnEpilogue::kStore) {
 #pragma unroll
-    for (int i = 0; i < kB; ++i) {
+    for (int i = 0; i < kBi; ++i) {
       const int row = row0 + wr + 32 * i + fr;
 #pragma unroll
-      for (int j = 0; j < kB; ++j) {
+      for (int j = 0; j < kBj; ++j) {
         const int block = col0 + wc + 32 * j;
         float x[16];
 #pragma unroll
@@ -597,7 +604,7 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
         }
       }
     }
-  } else if constexpr (kE == FfnEpilogue::kGate && TS == 64) {
+  } else if constexpr (kE == FfnEpilogue::kGate && TM == 64) {
     // waves 0 and 2 hold g of 32 rows each, 1 and 3 the u of the same: they meet through LDS
     __syncthreads();  // every wave's fragment reads are done
     f32x4* meet = reinterpret_cast<f32x4*>(smem) + (wave >> 1) * 256 + lane;
@@ -618,10 +625,10 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     gate_block(row, col0, gv, uv, h);
   } else if constexpr (kE == FfnEpilogue::kGate) {
 #pragma unroll
-    for (int i = 0; i < kB; ++i) {
+    for (int i = 0; i < kBi; ++i) {
       const int row = row0 + wr + 32 * i + fr;
 #pragma unroll
-      for (int j = 0; j < kB / 2; ++j) {
+      for (int j = 0; j < kBj / 2; ++j) {
         const int block = col0 + (wc + 64 * j) / 2;
         if (block >= ldc) continue;  // rows of the buffers are whole groups
         float gv[16], uv[16], h[16];
@@ -635,17 +642,17 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kB; ++i) {
+    for (int i = 0; i < kBi; ++i) {
       const int row = row0 + wr + 32 * i + fr;
       const bool inside = row < M;
 #pragma unroll
-      for (int j = 0; j < kB; ++j) {
+      for (int j = 0; j < kBj; ++j) {
         const int block = col0 + wc + 32 * j;
         const int64_t at = (int64_t)row * ldc + block;
         float gv[16], uv[16], h[16];
-        kept_values<kKeep>(kg[(i * kB + j) % kAhead], gv);
-        kept_values<kKeep>(ku[(i * kB + j) % kAhead], uv);
-        if (i * kB + j + kAhead < kB * kB) load_block(i * kB + j + kAhead);
+        kept_values<kKeep>(kg[(i * kBj + j) % kAhead], gv);
+        kept_values<kKeep>(ku[(i * kBj + j) % kAhead], uv);
+        if (i * kBj + j + kAhead < kBi * kBj) load_block(i * kBj + j + kAhead);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -676,32 +683,38 @@ __global__ __launch_bounds__(kFfnThreads, FfnTile<TS>::kPerCu) void ffn_tile_ker
 
 // ---- host ---------------------------------------------------------------------------
 
+// The tiles' shapes.
+enum FfnShape { kTile256, kTile256x128, kTile128, kTile64, kFfnShapes };
+constexpr int kFfnTileM[kFfnShapes] = {256, 256, 128, 64}, kFfnTileN[kFfnShapes] = {256, 128, 128, 64};
+
 // The forms that the block needs, each in a source file of its own kind:
 // gate: x gate^T and x up^T -> h and what is kept; rows: h down^T -> y; grad: dy down -> h, dg,
 // du; two: dg gate + du up -> dx; weights: dg^T x, du^T x, dy^T h.
-__attribute__((visibility("hidden"))) void ffn_tile_gate(int ts, int dtype, int keep, unsigned grid, hipStream_t s,
+__attribute__((visibility("hidden"))) void ffn_tile_gate(FfnShape shape, int dtype, int keep, unsigned grid, hipStream_t s,
                                                          const FfnTileArgs& a);
-__attribute__((visibility("hidden"))) void ffn_tile_rows(int ts, int dtype, unsigned grid, hipStream_t s,
+__attribute__((visibility("hidden"))) void ffn_tile_rows(FfnShape shape, int dtype, unsigned grid, hipStream_t s,
                                                          const FfnTileArgs& a);
-__attribute__((visibility("hidden"))) void ffn_tile_grad(int ts, int dtype, int keep, unsigned grid, hipStream_t s,
+__attribute__((visibility("hidden"))) void ffn_tile_grad(FfnShape shape, int dtype, int keep, unsigned grid, hipStream_t s,
                                                          const FfnTileArgs& a);
-__attribute__((visibility("hidden"))) void ffn_tile_two(int ts, int dtype, unsigned grid, hipStream_t s,
+__attribute__((visibility("hidden"))) void ffn_tile_two(FfnShape shape, int dtype, unsigned grid, hipStream_t s,
                                                         const FfnTileArgs& a);
-__attribute__((visibility("hidden"))) void ffn_tile_weights(int ts, int dtype, unsigned grid, hipStream_t s,
+__attribute__((visibility("hidden"))) void ffn_tile_weights(FfnShape shape, int dtype, unsigned grid, hipStream_t s,
                                                             const FfnTileArgs& a);
 
 template <bool kPCols, bool kQCols, bool kTwo, FfnEpilogue kE, int kKeep>
-void launch_ffn_tiles(int ts, int dtype, unsigned grid, hipStream_t s, const FfnTileArgs& a) {
+void launch_ffn_tiles(FfnShape shape, int dtype, unsigned grid, hipStream_t s, const FfnTileArgs& a) {
   const dim3 gd(grid), bd(kFfnThreads);
-  if (dtype == MORPH_DTYPE_F16) {
-    if (ts == 256) hipLaunchKernelGGL((ffn_tile_kernel<256, F16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-    else if (ts == 128) hipLaunchKernelGGL((ffn_tile_kernel<128, F16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-    else hipLaunchKernelGGL((ffn_tile_kernel<64, F16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-  } else {
-    if (ts == 256) hipLaunchKernelGGL((ffn_tile_kernel<256, BF16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-    else if (ts == 128) hipLaunchKernelGGL((ffn_tile_kernel<128, BF16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-    else hipLaunchKernelGGL((ffn_tile_kernel<64, BF16, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a);
-  }
+  auto with = [&](auto type) {
+    typedef decltype(type) T;
+    switch (shape) {
+      case kTile256: hipLaunchKernelGGL((ffn_tile_kernel<256, 256, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
+      case kTile256x128: hipLaunchKernelGGL((ffn_tile_kernel<256, 128, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
+      case kTile128: hipLaunchKernelGGL((ffn_tile_kernel<128, 128, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
+      default: hipLaunchKernelGGL((ffn_tile_kernel<64, 64, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
+    }
+  };
+  if (dtype == MORPH_DTYPE_F16) with(F16{});
+  else with(BF16{});
 }
 
 }  // namespace morph
