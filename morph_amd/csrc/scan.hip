@@ -222,39 +222,60 @@ __device__ __forceinline__ int take_tile(const ScanGrid& g, int& group) {
   return id / g.groups;
 }
 
-// What enters the tile (carry) and the (A, S) of its steps before this wave; first: what enters
-// the first tile, read in the first run.  `order`: the wave's place in the direction of the walk.
+// The way of a tile's state through its waves and to the next tile, in two steps with room for
+// work between them: start() publishes the tile's (A, S) as soon as its waves have met, and by
+// finish() the (A, S) of the tiles before have mostly arrived.  `order`: the wave's place in the
+// direction of the walk.
 template <int kVec>
-__device__ __forceinline__ void enter_tile(const ScanGrid& g, int tile, int group, int order, int lane,
-                                           const float (&A)[kVec], const float (&S)[kVec], const float (&first)[kVec],
-                                           float (&wa)[kVec], float (&ws)[kVec], float (&carry)[kVec]) {
-  __shared__ float sa[kWaves][kVec][64], ss[kWaves][kVec][64];
-  __shared__ float pa[kRun][kVec][64], ps[kRun][kVec][64], begin[kVec][64];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) sa[order][k][lane] = A[k], ss[order][k][lane] = S[k];
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) {
-    wa[k] = 1.0f, ws[k] = 0.0f;
-    for (int w = 0; w < order; ++w) {
-      ws[k] = __fmaf_rn(sa[w][k][lane], ws[k], ss[w][k][lane]);
-      wa[k] *= sa[w][k][lane];
-    }
-  }
-  // with this wave's: of the whole tile in the last one
-  float la[kVec], ls[kVec];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) ls[k] = __fmaf_rn(A[k], ws[k], S[k]), la[k] = wa[k] * A[k];
+struct Entering {
+  float wa[kVec], ws[kVec];  // (A, S) of the tile's steps before this wave
+  float la[kVec], ls[kVec];  // with this wave's: of the whole tile in the last one
+  float carry[kVec];         // what enters the tile
 
+  // Adds a wave's (A, S), and with kBack the backward's states' sums T over the same gates, whose
+  // walk is the other way: `state` goes from what enters the tile to what enters the wave.
+  template <bool kBack>
+  __device__ __forceinline__ void start(const ScanGrid& g, int tile, int group, int order, int lane,
+                                        const float (&A)[kVec], const float (&S)[kVec], const float (&T)[kVec],
+                                        float (&state)[kVec]) {
+    __shared__ float sa[kWaves][kVec][64], ss[kWaves][kVec][64], st[kBack ? kWaves : 1][kVec][64];
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) carry[k] = first[k];
-  const int run = tile / kRun, before = tile % kRun;
-  if (g.tiles > 1) {
-    const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
-    if (order == kWaves - 1 && before < kRun - 1 && tile + 1 < g.tiles) {
+    for (int k = 0; k < kVec; ++k) {
+      sa[order][k][lane] = A[k], ss[order][k][lane] = S[k];
+      if constexpr (kBack) st[order][k][lane] = T[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      wa[k] = 1.0f, ws[k] = 0.0f;
+      for (int w = 0; w < order; ++w) {
+        ws[k] = __fmaf_rn(sa[w][k][lane], ws[k], ss[w][k][lane]);
+        wa[k] *= sa[w][k][lane];
+      }
+      ls[k] = __fmaf_rn(A[k], ws[k], S[k]), la[k] = wa[k] * A[k];
+    }
+    const int before = tile % kRun;
+    if (g.tiles > 1 && order == kWaves - 1 && before < kRun - 1 && tile + 1 < g.tiles) {
+      const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
 #pragma unroll
       for (int k = 0; k < kVec; ++k) publish(g.parts + tile * stride + mine + k, la[k], ls[k]);
     }
+    if constexpr (kBack) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+        for (int w = kWaves - 1; w > order; --w) state[k] = __fmaf_rn(sa[w][k][lane], state[k], st[w][k][lane]);
+    }
+  }
+
+  // first: what enters the first tile, read in the first run.
+  __device__ __forceinline__ void finish(const ScanGrid& g, int tile, int group, int order, int lane,
+                                         const float (&first)[kVec]) {
+    __shared__ float pa[kRun][kVec][64], ps[kRun][kVec][64], begin[kVec][64];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) carry[k] = first[k];
+    if (g.tiles == 1) return;
+    const int run = tile / kRun, before = tile % kRun;
+    const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
     float x[kVec], y[kVec];
     if (order < before) {
       fetch<kVec>(g.parts + ((int64_t)run * kRun + order) * stride + mine, x, y);
@@ -280,7 +301,7 @@ __device__ __forceinline__ void enter_tile(const ScanGrid& g, int tile, int grou
       }
     }
   }
-}
+};
 
 // A wave's place: its tile's group, channels and steps.
 template <typename T, int kVec>
@@ -355,16 +376,30 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan
       }
     });
   }
-  float first[kVec], wa[kVec], ws[kVec], carry[kVec];
+  float first[kVec], none[kVec];
 #pragma unroll
   for (int k = 0; k < kVec; ++k) first[k] = tile < kRun && a.s0 ? a.s0[p.b * a.dim + p.c + k] : 0.0f;
-  enter_tile<kVec>(g, tile, group, wave, threadIdx.x & 63, A, S, first, wa, ws, carry);
+  Entering<kVec> e;
+  e.template start<false>(g, tile, group, wave, threadIdx.x & 63, A, S, A, none);
+  float act[kGated ? L : 1][kVec];  // silu(z), while the tiles before publish
+  if constexpr (kGated) {
+    if (p.n > 0) {
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          const float q = value<T, kVec>(z[i], k);
+          act[i][k] = q * gate_sigmoid(q);
+        }
+    }
+  }
+  e.finish(g, tile, group, wave, threadIdx.x & 63, first);
   if (!p.active || p.n <= 0) return;
   if (states && p.t0 % kSpan == 0) {
     const int64_t spans = (a.steps + kSpan - 1) / kSpan;
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
-      states[(p.b * spans + p.t0 / kSpan) * a.dim + p.c + k] = __fmaf_rn(wa[k], carry[k], ws[k]);
+      states[(p.b * spans + p.t0 / kSpan) * a.dim + p.c + k] = __fmaf_rn(e.wa[k], e.carry[k], e.ws[k]);
   }
   const Rows<T, kVec> ry(y, (p.b * a.steps + p.t0) * a.dim + p.channel, a.dim);
   whole_or_part(p.n == L, [&](auto whole) {
@@ -374,11 +409,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan
       float out[kVec];
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
-        s[k] = out[k] = __fmaf_rn(wa[k] * pa[i][k], carry[k], __fmaf_rn(pa[i][k], ws[k], ps[i][k]));
-        if constexpr (kGated) {
-          const float q = value<T, kVec>(z[i], k);
-          out[k] *= q * gate_sigmoid(q);
-        }
+        s[k] = out[k] = __fmaf_rn(e.wa[k] * pa[i][k], e.carry[k], __fmaf_rn(pa[i][k], e.ws[k], ps[i][k]));
+        if constexpr (kGated) out[k] *= act[i][k];
       }
       if (decltype(whole)::value || i < p.n) ry.store(i, p.lane, out);
     }
@@ -455,17 +487,12 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
 #pragma unroll
       for (int k = 0; k < kVec; ++k) R[k] = gate[i][k] * (w[i][k] + R[k]);
   }
-  // the state that enters each wave, from the one kept for the tile
-  {
-    __shared__ float sa[kWaves][kVec][64], ss[kWaves][kVec][64];
+  const int order = kWaves - 1 - wave;
+  float first[kVec];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) sa[wave][k][lane] = A[k], ss[wave][k][lane] = S[k];
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      for (int i = 0; i < wave; ++i) s[k] = __fmaf_rn(sa[i][k][lane], s[k], ss[i][k][lane]);
-    }
-  }
+  for (int k = 0; k < kVec; ++k) first[k] = walked < kRun && dlast ? dlast[p.b * a.dim + p.c + k] : 0.0f;
+  Entering<kVec> e;
+  e.template start<true>(g, walked, group, order, lane, A, R, S, s);
   const int64_t at = (p.b * a.steps + p.t0) * a.dim + p.channel;
   if (p.n > 0) {
     const Rows<T, kVec> oz(dz, at, a.dim);
@@ -485,13 +512,10 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
       }
     });
   }
-  float first[kVec], wa[kVec], wr[kVec], carry[kVec];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) first[k] = walked < kRun && dlast ? dlast[p.b * a.dim + p.c + k] : 0.0f;
-  enter_tile<kVec>(g, walked, group, kWaves - 1 - wave, lane, A, R, first, wa, wr, carry);
+  e.finish(g, walked, group, order, lane, first);
   if (!p.active || p.n <= 0) return;
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) r[k] = __fmaf_rn(wa[k], carry[k], wr[k]);
+  for (int k = 0; k < kVec; ++k) r[k] = __fmaf_rn(e.wa[k], e.carry[k], e.ws[k]);
   const Rows<T, kVec> of(df, at, a.dim), ov(dv, at, a.dim);
   whole_or_part(p.n == L, [&](auto whole) {
 #pragma unroll
