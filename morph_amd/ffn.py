@@ -9,6 +9,7 @@ FP32 and carry the gate in the products' epilogues.
     y = gated_ffn(x, gate, up, down)                              # serving: from one token on
     y, saved = gated_ffn_forward(x, gate, up, down, keep="fp8")   # training
     dx, dgate, dup, ddown = gated_ffn_backward(dy, saved, gate, up, down)
+    y = gated_feed_forward(x, gate, up, down, keep="fp8")         # the same under autograd
 
 The weight gradients have the weights' type and shape, as StageGradients.accumulate takes them.
 GatedFFN is the block as a module whose parameters carry the engine's names (gate.weight, ...).
@@ -192,6 +193,14 @@ class _GatedFFN(torch.autograd.Function):
         return *gated_ffn_backward(dy, ctx.saved, gate, up, down), None
 
 
+def gated_feed_forward(x, gate, up, down, keep="full"):
+    """gated_ffn under autograd: y, differentiable in x and the weights.  keep: as
+    gated_ffn_forward's."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, up, down)):
+        return _GatedFFN.apply(x, gate, up, down, keep)
+    return gated_ffn(x, gate, up, down)
+
+
 class GatedFFN(torch.nn.Module):
     """The block as a module: gate, up and down as bias-free Linear layers, so a state dict has
     gate.weight, up.weight and down.weight.  keep: as gated_ffn_forward's."""
@@ -206,7 +215,4 @@ class GatedFFN(torch.nn.Module):
         self.keep = keep
 
     def forward(self, x):
-        weights = self.gate.weight, self.up.weight, self.down.weight
-        if torch.is_grad_enabled() and (x.requires_grad or any(w.requires_grad for w in weights)):
-            return _GatedFFN.apply(x, *weights, self.keep)
-        return gated_ffn(x, *weights)
+        return gated_feed_forward(x, self.gate.weight, self.up.weight, self.down.weight, self.keep)

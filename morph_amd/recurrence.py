@@ -9,6 +9,7 @@ document begins), +inf passes it on unchanged (padding).  Kernels: csrc/scan.hip
     y, state = gated_scan(f, v, z, state)                  # a prompt, then token by token
     y, state, saved = gated_scan_forward(f, v, z, state)   # training
     df, dv, dz, dstate = gated_scan_backward(dy, saved, dlast)
+    y, state = gated_recurrence(f, v, z, state)            # the same under autograd
 """
 import ctypes
 
@@ -144,4 +145,6 @@ class _GatedScan(torch.autograd.Function):
 
 def gated_recurrence(f, v, z=None, state=None):
     """gated_scan under autograd: (y, last state), differentiable in f, v, z and state."""
-    return _GatedScan.apply(f, v, z, state)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, v, z, state)):
+        return _GatedScan.apply(f, v, z, state)
+    return gated_scan(f, v, z, state)
