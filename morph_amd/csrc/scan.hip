@@ -4,28 +4,32 @@
 // The recurrence of a stretch of steps is s -> A s + S with A the product of its gates and S
 // its result from a zero state, and two stretches compose: (A2, S2) after (A1, S1) is
 // (A2 A1, A2 S1 + S2).  So a workgroup takes a tile of steps and 128 channels, a lane two
-// channels, a wave kSteps consecutive steps, all loaded at once; each wave finds its (A, S) in
+// channels, a wave 16 (backward: 8) consecutive steps, all loaded at once; each wave finds its (A, S) in
 // registers, the waves' are joined through LDS, and the second pass over the registers starts from
-// the true state.  Every tensor is read and written once.
+// the true state.  Every tensor is read and written once.  HBM bounds it: 65536 steps of 3072 channels in
+// BF16 with z take 287 us forward (1.61 GB and 13 MB of states, 5.7 TB/s) and 540 us backward (2.82 GB, 5.3 TB/s).
+// Steps that fit one wave have a tile of one: 64 sequences of 2 to 16 steps of 3072 channels take
+// 7.2 to 8.5 us instead of 13.6 with the seven idle waves.
 //
 // Tiles of one channel group follow each other in time through memory, with the same sums
-// whatever their timing: kRun of them make a run.  A tile publishes its (A, S) before it waits for
-// anything; then it applies the (A, S) of the tiles before it in its run, in order, to the state
-// that the run begins with, which the last tile of the run before published.  (Taking
-// whichever is there, a predecessor's state or its (A, S), would round differently from call to
-// call.)  A published word is 64 bits and tells by itself whether it is there, so no ordering between
+// whatever their timing: kRun tiles make a run, kRuns runs a stretch.  A tile publishes its (A, S)
+// before it waits for anything, the last tile of a run the run's (A, S) as soon as the run's tiles
+// have theirs, the last of a stretch the state behind it.  What enters a tile is the state that its
+// stretch begins with, through the (A, S) of the runs and then of the tiles before it, in order.
+// (Taking whichever is there, a state or an (A, S), would round differently from call to call.)  So
+// only the stretches wait for each other, 0.7 us each time.  Where there are many channel groups a
+// stretch is a single run (kManyGroups).
+// A published word is 64 bits and tells by itself whether it is there, so no ordering between
 // words is needed.  Tiles are taken by ticket, earlier times first: what a tile waits for is always
 // running or done, so every wait ends (kSpins bounds it all the same).
 //
 // The forward applies every step's (A, S) from the tile's beginning to the state that enters
-// the tile, so the state behind a tile's last step is, bit for bit, the one that the next tile
-// begins with: where all gates are 1 the state stays as it is, across waves and tiles.
+// the tile, so the state behind a tile's last step is, bit for bit, the one that the next tile of
+// its run begins with; where all gates are 1 the state stays as it is, however long.
 //
 // The backward runs the tiles from the last to the first: r_t = w_t + a_(t+1) r_(t+1) is the same
 // recurrence in reversed time with the same A, and the states come again from the one that
 // the forward kept for each tile, in the same pass.
-//
-// A lane per channel that walks all steps (scan_walk_kernel) serves single steps.
 #include <type_traits>
 
 #include "layers.h"
@@ -34,7 +38,6 @@ namespace morph {
 namespace {
 
 constexpr int kSpan = MORPH_SCAN_SPAN;
-constexpr int kWalk = 1;  // steps up to which a lane walks them all
 
 template <typename T>
 __device__ __forceinline__ float load1(const void* p, int64_t i) {
@@ -51,75 +54,58 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float x) {
     static_cast<uint16_t*>(p)[i] = (uint16_t)from_float<T>(x);
 }
 
+// A step or none: a lane per channel, no workspace and no wait.  64 sequences of 3072 channels in BF16
+// with z take 3.0 us, 6.2 us with the call; two steps of them in a tile's one wave take 7.2 us.
 template <typename T>
-__global__ __launch_bounds__(64) void scan_walk_kernel(morph_scan a, void* __restrict__ y,
-                                                       float* __restrict__ last,
-                                                       float* __restrict__ states) {
-  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
+__global__ __launch_bounds__(64) void scan_one_kernel(morph_scan a, void* __restrict__ y, float* __restrict__ last,
+                                                      float* __restrict__ states) {
+  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y, at = b * a.dim + c;
   if (c >= a.dim) return;
-  float s = a.s0 ? a.s0[b * a.dim + c] : 0.0f;
-  const int64_t spans = (a.steps + kSpan - 1) / kSpan;
-  for (int64_t t = 0; t < a.steps; ++t) {
-    if (states && t % kSpan == 0) states[(b * spans + t / kSpan) * a.dim + c] = s;
-    const Sigmoid g = sigmoid(load1<T>(a.f, b * a.f_batch + t * a.f_step + c));
-    s = __fmaf_rn(g.a, s, g.b * load1<T>(a.v, b * a.v_batch + t * a.v_step + c));
+  float s = a.s0 ? a.s0[at] : 0.0f;
+  if (a.steps) {
+    if (states) states[at] = s;
+    const Sigmoid g = sigmoid(load1<T>(a.f, b * a.f_batch + c));
+    s = __fmaf_rn(g.a, s, g.b * load1<T>(a.v, b * a.v_batch + c));
     float out = s;
     if (a.z) {
-      const float z = load1<T>(a.z, b * a.z_batch + t * a.z_step + c);
+      const float z = load1<T>(a.z, b * a.z_batch + c);
       out = s * (z * sigmoid(z).a);
     }
-    store1<T>(y, (b * a.steps + t) * a.dim + c, out);
+    store1<T>(y, at, out);
   }
-  if (last) last[b * a.dim + c] = s;
+  if (last) last[at] = s;
 }
 
 template <typename T>
-__global__ __launch_bounds__(64) void scan_walk_back_kernel(morph_scan a, const float* __restrict__ states,
-                                                            const void* __restrict__ dy, int64_t dy_batch,
-                                                            int64_t dy_step, const float* __restrict__ dlast,
-                                                            void* __restrict__ df, void* __restrict__ dv,
-                                                            void* __restrict__ dz, float* __restrict__ ds0) {
-  __shared__ float before[kSpan][64];  // the state before each step of the span, a column per lane
-  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
+__global__ __launch_bounds__(64) void scan_one_back_kernel(morph_scan a, const float* __restrict__ states,
+                                                           const void* __restrict__ dy, int64_t dy_batch,
+                                                           const float* __restrict__ dlast, void* __restrict__ df,
+                                                           void* __restrict__ dv, void* __restrict__ dz,
+                                                           float* __restrict__ ds0) {
+  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y, at = b * a.dim + c;
   if (c >= a.dim) return;
-  const int lane = threadIdx.x;
-  const int64_t spans = (a.steps + kSpan - 1) / kSpan;
-  float r = dlast ? dlast[b * a.dim + c] : 0.0f;  // a_(t+1) r_(t+1)
-  for (int64_t k = spans - 1; k >= 0; --k) {
-    const int64_t t0 = k * kSpan;
-    const int n = (int)(a.steps - t0 < kSpan ? a.steps - t0 : kSpan);
-    float s = states[(b * spans + k) * a.dim + c];
-    for (int i = 0; i < n; ++i) {
-      before[i][lane] = s;
-      const Sigmoid g = sigmoid(load1<T>(a.f, b * a.f_batch + (t0 + i) * a.f_step + c));
-      s = __fmaf_rn(g.a, s, g.b * load1<T>(a.v, b * a.v_batch + (t0 + i) * a.v_step + c));
+  float r = dlast ? dlast[at] : 0.0f;
+  if (a.steps) {
+    const float s = states[at], v = load1<T>(a.v, b * a.v_batch + c);
+    const Sigmoid g = sigmoid(load1<T>(a.f, b * a.f_batch + c));
+    float w = load1<T>(dy, b * dy_batch + c);
+    if (a.z) {
+      const float z = load1<T>(a.z, b * a.z_batch + c);
+      const Sigmoid q = sigmoid(z);
+      store1<T>(dz, at, w * __fmaf_rn(g.a, s, g.b * v) * (q.a * __fmaf_rn(z, q.b, 1.0f)));
+      w *= z * q.a;
     }
-    for (int i = n - 1; i >= 0; --i) {
-      const int64_t t = t0 + i, at = (b * a.steps + t) * a.dim + c;
-      const Sigmoid g = sigmoid(load1<T>(a.f, b * a.f_batch + t * a.f_step + c));
-      const float v = load1<T>(a.v, b * a.v_batch + t * a.v_step + c);
-      float w = load1<T>(dy, b * dy_batch + t * dy_step + c);
-      const float prev = before[i][lane];
-      if (a.z) {
-        const float z = load1<T>(a.z, b * a.z_batch + t * a.z_step + c);
-        const Sigmoid q = sigmoid(z);
-        const float now = __fmaf_rn(g.a, prev, g.b * v);
-        store1<T>(dz, at, w * now * (q.a * __fmaf_rn(z, q.b, 1.0f)));
-        w *= z * q.a;
-      }
-      r += w;
-      store1<T>(dv, at, g.b * r);
-      store1<T>(df, at, r * (prev - v) * (g.a * g.b));
-      r *= g.a;
-    }
+    r += w;
+    store1<T>(dv, at, g.b * r);
+    store1<T>(df, at, r * (s - v) * (g.a * g.b));
+    r *= g.a;
   }
-  if (ds0) ds0[b * a.dim + c] = r;
+  if (ds0) ds0[at] = r;
 }
 
 // ---- tiles ----------------------------------------------------------------------
 
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kWaves = 8;  // of a tile; 1 where one wave has all steps
 constexpr int kForwardSteps = 16;  // of a wave: 128 steps a tile
 constexpr int kBackwardSteps = 8;  // 64: the backward holds four values per step and channel
 constexpr int kSpins = 1 << 20;
@@ -172,11 +158,15 @@ struct Rows {
 struct ScanGrid {
   uint32_t* ticket;  // the workspace: tickets given out, then
   uint64_t* parts;   // [tiles][groups][64 lanes][kVec]: A, S
-  uint64_t* runs;    // [runs][groups][64 lanes][kVec]: the state that run 1, 2, ... begins with, twice
+  uint64_t* runs;    // [runs][groups][64 lanes][kVec]: A, S
+  uint64_t* states;  // [stretches][groups][64 lanes][kVec]: what stretch 1, 2, ... begins with, twice
   int32_t tiles, groups, channel_groups;
+  int32_t in_stretch;  // runs of a stretch: kRuns or 1
 };
-constexpr int kRun = 8;  // tiles: one for each wave to fetch
-static_assert(kRun <= kWaves, "the last wave, which fetches the run's first state, has no tile's words to fetch");
+constexpr int kRun = 8;   // tiles of a run: a word of one for each wave to fetch
+constexpr int kRuns = 8;  // runs of a stretch, likewise
+static_assert(kRun <= kWaves && kRuns <= kWaves,
+              "the last wave, which fetches the stretch's first state, has no tile's or run's words to fetch");
 constexpr uint64_t kNothing = ~uint64_t(0);  // a word that is not published yet
 
 // Two floats as one word.  A pair of NaN that reads as kNothing is no result of arithmetic here
@@ -226,7 +216,7 @@ __device__ __forceinline__ int take_tile(const ScanGrid& g, int& group) {
 // work between them: start() publishes the tile's (A, S) as soon as its waves have met, and by
 // finish() the (A, S) of the tiles before have mostly arrived.  `order`: the wave's place in the
 // direction of the walk.
-template <int kVec>
+template <int kW, int kVec>
 struct Entering {
   float wa[kVec], ws[kVec];  // (A, S) of the tile's steps before this wave
   float la[kVec], ls[kVec];  // with this wave's: of the whole tile in the last one
@@ -238,7 +228,7 @@ struct Entering {
   __device__ __forceinline__ void start(const ScanGrid& g, int tile, int group, int order, int lane,
                                         const float (&A)[kVec], const float (&S)[kVec], const float (&T)[kVec],
                                         float (&state)[kVec]) {
-    __shared__ float sa[kWaves][kVec][64], ss[kWaves][kVec][64], st[kBack ? kWaves : 1][kVec][64];
+    __shared__ float sa[kW][kVec][64], ss[kW][kVec][64], st[kBack ? kW : 1][kVec][64];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
       sa[order][k][lane] = A[k], ss[order][k][lane] = S[k];
@@ -255,7 +245,7 @@ struct Entering {
       ls[k] = __fmaf_rn(A[k], ws[k], S[k]), la[k] = wa[k] * A[k];
     }
     const int before = tile % kRun;
-    if (g.tiles > 1 && order == kWaves - 1 && before < kRun - 1 && tile + 1 < g.tiles) {
+    if (g.tiles > 1 && order == kW - 1 && before < kRun - 1 && tile + 1 < g.tiles) {
       const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
 #pragma unroll
       for (int k = 0; k < kVec; ++k) publish(g.parts + tile * stride + mine + k, la[k], ls[k]);
@@ -263,18 +253,22 @@ struct Entering {
     if constexpr (kBack) {
 #pragma unroll
       for (int k = 0; k < kVec; ++k)
-        for (int w = kWaves - 1; w > order; --w) state[k] = __fmaf_rn(sa[w][k][lane], state[k], st[w][k][lane]);
+        for (int w = kW - 1; w > order; --w) state[k] = __fmaf_rn(sa[w][k][lane], state[k], st[w][k][lane]);
     }
   }
 
-  // first: what enters the first tile, read in the first run.
+  // first: this lane's share of what enters the first tile, read in the first stretch; null: zero.
   __device__ __forceinline__ void finish(const ScanGrid& g, int tile, int group, int order, int lane,
-                                         const float (&first)[kVec]) {
-    __shared__ float pa[kRun][kVec][64], ps[kRun][kVec][64], begin[kVec][64];
+                                         const float* first) {
+    __shared__ float pa[kRun][kVec][64], ps[kRun][kVec][64];    // the run's tiles
+    __shared__ float qa[kRuns][kVec][64], qs[kRuns][kVec][64];  // the stretch's runs
+    __shared__ float begin[kVec][64];
+    if (kW < kWaves || g.tiles == 1) {
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) carry[k] = first[k];
-    if (g.tiles == 1) return;
-    const int run = tile / kRun, before = tile % kRun;
+      for (int k = 0; k < kVec; ++k) carry[k] = first ? first[k] : 0.0f;
+      return;
+    }
+    const int run = tile / kRun, before = tile % kRun, stretch = g.in_stretch > 1 ? run / kRuns : run, earlier = g.in_stretch > 1 ? run % kRuns : 0;
     const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
     float x[kVec], y[kVec];
     if (order < before) {
@@ -282,29 +276,51 @@ struct Entering {
 #pragma unroll
       for (int k = 0; k < kVec; ++k) pa[order][k][lane] = x[k], ps[order][k][lane] = y[k];
     }
-    if (run > 0 && order == kWaves - 1) {
-      fetch<kVec>(g.runs + run * stride + mine, x, y);
+    if (before == kRun - 1 && earlier < g.in_stretch - 1 && tile + 1 < g.tiles) {
+      __syncthreads();
+      if (order == kW - 1) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          float A = 1.0f, S = 0.0f;
+          for (int i = 0; i < before; ++i) S = __fmaf_rn(pa[i][k][lane], S, ps[i][k][lane]), A *= pa[i][k][lane];
+          publish(g.runs + run * stride + mine + k, A * la[k], __fmaf_rn(la[k], S, ls[k]));
+        }
+      }
+    }
+    if (order < earlier) {
+      fetch<kVec>(g.runs + ((int64_t)stretch * kRuns + order) * stride + mine, x, y);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) qa[order][k][lane] = x[k], qs[order][k][lane] = y[k];
+    }
+    if (order == kW - 1) {
+      if (stretch > 0) {
+        fetch<kVec>(g.states + stretch * stride + mine, x, y);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) x[k] = first ? first[k] : 0.0f;
+      }
 #pragma unroll
       for (int k = 0; k < kVec; ++k) begin[k][lane] = x[k];
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      if (run > 0) carry[k] = begin[k][lane];
+      carry[k] = begin[k][lane];
+      for (int i = 0; i < earlier; ++i) carry[k] = __fmaf_rn(qa[i][k][lane], carry[k], qs[i][k][lane]);
       for (int i = 0; i < before; ++i) carry[k] = __fmaf_rn(pa[i][k][lane], carry[k], ps[i][k][lane]);
     }
-    if (order == kWaves - 1 && before == kRun - 1 && tile + 1 < g.tiles) {
+    if (order == kW - 1 && before == kRun - 1 && earlier == g.in_stretch - 1 && tile + 1 < g.tiles) {
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
         const float next = __fmaf_rn(la[k], carry[k], ls[k]);
-        publish(g.runs + (run + 1) * stride + mine + k, next, next);
+        publish(g.states + (stretch + 1) * stride + mine + k, next, next);
       }
     }
   }
 };
 
 // A wave's place: its tile's group, channels and steps.
-template <typename T, int kVec>
+template <typename T, int kW, int kVec>
 struct Place {
   int64_t b, channel, c, t0;  // channel: the group's first; c: the lane's first
   int n;                      // steps, <= 0: none
@@ -318,7 +334,7 @@ struct Place {
     const int own = active ? l * kVec : 0;  // lanes past the end repeat the first and store nothing
     c = channel + own;
     lane = (uint32_t)own * Fmt<T>::bytes;
-    t0 = ((int64_t)tile * kWaves + wave) * L;
+    t0 = ((int64_t)tile * kW + wave) * L;
     n = (int)(a.steps - t0 < L ? a.steps - t0 : L);
   }
 };
@@ -331,8 +347,8 @@ __device__ __forceinline__ void whole_or_part(bool whole, F&& body) {
   else body(std::false_type{});
 }
 
-template <typename T, int kVec, bool kGated, bool kStream>
-__global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan a, const ScanGrid g,
+template <typename T, int kW, int kVec, bool kGated, bool kStream>
+__global__ __launch_bounds__(64 * kW, 4) void scan_tile_kernel(const morph_scan a, const ScanGrid g,
                                                              void* __restrict__ y, float* __restrict__ last,
                                                              float* __restrict__ states) {
   constexpr int L = kForwardSteps;
@@ -340,7 +356,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan
   int group;
   const int tile = take_tile(g, group);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place<T, kVec> p(a, g, tile, group, wave, L);
+  const Place<T, kW, kVec> p(a, g, tile, group, wave, L);
 
   float A[kVec], S[kVec], pa[L][kVec], ps[L][kVec];  // (A, S) from the wave's first step on
   raw z[kGated ? L : 1];
@@ -376,10 +392,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan
       }
     });
   }
-  float first[kVec], none[kVec];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) first[k] = tile < kRun && a.s0 ? a.s0[p.b * a.dim + p.c + k] : 0.0f;
-  Entering<kVec> e;
+  float none[kVec];
+  Entering<kW, kVec> e;
   e.template start<false>(g, tile, group, wave, threadIdx.x & 63, A, S, A, none);
   float act[kGated ? L : 1][kVec];  // silu(z), while the tiles before publish
   if constexpr (kGated) {
@@ -393,7 +407,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan
         }
     }
   }
-  e.finish(g, tile, group, wave, threadIdx.x & 63, first);
+  e.finish(g, tile, group, wave, threadIdx.x & 63, a.s0 ? a.s0 + (p.b * a.dim + p.c) : nullptr);
   if (!p.active || p.n <= 0) return;
   if (states && p.t0 % kSpan == 0) {
     const int64_t spans = (a.steps + kSpan - 1) / kSpan;
@@ -421,8 +435,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(const morph_scan
   });
 }
 
-template <typename T, int kVec, bool kGated, bool kStream>
-__global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph_scan a, const ScanGrid g,
+template <typename T, int kW, int kVec, bool kGated, bool kStream>
+__global__ __launch_bounds__(64 * kW, 4) void scan_tile_back_kernel(const morph_scan a, const ScanGrid g,
                                                                   const float* __restrict__ states,
                                                                   const void* __restrict__ dy, int64_t dy_batch,
                                                                   int64_t dy_step, const float* __restrict__ dlast,
@@ -434,7 +448,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
   const int walked = take_tile(g, group);
   const int tile = g.tiles - 1 - walked;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place<T, kVec> p(a, g, tile, group, wave, L);
+  const Place<T, kW, kVec> p(a, g, tile, group, wave, L);
 
   // gate: a; pass: 1 - a; w: dy silu(z); x: v, then what r is multiplied by for df
   float gate[L][kVec], pass[L][kVec], w[L][kVec], x[L][kVec], slope[kGated ? L : 1][kVec];
@@ -487,11 +501,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
 #pragma unroll
       for (int k = 0; k < kVec; ++k) R[k] = gate[i][k] * (w[i][k] + R[k]);
   }
-  const int order = kWaves - 1 - wave;
-  float first[kVec];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) first[k] = walked < kRun && dlast ? dlast[p.b * a.dim + p.c + k] : 0.0f;
-  Entering<kVec> e;
+  const int order = kW - 1 - wave;
+  Entering<kW, kVec> e;
   e.template start<true>(g, walked, group, order, lane, A, R, S, s);
   const int64_t at = (p.b * a.steps + p.t0) * a.dim + p.channel;
   if (p.n > 0) {
@@ -512,7 +523,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_back_kernel(const morph
       }
     });
   }
-  e.finish(g, walked, group, order, lane, first);
+  e.finish(g, walked, group, order, lane, dlast ? dlast + (p.b * a.dim + p.c) : nullptr);
   if (!p.active || p.n <= 0) return;
 #pragma unroll
   for (int k = 0; k < kVec; ++k) r[k] = __fmaf_rn(e.wa[k], e.carry[k], e.ws[k]);
@@ -571,9 +582,10 @@ int64_t tiles_of(int64_t steps, bool backward) {
   const int64_t span = kWaves * (backward ? kBackwardSteps : kForwardSteps);
   return (steps + span - 1) / span;
 }
-// Words for either channel count per lane, channels rounded up to 128: one a tile, one a run.
+// Words for either channel count per lane, channels rounded up to 128: one a tile, a run and a stretch.
+int64_t runs_of(int64_t tiles) { return (tiles + kRun - 1) / kRun; }
 size_t scan_words(int64_t channels, int64_t tiles) {
-  return (size_t)channels * (size_t)(tiles + (tiles + kRun - 1) / kRun);
+  return (size_t)channels * (size_t)(tiles + 2 * runs_of(tiles));
 }
 size_t scan_workspace(int64_t batch, int64_t steps, int64_t dim, bool backward) {
   const int64_t tiles = tiles_of(steps, backward);
@@ -586,6 +598,12 @@ bool pairs(const void* p, int64_t batch, int64_t step, int64_t size) {
   return p == nullptr || (batch % 2 == 0 && step % 2 == 0 && reinterpret_cast<uintptr_t>(p) % (2 * size) == 0);
 }
 
+// From so many channel groups on a stretch is one run: few of the resident workgroups then belong to one
+// group and wait for each other, and the runs' words cost more than the waits.  Measured, us, stretches of 1 / 8 runs,
+// forward and backward of 65536 steps in BF16 with z: 24 groups 820 / 837, 16 566 / 577, 12 455 / 446,
+// 8 358 / 317; forward of 2 x 30574 x 238 (4 groups) 64 / 43.
+constexpr int64_t kManyGroups = 16;
+
 int scan_grid(const morph_scan* a, int kvec, bool backward, void* workspace, hipStream_t s, ScanGrid& g,
               unsigned& grid) {
   const int64_t groups_c = (a->dim + 64 * kvec - 1) / (64 * kvec), groups = groups_c * a->batch;
@@ -594,6 +612,8 @@ int scan_grid(const morph_scan* a, int kvec, bool backward, void* workspace, hip
   g.ticket = static_cast<uint32_t*>(workspace);
   g.parts = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kTicketBytes);
   g.runs = g.parts + total * 64 * kvec;
+  g.states = g.runs + runs_of(tiles) * groups * 64 * kvec;
+  g.in_stretch = groups < kManyGroups ? kRuns : 1;
   g.tiles = (int32_t)tiles, g.groups = (int32_t)groups, g.channel_groups = (int32_t)groups_c;
   grid = (unsigned)total;
   if (tiles > 1) {
@@ -614,22 +634,23 @@ bool streams(const morph_scan* a, int dtype, bool backward) {
   return a->batch * a->steps * a->dim * tensors * (dtype == MORPH_DTYPE_F32 ? 4 : 2) > (int64_t(256) << 20);
 }
 
-// A call's kernel by its types: F(T, two channels a lane, output gate, streams).
+// A call's kernel by its types: F(T, waves a tile, two channels a lane, output gate, streams).
 template <typename F>
-void by_form(int dtype, bool two, bool gated, bool stream, F&& f) {
-  auto with = [&](auto type, auto past) {
-    if (two && gated) f(type, std::integral_constant<int, 2>{}, std::true_type{}, past);
-    else if (two) f(type, std::integral_constant<int, 2>{}, std::false_type{}, past);
-    else if (gated) f(type, std::integral_constant<int, 1>{}, std::true_type{}, past);
-    else f(type, std::integral_constant<int, 1>{}, std::false_type{}, past);
+void by_form(int dtype, bool one_wave, bool two, bool gated, bool stream, F&& f) {
+  auto with = [&](auto type, auto waves, auto past) {
+    if (two && gated) f(type, waves, std::integral_constant<int, 2>{}, std::true_type{}, past);
+    else if (two) f(type, waves, std::integral_constant<int, 2>{}, std::false_type{}, past);
+    else if (gated) f(type, waves, std::integral_constant<int, 1>{}, std::true_type{}, past);
+    else f(type, waves, std::integral_constant<int, 1>{}, std::false_type{}, past);
   };
-  auto typed = [&](auto past) {
-    if (dtype == MORPH_DTYPE_F32) with(F32{}, past);
-    else if (dtype == MORPH_DTYPE_F16) with(F16{}, past);
-    else with(BF16{}, past);
+  auto typed = [&](auto waves, auto past) {
+    if (dtype == MORPH_DTYPE_F32) with(F32{}, waves, past);
+    else if (dtype == MORPH_DTYPE_F16) with(F16{}, waves, past);
+    else with(BF16{}, waves, past);
   };
-  if (stream) typed(std::true_type{});
-  else typed(std::false_type{});
+  if (one_wave) typed(std::integral_constant<int, 1>{}, std::false_type{});
+  else if (stream) typed(std::integral_constant<int, kWaves>{}, std::true_type{});
+  else typed(std::integral_constant<int, kWaves>{}, std::false_type{});
 }
 
 }  // namespace
@@ -652,10 +673,10 @@ extern "C" int morph_scan_forward(const morph_scan* scan, int dtype, void* y, fl
     return MORPH_EWORKSPACE;
   hipStream_t s = as_stream(stream);
   const morph_scan a = *scan;
-  if (a.steps <= kWalk) {
+  if (a.steps <= 1) {
     const dim3 grid((unsigned)((a.dim + 63) / 64), (unsigned)a.batch);
-    by_form(dtype, false, false, false, [&](auto type, auto, auto, auto) {
-      hipLaunchKernelGGL(scan_walk_kernel<decltype(type)>, grid, dim3(64), 0, s, a, y, last, states);
+    by_form(dtype, true, false, false, false, [&](auto type, auto, auto, auto, auto) {
+      hipLaunchKernelGGL(scan_one_kernel<decltype(type)>, grid, dim3(64), 0, s, a, y, last, states);
     });
     return launch_status();
   }
@@ -666,10 +687,12 @@ extern "C" int morph_scan_forward(const morph_scan* scan, int dtype, void* y, fl
   unsigned grid;
   const int shape = scan_grid(scan, two ? 2 : 1, false, workspace, s, g, grid);
   if (shape != MORPH_OK) return shape;
-  by_form(dtype, two, a.z != nullptr, streams(scan, dtype, false), [&](auto type, auto vec, auto gated, auto past) {
-    hipLaunchKernelGGL((scan_tile_kernel<decltype(type), decltype(vec)::value, decltype(gated)::value, decltype(past)::value>),
-                       dim3(grid), dim3(kThreads), 0, s, a, g, y, last, states);
-  });
+  auto launch = [&](auto type, auto waves, auto vec, auto gated, auto past) {
+    hipLaunchKernelGGL((scan_tile_kernel<decltype(type), decltype(waves)::value, decltype(vec)::value,
+                                         decltype(gated)::value, decltype(past)::value>),
+                       dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, y, last, states);
+  };
+  by_form(dtype, a.steps <= kForwardSteps, two, a.z != nullptr, streams(scan, dtype, false), launch);
   return launch_status();
 }
 
@@ -687,10 +710,10 @@ extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const floa
     return MORPH_EWORKSPACE;
   hipStream_t s = as_stream(stream);
   const morph_scan a = *scan;
-  if (a.steps <= kWalk) {
+  if (a.steps <= 1) {
     const dim3 grid((unsigned)((a.dim + 63) / 64), (unsigned)a.batch);
-    by_form(dtype, false, false, false, [&](auto type, auto, auto, auto) {
-      hipLaunchKernelGGL(scan_walk_back_kernel<decltype(type)>, grid, dim3(64), 0, s, a, states, dy, dy_batch, dy_step,
+    by_form(dtype, true, false, false, false, [&](auto type, auto, auto, auto, auto) {
+      hipLaunchKernelGGL(scan_one_back_kernel<decltype(type)>, grid, dim3(64), 0, s, a, states, dy, dy_batch,
                          dlast, df, dv, dz, ds0);
     });
     return launch_status();
@@ -703,9 +726,11 @@ extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const floa
   unsigned grid;
   const int shape = scan_grid(scan, two ? 2 : 1, true, workspace, s, g, grid);
   if (shape != MORPH_OK) return shape;
-  by_form(dtype, two, a.z != nullptr, streams(scan, dtype, true), [&](auto type, auto vec, auto gated, auto past) {
-    hipLaunchKernelGGL((scan_tile_back_kernel<decltype(type), decltype(vec)::value, decltype(gated)::value, decltype(past)::value>),
-                       dim3(grid), dim3(kThreads), 0, s, a, g, states, dy, dy_batch, dy_step, dlast, df, dv, dz, ds0);
-  });
+  auto launch = [&](auto type, auto waves, auto vec, auto gated, auto past) {
+    hipLaunchKernelGGL((scan_tile_back_kernel<decltype(type), decltype(waves)::value, decltype(vec)::value,
+                                         decltype(gated)::value, decltype(past)::value>),
+                       dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, states, dy, dy_batch, dy_step, dlast, df, dv, dz, ds0);
+  };
+  by_form(dtype, a.steps <= kBackwardSteps, two, a.z != nullptr, streams(scan, dtype, true), launch);
   return launch_status();
 }

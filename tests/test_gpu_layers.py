@@ -427,6 +427,26 @@ def test_scan(dtype, batch, steps, dim, gate, first):
     assert all(a is None or torch.equal(a, b) for a, b in zip(grads, twice))
 
 
+@pytest.mark.parametrize("batch,steps,dim", [(2, 16500, 40), (1, 33000, 3)])
+def test_scan_of_long_memory(batch, steps, dim):
+    """All gates but one in a thousand are 1: a state counts thousands of steps later, with the
+    roundings of a few, across every boundary that the kernels set between steps."""
+    gen = torch.Generator().manual_seed(steps)
+    f, v, z, s0 = _scan_inputs(gen, batch, steps, dim, torch.float32, True, True)
+    f = torch.where(torch.rand(f.shape, generator=gen) < .001, f.clamp(-4, 4), torch.tensor(math.inf))
+    dy, dlast = normal(gen, batch, steps, dim), normal(gen, batch, dim)
+    y, last, _ = R.scan(*_64(f, v, z, s0))
+    got, glast, saved = gated_scan_forward(*_dev(f, v, z, s0))
+    R.assert_scan(got, y, torch.float32, "y")
+    R.assert_scan(glast, last, torch.float32, "last")
+    grads = gated_scan_backward(dy.to(DEV), saved, dlast.to(DEV))
+    ref = R.scan_backward(*_64(f, v, z, s0), dy.double(), dlast.double())
+    for name, a, b in zip(("df", "dv", "dz", "ds0"), grads, ref):
+        R.assert_scan(a, b, torch.float32, name)
+    for a, b in zip(grads, gated_scan_backward(dy.to(DEV), saved, dlast.to(DEV))):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_scan_by_single_steps_equals_the_whole(dtype):
     """Token by token with the state handed on: FP32 states, so the same to their rounding."""
