@@ -154,9 +154,52 @@ bool fits(const Side& s, int64_t width) {
          (width % 8 == 0 || s.padded);
 }
 
+// Parts of K that 64 x 64 tiles of an output M x N of kt stages can be split into, 1, 2, 4 or 8: no more
+// than two workgroups per CU, and four stages, a tile's start, in each.  Measured, us, whole / in parts with
+// the launch that joins them: dx for 7 rows of 2880 x 6144 (8 parts) 70 / 20, for 126 of 1712 x 4096 (8) 41 / 17; a forward of
+// 128 rows of 3072 x 6144 (down in 4) 77 / 61; 512 rows (not split) 105.
+int splits_of(int64_t M, int64_t N, int64_t kt) {
+  const int64_t tiles = ((M + 63) / 64) * ((N + 63) / 64);
+  int n = 1;
+  while (n < 8 && 2 * n * tiles <= 512 && kt >= 8 * n) n *= 2;
+  return n;
+}
+int64_t parts_bytes(int64_t M, int64_t N, int64_t kt) {
+  const int n = splits_of(M, N, kt);
+  return n > 1 ? 4 * n * M * ((N + 63) / 64 * 64) : 0;
+}
+int64_t stages(int64_t K) { return (K + 63) / 64; }
+
+// What the sums of a split product's parts cost over one launch's stores, us.
+double join_us(int splits, int64_t M, int64_t N) { return 4.0 + (double)splits * (double)(M * N) * 8e-6 / 4.0; }
+
+// C [M, N] = the parts' sums, in order.  A thread takes eight columns.
+template <typename T, int kSplits>
+__global__ __launch_bounds__(kThreads) void ffn_join_kernel(const float* __restrict__ parts, int64_t M, int64_t N,
+                                                            int64_t ld, uint16_t* __restrict__ C, int64_t ldc,
+                                                            int vector) {
+  const int64_t row = blockIdx.y, col = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8;
+  if (col >= N) return;
+  f32x4 x[kSplits][2];
+#pragma unroll
+  for (int i = 0; i < kSplits; ++i) {
+    const f32x4* at = reinterpret_cast<const f32x4*>(parts + (i * M + row) * ld + col);
+    x[i][0] = at[0], x[i][1] = at[1];
+  }
+  float sum[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    sum[k] = x[0][k >> 2][k & 3];
+#pragma unroll
+    for (int i = 1; i < kSplits; ++i) sum[k] += x[i][k >> 2][k & 3];
+  }
+  store8(C + row * ldc + col, pack8<T>(sum), N - col, vector != 0);
+}
+
 struct Launch {
   FfnTileArgs a{};
   bool ok = true;
+  Launch() { a.splits = 1; }
   void add(const Side& p, const Side& q, int64_t p_width, int64_t q_width, int64_t M, int64_t N, void* c,
            int64_t ldc) {
     FfnTileProblem& o = a.p[a.count++];
@@ -168,10 +211,11 @@ struct Launch {
     ok = ok && fits(p, p_width) && fits(q, q_width);
   }
   // The tiles' shape for this K, and with it the outputs' tiles; split: 2 where a tile has half as
-  // many output columns (the gate's).
-  FfnShape choose(int64_t K, int split, double epilogue) {
+  // many output columns (the gate's).  parts: memory for the sums of K's parts (parts_bytes), which
+  // 64 x 64 tiles of one output of `kt` stages may then have.
+  FfnShape choose(int64_t K, int split, double epilogue, int64_t kt = 0, void* parts = nullptr) {
     a.K = (int32_t)K;
-    const int64_t kt = (K + 63) / 64;
+    if (kt == 0) kt = stages(K);
     auto tiles = [&](int shape) {
       const int tm = kFfnTileM[shape], tn = kFfnTileN[shape] / split;
       int64_t n = 0;
@@ -189,38 +233,77 @@ struct Launch {
       const double us = tiles_us((FfnShape)i, tiles(i), kt, epilogue);
       if (i == 0 || us < best) shape = i, best = us;
     }
+    if (parts != nullptr) {
+      const int n = splits_of(a.p[0].M, a.p[0].N, kt);
+      if (n > 1 && tiles_us(kTile64, n * tiles(kTile64), (kt + n - 1) / n, epilogue) + join_us(n, a.p[0].M, a.p[0].N) < best)
+        shape = kTile64, a.splits = n, a.parts = static_cast<float*>(parts);
+    }
     const int64_t n = tiles(shape);
     ok = ok && n <= (1 << 30);
     a.total = (int32_t)n;
     return (FfnShape)shape;
   }
   unsigned grid() const { return (unsigned)((a.total + 7) / 8 * 8); }
+  // Behind a launch: the sums of its parts, if it has some.
+  int join(int dtype, hipStream_t s) const {
+    const int status = launch_status();
+    if (status != MORPH_OK || a.splits == 1) return status;
+    const FfnTileProblem& o = a.p[0];
+    const dim3 grid((unsigned)((o.N + 8 * kThreads - 1) / (8 * kThreads)), (unsigned)o.M);
+    auto with = [&](auto type, auto splits) {
+      hipLaunchKernelGGL((ffn_join_kernel<decltype(type), decltype(splits)::value>), grid, dim3(kThreads), 0, s, a.parts,
+                         (int64_t)o.M, (int64_t)o.N, (int64_t)o.tiles_n * 64, o.C, o.ldc, (int)o.vector);
+    };
+    auto typed = [&](auto type) {
+      if (a.splits == 2) with(type, std::integral_constant<int, 2>{});
+      else if (a.splits == 4) with(type, std::integral_constant<int, 4>{});
+      else with(type, std::integral_constant<int, 8>{});
+    };
+    if (dtype == MORPH_DTYPE_F16) typed(F16{});
+    else typed(BF16{});
+    return launch_status();
+  }
 };
 
-// Up to five matrices copied to rows of whole 16-byte chunks, zero behind their width.
+// Up to five matrices copied to rows of whole 16-byte chunks, zero behind their width: a wave
+// per row, so that no thread divides to find its place.  Three weights of 2586 x 5905 (184 MB read and
+// written) in 29 us; a thread per chunk that it loaded value by value took 70.
 struct PadMatrix {
   const uint16_t* src;
   uint16_t* dst;
-  int64_t rows, cols, src_ld, dst_ld, first;  // first: its first chunk of the launch
+  int64_t cols, src_ld, dst_ld, first;  // first: its first row of the launch
 };
 struct PadArgs {
   PadMatrix m[5];
-  int64_t chunks;
+  int64_t rows;
   int32_t count;
 };
 __global__ __launch_bounds__(kThreads) void ffn_pad_kernel(const PadArgs a) {
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (at >= a.chunks) return;
+  const int64_t at = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (at >= a.rows) return;
   int i = 0;
   while (i + 1 < a.count && at >= a.m[i + 1].first) ++i;
   const PadMatrix& m = a.m[i];
-  const int64_t per_row = m.dst_ld / 8, row = (at - m.first) / per_row, c = (at - m.first - row * per_row) * 8;
-  const uint16_t* src = m.src + row * m.src_ld + c;
-  u32x4 v{0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (c + k < m.cols) v[k >> 1] |= (uint32_t)src[k] << (16 * (k & 1));
-  *reinterpret_cast<u32x4*>(m.dst + row * m.dst_ld + c) = v;
+  const int64_t row = at - m.first;
+  const uint16_t* src = m.src + row * m.src_ld;
+  uint16_t* dst = m.dst + row * m.dst_ld;
+  // Whole chunks as they lie behind the 4-byte boundary at or before them (of the row before, or the
+  // same allocation), and their last value.
+  const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 2) * 8;
+  const int64_t whole = m.cols / 8;
+#pragma unroll 4
+  for (int64_t c = threadIdx.x & 63; c < whole; c += 64) {
+    const uint16_t* p = src + 8 * c;
+    const u32x4 w = *reinterpret_cast<const u32x4_any*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+    const uint32_t last = p[7];
+    *reinterpret_cast<u32x4*>(dst + 8 * c) =
+        u32x4{__builtin_amdgcn_alignbit(w.y, w.x, shift), __builtin_amdgcn_alignbit(w.z, w.y, shift),
+              __builtin_amdgcn_alignbit(w.w, w.z, shift), __builtin_amdgcn_alignbit(last, w.w, shift)};
+  }
+  if ((threadIdx.x & 63) < 8) {  // the chunk that is not whole
+    const int64_t k = 8 * whole + (threadIdx.x & 63);
+    dst[k] = k < m.cols ? src[k] : (uint16_t)0;
+  }
 }
 
 int64_t padded_bytes(int64_t rows, int64_t cols) { return rows * ((cols + 7) / 8 * 8) * 2; }
@@ -234,23 +317,25 @@ struct Padding {
   void add(Side& s, int64_t rows, int64_t cols) {
     if (cols % 8 == 0 || rows == 0) return;
     PadMatrix& m = a.m[a.count++];
-    m = PadMatrix{static_cast<const uint16_t*>(s.p), reinterpret_cast<uint16_t*>(room), rows, cols, s.ld,
-                  (cols + 7) / 8 * 8, a.chunks};
-    a.chunks += rows * (m.dst_ld / 8);
+    m = PadMatrix{static_cast<const uint16_t*>(s.p), reinterpret_cast<uint16_t*>(room), cols, s.ld,
+                  (cols + 7) / 8 * 8, a.rows};
+    a.rows += rows;
     room += padded_bytes(rows, cols);
     s = Side{m.dst, m.dst_ld, true};
   }
   int launch(hipStream_t s) {
     if (a.count == 0) return MORPH_OK;
-    const int64_t grid = (a.chunks + kThreads - 1) / kThreads;
+    const int64_t grid = (a.rows + kThreads / 64 - 1) / (kThreads / 64);
     if (grid > 0x7FFFFFFF) return MORPH_ERANGE;
     hipLaunchKernelGGL(ffn_pad_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, a);
     return launch_status();
   }
 };
 
-// Whether a forward takes the few-rows kernels, which read any alignment.
-bool few_rows(int64_t rows, int keep) { return rows <= kFewRows && keep == MORPH_FFN_KEEP_NONE; }
+// Whether a forward's products take the few-rows kernels, which read any alignment (down for 7 rows
+// of 2880 x 6144: 14 us, 64 x 64 tiles 36); the gate's keeps nothing.
+bool few_down(int64_t rows) { return rows <= kFewRows; }
+bool few_gate(int64_t rows, int keep) { return rows <= kFewRows && keep == MORPH_FFN_KEEP_NONE; }
 
 int64_t whole_groups(int64_t n) { return (n + MORPH_ACT_GROUP - 1) / MORPH_ACT_GROUP * MORPH_ACT_GROUP; }
 
@@ -267,7 +352,7 @@ int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int
   const int keep = saved ? saved->keep : MORPH_FFN_KEEP_NONE;
   // The few-rows kernel reads P's fragments from memory for every weight row's: past 32 rows
   // the tiles are faster where they fit (33 to 64 rows of 3072 x 6144: 37 against 26 us).
-  if (few_rows(rows, keep) && (rows <= 32 || !(fits(x, d) && fits(gate, d) && fits(up, d))))
+  if (few_gate(rows, keep) && (rows <= 32 || !(fits(x, d) && fits(gate, d) && fits(up, d))))
     return ffn_few_rows(dtype, true, u16(x), x.ld, u16(gate), gate.ld, u16(up), up.ld, rows, ff, d, h, ld, s);
   Launch l;
   l.add(x, gate, d, d, rows, ff, h, ld);
@@ -290,16 +375,16 @@ int gate_product(int dtype, const Side& x, const Side& gate, const Side& up, int
 
 // y = h down^T.
 int down_product(int dtype, const Side& h, const Side& down, int64_t rows, int64_t d, int64_t ff, void* y,
-                 int64_t y_ld, int keep, hipStream_t s) {
-  if (few_rows(rows, keep))
+                 int64_t y_ld, void* parts, hipStream_t s) {
+  if (few_down(rows))
     return ffn_few_rows(dtype, false, u16(h), h.ld, u16(down), down.ld, nullptr, 0, rows, d, ff,
                         static_cast<uint16_t*>(y), y_ld, s);
   Launch l;
   l.add(h, down, ff, ff, rows, d, y, y_ld);
-  const FfnShape shape = l.choose(ff, 1, 0.0);
+  const FfnShape shape = l.choose(ff, 1, 0.0, stages(ff), parts);
   if (l.ok) {
     ffn_tile_rows(shape, dtype, l.grid(), s, l.a);
-    return launch_status();
+    return l.join(dtype, s);
   }
   FfnProduct p{};
   p.P[0] = along(h), p.Q[0] = along(down);
@@ -328,16 +413,16 @@ int grad_product(int dtype, const Side& dy, const Side& down, int64_t rows, int6
 
 // dx = dg gate + du up.
 int input_product(int dtype, const Side& dg, const Side& du, const Side& gate, const Side& up, int64_t rows,
-                  int64_t d, int64_t ff, void* dx, hipStream_t s) {
+                  int64_t d, int64_t ff, void* dx, void* parts, hipStream_t s) {
   Launch l;
   l.add(dg, gate, ff, d, rows, d, dx, d);
   l.ok = l.ok && fits(up, d) && gate.ld == up.ld;  // one set of offsets for both segments
   FfnTileProblem& o = l.a.p[0];
   o.P[1] = static_cast<const uint16_t*>(du.p), o.Q[1] = static_cast<const uint16_t*>(up.p);
-  const FfnShape shape = l.choose(ff, 1, 0.0);
+  const FfnShape shape = l.choose(ff, 1, 0.0, 2 * stages(ff), parts);
   if (l.ok) {
     ffn_tile_two(shape, dtype, l.grid(), s, l.a);
-    return launch_status();
+    return l.join(dtype, s);
   }
   FfnProduct p{};
   p.P[0] = along(dg), p.Q[0] = across(gate), p.P[1] = along(du), p.Q[1] = across(up);
@@ -412,10 +497,11 @@ extern "C" size_t morph_ffn_workspace_bytes(int64_t rows, int64_t d, int64_t ff,
   size_t bytes = 2 * (size_t)rows * (size_t)whole_groups(ff);  // h
   if (backward) bytes *= 3;                                     // and dg, du
   if (backward && keep == MORPH_FFN_KEEP_ACT8) bytes += 2 * (size_t)rows * (size_t)whole_groups(d);  // x
-  if (backward || !few_rows(rows, keep)) {  // copies of operands of odd widths
-    if (d % 8) bytes += (size_t)(padded_bytes(rows, d) * (backward ? 2 : 1) + 2 * padded_bytes(ff, d));
-    if (ff % 8) bytes += (size_t)padded_bytes(d, ff);
-  }
+  // copies of operands of odd widths
+  if (d % 8 && (backward || !few_gate(rows, keep)))
+    bytes += (size_t)(padded_bytes(rows, d) * (backward ? 2 : 1) + 2 * padded_bytes(ff, d));
+  if (ff % 8 && (backward || !few_down(rows))) bytes += (size_t)padded_bytes(d, ff);
+  if (backward || !few_down(rows)) bytes += (size_t)parts_bytes(rows, d, (backward ? 2 : 1) * stages(ff));
   return bytes;
 }
 
@@ -438,18 +524,18 @@ extern "C" int morph_ffn_forward(const morph_ffn* a, int dtype, const morph_ffn_
   }
   Side x{a->x, a->x_ld, false}, gate{a->gate, a->gate_ld, false}, up{a->up, a->up_ld, false};
   Side down{a->down, a->down_ld, false};
-  if (!few_rows(a->rows, keep)) {
-    Padding pad(h + a->rows * ld);
+  Padding pad(h + a->rows * ld);
+  if (!few_gate(a->rows, keep)) {
     pad.add(x, a->rows, a->d);
     pad.add(gate, a->ff, a->d);
     pad.add(up, a->ff, a->d);
-    pad.add(down, a->d, a->ff);
-    status = pad.launch(s);
-    if (status != MORPH_OK) return status;
   }
+  if (!few_down(a->rows)) pad.add(down, a->d, a->ff);
+  status = pad.launch(s);
+  if (status != MORPH_OK) return status;
   status = gate_product(dtype, x, gate, up, a->rows, a->d, a->ff, saved, h, ld, s);
   if (status != MORPH_OK) return status;
-  return down_product(dtype, Side{h, ld, true}, down, a->rows, a->d, a->ff, y, y_ld, keep, s);
+  return down_product(dtype, Side{h, ld, true}, down, a->rows, a->d, a->ff, y, y_ld, pad.room, s);
 }
 
 extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn_saved* saved,
@@ -472,8 +558,8 @@ extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn
   uint16_t *dg = h + a->rows * ld, *du = dg + a->rows * ld, *xs = du + a->rows * ld;  // xs: what else is needed
   Side x{a->x, a->x_ld, false}, gate{a->gate, a->gate_ld, false}, up{a->up, a->up_ld, false};
   Side down{a->down, a->down_ld, false}, sy{dy, dy_ld, false};
+  Padding pad(xs);
   if (a->rows > 0) {
-    Padding pad(xs);
     if (saved->keep == MORPH_FFN_KEEP_ACT8) {
       x = Side{xs, whole_groups(a->d), true};
       pad.room += 2 * a->rows * x.ld;
@@ -492,7 +578,7 @@ extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn
   const Side sh{h, ld, true}, sg{dg, ld, true}, su{du, ld, true};
   if (a->rows > 0) {
     status = grad_product(dtype, sy, down, a->rows, a->d, a->ff, saved, h, dg, du, ld, s);
-    if (status == MORPH_OK) status = input_product(dtype, sg, su, gate, up, a->rows, a->d, a->ff, dx, s);
+    if (status == MORPH_OK) status = input_product(dtype, sg, su, gate, up, a->rows, a->d, a->ff, dx, pad.room, s);
   }
   if (status == MORPH_OK)
     status = weight_products(dtype, sg, su, x, sy, sh, a->rows, a->d, a->ff, dgate, dup, ddown, s);

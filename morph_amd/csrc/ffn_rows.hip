@@ -23,14 +23,14 @@
 namespace morph {
 namespace {
 
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
 
 // Eight values at p as loaded.  kOdd: the four words from the boundary at or before p (a value
 // more in front, of the row before or the same allocation), and behind them the last value.
 template <bool kOdd>
 struct Eight {
   u32x4 w;
-  __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const u32x4_any*>(p); }
+  __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const u32x4_any2*>(p); }
   __device__ __forceinline__ u32x4 values(uint32_t) const { return w; }
 };
 template <>
@@ -38,7 +38,7 @@ struct Eight<true> {
   u32x4 w;
   uint32_t last;
   __device__ __forceinline__ void load(const uint16_t* p) {
-    w = *reinterpret_cast<const u32x4_any*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+    w = *reinterpret_cast<const u32x4_any2*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
     last = p[7];
   }
   __device__ __forceinline__ u32x4 values(uint32_t shift) const {  // 16 for an odd row, else 0

@@ -54,6 +54,8 @@ struct FfnTileArgs {
   int32_t count;
   int32_t K;         // of each segment
   int32_t total;     // tiles
+  int32_t splits;    // parts of K, of one workgroup each (64 x 64 tiles of one output; else 1)
+  float* parts;      // [splits][M][64 tiles_n]: their sums, where there are several
   uint16_t *dg, *du;
   void *g, *u;
   uint8_t *g_exponents, *u_exponents;
@@ -218,6 +220,8 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
   const int K = __builtin_amdgcn_readfirstlane(g.K);
   const int KS = (K + BK - 1) / BK;         // stages of a segment, >= 1
   const int KT = kTwo ? 2 * KS : KS;        // of the product
+  constexpr bool kParts = TM == 64 && kE == FfnEpilogue::kStore;
+  const int part = kParts ? (int)blockIdx.y : 0;
   const int rest = K - (KS - 1) * BK;       // K in a segment's last stage, 1 .. 64
 
   // One operand's tile: its base, and the descriptor's limits.  "rows": offsets of rows past
@@ -382,7 +386,7 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
   };
 
   // kGateGrad: what was kept of the first blocks is on its way under the last stage's MFMAs, and
-  // kAhead blocks ahead of its use from then on (a wait per block was 70 us of a 4096 x 6144 launch).
+  // kAhead blocks ahead of its use from then on (4096 rows of 3072 x 6144: 278 us, 296 with a wait per block).
   constexpr int kAhead = kE != FfnEpilogue::kGateGrad || TM == 64 ? 1 : kKeep == MORPH_FFN_KEEP_FULL ? 3 : 4;
   [[maybe_unused]] KeptBlock<kKeep> kg[kAhead], ku[kAhead] = {};
   auto load_block = [&](int n) {
@@ -407,14 +411,16 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
     // waits until stage t + 1 has landed, the barrier publishes it and frees stage t's slots, and
     // the reads of t + 1 and the loads of t + 3 run under stage t's MFMAs.
     constexpr int kRing = kSlots / 2, kStageLoads = kLoadsP + kLoadsQ;
+    const int first = kParts ? part * KT / g.splits : 0;  // stage 0 here, of `count`
+    const int count = kParts ? (part + 1) * KT / g.splits - first : KT;
     struct Stage {
       Frags f[4];
     };
     auto load_stage = [&](int slot, int stage) {
 #pragma unroll
-      for (int j = 0; j < kLoadsP; ++j) issue_load(false, 2 * slot, stage, j);
+      for (int j = 0; j < kLoadsP; ++j) issue_load(false, 2 * slot, first + stage, j);
 #pragma unroll
-      for (int j = 0; j < kLoadsQ; ++j) issue_load(true, 2 * slot + 1, stage, j);
+      for (int j = 0; j < kLoadsQ; ++j) issue_load(true, 2 * slot + 1, first + stage, j);
     };
     auto read_stage = [&](Stage& st, int slot) {
 #pragma unroll
@@ -433,11 +439,11 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
     int slot = 0;  // of stage t
     auto step = [&](int t, const Stage& cur, Stage& nxt) {
       const int nslot = slot + 1 == kRing ? 0 : slot + 1;
-      if (t + 1 < KT) {
-        wait_pending(min(kRing - 1, KT - 1 - t) - 1);
+      if (t + 1 < count) {
+        wait_pending(min(kRing - 1, count - 1 - t) - 1);
         lds_barrier();
         read_stage(nxt, nslot);
-        if (t + kRing < KT) load_stage(slot, t + kRing);
+        if (t + kRing < count) load_stage(slot, t + kRing);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -447,17 +453,17 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
     };
 #pragma unroll
     for (int k = 0; k < kRing; ++k)
-      if (k < KT) load_stage(k, k);
-    wait_pending(min(kRing, KT) - 1);
+      if (k < count) load_stage(k, k);
+    wait_pending(min(kRing, count) - 1);
     lds_barrier();
     read_stage(s0, 0);
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-    for (int t = 0; t + 1 < KT; t += 2) {
+    for (int t = 0; t + 1 < count; t += 2) {
       step(t, s0, s1);
       step(t + 1, s1, s0);
     }
     load_ahead();
-    if (KT & 1) step(KT - 1, s0, s1);
+    if (count & 1) step(count - 1, s0, s1);
   } else {
     Frags f0, f1;
     constexpr int kHalfP = kLoadsP / 2, kHalfQ = kLoadsQ / 2;
@@ -588,20 +594,21 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
         float x[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = acc[i][j][r];
+        if (kParts && g.splits > 1) {
+          if (row >= M) continue;
+          float* at = g.parts + ((int64_t)part * M + row) * (o.tiles_n * TN) + block + 4 * fh;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4*>(at + 8 * q) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+          continue;
+        }
         u32x4 w[2];
         row_words<T>(x, w[0], w[1]);
         const int col = block + 16 * fh;
         uint16_t* at = o.C + (int64_t)row * ldc + col;
         if (row >= M) continue;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (o.vector && col + 8 * k + 8 <= N) {
-            *reinterpret_cast<u32x4*>(at + 8 * k) = w[k];
-          } else {
-            for (int e = 0; e < 8; ++e)
-              if (col + 8 * k + e < N) at[8 * k + e] = (uint16_t)(w[k][e >> 1] >> (16 * (e & 1)));
-          }
-        }
+        for (int k = 0; k < 2; ++k) store8(at + 8 * k, w[k], N - col - 8 * k, o.vector != 0);
       }
     }
   } else if constexpr (kE == FfnEpilogue::kGate && TM == 64) {
@@ -710,7 +717,10 @@ void launch_ffn_tiles(FfnShape shape, int dtype, unsigned grid, hipStream_t s, c
       case kTile256: hipLaunchKernelGGL((ffn_tile_kernel<256, 256, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
       case kTile256x128: hipLaunchKernelGGL((ffn_tile_kernel<256, 128, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
       case kTile128: hipLaunchKernelGGL((ffn_tile_kernel<128, 128, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
-      default: hipLaunchKernelGGL((ffn_tile_kernel<64, 64, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
+      default:
+        hipLaunchKernelGGL((ffn_tile_kernel<64, 64, T, kPCols, kQCols, kTwo, kE, kKeep>), dim3(grid, (unsigned)a.splits), bd,
+                           0, s, a);
+        break;
     }
   };
   if (dtype == MORPH_DTYPE_F16) with(F16{});

@@ -186,6 +186,15 @@ def test_ffn_training_step(dtype, rows, d, ff, keep):
 
 
 @pytest.mark.parametrize("keep", ["full", "fp8"])
+@pytest.mark.parametrize("rows,d,ff", [(3, 40, 3001), (70, 72, 2056), (130, 265, 2500), (257, 65, 5001),
+                                       (400, 513, 1027)])
+def test_ffn_wide_middle(rows, d, ff, keep):
+    """ff far above d: sums over ff for few outputs, and results at odd addresses."""
+    test_ffn_forward(torch.bfloat16, rows, d, ff)
+    test_ffn_training_step(torch.bfloat16, rows, d, ff, keep)
+
+
+@pytest.mark.parametrize("keep", ["full", "fp8"])
 @pytest.mark.parametrize("rows,d,ff", [(3, 64, 96), (200, 128, 192)])
 def test_ffn_strides(rows, d, ff, keep):
     """Operands that are views: rows of wider tensors, at odd offsets, transposed, expanded, and
@@ -617,3 +626,54 @@ def test_native_path_under_autograd_keeps_no_graph():
     assert not y.requires_grad and not saved.x.requires_grad
     _, _, kept = gated_scan_forward(x[None], x[None])
     assert not kept.f.requires_grad
+
+
+def test_operators_in_a_graph():
+    """Captured once and replayed, with other inputs in the same places and eager work between:
+    each time what the eager calls give."""
+    gen = torch.Generator().manual_seed(13)
+    rows, d, ff = 130, 72, 2056
+    x, dy = (normal(gen, rows, d, dtype=torch.bfloat16).to(DEV) for _ in range(2))
+    weights = [w.to(DEV) for w in _weights(gen, d, ff, torch.bfloat16)]
+    f, v, z = (normal(gen, 2, 1300, d, mean=m, dtype=torch.bfloat16).to(DEV) for m in (2.0, 0.0, 0.0))
+
+    def step():
+        y, saved = gated_ffn_forward(x, *weights, keep="fp8")
+        out = [y, *gated_ffn_backward(dy, saved, *weights), gated_ffn(x[:5], *weights)]
+        ys, last, kept = gated_scan_forward(f, v, z)
+        out += [ys, last, *gated_scan_backward(ys, kept, last)[:3], *gated_scan(f[:, :1], v[:, :1], z[:, :1], last)]
+        return out + [unpack_activation(pack_activation(dy))]
+
+    step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for k in range(4):
+        for t in (x, dy, f, v, z):
+            t.copy_(normal(gen, *t.shape, dtype=t.dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), k
+
+
+def test_another_stream_is_the_callers():
+    """On a stream of the caller's own the calls, their workspaces and results stay in its order."""
+    gen = torch.Generator().manual_seed(17)
+    x = normal(gen, 300, 64, dtype=torch.bfloat16).to(DEV)
+    weights = [w.to(DEV) for w in _weights(gen, 64, 2048, torch.bfloat16)]
+    f = normal(gen, 1, 4200, 64, dtype=torch.bfloat16).to(DEV)
+    y, (s, last) = gated_ffn(x, *weights), gated_scan(f, f)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            again, (s2, last2) = gated_ffn(x * 1, *weights), gated_scan(f * 1, f * 1)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(y, again) and torch.equal(s, s2) and torch.equal(last, last2)
