@@ -18,16 +18,18 @@ namespace {
 
 constexpr int kGroup = MORPH_ACT_GROUP;
 constexpr int kThreads = 256;
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // Values c .. c + 7 of a row of `cols` (zeros behind its end); wide: the row's address and
-// stride allow 16-byte accesses.
+// stride allow 16-byte accesses.  Others go by words: 11308 x 2763 in BF16, pack and unpack, 39 us (value by
+// value 85), 2762 in FP32 59 (140).
 template <typename T>
 __device__ __forceinline__ void load8(const void* row, int64_t c, int64_t cols, bool wide,
                                       float (&x)[8]) {
   if constexpr (std::is_same_v<T, F32>) {
     const float* p = static_cast<const float*>(row) + c;
-    if (wide && c + 8 <= cols) {
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
+    if (c + 8 <= cols) {
+      const f32x4 lo = *reinterpret_cast<const f32x4_any*>(p), hi = *reinterpret_cast<const f32x4_any*>(p + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[k] = lo[k], x[4 + k] = hi[k];
       return;
@@ -36,8 +38,8 @@ __device__ __forceinline__ void load8(const void* row, int64_t c, int64_t cols, 
     for (int k = 0; k < 8; ++k) x[k] = c + k < cols ? p[k] : 0.0f;
   } else {
     const uint16_t* p = static_cast<const uint16_t*>(row) + c;
-    if (wide && c + 8 <= cols) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+    if (c + 8 <= cols) {
+      const u32x4 v = wide ? *reinterpret_cast<const u32x4*>(p) : load_eight(p);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[2 * k] = to_float<T>(v[k] & 0xFFFFu);
@@ -55,24 +57,18 @@ __device__ __forceinline__ void store8(void* row, int64_t c, int64_t cols, bool 
                                        const float (&x)[8]) {
   if constexpr (std::is_same_v<T, F32>) {
     float* p = static_cast<float*>(row) + c;
-    if (wide && c + 8 <= cols) {
-      *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    if (c + 8 <= cols) {  // any row is a multiple of 4 bytes
+      *reinterpret_cast<f32x4_any*>(p) = f32x4_any{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4_any*>(p + 4) = f32x4_any{x[4], x[5], x[6], x[7]};
       return;
     }
     for (int k = 0; k < 8; ++k)
       if (c + k < cols) p[k] = x[k];
   } else {
-    uint16_t* p = static_cast<uint16_t*>(row) + c;
-    if (wide && c + 8 <= cols) {
-      u32x4 v;
+    u32x4 v;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = from_float<T>(x[2 * k]) | (from_float<T>(x[2 * k + 1]) << 16);
-      *reinterpret_cast<u32x4*>(p) = v;
-      return;
-    }
-    for (int k = 0; k < 8; ++k)
-      if (c + k < cols) p[k] = (uint16_t)from_float<T>(x[k]);
+    for (int k = 0; k < 4; ++k) v[k] = from_float<T>(x[2 * k]) | (from_float<T>(x[2 * k + 1]) << 16);
+    store_eight(static_cast<uint16_t*>(row) + c, v, cols - c, wide);
   }
 }
 

@@ -56,32 +56,6 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
   return u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
 }
 
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t u32x3_any __attribute__((ext_vector_type(3), aligned(4)));
-
-// The first n of eight values to any place; vector: a multiple of 16 bytes.  At 2 mod 4 three
-// stores, the middle one on 4-byte words (the weights' gradients of 3 rows of 2586 x 5905: 57 us, value by
-// value 169).
-__device__ __forceinline__ void store8(uint16_t* at, const u32x4 w, int64_t n, bool vector) {
-  if (n >= 8) {
-    if (vector) {
-      *reinterpret_cast<u32x4*>(at) = w;
-    } else if (reinterpret_cast<uintptr_t>(at) % 4 == 0) {
-      *reinterpret_cast<u32x4_any*>(at) = w;
-    } else {
-      at[0] = (uint16_t)w.x;
-      *reinterpret_cast<u32x3_any*>(at + 1) =
-          u32x3_any{__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16),
-                    __builtin_amdgcn_alignbit(w.w, w.z, 16)};
-      at[7] = (uint16_t)(w.w >> 16);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) at[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-  }
-}
-
 // Keep eight consecutive values at index `at` of a row-major buffer whose rows are whole
 // groups: FP32, or codes and the group's exponent, of which a quad of lanes holds four parts.
 __device__ __forceinline__ void ffn_keep8(int keep, void* buffer, uint8_t* exponents, int64_t at,

@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kThreads) void ffn_join_kernel(const float* __restr
 #pragma unroll
     for (int i = 1; i < kSplits; ++i) sum[k] += x[i][k >> 2][k & 3];
   }
-  store8(C + row * ldc + col, pack8<T>(sum), N - col, vector != 0);
+  store_eight(C + row * ldc + col, pack8<T>(sum), N - col, vector != 0);
 }
 
 struct Launch {
@@ -287,19 +287,9 @@ __global__ __launch_bounds__(kThreads) void ffn_pad_kernel(const PadArgs a) {
   const int64_t row = at - m.first;
   const uint16_t* src = m.src + row * m.src_ld;
   uint16_t* dst = m.dst + row * m.dst_ld;
-  // Whole chunks as they lie behind the 4-byte boundary at or before them (of the row before, or the
-  // same allocation), and their last value.
-  const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 2) * 8;
   const int64_t whole = m.cols / 8;
 #pragma unroll 4
-  for (int64_t c = threadIdx.x & 63; c < whole; c += 64) {
-    const uint16_t* p = src + 8 * c;
-    const u32x4 w = *reinterpret_cast<const u32x4_any*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
-    const uint32_t last = p[7];
-    *reinterpret_cast<u32x4*>(dst + 8 * c) =
-        u32x4{__builtin_amdgcn_alignbit(w.y, w.x, shift), __builtin_amdgcn_alignbit(w.z, w.y, shift),
-              __builtin_amdgcn_alignbit(w.w, w.z, shift), __builtin_amdgcn_alignbit(last, w.w, shift)};
-  }
+  for (int64_t c = threadIdx.x & 63; c < whole; c += 64) *reinterpret_cast<u32x4*>(dst + 8 * c) = load_eight(src + 8 * c);
   if ((threadIdx.x & 63) < 8) {  // the chunk that is not whole
     const int64_t k = 8 * whole + (threadIdx.x & 63);
     dst[k] = k < m.cols ? src[k] : (uint16_t)0;

@@ -608,7 +608,7 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
         uint16_t* at = o.C + (int64_t)row * ldc + col;
         if (row >= M) continue;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) store8(at + 8 * k, w[k], N - col - 8 * k, o.vector != 0);
+        for (int k = 0; k < 2; ++k) store_eight(at + 8 * k, w[k], N - col - 8 * k, o.vector != 0);
       }
     }
   } else if constexpr (kE == FfnEpilogue::kGate && TM == 64) {

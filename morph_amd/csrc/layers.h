@@ -139,4 +139,39 @@ __device__ __forceinline__ GateGrad ffn_gate_grad(float dh, float g, float u) {
   return GateGrad{s.y * u, dh * u * s.slope, dh * s.y};
 }
 
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x3_any __attribute__((ext_vector_type(3), aligned(4)));
+
+// Eight values at any place, as they lie behind the 4-byte boundary at or before them (a value more in front, of
+// the same allocation), and the last of them.
+__device__ __forceinline__ u32x4 load_eight(const uint16_t* p) {
+  const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 2) * 8, last = p[7];
+  const u32x4 w = *reinterpret_cast<const u32x4_any*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+  return u32x4{__builtin_amdgcn_alignbit(w.y, w.x, shift), __builtin_amdgcn_alignbit(w.z, w.y, shift),
+               __builtin_amdgcn_alignbit(w.w, w.z, shift), __builtin_amdgcn_alignbit(last, w.w, shift)};
+}
+
+// The first n of eight values to any place; vector: a multiple of 16 bytes.  At 2 mod 4 three
+// stores, the middle one on 4-byte words (the weights' gradients of 3 rows of 2586 x 5905: 57 us, value by
+// value 169).
+__device__ __forceinline__ void store_eight(uint16_t* at, const u32x4 w, int64_t n, bool vector) {
+  if (n >= 8) {
+    if (vector) {
+      *reinterpret_cast<u32x4*>(at) = w;
+    } else if (reinterpret_cast<uintptr_t>(at) % 4 == 0) {
+      *reinterpret_cast<u32x4_any*>(at) = w;
+    } else {
+      at[0] = (uint16_t)w.x;
+      *reinterpret_cast<u32x3_any*>(at + 1) =
+          u32x3_any{__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16),
+                    __builtin_amdgcn_alignbit(w.w, w.z, 16)};
+      at[7] = (uint16_t)(w.w >> 16);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) at[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
 }  // namespace morph

@@ -677,3 +677,34 @@ def test_another_stream_is_the_callers():
             again, (s2, last2) = gated_ffn(x * 1, *weights), gated_scan(f * 1, f * 1)
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(y, again) and torch.equal(s, s2) and torch.equal(last, last2)
+
+
+def test_offsets_past_32_bits():
+    """Arrays of more than 2^31 values, whose last rows, steps and groups are those of a small call."""
+    rows = 64 * 10990
+    x = torch.empty(rows, 3072, dtype=torch.bfloat16, device=DEV)
+    assert x.numel() > 1 << 31
+    gen = torch.Generator(DEV).manual_seed(19)
+    for part in x.split(1 << 16):
+        part.normal_(generator=gen)
+
+    packed, tail = pack_activation(x), pack_activation(x[-300:])
+    assert torch.equal(packed.codes[-300:], tail.codes) and torch.equal(packed.exponents[-300:], tail.exponents)
+    assert torch.equal(unpack_activation(packed)[-300:], unpack_activation(tail))
+    del packed, tail
+
+    narrow = x.view(-1, 64)[:1 << 21]
+    wide = [(torch.randn(s, generator=gen, device=DEV) / 8).bfloat16() for s in ((1088, 64), (1088, 64), (64, 1088))]
+    assert narrow.shape[0] * 1088 > 1 << 31
+    assert torch.equal(gated_ffn(narrow, *wide)[-512:], gated_ffn(narrow[-(1 << 19):], *wide)[-512:])
+
+    f, state = x[None], torch.randn(1, 3072, generator=gen, device=DEV)
+    y, last, saved = gated_scan_forward(f, f, None, state)
+    grads = gated_scan_backward(f, saved, last)
+    end = f[:, -128:]
+    y2, last2, saved2 = gated_scan_forward(end, end, None, saved.states[:, -2].contiguous())
+    # the same formulas on the same values: FP32 sums in another order, each rounded to a step of 2^-7 at most
+    for a, b in zip((y, *grads[:2]), (y2, *gated_scan_backward(end, saved2, last2)[:2])):
+        a, b = a[:, -128:].float(), b.float()
+        assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 1e-4).all()
+    R.assert_scan(last, last2.double().cpu(), torch.float32, "last")
