@@ -593,10 +593,12 @@ size_t scan_workspace(int64_t batch, int64_t steps, int64_t dim, bool backward) 
   return kTicketBytes + 8 * scan_words(batch * ((dim + 127) / 128 * 128), tiles);
 }
 
-// Whether two channels a lane fit: even rows, and pairs aligned.
-bool pairs(const void* p, int64_t batch, int64_t step, int64_t size) {
-  return p == nullptr || (batch % 2 == 0 && step % 2 == 0 && reinterpret_cast<uintptr_t>(p) % (2 * size) == 0);
+// Whether all of a tensor's rows begin at multiples of `bytes`.
+bool starts(const void* p, int64_t batch, int64_t step, int64_t size, int64_t bytes) {
+  return p == nullptr ||
+         (batch * size % bytes == 0 && step * size % bytes == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0);
 }
+constexpr int64_t kLine = 128;
 
 // From so many channel groups on a stretch is one run: few of the resident workgroups then belong to one
 // group and wait for each other, and the runs' words cost more than the waits.  Measured, us, stretches of 1 / 8 runs,
@@ -628,10 +630,12 @@ int scan_grid(const morph_scan* a, int kvec, bool backward, void* workspace, hip
 // written past the caches loses nothing to whoever comes next.  Measured, us, ordinary / past
 // the caches, BF16 with z: forward and backward of 65536 x 3072 341 / 293 and 632 / 545, of
 // 8 x 4096 x 3072 156 / 150 and 297 / 268; of 4 x 1024 x 3072 (100 and 176 MB, partly in the
-// cache from the kernel before) 31.0 / 31.4 and 45 / 48.
-bool streams(const morph_scan* a, int dtype, bool backward) {
+// cache from the kernel before) 31.0 / 31.4 and 45 / 48.  Not where a channel group's rows end within a cache
+// line, which two groups then share: forward and backward of 20 x 2694 steps, FP16 with z, 2048 channels
+// 528 / 484, 2040 635 / 769, 2032 615 / 648; 7 x 6200 x 2200 in FP32 936 / 1015.
+bool streams(const morph_scan* a, int dtype, bool backward, bool lines) {
   const int64_t tensors = (a->z != nullptr ? 3 : 2) * (backward ? 2 : 1) + 1;
-  return a->batch * a->steps * a->dim * tensors * (dtype == MORPH_DTYPE_F32 ? 4 : 2) > (int64_t(256) << 20);
+  return lines && a->batch * a->steps * a->dim * tensors * (dtype == MORPH_DTYPE_F32 ? 4 : 2) > (int64_t(256) << 20);
 }
 
 // A call's kernel by its types: F(T, waves a tile, two channels a lane, output gate, streams).
@@ -681,8 +685,12 @@ extern "C" int morph_scan_forward(const morph_scan* scan, int dtype, void* y, fl
     return launch_status();
   }
   const int64_t size = dtype == MORPH_DTYPE_F32 ? 4 : 2;
-  const bool two = a.dim % 2 == 0 && pairs(a.f, a.f_batch, a.f_step, size) && pairs(a.v, a.v_batch, a.v_step, size) &&
-                   pairs(a.z, a.z_batch, a.z_step, size) && pairs(y, 0, 0, size);
+  auto all = [&](int64_t bytes) {
+    return a.dim * size % bytes == 0 && starts(a.f, a.f_batch, a.f_step, size, bytes) &&
+           starts(a.v, a.v_batch, a.v_step, size, bytes) && starts(a.z, a.z_batch, a.z_step, size, bytes) &&
+           starts(y, 0, 0, size, bytes);
+  };
+  const bool two = all(2 * size);  // channels a lane
   ScanGrid g;
   unsigned grid;
   const int shape = scan_grid(scan, two ? 2 : 1, false, workspace, s, g, grid);
@@ -692,7 +700,7 @@ extern "C" int morph_scan_forward(const morph_scan* scan, int dtype, void* y, fl
                                          decltype(gated)::value, decltype(past)::value>),
                        dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, y, last, states);
   };
-  by_form(dtype, a.steps <= kForwardSteps, two, a.z != nullptr, streams(scan, dtype, false), launch);
+  by_form(dtype, a.steps <= kForwardSteps, two, a.z != nullptr, streams(scan, dtype, false, all(kLine)), launch);
   return launch_status();
 }
 
@@ -719,9 +727,13 @@ extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const floa
     return launch_status();
   }
   const int64_t size = dtype == MORPH_DTYPE_F32 ? 4 : 2;
-  const bool two = a.dim % 2 == 0 && pairs(a.f, a.f_batch, a.f_step, size) && pairs(a.v, a.v_batch, a.v_step, size) &&
-                   pairs(a.z, a.z_batch, a.z_step, size) && pairs(dy, dy_batch, dy_step, size) &&
-                   pairs(df, 0, 0, size) && pairs(dv, 0, 0, size) && pairs(dz, 0, 0, size);
+  auto all = [&](int64_t bytes) {
+    return a.dim * size % bytes == 0 && starts(a.f, a.f_batch, a.f_step, size, bytes) &&
+           starts(a.v, a.v_batch, a.v_step, size, bytes) && starts(a.z, a.z_batch, a.z_step, size, bytes) &&
+           starts(dy, dy_batch, dy_step, size, bytes) && starts(df, 0, 0, size, bytes) &&
+           starts(dv, 0, 0, size, bytes) && starts(dz, 0, 0, size, bytes);
+  };
+  const bool two = all(2 * size);  // channels a lane
   ScanGrid g;
   unsigned grid;
   const int shape = scan_grid(scan, two ? 2 : 1, true, workspace, s, g, grid);
@@ -731,6 +743,6 @@ extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const floa
                                          decltype(gated)::value, decltype(past)::value>),
                        dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, states, dy, dy_batch, dy_step, dlast, df, dv, dz, ds0);
   };
-  by_form(dtype, a.steps <= kBackwardSteps, two, a.z != nullptr, streams(scan, dtype, true), launch);
+  by_form(dtype, a.steps <= kBackwardSteps, two, a.z != nullptr, streams(scan, dtype, true, all(kLine)), launch);
   return launch_status();
 }
