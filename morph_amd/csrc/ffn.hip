@@ -154,31 +154,32 @@ bool fits(const Side& s, int64_t width) {
          (width % 8 == 0 || s.padded);
 }
 
-// Parts of K that 64 x 64 tiles of an output M x N of kt stages can be split into, 1, 2, 4 or 8: no more
-// than two workgroups per CU, and four stages, a tile's start, in each.  Measured, us, whole / in parts with
-// the launch that joins them: dx for 7 rows of 2880 x 6144 (8 parts) 70 / 20, for 126 of 1712 x 4096 (8) 41 / 17; a forward of
-// 128 rows of 3072 x 6144 (down in 4) 77 / 61; 512 rows (not split) 105.
-int splits_of(int64_t M, int64_t N, int64_t kt) {
-  const int64_t tiles = ((M + 63) / 64) * ((N + 63) / 64);
+// The most parts of K that tiles of `edge` of an output M x N of kt stages are split into: no more than two
+// workgroups per CU, and eight stages, twice a tile's start, in each.  Measured, us, whole in the best tiles / in
+// parts with the launch that joins them, as choose() takes them: forward of 100 rows of 3072 x 6144 72 / 53 (128 x 128,
+// 8 parts), 256 84 / 75 (128, 4), 512 104 / 94 (128, 4), 1024 146 / 138 (128, 2), 256 rows of 640 x 2336 24 / 21 (64, 4),
+// dx of 7 rows of 2880 x 6144 70 / 20 (64, 8); left whole: 1413 rows of 1408 x 5528 108 / 117, 2048 of 512 x 2048, forward
+// and backward, 103 / 105.
+int splits_of(int64_t edge, int64_t M, int64_t N, int64_t kt) {
+  const int64_t tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
   int n = 1;
-  while (n < 8 && 2 * n * tiles <= 512 && kt >= 8 * n) n *= 2;
+  while (n < 8 && 2 * n * tiles <= 512 && kt >= 16 * n) n *= 2;
   return n;
 }
 int64_t parts_bytes(int64_t M, int64_t N, int64_t kt) {
-  const int n = splits_of(M, N, kt);
-  return n > 1 ? 4 * n * M * ((N + 63) / 64 * 64) : 0;
+  const int n = std::max(splits_of(64, M, N, kt), splits_of(128, M, N, kt));
+  return n > 1 ? 4 * n * M * ((N + 127) / 128 * 128) : 0;
 }
 int64_t stages(int64_t K) { return (K + 63) / 64; }
 
 // What the sums of a split product's parts cost over one launch's stores, us.
-double join_us(int splits, int64_t M, int64_t N) { return 4.0 + (double)splits * (double)(M * N) * 8e-6 / 4.0; }
+double join_us(int splits, int64_t M, int64_t N) { return 4.0 + (double)splits * (double)(M * N) * 5e-7; }
 
 // C [M, N] = the parts' sums, in order.  A thread takes eight columns.
 template <typename T, int kSplits>
-__global__ __launch_bounds__(kThreads) void ffn_join_kernel(const float* __restrict__ parts, int64_t M, int64_t N,
-                                                            int64_t ld, uint16_t* __restrict__ C, int64_t ldc,
-                                                            int vector) {
-  const int64_t row = blockIdx.y, col = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8;
+__global__ __launch_bounds__(64) void ffn_join_kernel(const float* __restrict__ parts, int64_t M, int64_t N,
+                                                      int64_t ld, uint16_t* __restrict__ C, int64_t ldc, int vector) {
+  const int64_t row = blockIdx.y, col = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 8;
   if (col >= N) return;
   f32x4 x[kSplits][2];
 #pragma unroll
@@ -212,7 +213,7 @@ struct Launch {
   }
   // The tiles' shape for this K, and with it the outputs' tiles; split: 2 where a tile has half as
   // many output columns (the gate's).  parts: memory for the sums of K's parts (parts_bytes), which
-  // 64 x 64 tiles of one output of `kt` stages may then have.
+  // small tiles of one output of `kt` stages may then have.
   FfnShape choose(int64_t K, int split, double epilogue, int64_t kt = 0, void* parts = nullptr) {
     a.K = (int32_t)K;
     if (kt == 0) kt = stages(K);
@@ -233,11 +234,15 @@ struct Launch {
       const double us = tiles_us((FfnShape)i, tiles(i), kt, epilogue);
       if (i == 0 || us < best) shape = i, best = us;
     }
-    if (parts != nullptr) {
-      const int n = splits_of(a.p[0].M, a.p[0].N, kt);
-      if (n > 1 && tiles_us(kTile64, n * tiles(kTile64), (kt + n - 1) / n, epilogue) + join_us(n, a.p[0].M, a.p[0].N) < best)
-        shape = kTile64, a.splits = n, a.parts = static_cast<float*>(parts);
+    const double whole = best;
+    for (int i = kTile128; parts != nullptr && i <= kTile64; ++i) {
+      const int most = splits_of(kFfnTileM[i], a.p[0].M, a.p[0].N, kt);
+      for (int n = 2; n <= most; n *= 2) {
+        const double us = tiles_us((FfnShape)i, n * tiles(i), (kt + n - 1) / n, epilogue) + join_us(n, a.p[0].M, a.p[0].N);
+        if (us < 0.95 * whole && us < best) shape = i, best = us, a.splits = n;
+      }
     }
+    if (a.splits > 1) a.parts = static_cast<float*>(parts);
     const int64_t n = tiles(shape);
     ok = ok && n <= (1 << 30);
     a.total = (int32_t)n;
@@ -245,14 +250,15 @@ struct Launch {
   }
   unsigned grid() const { return (unsigned)((a.total + 7) / 8 * 8); }
   // Behind a launch: the sums of its parts, if it has some.
-  int join(int dtype, hipStream_t s) const {
+  int join(FfnShape shape, int dtype, hipStream_t s) const {
     const int status = launch_status();
     if (status != MORPH_OK || a.splits == 1) return status;
     const FfnTileProblem& o = a.p[0];
-    const dim3 grid((unsigned)((o.N + 8 * kThreads - 1) / (8 * kThreads)), (unsigned)o.M);
+    const int tile_n = kFfnTileN[shape];
+    const dim3 grid((unsigned)((o.N + 511) / 512), (unsigned)o.M);
     auto with = [&](auto type, auto splits) {
-      hipLaunchKernelGGL((ffn_join_kernel<decltype(type), decltype(splits)::value>), grid, dim3(kThreads), 0, s, a.parts,
-                         (int64_t)o.M, (int64_t)o.N, (int64_t)o.tiles_n * 64, o.C, o.ldc, (int)o.vector);
+      hipLaunchKernelGGL((ffn_join_kernel<decltype(type), decltype(splits)::value>), grid, dim3(64), 0, s, a.parts,
+                         (int64_t)o.M, (int64_t)o.N, (int64_t)o.tiles_n * tile_n, o.C, o.ldc, (int)o.vector);
     };
     auto typed = [&](auto type) {
       if (a.splits == 2) with(type, std::integral_constant<int, 2>{});
@@ -374,7 +380,7 @@ int down_product(int dtype, const Side& h, const Side& down, int64_t rows, int64
   const FfnShape shape = l.choose(ff, 1, 0.0, stages(ff), parts);
   if (l.ok) {
     ffn_tile_rows(shape, dtype, l.grid(), s, l.a);
-    return l.join(dtype, s);
+    return l.join(shape, dtype, s);
   }
   FfnProduct p{};
   p.P[0] = along(h), p.Q[0] = along(down);
@@ -412,7 +418,7 @@ int input_product(int dtype, const Side& dg, const Side& du, const Side& gate, c
   const FfnShape shape = l.choose(ff, 1, 0.0, 2 * stages(ff), parts);
   if (l.ok) {
     ffn_tile_two(shape, dtype, l.grid(), s, l.a);
-    return l.join(dtype, s);
+    return l.join(shape, dtype, s);
   }
   FfnProduct p{};
   p.P[0] = along(dg), p.Q[0] = across(gate), p.P[1] = along(du), p.Q[1] = across(up);

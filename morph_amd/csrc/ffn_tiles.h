@@ -14,6 +14,9 @@
 // two stages ahead, two register sets of fragments; one barrier per stage.  Every 16-byte
 // chunk of an LDS row is stored XOR-swizzled, chosen by which chunk each lane fetches.
 //
+// Few tiles.  Where an output has fewer tiles than the chip has room for, workgroups of the small shapes take parts
+// of K, and their FP32 sums are joined in order by a launch of their own (ffn.hip).
+//
 // Ragged sizes.  Every load goes through a buffer descriptor that ends with the operand, and
 // the hardware gives zeros beyond it: rows past M or N, and for a "cols" operand the rows past K.
 // A "rows" operand's chunks past K lie inside the buffer (in the next row), so in the last stage
@@ -54,8 +57,8 @@ struct FfnTileArgs {
   int32_t count;
   int32_t K;         // of each segment
   int32_t total;     // tiles
-  int32_t splits;    // parts of K, of one workgroup each (64 x 64 tiles of one output; else 1)
-  float* parts;      // [splits][M][64 tiles_n]: their sums, where there are several
+  int32_t splits;    // parts of K, of one workgroup each (small tiles of one output; else 1)
+  float* parts;      // [splits][M][tiles_n tiles' columns]: their sums, where there are several
   uint16_t *dg, *du;
   void *g, *u;
   uint8_t *g_exponents, *u_exponents;
@@ -220,8 +223,10 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
   const int K = __builtin_amdgcn_readfirstlane(g.K);
   const int KS = (K + BK - 1) / BK;         // stages of a segment, >= 1
   const int KT = kTwo ? 2 * KS : KS;        // of the product
-  constexpr bool kParts = TM == 64 && kE == FfnEpilogue::kStore;
+  constexpr bool kParts = TM <= 128 && kE == FfnEpilogue::kStore;
   const int part = kParts ? (int)blockIdx.y : 0;
+  const int first = kParts ? part * KT / g.splits : 0;  // the part's first stage, and how many
+  const int count = kParts ? (part + 1) * KT / g.splits - first : KT;
   const int rest = K - (KS - 1) * BK;       // K in a segment's last stage, 1 .. 64
 
   // One operand's tile: its base, and the descriptor's limits.  "rows": offsets of rows past
@@ -297,7 +302,8 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
   }
   // With a "cols" operand the load is inline assembly: the compiler then adds no waits of its
   // own before the transposing reads.  Completion is managed by the vmcnt waits below.
-  auto issue_load = [&](bool q, int slot, int stage, int j) {
+  auto issue_load = [&](bool q, int slot, int at, int j) {
+    const int stage = first + at;
     const bool second = kTwo && stage >= KS;
     const int s = second ? stage - KS : stage;
     const bool last = s == KS - 1;
@@ -411,16 +417,14 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
     // waits until stage t + 1 has landed, the barrier publishes it and frees stage t's slots, and
     // the reads of t + 1 and the loads of t + 3 run under stage t's MFMAs.
     constexpr int kRing = kSlots / 2, kStageLoads = kLoadsP + kLoadsQ;
-    const int first = kParts ? part * KT / g.splits : 0;  // stage 0 here, of `count`
-    const int count = kParts ? (part + 1) * KT / g.splits - first : KT;
     struct Stage {
       Frags f[4];
     };
     auto load_stage = [&](int slot, int stage) {
 #pragma unroll
-      for (int j = 0; j < kLoadsP; ++j) issue_load(false, 2 * slot, first + stage, j);
+      for (int j = 0; j < kLoadsP; ++j) issue_load(false, 2 * slot, stage, j);
 #pragma unroll
-      for (int j = 0; j < kLoadsQ; ++j) issue_load(true, 2 * slot + 1, first + stage, j);
+      for (int j = 0; j < kLoadsQ; ++j) issue_load(true, 2 * slot + 1, stage, j);
     };
     auto read_stage = [&](Stage& st, int slot) {
 #pragma unroll
@@ -540,7 +544,7 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
     for (int j = 0; j < kLoadsP; ++j) issue_load(false, 0, 0, j);
 #pragma unroll
     for (int j = 0; j < kLoadsQ; ++j) issue_load(true, 1, 0, j);
-    if (KT > 1) {
+    if (count > 1) {
 #pragma unroll
       for (int j = 0; j < kLoadsP; ++j) issue_load(false, 2, 1, j);
 #pragma unroll
@@ -555,16 +559,16 @@ __global__ __launch_bounds__(kFfnThreads, (FfnTile<TM, TN>::kPerCu)) void ffn_ti
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     int ps = 0;
     auto advance = [&]() { ps = ps + 2 >= kSlots ? ps + 2 - kSlots : ps + 2; };
-    for (int t = 0; t + 2 < KT; ++t) {
+    for (int t = 0; t + 2 < count; ++t) {
       step(t, ps, std::integral_constant<int, 0>{});
       advance();
     }
-    if (KT > 1) {
-      step(KT - 2, ps, std::integral_constant<int, 1>{});
+    if (count > 1) {
+      step(count - 2, ps, std::integral_constant<int, 1>{});
       advance();
     }
     load_ahead();
-    step(KT - 1, ps, std::integral_constant<int, 2>{});
+    step(count - 1, ps, std::integral_constant<int, 2>{});
   }
 
   // ---- epilogue: straight from the registers ------------------------------------
@@ -710,17 +714,14 @@ __attribute__((visibility("hidden"))) void ffn_tile_weights(FfnShape shape, int 
 
 template <bool kPCols, bool kQCols, bool kTwo, FfnEpilogue kE, int kKeep>
 void launch_ffn_tiles(FfnShape shape, int dtype, unsigned grid, hipStream_t s, const FfnTileArgs& a) {
-  const dim3 gd(grid), bd(kFfnThreads);
+  const dim3 gd(grid, (unsigned)a.splits), bd(kFfnThreads);
   auto with = [&](auto type) {
     typedef decltype(type) T;
     switch (shape) {
       case kTile256: hipLaunchKernelGGL((ffn_tile_kernel<256, 256, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
       case kTile256x128: hipLaunchKernelGGL((ffn_tile_kernel<256, 128, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
       case kTile128: hipLaunchKernelGGL((ffn_tile_kernel<128, 128, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
-      default:
-        hipLaunchKernelGGL((ffn_tile_kernel<64, 64, T, kPCols, kQCols, kTwo, kE, kKeep>), dim3(grid, (unsigned)a.splits), bd,
-                           0, s, a);
-        break;
+      default: hipLaunchKernelGGL((ffn_tile_kernel<64, 64, T, kPCols, kQCols, kTwo, kE, kKeep>), gd, bd, 0, s, a); break;
     }
   };
   if (dtype == MORPH_DTYPE_F16) with(F16{});

@@ -194,6 +194,12 @@ def test_ffn_wide_middle(rows, d, ff, keep):
     test_ffn_training_step(torch.bfloat16, rows, d, ff, keep)
 
 
+@pytest.mark.parametrize("rows,d,ff", [(100, 1536, 3000), (390, 1001, 4100)])
+def test_ffn_some_hundred_rows(rows, d, ff):
+    test_ffn_forward(torch.float16, rows, d, ff)
+    test_ffn_training_step(torch.float16, rows, d, ff, "full")
+
+
 @pytest.mark.parametrize("keep", ["full", "fp8"])
 @pytest.mark.parametrize("rows,d,ff", [(3, 64, 96), (200, 128, 192)])
 def test_ffn_strides(rows, d, ff, keep):
