@@ -202,8 +202,8 @@ extern "C" int morph_act_pack(const void* src, int dtype, int64_t rows, int64_t 
   const int status = act_shape(src, dtype, rows, cols, ld, codes, exponents, groups, total, grid, per, wide);
   if (status != MORPH_OK || grid == 0) return status;
   by_type(dtype, ld == cols && cols % kGroup == 0, per, [&](auto type, auto flat, auto count) {
-    hipLaunchKernelGGL((act_pack_kernel<decltype(type), decltype(flat)::value, decltype(count)::value>), dim3((unsigned)grid), dim3(kThreads),
-                       0, as_stream(stream), src, cols, ld, codes, exponents, groups, total, wide);
+    hipLaunchKernelGGL((act_pack_kernel<decltype(type), decltype(flat)::value, decltype(count)::value>),
+                       dim3((unsigned)grid), dim3(kThreads), 0, as_stream(stream), src, cols, ld, codes, exponents, groups, total, wide);
   });
   return launch_status();
 }
@@ -216,8 +216,8 @@ extern "C" int morph_act_unpack(const uint8_t* codes, const uint8_t* exponents, 
   const int status = act_shape(dst, dtype, rows, cols, ld, codes, exponents, groups, total, grid, per, wide);
   if (status != MORPH_OK || grid == 0) return status;
   by_type(dtype, ld == cols && cols % kGroup == 0, per, [&](auto type, auto flat, auto count) {
-    hipLaunchKernelGGL((act_unpack_kernel<decltype(type), decltype(flat)::value, decltype(count)::value>), dim3((unsigned)grid),
-                       dim3(kThreads), 0, as_stream(stream), codes, exponents, cols, dst, ld, groups, total, wide);
+    hipLaunchKernelGGL((act_unpack_kernel<decltype(type), decltype(flat)::value, decltype(count)::value>),
+                       dim3((unsigned)grid), dim3(kThreads), 0, as_stream(stream), codes, exponents, cols, dst, ld, groups, total, wide);
   });
   return launch_status();
 }

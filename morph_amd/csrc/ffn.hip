@@ -10,8 +10,9 @@
 //
 // The tiles of ffn_tiles.h take operands whose rows are 16-byte aligned and a multiple of 8
 // values long; operands of other widths are copied to such rows first (ffn_pad_kernel: a
-// read and a write of them beside the product's many reads).  ffn_any_kernel takes operands of any stride and alignment, any size: 64 x 64
-// tiles through LDS, loaded element by element along whichever index is contiguous.
+// read and a write of them beside the product's many reads).  ffn_any_kernel takes operands of any stride
+// and alignment, any size: 64 x 64 tiles through LDS, loaded element by element along whichever index is
+// contiguous.
 #include <algorithm>
 #include <cmath>
 

@@ -179,7 +179,8 @@ void launch_few(const uint16_t* P, int64_t ldp, const uint16_t* Q0, int64_t ldq0
     hipLaunchKernelGGL((ffn_few_rows_kernel<T, kGated, kTiles, kWaves, kBlocks, kRows, true>), grid, block, 0, s,
                        P, ldp, Q0, ldq0, Q1, ldq1, M, N, K, C, ldc);
   else
-    hipLaunchKernelGGL((ffn_few_rows_kernel<T, kGated, kTiles, kWaves, kBlocks, kRows, false>), grid, block, 0, s, P, ldp, Q0, ldq0, Q1, ldq1, M, N, K, C, ldc);
+    hipLaunchKernelGGL((ffn_few_rows_kernel<T, kGated, kTiles, kWaves, kBlocks, kRows, false>), grid, block, 0, s,
+                       P, ldp, Q0, ldq0, Q1, ldq1, M, N, K, C, ldc);
 }
 
 template <typename T, bool kGated, typename... Args>

@@ -9,8 +9,8 @@
 //
 // Tiling and pipeline are the Newton-Schulz products' (gemm.hip, where the constants were
 // measured): a tile of 256 x 256 (or 256 x 128, or 128 x 128 with two workgroups per CU, or 64 x 64,
-// three with a pipeline of whole stages, where those fill the chip better), four waves with a quarter each as 32 x 32 x 16 MFMAs, K in stages of 64, a
-// ring of five LDS slots that hold the P or the Q of one stage, filled by direct loads
+// three with a pipeline of whole stages, where those fill the chip better), four waves with a quarter each
+// as 32 x 32 x 16 MFMAs, K in stages of 64, a ring of five LDS slots that hold the P or the Q of one stage, filled by direct loads
 // two stages ahead, two register sets of fragments; one barrier per stage.  Every 16-byte
 // chunk of an LDS row is stored XOR-swizzled, chosen by which chunk each lane fetches.
 //

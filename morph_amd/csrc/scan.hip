@@ -268,7 +268,8 @@ struct Entering {
       for (int k = 0; k < kVec; ++k) carry[k] = first ? first[k] : 0.0f;
       return;
     }
-    const int run = tile / kRun, before = tile % kRun, stretch = g.in_stretch > 1 ? run / kRuns : run, earlier = g.in_stretch > 1 ? run % kRuns : 0;
+    const int run = tile / kRun, before = tile % kRun;
+    const int stretch = g.in_stretch > 1 ? run / kRuns : run, earlier = g.in_stretch > 1 ? run % kRuns : 0;
     const int64_t mine = ((int64_t)group * 64 + lane) * kVec, stride = (int64_t)g.groups * 64 * kVec;
     float x[kVec], y[kVec];
     if (order < before) {
@@ -741,7 +742,8 @@ extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const floa
   auto launch = [&](auto type, auto waves, auto vec, auto gated, auto past) {
     hipLaunchKernelGGL((scan_tile_back_kernel<decltype(type), decltype(waves)::value, decltype(vec)::value,
                                          decltype(gated)::value, decltype(past)::value>),
-                       dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, states, dy, dy_batch, dy_step, dlast, df, dv, dz, ds0);
+                       dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, states, dy, dy_batch, dy_step, dlast,
+                       df, dv, dz, ds0);
   };
   by_form(dtype, a.steps <= kBackwardSteps, two, a.z != nullptr, streams(scan, dtype, true, all(kLine)), launch);
   return launch_status();
