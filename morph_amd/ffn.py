@@ -62,7 +62,7 @@ class SavedFFN:
 
 
 def _weights(x, gate, up, down):
-    """The weights as rows, and ff; checked against x."""
+    """ff of the weights, which are checked against x."""
     require_gpu(x, "x", HALF)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("x must be [..., d] with d >= 1")
@@ -73,7 +73,7 @@ def _weights(x, gate, up, down):
     ff = gate.shape[0]
     require_gpu(up, "up", (x.dtype,), (ff, d), device)
     require_gpu(down, "down", (x.dtype,), (d, ff), device)
-    return as_rows(gate), as_rows(up), as_rows(down), ff
+    return ff
 
 
 def _block(x, gate, up, down, rows, d, ff):
@@ -108,11 +108,11 @@ def _forward(x, gate, up, down, keep, stream):
                 return y, SavedFFN(keep, x.detach().view(-1, x.shape[-1]), kept[0], None, x.shape, ff, x.dtype)
             packed = _packings(kept, x.shape, kept[0].shape[0], ff, x.dtype)
             return y, SavedFFN(keep, packed[0], None, packed, x.shape, ff, x.dtype)
-    gate, up, down, ff = _weights(x, gate, up, down)
+    ff = _weights(x, gate, up, down)
     d, device, dtype = x.shape[-1], x.device, x.dtype
     rows = x.numel() // d
     with running_on(device, stream, (x, gate, up, down)):
-        flat = as_rows(x.detach())
+        flat, gate, up, down = (as_rows(t.detach()) for t in (x, gate, up, down))
         y = torch.empty(x.shape, dtype=dtype, device=device)
         saved = None
         if keep == "full":
@@ -158,13 +158,13 @@ def gated_ffn_backward(dy, saved, gate, up, down, stream=None):
         made = layer_calls().ffn_backward(dy, saved.tensors(), gate, up, down, KEEP[saved.keep])
         if made is not None:
             return native(made)
-    gate, up, down, ff = _weights(dy, gate, up, down)
+    ff = _weights(dy, gate, up, down)
     if ff != saved.ff:
         raise ValueError(f"the weights have {ff} hidden units, the forward had {saved.ff}")
     d, dtype = dy.shape[-1], dy.dtype
     rows = dy.numel() // d
     with running_on(device, stream, (dy, gate, up, down, *saved.tensors())):
-        flat = as_rows(dy.detach())
+        flat, gate, up, down = (as_rows(t.detach()) for t in (dy, gate, up, down))
         dx = torch.empty(saved.shape, dtype=dtype, device=device)
         dgate, dup = (torch.empty((ff, d), dtype=dtype, device=device) for _ in range(2))
         ddown = torch.empty((d, ff), dtype=dtype, device=device)

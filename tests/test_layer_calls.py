@@ -1,0 +1,101 @@
+"""What the layer operators' wrappers do before and around their launches, with the launches taken
+out, on the CPU."""
+import contextlib
+
+import pytest
+import torch
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from morph_amd import activations, ffn, layers, recurrence
+
+
+class _Library:
+    """Entry points that launch nothing and succeed; workspaces of no bytes."""
+
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+class _NoNativePath:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+class _Copies(TorchDispatchMode):
+    """Notes for every copy of a tensor whether it was made on the call's stream."""
+
+    def __init__(self, place):
+        super().__init__()
+        self.place, self.made = place, []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.overloadpacket in (torch.ops.aten.clone, torch.ops.aten.copy_, torch.ops.aten._to_copy):
+            self.made.append(self.place["entered"])
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.fixture
+def wrappers(monkeypatch):
+    """The wrappers on CPU tensors: {"entered": whether the call's stream is current, "inputs": the
+    storages that were kept alive for it}."""
+    place = {"entered": False, "inputs": set()}
+
+    @contextlib.contextmanager
+    def running_on(device, stream, inputs=()):
+        place["inputs"] |= {t.untyped_storage().data_ptr() for t in inputs if t is not None}
+        place["entered"] = True
+        yield
+        place["entered"] = False
+
+    def require(t, name, dtypes=None, shape=None, device=None):
+        assert shape is None or tuple(t.shape) == tuple(shape)
+        return t
+    for module in (activations, ffn, recurrence):
+        monkeypatch.setattr(module, "running_on", running_on)
+        monkeypatch.setattr(module, "require_gpu", require)
+        monkeypatch.setattr(module, "lib", _Library)
+        monkeypatch.setattr(module, "layer_calls", _NoNativePath)
+        monkeypatch.setattr(module, "current_stream", lambda: None)
+    return place
+
+
+def _ffn_inputs(rows=5, d=16, ff=24):
+    half = torch.float16
+    x, dy = torch.zeros(d, rows, dtype=half).t(), torch.zeros(1, d, dtype=half).expand(rows, d)
+    return x, dy, [torch.zeros(d, ff, dtype=half).t(), torch.zeros(1, d, dtype=half).expand(ff, d),
+                   torch.zeros(ff, d, dtype=half).t()]
+
+
+@pytest.mark.parametrize("keep", ["full", "fp8"])
+def test_ffn_copies_its_operands_on_the_calls_stream(wrappers, keep):
+    """Views that are no rows are copied; a copy made on the stream that is current outside the call
+    would not be ordered with the kernels that read it, nor with what wrote the view."""
+    x, dy, weights = _ffn_inputs()
+    for call in (lambda: ffn.gated_ffn(x, *weights, stream=object()),
+                 lambda: ffn.gated_ffn_forward(x, *weights, keep=keep, stream=object())):
+        wrappers["inputs"].clear()
+        with _Copies(wrappers) as copies:
+            call()
+        assert copies.made == [True] * 4
+        assert {t.untyped_storage().data_ptr() for t in (x, *weights)} <= wrappers["inputs"]
+    _, saved = ffn.gated_ffn_forward(x, *weights, keep=keep, stream=object())
+    wrappers["inputs"].clear()
+    with _Copies(wrappers) as copies:
+        ffn.gated_ffn_backward(dy, saved, *weights, stream=object())
+    assert copies.made == [True] * 4
+    assert {t.untyped_storage().data_ptr() for t in (dy, *weights)} <= wrappers["inputs"]
+
+
+def test_other_operators_copy_on_the_calls_stream(wrappers):
+    x = torch.zeros(16, 5).t()
+    with _Copies(wrappers) as copies:
+        activations.pack_activation(x, stream=object())
+    assert copies.made == [True]
+    f = torch.zeros(2, 16, 5).transpose(1, 2)
+    state = torch.zeros(16, 2).t()
+    with _Copies(wrappers) as copies:
+        _, _, saved = recurrence.gated_scan_forward(f, f, f, state, stream=object())
+    assert copies.made == [True] * 4
+    with _Copies(wrappers) as copies:
+        recurrence.gated_scan_backward(f, saved, state, stream=object())
+    assert copies.made == [True] * 2
