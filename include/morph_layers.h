@@ -35,7 +35,11 @@ extern "C" {
 /* src: [rows, cols] of dtype F32, F16 or BF16, row stride ld >= cols. */
 int morph_act_pack(const void* src, int dtype, int64_t rows, int64_t cols, int64_t ld,
                    uint8_t* codes, uint8_t* exponents, void* stream);
-/* dst: [rows, cols] = dtype(code * 2^(e - 127)), row stride ld >= cols. */
+/* dst: [rows, cols] = dtype(code * 2^(e - 127)), row stride ld >= cols.  The nearest code may stand
+ * for more than the value did: 63488 and above become 65536, as 1.9375 * 2^127 and above become 2^128.
+ * In F16, and in F32 and BF16, that is infinite.  With MORPH_ACT_SATURATE added to dtype it becomes the
+ * dtype's largest value, so that what was finite in this dtype comes back finite; NaN stays NaN. */
+#define MORPH_ACT_SATURATE 0x100
 int morph_act_unpack(const uint8_t* codes, const uint8_t* exponents, int64_t rows, int64_t cols,
                      void* dst, int dtype, int64_t ld, void* stream);
 
@@ -52,7 +56,8 @@ int morph_act_unpack(const uint8_t* codes, const uint8_t* exponents, int64_t row
 enum morph_ffn_keep {
   MORPH_FFN_KEEP_NONE = 0, /* nothing: no backward follows */
   MORPH_FFN_KEEP_FULL = 1, /* g and u in FP32, and the caller keeps x */
-  MORPH_FFN_KEEP_ACT8 = 2  /* g, u and x in 8 bits (the groups above) */
+  MORPH_FFN_KEEP_ACT8 = 2  /* g, u and x in 8 bits (the groups above); the backward decodes x with
+                              MORPH_ACT_SATURATE, g and u in FP32 (infinite from 1.9375 * 2^127 on) */
 };
 
 typedef struct morph_ffn {

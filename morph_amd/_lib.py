@@ -41,6 +41,7 @@ EXPORTS = (
     "morph_scan_workspace_bytes", "morph_scan_forward", "morph_scan_backward",
 )
 SCAN_SPAN = 64  # MORPH_SCAN_SPAN
+ACT_SATURATE = 0x100  # MORPH_ACT_SATURATE
 GEMM_TILE_M, GEMM_TILE_N, GEMM_TILE_K = 256, 256, 64
 GEMM_SYMMETRIC = 1
 GEMM_Q_KN = 2

@@ -3,7 +3,9 @@
 The streamed engine keeps one boundary activation per stage and micro-batch from the forward to
 the replayed backward (disk.py:365-396), on the device or on the host.  pack_activation holds
 one in 33/64 of its 16 bits: E4M3 codes with a power-of-two scale per 32 consecutive values of a
-row (csrc/act8.hip), relative error 2^-4 at most within 2^14 of a group's largest value.
+row (csrc/act8.hip), relative error 2^-4 at most within 2^14 of a group's largest value.  The topmost
+values of a type (FP16's from 63488 on) are nearest to a code beyond its range; back in that type they are
+its largest value.
 gated_ffn_forward(keep="fp8") keeps its own activations the same way.
 
 A value that is not finite is held as NaN and comes back as NaN: in a step under a dynamic loss
@@ -11,7 +13,7 @@ scale it reaches the gradients, and the detector skips the step.
 """
 import torch
 
-from ._lib import check, layer_calls, lib
+from ._lib import ACT_SATURATE, check, layer_calls, lib
 from .layers import (GROUP, address, as_rows, current_stream, dtype_code, native, require_gpu, row_stride,
                      running_on)
 
@@ -68,14 +70,16 @@ def pack_activation(x, stream=None):
 
 
 def unpack_activation(packed, dtype=None, stream=None):
-    """The activation that `packed` stands for, contiguous, in its own dtype or `dtype`."""
+    """The activation that `packed` stands for, contiguous: in its own dtype, where what was finite comes
+    back finite, or converted to `dtype` as a cast converts it (beyond that type's range: infinite)."""
     if not isinstance(packed, PackedActivation):
         raise TypeError("packed must be a PackedActivation")
+    saturate = ACT_SATURATE if dtype is None else 0
     dtype = packed.dtype if dtype is None else dtype
     if dtype not in FLOATS:
         raise TypeError(f"unsupported dtype {dtype}; expected float32, float16 or bfloat16")
     if stream is None:
-        out = layer_calls().unpack(packed.codes, packed.exponents, packed.shape, dtype_code(dtype))
+        out = layer_calls().unpack(packed.codes, packed.exponents, packed.shape, dtype_code(dtype) | saturate)
         if out is not None:
             return native(out)
     cols = packed.shape[-1]
@@ -89,5 +93,5 @@ def unpack_activation(packed, dtype=None, stream=None):
         out = torch.empty(packed.shape, dtype=dtype, device=codes.device)
         if rows:
             check(lib().morph_act_unpack(address(codes), address(exponents), rows, cols, address(out),
-                                         dtype_code(dtype), cols, current_stream()))
+                                         dtype_code(dtype) | saturate, cols, current_stream()))
         return out

@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void act_unpack_kernel(const uint8_t* __r
                                                               const uint8_t* __restrict__ exponents,
                                                               int64_t cols, void* __restrict__ dst,
                                                               int64_t ld, int64_t groups, int64_t total,
-                                                              bool wide) {
+                                                              bool wide, bool saturate) {
   const int part = threadIdx.x & 3;
   const int64_t first = (int64_t)blockIdx.x * kPer * kQuads + (threadIdx.x >> 2);
   u32x2 w[kPer];
@@ -142,7 +142,8 @@ __global__ __launch_bounds__(kThreads) void act_unpack_kernel(const uint8_t* __r
     float lo[4], hi[4];
     act_decode4(w[i].x, scale, lo);
     act_decode4(w[i].y, scale, hi);
-    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    if (saturate && __any((int)e[i] >= kActTop<T>)) act_saturate<T>(x);
     store8<T>(static_cast<char*>(dst) + p.row * ld * Fmt<T>::bytes, p.c, kFlat ? total * kGroup : cols, wide, x);
   }
 }
@@ -213,11 +214,14 @@ extern "C" int morph_act_unpack(const uint8_t* codes, const uint8_t* exponents, 
   int64_t groups, total, grid;
   int per;
   bool wide;
+  const bool saturate = dtype >= 0 && (dtype & MORPH_ACT_SATURATE) != 0;
+  if (saturate) dtype &= ~MORPH_ACT_SATURATE;
   const int status = act_shape(dst, dtype, rows, cols, ld, codes, exponents, groups, total, grid, per, wide);
   if (status != MORPH_OK || grid == 0) return status;
   by_type(dtype, ld == cols && cols % kGroup == 0, per, [&](auto type, auto flat, auto count) {
     hipLaunchKernelGGL((act_unpack_kernel<decltype(type), decltype(flat)::value, decltype(count)::value>),
-                       dim3((unsigned)grid), dim3(kThreads), 0, as_stream(stream), codes, exponents, cols, dst, ld, groups, total, wide);
+                       dim3((unsigned)grid), dim3(kThreads), 0, as_stream(stream), codes, exponents, cols, dst, ld, groups, total, wide,
+                       saturate);
   });
   return launch_status();
 }

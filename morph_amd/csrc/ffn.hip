@@ -560,7 +560,8 @@ extern "C" int morph_ffn_backward(const morph_ffn* a, int dtype, const morph_ffn
     if (saved->keep == MORPH_FFN_KEEP_ACT8) {
       x = Side{xs, whole_groups(a->d), true};
       pad.room += 2 * a->rows * x.ld;
-      status = morph_act_unpack(saved->x_codes, saved->x_exponents, a->rows, a->d, xs, dtype, x.ld, stream);
+      status = morph_act_unpack(saved->x_codes, saved->x_exponents, a->rows, a->d, xs, dtype | MORPH_ACT_SATURATE,
+                                x.ld, stream);
       if (status != MORPH_OK) return status;
     } else {
       pad.add(x, a->rows, a->d);

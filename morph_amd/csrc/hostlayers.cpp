@@ -98,7 +98,8 @@ class LayerCalls {
     return py::make_tuple(wrap(std::move(codes)), wrap(std::move(exps)));
   }
 
-  // What codes and exponents of a [.., cols] activation stand for, in the type of this dtype code.
+  // What codes and exponents of a [.., cols] activation stand for, in the type of this dtype code (with
+  // MORPH_ACT_SATURATE or without).
   py::object unpack(py::handle ocodes, py::handle oexps, const std::vector<int64_t>& shape, int dtype) const {
     if (c10::impl::dispatch_mode_enabled() || shape.empty() || dtype < 0) return py::none();
     const Here here(ocodes);
@@ -114,7 +115,8 @@ class LayerCalls {
              t.is_contiguous();
     };
     if (!fits(*codes, groups * MORPH_ACT_GROUP) || !fits(*exps, groups)) return py::none();
-    at::Tensor out = here.empty(shape, dtype == MORPH_DTYPE_F32 ? at::kFloat : dtype == MORPH_DTYPE_F16 ? at::kHalf : at::kBFloat16);
+    const int type = dtype & ~MORPH_ACT_SATURATE;
+    at::Tensor out = here.empty(shape, type == MORPH_DTYPE_F32 ? at::kFloat : type == MORPH_DTYPE_F16 ? at::kHalf : at::kBFloat16);
     const int rc = released([&] {
       return c_.act_unpack(codes->const_data_ptr<uint8_t>(), exps->const_data_ptr<uint8_t>(), rows, cols,
                            out.data_ptr(), dtype, cols, here.stream());

@@ -119,6 +119,18 @@ __device__ __forceinline__ void act_decode4(uint32_t w, float scale, float (&x)[
   x[3] = hi[1] * scale;
 }
 
+// Values decoded for the type T, where an infinity (the code above the largest values) becomes T's largest
+// value; NaN fails both comparisons.  Only groups of this exponent byte on hold such codes: 448 * 2^(e - 127)
+// is in the range below it.
+template <typename T>
+constexpr int kActTop = std::is_same_v<T, F16> ? 135 : 247;
+template <typename T, int kCount>
+__device__ __forceinline__ void act_saturate(float (&x)[kCount]) {
+  constexpr float kMost = std::is_same_v<T, F16> ? 65504.0f : std::is_same_v<T, BF16> ? 0x1.FEp127f : 0x1.FFFFFEp127f;
+#pragma unroll
+  for (int k = 0; k < kCount; ++k) x[k] = x[k] > kMost ? kMost : x[k] < -kMost ? -kMost : x[k];
+}
+
 // The largest value of a quad of lanes, in all four.
 __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
   x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]

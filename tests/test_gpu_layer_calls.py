@@ -1,8 +1,12 @@
 """Calls of the layer operators as users make them: on another stream, under autograd, at the ends
 of a type's range, and with what they refuse."""
+import math
+
 import pytest
 import torch
 
+import layer_reference as R
+from morph_amd.activations import pack_activation, unpack_activation
 from morph_amd.ffn import gated_ffn, gated_ffn_backward, gated_ffn_forward
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +55,56 @@ def test_ffn_views_written_on_the_calls_stream(keep):
         side.synchronize()
         assert torch.equal(got, y) and torch.equal(served, gated_ffn(x, *copies))
         assert all(torch.equal(a, b) for a, b in zip(back, grads))
+
+
+# ---- the top of a type's range in 8 bits ----------------------------------------
+def _top_values(dtype, gen, rows, cols):
+    """Values of the type's last two binades, either sign, some that are not finite; a row that holds its
+    largest value only, and one far below."""
+    x = (torch.rand(rows, cols, generator=gen, dtype=torch.float64) * .75 + .25) * torch.finfo(dtype).max
+    x[torch.rand(rows, cols, generator=gen) < .5] *= -1
+    x = x.to(dtype)
+    bad = torch.rand(rows, cols, generator=gen)
+    for k, value in enumerate((math.nan, math.inf, -math.inf)):
+        x[(bad > .01 * k) & (bad < .01 * (k + 1))] = value
+    x[0], x[-1] = torch.finfo(dtype).max, 1.0
+    return x
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(3, 40), (7, 64), (5, 37), (20000, 1024), (20001, 1021)])
+def test_unpacked_in_its_own_type_the_finite_stays_finite(dtype, rows, cols):
+    x = _top_values(dtype, torch.Generator().manual_seed(rows), rows, cols).to(DEV)
+    packed = pack_activation(x)
+    out = unpack_activation(packed)
+    assert torch.equal(out.isfinite(), x.isfinite()) and torch.equal(out.isnan(), ~x.isfinite())
+    fine = x.isfinite()
+    assert ((out - x).abs()[fine] <= x.abs()[fine] / 16).all()
+    assert (out[0] == torch.finfo(dtype).max).all() and (out[-1] == 1).all()
+    assert torch.equal(unpack_activation(packed, stream=torch.cuda.current_stream()).nan_to_num(7.0), out.nan_to_num(7.0))
+    # another type asked for: a cast, and what lies beyond its range is infinite
+    wide = unpack_activation(packed, torch.float16)
+    assert torch.isinf(wide[0]).all()
+    if dtype == torch.float16:
+        assert (unpack_activation(packed, torch.float32)[0] == 65536).all()
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_ffn_kept_in_8_bits_takes_the_top_of_fp16(rows):
+    """x near 65504, kept in 8 bits: finite gradients, those of the formula on x saturated."""
+    gen = torch.Generator().manual_seed(23)
+    d, ff, dtype = 72, 104, torch.float16
+    x = normal(gen, rows, d, dtype=dtype)
+    x[2, 3], x[3, 50], x[1, 71] = 65504, -63488, 64000
+    weights = [normal(gen, ff, d, scale=2.0 ** -14, dtype=dtype), normal(gen, ff, d, scale=2.0 ** -14, dtype=dtype),
+               normal(gen, d, ff, scale=ff ** -.5, dtype=dtype)]
+    dy = normal(gen, rows, d, scale=2.0 ** -7, dtype=dtype)
+    dev = [w.to(DEV) for w in weights]
+    y, saved = gated_ffn_forward(x.to(DEV), *dev, keep="fp8")
+    dx, dgate, dup, ddown = gated_ffn_backward(dy.to(DEV), saved, *dev)
+    assert all(t.isfinite().all() for t in (y, dx, dgate, dup, ddown))
+    xk, g, u = (R.unpack(p.codes, p.exponents, p.shape[-1]) for p in (saved.x, saved.gate, saved.up))
+    assert xk.abs().max() == 65536
+    ref = R.ffn_backward(dy.double(), xk.clamp(-65504, 65504), g, u, *(w.double() for w in weights))
+    R.assert_product(dgate, ref["dg"].T, xk.clamp(-65504, 65504), dtype, "dgate")
+    R.assert_product(dup, ref["du"].T, xk.clamp(-65504, 65504), dtype, "dup")

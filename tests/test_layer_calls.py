@@ -1,12 +1,15 @@
 """What the layer operators' wrappers do before and around their launches, with the launches taken
 out, on the CPU."""
 import contextlib
+import ctypes
+from pathlib import Path
 
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from morph_amd import activations, ffn, layers, recurrence
+from morph_amd import _lib, activations, ffn, recurrence
+from test_abi import no_gpu_visible
 
 
 class _Library:
@@ -99,3 +102,15 @@ def test_other_operators_copy_on_the_calls_stream(wrappers):
     with _Copies(wrappers) as copies:
         recurrence.gated_scan_backward(f, saved, state, stream=object())
     assert copies.made == [True] * 2
+
+
+@no_gpu_visible
+def test_saturate_is_unpacks_alone():
+    """MORPH_ACT_SATURATE goes with a dtype that there is, and with the unpack."""
+    header = (Path(__file__).resolve().parents[1] / "include" / "morph_layers.h").read_text()
+    assert f"#define MORPH_ACT_SATURATE {_lib.ACT_SATURATE:#x}\n" in header
+    p = ctypes.c_void_p(0x10000)
+    for dtype in (-1, 3, _lib.ACT_SATURATE | 3, 0x200):
+        assert _lib.lib().morph_act_unpack(p, p, 1, 1, p, dtype, 1, None) == -2
+    assert _lib.lib().morph_act_unpack(p, p, 0, 1, p, _lib.ACT_SATURATE | 1, 1, None) == 0
+    assert _lib.lib().morph_act_pack(p, _lib.ACT_SATURATE | 1, 1, 1, 1, p, p, None) == -2
