@@ -20,8 +20,8 @@ import torch
 
 from ._lib import FfnBlock, FfnSaved, check, layer_calls, lib
 from .activations import PackedActivation
-from .layers import (GROUP, HALF, address, as_rows, current_stream, dtype_code, native, require_gpu,
-                     row_stride, running_on)
+from .layers import (GROUP, HALF, address, as_rows, current_stream, dtype_code, first_order, native,
+                     require_gpu, row_stride, running_on)
 
 KEEP = {"none": 0, "full": 1, "fp8": 2}
 
@@ -190,11 +190,12 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         gate, up, down = ctx.saved_tensors[:3]
-        return *gated_ffn_backward(dy, ctx.saved, gate, up, down), None
+        grads = gated_ffn_backward(dy, ctx.saved, gate, up, down)
+        return *first_order("gated_feed_forward", grads), None
 
 
 def gated_feed_forward(x, gate, up, down, keep="full"):
-    """gated_ffn under autograd: y, differentiable in x and the weights.  keep: as
+    """gated_ffn under autograd: y, differentiable once in x and the weights.  keep: as
     gated_ffn_forward's."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, up, down)):
         return _GatedFFN.apply(x, gate, up, down, keep)

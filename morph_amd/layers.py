@@ -1,4 +1,5 @@
-"""What the layer operators' wrappers share: checks of tensors, and the stream a call runs on."""
+"""What the layer operators' wrappers share: checks of tensors, the stream a call runs on, and the
+order of their derivatives."""
 import contextlib
 import ctypes
 
@@ -61,6 +62,27 @@ def running_on(device, stream, inputs=()):
     if stream is None and device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return _elsewhere(device, stream, inputs if stream is not None else ())
+
+
+class _FirstOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, anchor, *grads):
+        ctx.name = name
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} can be differentiated once: its gradients have no backward of their own")
+
+
+def first_order(name, grads):
+    """The gradients that a backward returns.  Under create_graph=True they would count as constants, and
+    their own derivatives would be missing from a sum without an error: there they raise where they
+    are differentiated.  (torch's once_differentiable does so only where the gradient that comes in
+    requires one: not for the gradient of y.sum().)"""
+    if not torch.is_grad_enabled():
+        return grads
+    return _FirstOrder.apply(name, torch.empty(0, requires_grad=True), *grads)
 
 
 def native(result):

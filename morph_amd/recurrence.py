@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from ._lib import SCAN_SPAN, ScanArgs, check, layer_calls, lib
-from .layers import address, current_stream, dtype_code, native, require_gpu, running_on
+from .layers import address, current_stream, dtype_code, first_order, native, require_gpu, running_on
 
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -140,11 +140,11 @@ class _GatedScan(torch.autograd.Function):
         if dy is None:
             dy = torch.zeros_like(saved.f)
         df, dv, dz, dstate = gated_scan_backward(dy, saved, dlast)
-        return df, dv, dz, dstate if saved.state is not None else None
+        return first_order("gated_recurrence", (df, dv, dz, dstate if saved.state is not None else None))
 
 
 def gated_recurrence(f, v, z=None, state=None):
-    """gated_scan under autograd: (y, last state), differentiable in f, v, z and state."""
+    """gated_scan under autograd: (y, last state), differentiable once in f, v, z and state."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, v, z, state)):
         return _GatedScan.apply(f, v, z, state)
     return gated_scan(f, v, z, state)

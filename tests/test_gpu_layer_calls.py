@@ -7,7 +7,8 @@ import torch
 
 import layer_reference as R
 from morph_amd.activations import pack_activation, unpack_activation
-from morph_amd.ffn import gated_ffn, gated_ffn_backward, gated_ffn_forward
+from morph_amd.ffn import gated_feed_forward, gated_ffn, gated_ffn_backward, gated_ffn_forward
+from morph_amd.recurrence import gated_recurrence
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -108,3 +109,40 @@ def test_ffn_kept_in_8_bits_takes_the_top_of_fp16(rows):
     ref = R.ffn_backward(dy.double(), xk.clamp(-65504, 65504), g, u, *(w.double() for w in weights))
     R.assert_product(dgate, ref["dg"].T, xk.clamp(-65504, 65504), dtype, "dgate")
     R.assert_product(dup, ref["du"].T, xk.clamp(-65504, 65504), dtype, "dup")
+
+
+# ---- derivatives ------------------------------------------------------------------
+def _differentiable(kind):
+    """An operator as a function of tensors, and the tensors."""
+    gen = torch.Generator().manual_seed(29)
+    if kind in ("full", "fp8"):
+        tensors = [normal(gen, 5, 64, dtype=torch.bfloat16), normal(gen, 96, 64, scale=.1, dtype=torch.bfloat16),
+                   normal(gen, 96, 64, scale=.1, dtype=torch.bfloat16), normal(gen, 64, 96, scale=.1, dtype=torch.bfloat16)]
+        return lambda *t: gated_feed_forward(*t, keep=kind), [t.to(DEV) for t in tensors]
+    f, v, z = (normal(gen, 2, 150, 40, mean=m).to(DEV) for m in (2.0, 0.0, 0.0))
+    if kind == "scan":
+        return lambda f, v: gated_recurrence(f, v)[0], [f, v]
+    return lambda f, v, z, s: torch.cat([t.flatten() for t in gated_recurrence(f, v, z, s)]), [f, v, z, normal(gen, 2, 40).to(DEV)]
+
+
+@pytest.mark.parametrize("loss", [lambda y: y.float().sum(), lambda y: y.float().square().sum()])
+@pytest.mark.parametrize("kind", ["full", "fp8", "scan", "scan_gated"])
+def test_second_derivatives_raise(kind, loss):
+    """A gradient penalty, in every input: an error, not the penalty's missing share; the first
+    derivatives under create_graph are the ordinary ones."""
+    run, tensors = _differentiable(kind)
+    for i in range(len(tensors)):
+        leaves = [t.detach().requires_grad_(i == k) for k, t in enumerate(tensors)]
+        plain, = torch.autograd.grad(loss(run(*leaves)), leaves[i])
+        assert not plain.requires_grad
+        grad, = torch.autograd.grad(loss(run(*leaves)), leaves[i], create_graph=True)
+        assert torch.equal(grad.detach(), plain) and grad.requires_grad
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            (grad.float().square().sum() + leaves[i].float().square().sum()).backward()
+    leaves = [t.detach().requires_grad_() for t in tensors]
+    loss(run(*leaves)).backward(create_graph=True)
+    grads = [t.grad.detach() for t in leaves]
+    for t in leaves:
+        t.grad = None
+    loss(run(*leaves)).backward()
+    assert all(torch.equal(a, t.grad) for a, t in zip(grads, leaves))
