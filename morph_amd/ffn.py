@@ -21,7 +21,7 @@ import torch
 from ._lib import FfnBlock, FfnSaved, check, layer_calls, lib
 from .activations import PackedActivation
 from .layers import (GROUP, HALF, address, as_rows, current_stream, dtype_code, first_order, native,
-                     require_gpu, row_stride, running_on)
+                     require_gpu, requires_grad, row_stride, running_on)
 
 KEEP = {"none": 0, "full": 1, "fp8": 2}
 
@@ -197,7 +197,7 @@ class _GatedFFN(torch.autograd.Function):
 def gated_feed_forward(x, gate, up, down, keep="full"):
     """gated_ffn under autograd: y, differentiable once in x and the weights.  keep: as
     gated_ffn_forward's."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, up, down)):
+    if requires_grad("gated_feed_forward", x, gate, up, down):
         return _GatedFFN.apply(x, gate, up, down, keep)
     return gated_ffn(x, gate, up, down)
 

@@ -4,6 +4,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, dtype_code
 
@@ -62,6 +63,15 @@ def running_on(device, stream, inputs=()):
     if stream is None and device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return _elsewhere(device, stream, inputs if stream is not None else ())
+
+
+def requires_grad(name, *tensors):
+    """Whether a call under autograd has to keep something for its backward.  Tangents of forward mode
+    are refused: the kernels would drop them."""
+    tensors = [t for t in tensors if t is not None]
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative (an input is a dual tensor)")
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 class _FirstOrder(torch.autograd.Function):

@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from ._lib import SCAN_SPAN, ScanArgs, check, layer_calls, lib
-from .layers import address, current_stream, dtype_code, first_order, native, require_gpu, running_on
+from .layers import address, current_stream, dtype_code, first_order, native, require_gpu, requires_grad, running_on
 
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -145,6 +145,6 @@ class _GatedScan(torch.autograd.Function):
 
 def gated_recurrence(f, v, z=None, state=None):
     """gated_scan under autograd: (y, last state), differentiable once in f, v, z and state."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, v, z, state)):
+    if requires_grad("gated_recurrence", f, v, z, state):
         return _GatedScan.apply(f, v, z, state)
     return gated_scan(f, v, z, state)

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import layer_reference as R
 from morph_amd.activations import pack_activation, unpack_activation
@@ -146,3 +147,23 @@ def test_second_derivatives_raise(kind, loss):
         t.grad = None
     loss(run(*leaves)).backward()
     assert all(torch.equal(a, t.grad) for a, t in zip(grads, leaves))
+
+
+@pytest.mark.parametrize("kind", ["full", "fp8", "scan", "scan_gated"])
+def test_forward_mode_raises(kind):
+    """Tangents (dual tensors, torch.func.jvp), in every input and with gradients on or off: an error, not a
+    result without its tangent; tensors without one are computed as ever."""
+    run, tensors = _differentiable(kind)
+    plain = run(*tensors)
+    for i in range(len(tensors)):
+        for leaf in (False, True):
+            with forward_ad.dual_level():
+                duals = [t.detach().requires_grad_(leaf) for t in tensors]
+                assert torch.equal(run(*duals), plain)
+                duals[i] = forward_ad.make_dual(duals[i], torch.ones_like(duals[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    run(*duals)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    run(*duals)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda t: run(*tensors[:i], t, *tensors[i + 1:]), (tensors[i],), (torch.ones_like(tensors[i]),))
