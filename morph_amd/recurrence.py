@@ -37,7 +37,7 @@ def _channels_last(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _checked(f, v, z, state):
+def _check(f, v, z, state):
     require_gpu(f, "f", FLOATS)
     if f.dim() != 3:
         raise ValueError(f"f must be [batch, steps, dim], got {tuple(f.shape)}")
@@ -46,8 +46,6 @@ def _checked(f, v, z, state):
         require_gpu(z, "z", (f.dtype,), f.shape, f.device)
     if state is not None:
         require_gpu(state, "state", (torch.float32,), (f.shape[0], f.shape[2]), f.device)
-    return (_channels_last(f), _channels_last(v), _channels_last(z) if z is not None else None,
-            state.detach().contiguous() if state is not None else None)
 
 
 def _args(f, v, z, state):
@@ -71,9 +69,11 @@ def _forward(f, v, z, state, train, stream):
             y, last, states = native(made)
             return y, last, SavedScan(f.detach(), v.detach(), z.detach() if z is not None else None,
                                       state.detach() if state is not None else None, states)
-    require_gpu(f, "f", FLOATS)
+    _check(f, v, z, state)
     with running_on(f.device, stream, (f, v, z, state)):
-        f, v, z, state = _checked(f, v, z, state)
+        f, v = _channels_last(f), _channels_last(v)
+        z = _channels_last(z) if z is not None else None
+        state = state.detach().contiguous() if state is not None else None
         batch, steps, dim = f.shape
         y = torch.empty((batch, steps, dim), dtype=f.dtype, device=f.device)
         last = torch.empty((batch, dim), dtype=torch.float32, device=f.device)

@@ -9,7 +9,7 @@ from torch.autograd import forward_ad
 import layer_reference as R
 from morph_amd.activations import pack_activation, unpack_activation
 from morph_amd.ffn import gated_feed_forward, gated_ffn, gated_ffn_backward, gated_ffn_forward
-from morph_amd.recurrence import gated_recurrence
+from morph_amd.recurrence import gated_recurrence, gated_scan, gated_scan_backward, gated_scan_forward
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -167,3 +167,19 @@ def test_forward_mode_raises(kind):
                     run(*duals)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(lambda t: run(*tensors[:i], t, *tensors[i + 1:]), (tensors[i],), (torch.ones_like(tensors[i]),))
+
+
+# ---- refusals ---------------------------------------------------------------------
+def test_scan_refuses_on_another_stream():
+    """The documented errors with stream= too, whichever argument is wrong."""
+    f, side = torch.zeros(2, 5, 64, device=DEV), torch.cuda.Stream()
+    for args, error in (((f, "v"), TypeError), ((f, f.cpu()), ValueError), ((f, f, [1]), TypeError),
+                        ((f, f, f.cpu()), ValueError), ((f, f, None, 1.0), TypeError),
+                        ((f, f, None, f[:, 0].cpu()), ValueError), (([1], f), TypeError), ((f[0], f), ValueError)):
+        for call in (gated_scan, gated_scan_forward):
+            with pytest.raises(error):
+                call(*args, stream=side)
+    _, _, saved = gated_scan_forward(f, f)
+    for args, error in (((f, saved, "dlast"), TypeError), ((f.cpu(), saved), ValueError), ((f, saved, f[:, 0].cpu()), ValueError)):
+        with pytest.raises(error):
+            gated_scan_backward(*args, stream=side)
