@@ -61,6 +61,11 @@ class SavedFFN:
         return 4 * self.projections.numel()
 
 
+def _check_keep(keep):
+    if keep not in ("full", "fp8"):
+        raise ValueError('keep must be "full" or "fp8"')
+
+
 def _weights(x, gate, up, down):
     """ff of the weights, which are checked against x."""
     require_gpu(x, "x", HALF)
@@ -143,8 +148,7 @@ def gated_ffn_forward(x, gate, up, down, keep="full", stream=None):
     roundings of the matrix instructions' 16-bit operands (8 ff bytes a row, and x by reference:
     it may not change before the backward); "fp8" holds x and both projections in 8 bits, about
     d + 2 ff bytes a row, and the backward takes them for x and the projections."""
-    if keep not in ("full", "fp8"):
-        raise ValueError('keep must be "full" or "fp8"')
+    _check_keep(keep)
     return _forward(x, gate, up, down, keep, stream)
 
 
@@ -197,6 +201,7 @@ class _GatedFFN(torch.autograd.Function):
 def gated_feed_forward(x, gate, up, down, keep="full"):
     """gated_ffn under autograd: y, differentiable once in x and the weights.  keep: as
     gated_ffn_forward's."""
+    _check_keep(keep)
     if requires_grad("gated_feed_forward", x, gate, up, down):
         return _GatedFFN.apply(x, gate, up, down, keep)
     return gated_ffn(x, gate, up, down)
@@ -208,8 +213,7 @@ class GatedFFN(torch.nn.Module):
 
     def __init__(self, d, ff, keep="full", device=None, dtype=torch.float16):
         super().__init__()
-        if keep not in ("full", "fp8"):
-            raise ValueError('keep must be "full" or "fp8"')
+        _check_keep(keep)
         self.gate = torch.nn.Linear(d, ff, bias=False, device=device, dtype=dtype)
         self.up = torch.nn.Linear(d, ff, bias=False, device=device, dtype=dtype)
         self.down = torch.nn.Linear(ff, d, bias=False, device=device, dtype=dtype)

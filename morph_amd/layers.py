@@ -68,7 +68,7 @@ def running_on(device, stream, inputs=()):
 def requires_grad(name, *tensors):
     """Whether a call under autograd has to keep something for its backward.  Tangents of forward mode
     are refused: the kernels would drop them."""
-    tensors = [t for t in tensors if t is not None]
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor)]  # the operator refuses what is none
     if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{name} has no forward-mode derivative (an input is a dual tensor)")
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)

@@ -183,3 +183,23 @@ def test_scan_refuses_on_another_stream():
     for args, error in (((f, saved, "dlast"), TypeError), ((f.cpu(), saved), ValueError), ((f, saved, f[:, 0].cpu()), ValueError)):
         with pytest.raises(error):
             gated_scan_backward(*args, stream=side)
+
+
+def test_calls_under_autograd_refuse():
+    """What is no tensor, and a keep that there is none, raise as in the calls without autograd."""
+    x = torch.zeros(4, 64, dtype=torch.float16, device=DEV)
+    gate, up, down = (torch.zeros(s, dtype=torch.float16, device=DEV) for s in ((96, 64), (96, 64), (64, 96)))
+    for args in ((None, gate, up, down), (x, None, up, down), (x, gate, 3, down), (x, gate, up, [down])):
+        with pytest.raises(TypeError):
+            gated_feed_forward(*args)
+        with pytest.raises(TypeError):
+            gated_feed_forward(x.requires_grad_() if args[0] is not None else None, *args[1:])
+    for leaf in (x, x.detach()):
+        with pytest.raises(ValueError, match="keep"):
+            gated_feed_forward(leaf, gate, up, down, keep="none")
+    with torch.no_grad(), pytest.raises(ValueError, match="keep"):
+        gated_feed_forward(x, gate, up, down, keep="bf16")
+    f = torch.zeros(2, 5, 64, device=DEV)
+    for args in ((f, "v"), (None, f), (f, f, 1), (f, f, None, [0])):
+        with pytest.raises(TypeError):
+            gated_recurrence(*args)
