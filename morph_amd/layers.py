@@ -60,6 +60,8 @@ def running_on(device, stream, inputs=()):
     """A context whose current device and stream are the call's, so that what it allocates
     belongs to that stream.  Inputs are kept alive for the work queued there; their
     contents are the caller's to order, as for any stream."""
+    if stream is not None and stream.device != device:
+        raise ValueError(f"stream is on {stream.device}, expected {device}")
     if stream is None and device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return _elsewhere(device, stream, inputs if stream is not None else ())

@@ -3,12 +3,13 @@ out, on the CPU."""
 import contextlib
 import ctypes
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from morph_amd import _lib, activations, ffn, recurrence
+from morph_amd import _lib, activations, ffn, layers, recurrence
 from test_abi import no_gpu_visible
 
 
@@ -114,3 +115,11 @@ def test_saturate_is_unpacks_alone():
         assert _lib.lib().morph_act_unpack(p, p, 1, 1, p, dtype, 1, None) == -2
     assert _lib.lib().morph_act_unpack(p, p, 0, 1, p, _lib.ACT_SATURATE | 1, 1, None) == 0
     assert _lib.lib().morph_act_pack(p, _lib.ACT_SATURATE | 1, 1, 1, 1, p, p, None) == -2
+
+
+def test_a_stream_of_another_device_is_refused():
+    """Launched there, the kernels would read this device's memory from the other one."""
+    there = SimpleNamespace(device=torch.device("cuda", 1))
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        layers.running_on(torch.device("cuda", 0), there)
+    layers.running_on(torch.device("cuda", 1), there)
