@@ -44,6 +44,14 @@ class SavedFFN:
     def up(self):
         return self.packed[2] if self.keep == "fp8" else self.projections[1]
 
+    @classmethod
+    def of(cls, tensors, keep, shape, ff, dtype):
+        """From tensors() and the rest."""
+        if keep == "fp8":
+            packed = _packings(tensors, shape, tensors[0].shape[0], ff, dtype)
+            return cls(keep, packed[0], None, packed, shape, ff, dtype)
+        return cls(keep, *tensors, None, shape, ff, dtype)
+
     def tensors(self):
         if self.keep == "fp8":
             return tuple(t for p in self.packed for t in (p.codes, p.exponents))
@@ -110,9 +118,8 @@ def _forward(x, gate, up, down, keep, stream):
             y, kept = made
             ff = gate.shape[0]
             if keep == "full":
-                return y, SavedFFN(keep, x.detach().view(-1, x.shape[-1]), kept[0], None, x.shape, ff, x.dtype)
-            packed = _packings(kept, x.shape, kept[0].shape[0], ff, x.dtype)
-            return y, SavedFFN(keep, packed[0], None, packed, x.shape, ff, x.dtype)
+                kept = x.detach().view(-1, x.shape[-1]), kept[0]
+            return y, SavedFFN.of(kept, keep, x.shape, ff, x.dtype)
     ff = _weights(x, gate, up, down)
     d, device, dtype = x.shape[-1], x.device, x.dtype
     rows = x.numel() // d
@@ -122,12 +129,12 @@ def _forward(x, gate, up, down, keep, stream):
         saved = None
         if keep == "full":
             wide = -(-ff // GROUP) * GROUP
-            saved = SavedFFN(keep, flat, torch.empty((2, rows, wide), dtype=torch.float32, device=device), None,
-                             x.shape, ff, dtype)
+            projections = torch.empty((2, rows, wide), dtype=torch.float32, device=device)
+            saved = SavedFFN.of((flat, projections), keep, x.shape, ff, dtype)
         elif keep == "fp8":
-            packed = _packings([torch.empty((rows, -(-n // GROUP) * size), dtype=torch.uint8, device=device)
-                                for n in (d, ff, ff) for size in (GROUP, 1)], x.shape, rows, ff, dtype)
-            saved = SavedFFN(keep, packed[0], None, packed, x.shape, ff, dtype)
+            codes = [torch.empty((rows, -(-n // GROUP) * size), dtype=torch.uint8, device=device)
+                     for n in (d, ff, ff) for size in (GROUP, 1)]
+            saved = SavedFFN.of(codes, keep, x.shape, ff, dtype)
         if rows:
             L = lib()
             size = L.morph_ffn_workspace_bytes(rows, d, ff, KEEP[keep], 0)
@@ -186,15 +193,15 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, up, down, keep):
         y, saved = gated_ffn_forward(x, gate, up, down, keep)
-        ctx.saved = saved
-        # tensors that autograd should guard against changes in place
-        ctx.save_for_backward(gate, up, down, *((x,) if keep == "full" else ()))
+        # what was kept is autograd's to hold and release; x for its guard against changes in place
+        ctx.save_for_backward(gate, up, down, x if keep == "full" else None, *saved.tensors())
+        ctx.kept = keep, saved.shape, saved.ff, saved.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        gate, up, down = ctx.saved_tensors[:3]
-        grads = gated_ffn_backward(dy, ctx.saved, gate, up, down)
+        gate, up, down, _, *tensors = ctx.saved_tensors
+        grads = gated_ffn_backward(dy, SavedFFN.of(tensors, *ctx.kept), gate, up, down)
         return *first_order("gated_feed_forward", grads), None
 
 

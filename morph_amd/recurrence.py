@@ -128,15 +128,14 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, f, v, z, state):
         y, last, saved = gated_scan_forward(f, v, z, state)
-        ctx.save_for_backward(*(t for t in (f, v, z, state) if t is not None))
-        ctx.saved = saved
+        # what was kept is autograd's to hold and release; the inputs for its guard against changes in place
+        ctx.save_for_backward(f, v, z, state, *(getattr(saved, name) for name in SavedScan.__slots__))
         ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
     def backward(ctx, dy, dlast):
-        ctx.saved_tensors  # raises where an input was changed in place
-        saved = ctx.saved
+        saved = SavedScan(*ctx.saved_tensors[4:])
         if dy is None:
             dy = torch.zeros_like(saved.f)
         df, dv, dz, dstate = gated_scan_backward(dy, saved, dlast)

@@ -203,3 +203,47 @@ def test_calls_under_autograd_refuse():
     for args in ((f, "v"), (None, f), (f, f, 1), (f, f, None, [0])):
         with pytest.raises(TypeError):
             gated_recurrence(*args)
+
+
+@pytest.mark.parametrize("kind", ["full", "fp8", "scan", "scan_gated"])
+def test_backward_releases_what_was_kept(kind):
+    """Behind a backward only inputs, outputs and gradients are held, as torch's own operators do, also
+    while an output is kept; and what is kept passes through saved_tensors_hooks (offloading)."""
+    run, tensors = _differentiable(kind)
+    leaves = [torch.cat([t.detach()] * 200).requires_grad_() if i == 0 or kind.startswith("scan") else
+              t.detach().requires_grad_() for i, t in enumerate(tensors)]
+    before = torch.cuda.memory_allocated()
+    out = run(*leaves)
+    size = out.untyped_storage().nbytes()
+    held = torch.cuda.memory_allocated() - before - size
+    assert held > (1 << 16)
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    del grads
+    assert torch.cuda.memory_allocated() - before - size < held // 8
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, leaves, torch.ones_like(out))
+
+    plain = torch.autograd.grad(run(*leaves), leaves, torch.ones_like(out))
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        out = run(*leaves)
+    assert torch.cuda.memory_allocated() - before - size < held // 8
+    for a, b in zip(torch.autograd.grad(out, leaves, torch.ones_like(out)), plain):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["full", "fp8", "scan", "scan_gated"])
+def test_inputs_changed_before_the_backward_raise(kind):
+    """Every input that the backward reads; of the block's x the 8-bit form has a copy."""
+    run, tensors = _differentiable(kind)
+    for i in range(len(tensors)):
+        if kind.startswith("scan") and i == 3:
+            continue  # the first state is read by the forward alone
+        leaves = [t.clone().requires_grad_(k != i) for k, t in enumerate(tensors)]
+        out = run(*leaves)
+        leaves[i].add_(1)
+        if kind == "fp8" and i == 0:
+            out.float().sum().backward()
+        else:
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                out.float().sum().backward()
