@@ -352,6 +352,7 @@ template <typename T, int kW, int kVec, bool kGated, bool kStream>
 __global__ __launch_bounds__(64 * kW, 4) void scan_tile_kernel(const morph_scan a, const ScanGrid g,
                                                              void* __restrict__ y, float* __restrict__ last,
                                                              float* __restrict__ states) {
+  static_assert(kVec == 2 || !kStream, "what by_form asks for");
   constexpr int L = kForwardSteps;
   typedef typename Raw<T, kVec>::type raw;
   int group;
@@ -443,6 +444,7 @@ __global__ __launch_bounds__(64 * kW, 4) void scan_tile_back_kernel(const morph_
                                                                   int64_t dy_step, const float* __restrict__ dlast,
                                                                   void* __restrict__ df, void* __restrict__ dv,
                                                                   void* __restrict__ dz, float* __restrict__ ds0) {
+  static_assert(kVec == 2 || !kStream, "what by_form asks for");
   constexpr int L = kBackwardSteps;
   typedef typename Raw<T, kVec>::type raw;
   int group;
@@ -639,14 +641,18 @@ bool streams(const morph_scan* a, int dtype, bool backward, bool lines) {
   return lines && a->batch * a->steps * a->dim * tensors * (dtype == MORPH_DTYPE_F32 ? 4 : 2) > (int64_t(256) << 20);
 }
 
-// A call's kernel by its types: F(T, waves a tile, two channels a lane, output gate, streams).
+// A call's kernel by its types: F(T, waves a tile, channels a lane, output gate, streams).  What streams has two
+// channels a lane: its rows are whole cache lines.
 template <typename F>
 void by_form(int dtype, bool one_wave, bool two, bool gated, bool stream, F&& f) {
   auto with = [&](auto type, auto waves, auto past) {
-    if (two && gated) f(type, waves, std::integral_constant<int, 2>{}, std::true_type{}, past);
-    else if (two) f(type, waves, std::integral_constant<int, 2>{}, std::false_type{}, past);
-    else if (gated) f(type, waves, std::integral_constant<int, 1>{}, std::true_type{}, past);
-    else f(type, waves, std::integral_constant<int, 1>{}, std::false_type{}, past);
+    auto lanes = [&](auto channels) {
+      if (gated) f(type, waves, channels, std::true_type{}, past);
+      else f(type, waves, channels, std::false_type{}, past);
+    };
+    if constexpr (decltype(past)::value) lanes(std::integral_constant<int, 2>{});
+    else if (two) lanes(std::integral_constant<int, 2>{});
+    else lanes(std::integral_constant<int, 1>{});
   };
   auto typed = [&](auto waves, auto past) {
     if (dtype == MORPH_DTYPE_F32) with(F32{}, waves, past);
