@@ -169,7 +169,7 @@ int act_shape(const void* values, int dtype, int64_t rows, int64_t cols, int64_t
   total = rows * groups;
   per = total >= kMany ? 4 : 1;
   grid = (total + per * kQuads - 1) / (per * kQuads);
-  if (grid > 0x7FFFFFFF) return MORPH_ERANGE;
+  if (!launchable(grid, kThreads)) return MORPH_ERANGE;
   wide = !misaligned(values, 16) && (rows == 1 || ld * size % 16 == 0);
   return MORPH_OK;
 }

@@ -245,7 +245,7 @@ struct Launch {
     }
     if (a.splits > 1) a.parts = static_cast<float*>(parts);
     const int64_t n = tiles(shape);
-    ok = ok && n <= (1 << 30);
+    ok = ok && launchable(n + 7, kFfnThreads);
     a.total = (int32_t)n;
     return (FfnShape)shape;
   }
@@ -323,7 +323,7 @@ struct Padding {
   int launch(hipStream_t s) {
     if (a.count == 0) return MORPH_OK;
     const int64_t grid = (a.rows + kThreads / 64 - 1) / (kThreads / 64);
-    if (grid > 0x7FFFFFFF) return MORPH_ERANGE;
+    if (!launchable(grid, kThreads)) return MORPH_ERANGE;
     hipLaunchKernelGGL(ffn_pad_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, a);
     return launch_status();
   }

@@ -10,6 +10,11 @@ namespace morph {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+// Whether so many workgroups of `threads` may be launched along a dimension: fewer than 2^32 threads.
+inline bool launchable(int64_t workgroups, int64_t threads) {
+  return workgroups <= int64_t(0xFFFFFFFF) / threads;
+}
+
 // Two floats in one word, each rounded to nearest even (overflow to inf, as a conversion).
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {

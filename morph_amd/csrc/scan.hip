@@ -609,11 +609,11 @@ constexpr int64_t kLine = 128;
 // 8 358 / 317; forward of 2 x 30574 x 238 (4 groups) 64 / 43.
 constexpr int64_t kManyGroups = 16;
 
-int scan_grid(const morph_scan* a, int kvec, bool backward, void* workspace, hipStream_t s, ScanGrid& g,
+int scan_grid(const morph_scan* a, int waves, int kvec, bool backward, void* workspace, hipStream_t s, ScanGrid& g,
               unsigned& grid) {
   const int64_t groups_c = (a->dim + 64 * kvec - 1) / (64 * kvec), groups = groups_c * a->batch;
   const int64_t tiles = tiles_of(a->steps, backward), total = tiles * groups;
-  if (total > 0x7FFFFFFF) return MORPH_ERANGE;
+  if (!launchable(total, 64 * waves)) return MORPH_ERANGE;
   g.ticket = static_cast<uint32_t*>(workspace);
   g.parts = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kTicketBytes);
   g.runs = g.parts + total * 64 * kvec;
@@ -698,16 +698,17 @@ extern "C" int morph_scan_forward(const morph_scan* scan, int dtype, void* y, fl
            starts(y, 0, 0, size, bytes);
   };
   const bool two = all(2 * size);  // channels a lane
+  const bool one_wave = a.steps <= kForwardSteps;
   ScanGrid g;
   unsigned grid;
-  const int shape = scan_grid(scan, two ? 2 : 1, false, workspace, s, g, grid);
+  const int shape = scan_grid(scan, one_wave ? 1 : kWaves, two ? 2 : 1, false, workspace, s, g, grid);
   if (shape != MORPH_OK) return shape;
   auto launch = [&](auto type, auto waves, auto vec, auto gated, auto past) {
     hipLaunchKernelGGL((scan_tile_kernel<decltype(type), decltype(waves)::value, decltype(vec)::value,
                                          decltype(gated)::value, decltype(past)::value>),
                        dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, y, last, states);
   };
-  by_form(dtype, a.steps <= kForwardSteps, two, a.z != nullptr, streams(scan, dtype, false, all(kLine)), launch);
+  by_form(dtype, one_wave, two, a.z != nullptr, streams(scan, dtype, false, all(kLine)), launch);
   return launch_status();
 }
 
@@ -741,9 +742,10 @@ extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const floa
            starts(dv, 0, 0, size, bytes) && starts(dz, 0, 0, size, bytes);
   };
   const bool two = all(2 * size);  // channels a lane
+  const bool one_wave = a.steps <= kBackwardSteps;
   ScanGrid g;
   unsigned grid;
-  const int shape = scan_grid(scan, two ? 2 : 1, true, workspace, s, g, grid);
+  const int shape = scan_grid(scan, one_wave ? 1 : kWaves, two ? 2 : 1, true, workspace, s, g, grid);
   if (shape != MORPH_OK) return shape;
   auto launch = [&](auto type, auto waves, auto vec, auto gated, auto past) {
     hipLaunchKernelGGL((scan_tile_back_kernel<decltype(type), decltype(waves)::value, decltype(vec)::value,
@@ -751,6 +753,6 @@ extern "C" int morph_scan_backward(const morph_scan* scan, int dtype, const floa
                        dim3(grid), dim3(64 * decltype(waves)::value), 0, s, a, g, states, dy, dy_batch, dy_step, dlast,
                        df, dv, dz, ds0);
   };
-  by_form(dtype, a.steps <= kBackwardSteps, two, a.z != nullptr, streams(scan, dtype, true, all(kLine)), launch);
+  by_form(dtype, one_wave, two, a.z != nullptr, streams(scan, dtype, true, all(kLine)), launch);
   return launch_status();
 }

@@ -123,3 +123,19 @@ def test_a_stream_of_another_device_is_refused():
     with pytest.raises(ValueError, match="stream is on cuda:1"):
         layers.running_on(torch.device("cuda", 0), there)
     layers.running_on(torch.device("cuda", 1), there)
+
+
+@no_gpu_visible
+def test_grids_past_the_launch_limit_are_refused():
+    """A launch has fewer than 2^32 threads along a dimension: more are MORPH_ERANGE, with nothing enqueued,
+    not a launch that fails behind another one (a recurrence's first kernel clears its workspace)."""
+    lib, p = _lib.lib(), ctypes.c_void_p(0x10000)
+    for dtype in (0, 1, 2):
+        for rows in (1 << 34, (1 << 32) + 1):  # 2^24 workgroups and more of 256 groups
+            assert lib.morph_act_pack(p, dtype, rows, 1, 1, p, p, None) == -4
+            assert lib.morph_act_unpack(p, p, rows, 1, p, dtype, 1, None) == -4
+        for batch, steps, dim in ((65535, 16640, 8), (65535, 1 << 20, 1), (1, 1 << 31, 130), (4096, 1 << 19, 64)):
+            args = _lib.ScanArgs(0x10000, 0x10000, 0x10000, None, batch, steps, dim, *[steps * dim, dim] * 3)
+            assert lib.morph_scan_forward(ctypes.byref(args), dtype, p, p, p, p, 1 << 50, None) == -4
+            assert lib.morph_scan_backward(ctypes.byref(args), dtype, p, p, steps * dim, dim, None, p, p, p, p, p,
+                                           1 << 50, None) == -4
