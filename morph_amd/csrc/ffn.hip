@@ -12,7 +12,10 @@
 // values long; operands of other widths are copied to such rows first (ffn_pad_kernel: a
 // read and a write of them beside the product's many reads).  ffn_any_kernel takes operands of any stride
 // and alignment, any size: 64 x 64 tiles through LDS, loaded element by element along whichever index is
-// contiguous.
+// contiguous.  It runs where a width is a multiple of 8 but the address is off 16 bytes or the row stride is no
+// multiple of 8, and for dx where gate and up differ in their row strides, and it is slow: 2048 rows of 3072 x 6144
+// in BF16 take 4490 us with such a gate (255 with none, 253 with a copy of it ahead of the call), forward and
+// backward 8090 (794).
 #include <algorithm>
 #include <cmath>
 
@@ -130,6 +133,12 @@ int launch_any(FfnEpilogue e, const FfnProduct& a, hipStream_t s) {
 //   gate's gradient: 512 40 / 38 / 49 / 78, 2048: 139 / 98 / 112 / 104, 4096 (FP32 kept): 283 / 224 / 223 / 244;
 //   dx: 512 88 / 108 / 143 / 223, 2048: 282 / 197 / 173 / 247, 4096: 551 / 348 / 348 / 285;
 //   weights: 512 104 / 76 / 87 / 81, 2048: 360 / 234 / 237 / 219, 4096: 800 / 459 / 458 / 412.
+// Other widths, FP16, FP32 kept, 333 x 200 x 536 / 1024 x 768 x 2048 / 512 x 1536 x 4096 / 4096 x 768 x 2048 /
+// 2048 x 1408 x 5528 / 4096 x 2048 x 5504, all four shapes of each (K whole): what the rule takes over the best of them:
+//   gate: 1.00 / 1.00 / 1.00 / 1.00 / 1.06 / 1.00, nothing kept the same but 1.08 at 2048 x 1408 x 5528;
+//   down: 1.00 / 1.00 / 1.00 / 1.00 / 1.00 / 1.11; dx: 1.00 / 1.00 / 1.00 / 1.00 / 1.00 / 1.11;
+//   gate's gradient: 1.00 / 1.00 / 1.00 / 1.12 / 1.00 / 1.00; weights: 1.00 / 1.00 / 1.00 / 1.00 / 1.02 / 1.02.
+// So 5.9 against 8.6 to 18.1 us for down at 333 x 200 x 536, 101.7 against 158 / 91.9 / 120 at 4096 x 2048 x 5504.
 double tiles_us(FfnShape shape, int64_t tiles, int64_t kt, double epilogue) {
   const double q = (double)tiles / 256.0, n = std::ceil(q), full = q / n;
   switch (shape) {

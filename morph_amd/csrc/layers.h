@@ -27,8 +27,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 // sigmoid(x) and sigmoid(-x) from one exponential of -|x|, which neither overflows nor
-// cancels: both are accurate to a few ulp at either end, where 1 - sigmoid(x) would keep no
-// digit.  +-inf give exactly 1 and 0, NaN gives NaN.
+// cancels, so that the smaller one keeps its digits where 1 - sigmoid(x) would keep none.  The larger
+// one is accurate to a few ulp.  The smaller one's relative error grows with |x|, since the product
+// with log2(e) is rounded: up to 8 units of 2^-24 at |x| = 10, 16 at 20, 56 at 50 and 64 at 87
+// (evaluated with an exact exponential).  +-inf give exactly 1 and 0, NaN gives NaN.
 struct Sigmoid {
   float a, b;
 };

@@ -169,8 +169,8 @@ static_assert(kRun <= kWaves && kRuns <= kWaves,
               "the last wave, which fetches the stretch's first state, has no tile's or run's words to fetch");
 constexpr uint64_t kNothing = ~uint64_t(0);  // a word that is not published yet
 
-// Two floats as one word.  A pair of NaN that reads as kNothing is no result of arithmetic here
-// (the device's NaN has another payload), and would only be waited for until kSpins.
+// Two floats as one word.  A pair of NaN that reads as kNothing loses a bit of its payload, so that it
+// is not waited for.
 __device__ __forceinline__ void publish(uint64_t* at, float x, float y) {
   const uint64_t w = ((uint64_t)__builtin_bit_cast(uint32_t, y) << 32) | __builtin_bit_cast(uint32_t, x);
   __hip_atomic_store(at, w == kNothing ? w ^ 1 : w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

@@ -1,4 +1,4 @@
-"""The gated linear recurrence of a stage's mixer, over sequences and by single steps.
+"""A gated linear recurrence over sequences and by single steps.
 
     a_t = sigmoid(f_t),   s_t = a_t s_(t-1) + (1 - a_t) v_t,   y_t = s_t silu(z_t)
 
