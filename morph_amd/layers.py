@@ -80,7 +80,8 @@ class _FirstOrder(torch.autograd.Function):
     @staticmethod
     def forward(ctx, name, anchor, *grads):
         ctx.name = name
-        return grads
+        # aliases: inputs handed through would count as views of each other and refuse changes in place
+        return tuple(g.detach() if g is not None else None for g in grads)
 
     @staticmethod
     def backward(ctx, *_):

@@ -139,3 +139,19 @@ def test_grids_past_the_launch_limit_are_refused():
             assert lib.morph_scan_forward(ctypes.byref(args), dtype, p, p, p, p, 1 << 50, None) == -4
             assert lib.morph_scan_backward(ctypes.byref(args), dtype, p, p, steps * dim, dim, None, p, p, p, p, p,
                                            1 << 50, None) == -4
+
+
+def test_gradients_under_create_graph_take_changes_in_place():
+    """They are scaled and clipped as others are, share the kernels' memory, and still raise."""
+    given = torch.ones(3), None, torch.ones(2)
+    grads = layers.first_order("operator", given)
+    assert grads[1] is None and grads[0].data_ptr() == given[0].data_ptr()
+    with torch.no_grad():
+        grads[0].mul_(2)
+    scaled = grads[2].mul_(3)
+    assert (given[0] == 2).all() and (given[2] == 3).all()
+    for g in (grads[0], scaled):
+        with pytest.raises(RuntimeError, match="operator can be differentiated once"):
+            g.sum().backward()
+    with torch.no_grad():
+        assert layers.first_order("operator", given) is given
