@@ -284,6 +284,52 @@ int morph_nonfinite_table(const void* d_table, const morph_adamw_tensor* tensors
                           int grad_dtype, morph_step_state* d_state, int slot, int64_t* d_clocks,
                           const int32_t* d_prev_clock_list, int n_prev, int close, void* stream);
 
+/* ---- AdamW with its moments in 8 bits ---------------------------------------
+ * A moment of n values is G = ceil(n / 32) groups of 32 consecutive ones: 32 G codes (zeros behind
+ * the last value), then G exponent bytes, 33 G bytes in all, 4-byte aligned.  A group's scale is
+ * 2^(e - 127) with e its exponent byte.  A first moment is an E4M3 code times the scale, e the least of
+ * 1 .. 247 with every value at most 448 scales.  A second moment is an unsigned code, 5 exponent bits
+ * (bias 31) over 3 mantissa bits, times the scale, e the least of 11 .. 254 with every value at most
+ * 1.75 scales: from 2^-33 to 1.75 scales, whose root has the first moment's range.
+ *
+ * A step decodes both, updates them in FP32 as morph_adamw_multi_dev does, updates the master from those FP32
+ * values, and rounds them to codes: a value between two codes goes up with the probability of its
+ * place between them (16 bits of it), so that changes of less than a code's step, a thousandth a step with
+ * beta2 = 0.999, are not lost but happen as often as they add up to one.  A second moment that is not
+ * 0 keeps the least code at least, so that no first moment is divided by eps alone.  The 16 bits
+ * are the low (first moment) or high half (second) of
+ *   mix(place ^ mix(mix(seed + (clock_index + 1) * 0x9E3779B9) ^ t))        all modulo 2^32,
+ *   mix(x): x ^= x >> 16, x *= 0x6A09E667, x ^= x >> 15, x *= 0xBB67AE85, x ^= x >> 16
+ * with the seed in the constant set's `reserved`, t the step and place the element's index, so a step gives
+ * the same bits each time.  A moment beyond the largest float becomes it.
+ */
+#define MORPH_MOMENT_GROUP 32
+#define MORPH_MOMENT_LEAST_SECOND 11 /* 2^-33 scales are the least float then */
+
+/* morph_adamw_multi_dev, morph_adamw_table_dev with exp_avg and exp_avg_sq in this form; at most 2^30
+ * elements a tensor (MORPH_ERANGE).  Tables as morph_adamw_table_fill makes them. */
+int morph_adamw8_multi_dev(const morph_adamw_tensor* tensors, int count, int grad_dtype,
+                           int out_dtype, const morph_adamw_hp* hps,
+                           const morph_adamw_sched* scheds, int n_hp, const int64_t* d_clocks,
+                           const morph_step_state* d_state, int slot, void* start_event,
+                           void* stop_event, void* stream);
+int morph_adamw8_table_dev(const void* d_table, const morph_adamw_tensor* tensors, int count,
+                           int grad_dtype, int out_dtype, const morph_adamw_hp* hps,
+                           const morph_adamw_sched* scheds, int n_hp, const int64_t* d_clocks,
+                           const morph_step_state* d_state, int slot, void* start_event,
+                           void* stop_event, void* stream);
+
+typedef struct morph_moment_values {
+  const void* exp_avg;    /* the two moments in 8 bits */
+  const void* exp_avg_sq;
+  void* exp_avg_out;      /* numel values each */
+  void* exp_avg_sq_out;
+  int64_t numel;          /* at most 2^30 */
+} morph_moment_values;
+
+/* The values that the codes stand for, as F32, F16 or BF16. */
+int morph_moment_decode(const morph_moment_values* tensors, int count, int dtype, void* stream);
+
 /* ---- Stage-gradient accumulation ------------------------------------------
  * Replaces the reference's per-micro-batch
  *   destination.add_(g.detach().float() / loss_scale)

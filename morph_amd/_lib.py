@@ -1,4 +1,5 @@
-"""ctypes binding of libmorph_optim.so (the C ABI in include/morph_optim.h and morph_layers.h).
+"""ctypes binding of libmorph_optim.so (the C ABI in include/morph_optim.h, morph_layers.h and
+morph_state_space.h).
 
 The shared library is built in-tree by morph_amd.build into morph_amd/lib/.
 It links the same HIP runtime soname torch carries (libamdhip64.so.7), so
@@ -23,12 +24,13 @@ ADAMW_TABLE_SETS, ADAMW_TABLE_NUMEL = 8, 1 << 30  # limits of morph_adamw_table_
 DTYPE_NONE, DTYPE_F32, DTYPE_F16, DTYPE_BF16 = -1, 0, 1, 2
 HP_DIVIDE_SCALE, HP_APPLY_CLIP, HP_APPLY_DECAY, HP_LERP_LARGE = 1, 2, 4, 8
 
-# Every symbol that include/morph_optim.h and include/morph_layers.h declare.
+# Every symbol that the headers in include/ declare.
 EXPORTS = (
     "morph_abi_version", "morph_strerror", "morph_flag_clear", "morph_nonfinite_or",
     "morph_nonfinite_or_multi", "morph_adamw_fused", "morph_adamw_multi",
     "morph_adamw_multi_dev", "morph_adamw_table_bytes", "morph_adamw_table_fill",
-    "morph_adamw_table_dev", "morph_nonfinite_table", "morph_step_end", "morph_nonfinite_or_close",
+    "morph_adamw_table_dev", "morph_adamw8_multi_dev", "morph_adamw8_table_dev", "morph_moment_decode",
+    "morph_nonfinite_table", "morph_step_end", "morph_nonfinite_or_close",
     "morph_grad_partials", "morph_grad_accumulate", "morph_grad_accumulate_final_noalloc",
     "morph_sumsq_total", "morph_convert_f32", "morph_fp8_pack", "morph_fp8_unpack",
     "morph_gemm_nt_bf16", "morph_gemm_tile_edge",
@@ -39,8 +41,15 @@ EXPORTS = (
     "morph_act_pack", "morph_act_unpack",
     "morph_ffn_workspace_bytes", "morph_ffn_forward", "morph_ffn_backward",
     "morph_scan_workspace_bytes", "morph_scan_forward", "morph_scan_backward",
+    "morph_norm_workspace_bytes", "morph_norm_forward", "morph_norm_backward",
+    "morph_conv_workspace_bytes", "morph_conv_forward", "morph_conv_backward",
+    "morph_ssm_workspace_bytes", "morph_ssm_forward", "morph_ssm_backward",
 )
 SCAN_SPAN = 64  # MORPH_SCAN_SPAN
+CONV_MAX_TAPS = 4  # MORPH_CONV_MAX_TAPS
+SSM_SPAN, SSM_MAX_STATES = 64, 64  # MORPH_SSM_SPAN, MORPH_SSM_MAX_STATES
+MOMENT_GROUP = 32  # MORPH_MOMENT_GROUP
+MOMENT_NUMEL = 1 << 30  # elements of a tensor with moments in 8 bits
 ACT_SATURATE = 0x100  # MORPH_ACT_SATURATE
 GEMM_TILE_M, GEMM_TILE_N, GEMM_TILE_K = 256, 256, 64
 GEMM_SYMMETRIC = 1
@@ -69,6 +78,12 @@ class AdamwTensor(ctypes.Structure):
                 ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
                 ("out", ctypes.c_void_p), ("numel", ctypes.c_int64),
                 ("hp_index", ctypes.c_int32), ("clock_index", ctypes.c_int32)]
+
+
+class MomentValues(ctypes.Structure):
+    """morph_moment_values."""
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "exp_avg", "exp_avg_sq", "exp_avg_out", "exp_avg_sq_out")] + [("numel", ctypes.c_int64)]
 
 
 class StepState(ctypes.Structure):
@@ -126,6 +141,36 @@ class ScanArgs(ctypes.Structure):
                                             "v_step", "z_batch", "z_step")]
 
 
+class NormArgs(ctypes.Structure):
+    """morph_norm."""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "weight", "bias")] + [
+        (name, ctypes.c_int64) for name in ("rows", "cols", "x_ld")] + [
+        ("eps", ctypes.c_float), ("weight_dtype", ctypes.c_int32)]
+
+
+class ConvArgs(ctypes.Structure):
+    """morph_conv."""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "before", "weight", "bias")] + [
+        (name, ctypes.c_int64) for name in ("batch", "steps", "dim", "x_batch", "x_step")] + [
+        ("taps", ctypes.c_int32), ("weight_dtype", ctypes.c_int32)]
+
+
+class SsmArgs(ctypes.Structure):
+    """morph_ssm."""
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "x", "dt", "z", "B", "C", "A", "skip", "dt_bias", "first")] + [
+        (name, ctypes.c_int64) for name in (
+            "batch", "steps", "dim", "x_batch", "x_step", "dt_batch", "dt_step", "z_batch", "z_step",
+            "B_batch", "B_step", "C_batch", "C_step")] + [
+        ("states", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class SsmGrads(ctypes.Structure):
+    """morph_ssm_grads."""
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "dx", "ddt", "dz", "dB", "dC", "dA", "dskip", "ddt_bias", "dfirst")]
+
+
 _lib = None
 _load_lock = threading.Lock()
 
@@ -166,6 +211,13 @@ def _load():
         "morph_adamw_table_dev": ([vp, ctypes.POINTER(AdamwTensor), i32, i32, i32,
                                    ctypes.POINTER(AdamwHP), ctypes.POINTER(AdamwSched), i32,
                                    vp, vp, i32, vp, vp, vp], i32),
+        "morph_adamw8_multi_dev": ([ctypes.POINTER(AdamwTensor), i32, i32, i32,
+                                    ctypes.POINTER(AdamwHP), ctypes.POINTER(AdamwSched), i32,
+                                    vp, vp, i32, vp, vp, vp], i32),
+        "morph_adamw8_table_dev": ([vp, ctypes.POINTER(AdamwTensor), i32, i32, i32,
+                                    ctypes.POINTER(AdamwHP), ctypes.POINTER(AdamwSched), i32,
+                                    vp, vp, i32, vp, vp, vp], i32),
+        "morph_moment_decode": ([vp, i32, i32, vp], i32),
         "morph_nonfinite_table": ([vp, ctypes.POINTER(AdamwTensor), i32, i32, vp, i32, vp, vp,
                                    i32, i32, vp], i32),
         "morph_step_end": ([vp, vp, vp, i32, i32, vp], i32),
@@ -215,6 +267,17 @@ def _load():
         "morph_scan_forward": ([vp, i32, vp, vp, vp, vp, ctypes.c_size_t, vp], i32),
         "morph_scan_backward": ([vp, i32, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, ctypes.c_size_t,
                                  vp], i32),
+        "morph_norm_workspace_bytes": ([i64, i64], ctypes.c_size_t),
+        "morph_norm_forward": ([vp, i32, vp, vp, vp], i32),
+        "morph_norm_backward": ([vp, i32, vp, vp, i64, vp, vp, vp, vp, ctypes.c_size_t, vp], i32),
+        "morph_conv_workspace_bytes": ([i64, i64, i64, i32], ctypes.c_size_t),
+        "morph_conv_forward": ([vp, i32, vp, vp, vp], i32),
+        "morph_conv_backward": ([vp, i32, vp, i64, i64, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp],
+                                i32),
+        "morph_ssm_workspace_bytes": ([i64, i64, i64, i32], ctypes.c_size_t),
+        "morph_ssm_forward": ([vp, i32, vp, vp, vp, vp], i32),
+        "morph_ssm_backward": ([vp, i32, vp, vp, i64, i64, vp, ctypes.POINTER(SsmGrads), vp,
+                                ctypes.c_size_t, vp], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(handle, name)

@@ -38,6 +38,7 @@
 
 #include "adamw_table.h"
 #include "common.h"
+#include "layers.h"
 
 #ifndef MORPH_ADAMW_UNROLL
 #define MORPH_ADAMW_UNROLL 1
@@ -192,6 +193,128 @@ __device__ __forceinline__ void store_out1(void* out, int64_t i, float p) {
   }
 }
 
+// ---- moments in 8 bits (morph_optim.h) -------------------------------------------
+// A lane's four elements are a word of codes of each moment, and eight lanes have a group: its largest
+// value is found across them, its exponent byte written by the first.  Codes are padded to whole groups,
+// so a word of them never ends behind the state.
+constexpr int kGroup = MORPH_MOMENT_GROUP;
+
+__device__ __forceinline__ uint32_t mix32(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x6A09E667u;
+  x ^= x >> 15;
+  x *= 0xBB67AE85u;
+  return x ^ (x >> 16);
+}
+// The largest value of the eight lanes that share a group, in all of them.
+__device__ __forceinline__ uint32_t group_max(uint32_t x) {
+  x = quad_max(x);
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, false));  // row_half_mirror
+}
+__device__ __forceinline__ void decode_second4(uint32_t w, int e, float (&x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    x[k] = __builtin_amdgcn_ldexpf(__builtin_bit_cast(float, ((w >> (8 * k)) & 0xFFu) << 20), e - 31);
+}
+// x >= 0 scaled so that its exponent field is the code's, rounded down after 16 random bits were added
+// below the code's last one: up with the probability of the part that is cut off.
+__device__ __forceinline__ uint32_t round_code(float x, int shift, uint32_t random16) {
+  return (__builtin_bit_cast(uint32_t, __builtin_amdgcn_ldexpf(x, shift)) + (random16 << 4)) >> 20;
+}
+__device__ __forceinline__ float saturated(float x) {
+  constexpr float kMost = 0x1.FFFFFEp127f;
+  return __builtin_amdgcn_fmed3f(x, -kMost, kMost);
+}
+
+static_assert(kPerBlock == 4 * kBlock && kPerBlock % kGroup == 0, "a lane has one word of codes");
+
+struct VecRegs8 {
+  f32x4 P;
+  uint32_t M, V;
+  int em, ev;
+  float G[4];
+};
+
+template <typename GT>
+__device__ __forceinline__ void load_vector8(const TensorArg& T, int64_t base, VecRegs8& r) {
+  const int64_t e = base + threadIdx.x * 4, codes = (T.n + kGroup - 1) / kGroup * kGroup;
+  const uint8_t* m = reinterpret_cast<const uint8_t*>(T.m);
+  const uint8_t* v = reinterpret_cast<const uint8_t*>(T.v);
+  if (T.vector_ok && base + kPerBlock <= T.n) {
+    load_grad4<GT>(T.grad, e, r.G);
+    r.P = load_stream<kNT>(reinterpret_cast<const f32x4*>(T.p + e));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      r.G[k] = e + k < T.n ? load_grad1<GT>(T.grad, e + k) : 0.0f;
+      r.P[k] = e + k < T.n ? T.p[e + k] : 0.0f;
+    }
+  }
+  r.M = r.V = 0, r.em = r.ev = 1;
+  if (e < codes) {
+    r.M = load_stream<kNT>(reinterpret_cast<const uint32_t*>(m + e));
+    r.V = load_stream<kNT>(reinterpret_cast<const uint32_t*>(v + e));
+    r.em = m[codes + e / kGroup];
+    r.ev = v[codes + e / kGroup];
+  }
+}
+
+template <typename OT>
+__device__ __forceinline__ void update_vector8(const TensorArg& T, const morph_adamw_hp& hp, uint32_t key,
+                                               int64_t base, VecRegs8& r) {
+  const int64_t e = base + threadIdx.x * 4, codes = (T.n + kGroup - 1) / kGroup * kGroup;
+  float m[4], v[4];
+  uint32_t most_m = 0, most_v = 0;
+  act_decode4(r.M, act_scale(r.em), m);
+  decode_second4(r.V, r.ev, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float p = r.P[k];
+    adamw_update(r.G[k], p, m[k], v[k], hp);
+    r.P[k] = p;
+    m[k] = e + k < T.n ? saturated(m[k]) : 0.0f;
+    v[k] = e + k < T.n ? saturated(v[k]) : 0.0f;
+    most_m = max(most_m, magnitude(m[k]));
+    most_v = max(most_v, magnitude(v[k]));
+  }
+  const int em = act_exponent(group_max(most_m));
+  int ev = (int)((group_max(most_v) + 0x1FFFFFu) >> 23);
+  ev = ev < MORPH_MOMENT_LEAST_SECOND ? MORPH_MOMENT_LEAST_SECOND : ev > 254 ? 254 : ev;
+  r.M = r.V = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t random = mix32((uint32_t)(e + k) ^ key);
+    const uint32_t first = round_code(__builtin_fabsf(m[k]), 7 - em, random & 0xFFFFu) |
+                           (__builtin_bit_cast(uint32_t, m[k]) >> 31) << 7;
+    uint32_t second = round_code(v[k], 31 - ev, random >> 16);
+    second = second > 254u ? 254u : second;
+    if (v[k] > 0.0f && second == 0u) second = 1u;
+    r.M |= first << (8 * k);
+    r.V |= second << (8 * k);
+  }
+  if (T.vector_ok && base + kPerBlock <= T.n) {
+    store_stream<kNT>(reinterpret_cast<f32x4*>(T.p + e), r.P);
+    if (T.out != nullptr) store_out4<OT>(T.out, e, r.P);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (e + k < T.n) {
+        T.p[e + k] = r.P[k];
+        if (T.out != nullptr) store_out1<OT>(T.out, e + k, r.P[k]);
+      }
+  }
+  if (e < codes) {
+    uint8_t* sm = reinterpret_cast<uint8_t*>(T.m);
+    uint8_t* sv = reinterpret_cast<uint8_t*>(T.v);
+    store_stream<kNT>(reinterpret_cast<uint32_t*>(sm + e), r.M);
+    store_stream<kNT>(reinterpret_cast<uint32_t*>(sv + e), r.V);
+    if (threadIdx.x % 8 == 0) {
+      sm[codes + e / kGroup] = (uint8_t)em;
+      sv[codes + e / kGroup] = (uint8_t)ev;
+    }
+  }
+}
+
 // One lane's share of a vector chunk, held between the loads and the update.
 struct VecRegs {
   f32x4 P[kUnroll], M[kUnroll], V[kUnroll];
@@ -273,13 +396,24 @@ __device__ __forceinline__ bool control(const Args& a, const TensorArg& T,
   return true;
 }
 
+// The words that round this tensor's moments in this step are mix32(place ^ key).
+template <typename Args>
+__device__ __forceinline__ uint32_t rounding_key(const Args& a, const TensorArg& T, const morph_adamw_hp& hp) {
+  return mix32(mix32(hp.reserved + (uint32_t)(T.clock + 1) * 0x9E3779B9u) ^ (uint32_t)(a.clocks[T.clock] + 1));
+}
+
 // Block b of tensor T.
-template <typename GT, typename OT, bool kDev, typename Args>
+template <typename GT, typename OT, bool kDev, int kBits, typename Args>
 __device__ __forceinline__ void run_block(const Args& a, const TensorArg& T, int b,
                                           const uint32_t* skip) {
   const int64_t base = (int64_t)(b - T.first_block) * kPerBlock;
   morph_adamw_hp hp;
-  if (T.vector_ok && base + kPerBlock <= T.n) {
+  if constexpr (kBits == 8) {
+    VecRegs8 r;
+    load_vector8<GT>(T, base, r);
+    if (!control<kDev>(a, T, skip, hp)) return;
+    update_vector8<OT>(T, hp, rounding_key(a, T, hp), base, r);
+  } else if (T.vector_ok && base + kPerBlock <= T.n) {
     // The streams are requested before the control words, so their latency
     // overlaps; a skipped step (control false) still writes nothing.
     VecRegs r;
@@ -292,11 +426,11 @@ __device__ __forceinline__ void run_block(const Args& a, const TensorArg& T, int
   }
 }
 
-template <typename GT, typename OT, bool kDev>
+template <typename GT, typename OT, bool kDev, int kBits>
 __global__ __launch_bounds__(kBlock) void adamw_multi_kernel(const LaunchArgs a,
                                                              const uint32_t* __restrict__ skip) {
   const int b = a.reverse ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
-  run_block<GT, OT, kDev>(a, a.t[segment_of(a.t, a.count, b)], b, skip);
+  run_block<GT, OT, kDev, kBits>(a, a.t[segment_of(a.t, a.count, b)], b, skip);
 }
 
 // Many tensors in one launch (adamw_table.h): the descriptors lie in device memory, the
@@ -312,7 +446,7 @@ struct TableArgs {
 };
 static_assert(sizeof(TableArgs) + 64 <= kMaxKernargBytes, "launch table fits the kernel arguments");
 
-template <typename GT, typename OT>
+template <typename GT, typename OT, int kBits>
 __global__ __launch_bounds__(kBlock) void adamw_table_kernel(const TableArgs a,
                                                              const TableRow* __restrict__ rows,
                                                              const int32_t* __restrict__ map,
@@ -324,7 +458,7 @@ __global__ __launch_bounds__(kBlock) void adamw_table_kernel(const TableArgs a,
   const uint64_t g = a.grad[row - a.first_row];
   const TensorArg T{reinterpret_cast<const void*>(g & ~uint64_t(1)), R.p, R.m, R.v, R.out, R.n,
                     R.hp, R.first_block, (int32_t)(~g & 1), R.clock};
-  run_block<GT, OT, true>(a, T, b, skip);
+  run_block<GT, OT, true, kBits>(a, T, b, skip);
 }
 
 // Events (nullable) are stamped by the dispatch itself (hipExtLaunchKernel):
@@ -344,34 +478,39 @@ void launch_kernel(K kernel, int blocks, const LaunchArgs& a, const uint32_t* sk
                           a, skip);
 }
 
+// How a call's launches run: constants from the host, or from the device with moments in 32 or 8 bits.
+enum class Form { kHost, kDev, kDev8 };
+
 template <typename GT, typename OT>
-int launch(bool dev, const LaunchArgs& a, int blocks, const uint32_t* skip, hipStream_t s,
+int launch(Form form, const LaunchArgs& a, int blocks, const uint32_t* skip, hipStream_t s,
            Stamps ev) {
-  if (dev)
-    launch_kernel(adamw_multi_kernel<GT, OT, true>, blocks, a, skip, s, ev);
+  if (form == Form::kDev8)
+    launch_kernel(adamw_multi_kernel<GT, OT, true, 8>, blocks, a, skip, s, ev);
+  else if (form == Form::kDev)
+    launch_kernel(adamw_multi_kernel<GT, OT, true, 32>, blocks, a, skip, s, ev);
   else
-    launch_kernel(adamw_multi_kernel<GT, OT, false>, blocks, a, skip, s, ev);
+    launch_kernel(adamw_multi_kernel<GT, OT, false, 32>, blocks, a, skip, s, ev);
   return launch_status();
 }
 
 template <typename GT>
-int launch_out(bool dev, int out_dtype, const LaunchArgs& a, int blocks, const uint32_t* skip,
+int launch_out(Form form, int out_dtype, const LaunchArgs& a, int blocks, const uint32_t* skip,
                hipStream_t s, Stamps ev) {
   switch (out_dtype) {
-    case MORPH_DTYPE_NONE: return launch<GT, NoOut>(dev, a, blocks, skip, s, ev);
-    case MORPH_DTYPE_F32: return launch<GT, F32>(dev, a, blocks, skip, s, ev);
-    case MORPH_DTYPE_F16: return launch<GT, F16>(dev, a, blocks, skip, s, ev);
-    case MORPH_DTYPE_BF16: return launch<GT, BF16>(dev, a, blocks, skip, s, ev);
+    case MORPH_DTYPE_NONE: return launch<GT, NoOut>(form, a, blocks, skip, s, ev);
+    case MORPH_DTYPE_F32: return launch<GT, F32>(form, a, blocks, skip, s, ev);
+    case MORPH_DTYPE_F16: return launch<GT, F16>(form, a, blocks, skip, s, ev);
+    case MORPH_DTYPE_BF16: return launch<GT, BF16>(form, a, blocks, skip, s, ev);
     default: return MORPH_EDTYPE;
   }
 }
 
-int dispatch(bool dev, int grad_dtype, int out_dtype, const LaunchArgs& a, int blocks,
+int dispatch(Form form, int grad_dtype, int out_dtype, const LaunchArgs& a, int blocks,
              const uint32_t* skip, hipStream_t s, Stamps ev) {
   switch (grad_dtype) {
-    case MORPH_DTYPE_F32: return launch_out<F32>(dev, out_dtype, a, blocks, skip, s, ev);
-    case MORPH_DTYPE_F16: return launch_out<F16>(dev, out_dtype, a, blocks, skip, s, ev);
-    case MORPH_DTYPE_BF16: return launch_out<BF16>(dev, out_dtype, a, blocks, skip, s, ev);
+    case MORPH_DTYPE_F32: return launch_out<F32>(form, out_dtype, a, blocks, skip, s, ev);
+    case MORPH_DTYPE_F16: return launch_out<F16>(form, out_dtype, a, blocks, skip, s, ev);
+    case MORPH_DTYPE_BF16: return launch_out<BF16>(form, out_dtype, a, blocks, skip, s, ev);
     default: return MORPH_EDTYPE;
   }
 }
@@ -401,8 +540,9 @@ bool vector_ok(const void* p, const void* m, const void* v, const void* grad, in
 int enqueue(const morph_adamw_tensor* tensors, int count, int grad_dtype, int out_dtype,
             const morph_adamw_hp* hps, const morph_adamw_sched* scheds, int n_hp,
             const int64_t* clocks, const morph_step_state* state, const uint32_t* d_skip,
-            void* stream, Stamps stamps = Stamps{nullptr, nullptr}) {
+            void* stream, Stamps stamps = Stamps{nullptr, nullptr}, int bits = 32) {
   const bool dev = state != nullptr;
+  const Form form = !dev ? Form::kHost : bits == 8 ? Form::kDev8 : Form::kDev;
   if (count < 0 || (count > 0 && (tensors == nullptr || hps == nullptr)) || n_hp < 0)
     return MORPH_EINVAL;
   if (dev && (scheds == nullptr || clocks == nullptr)) return MORPH_EINVAL;
@@ -417,6 +557,10 @@ int enqueue(const morph_adamw_tensor* tensors, int count, int grad_dtype, int ou
                         t.exp_avg_sq == nullptr))
       return MORPH_EINVAL;
     if (dev && t.clock_index < 0) return MORPH_EINVAL;
+    if (bits == 8) {
+      if (t.numel > kMaxSegment) return MORPH_ERANGE;  // the exponents lie behind all codes
+      if (!aligned(t.exp_avg, 4) || !aligned(t.exp_avg_sq, 4)) return MORPH_EINVAL;
+    }
   }
   if (dev)
     for (int k = 0; k < n_hp; ++k)
@@ -438,7 +582,7 @@ int enqueue(const morph_adamw_tensor* tensors, int count, int grad_dtype, int ou
     const Stamps ev{first_launch ? stamps.e0 : nullptr, last ? stamps.e1 : nullptr};
     first_launch = false;
     a.reverse = grad_bytes > kReverseAboveBytes ? 1 : 0;
-    const int rc = dispatch(dev, grad_dtype, out_dtype, a, blocks, d_skip, s, ev);
+    const int rc = dispatch(form, grad_dtype, out_dtype, a, blocks, d_skip, s, ev);
     a.count = 0;
     n_local_hp = 0;
     blocks = 0;
@@ -516,28 +660,28 @@ int64_t table_bytes(int count, const TableShape& t) {
   return (int64_t)count * (int64_t)sizeof(TableRow) + 4 * (t.blocks + t.det_blocks);
 }
 
-template <typename GT, typename OT>
+template <typename GT, typename OT, int kBits>
 int launch_table(const TableArgs& a, const void* d_table, int count, int blocks,
                  const uint32_t* skip, hipStream_t s, Stamps ev) {
   const TableRow* rows = static_cast<const TableRow*>(d_table);
   const int32_t* map = reinterpret_cast<const int32_t*>(rows + count);
   if (ev.e0 == nullptr && ev.e1 == nullptr)
-    hipLaunchKernelGGL((adamw_table_kernel<GT, OT>), dim3(blocks), dim3(kBlock), kOccupancyLds, s,
-                       a, rows, map, skip);
+    hipLaunchKernelGGL((adamw_table_kernel<GT, OT, kBits>), dim3(blocks), dim3(kBlock), kOccupancyLds,
+                       s, a, rows, map, skip);
   else
-    hipExtLaunchKernelGGL((adamw_table_kernel<GT, OT>), dim3(blocks), dim3(kBlock), kOccupancyLds,
-                          s, ev.e0, ev.e1, 0u, a, rows, map, skip);
+    hipExtLaunchKernelGGL((adamw_table_kernel<GT, OT, kBits>), dim3(blocks), dim3(kBlock),
+                          kOccupancyLds, s, ev.e0, ev.e1, 0u, a, rows, map, skip);
   return launch_status();
 }
 
-template <typename GT>
+template <typename GT, int kBits>
 int launch_table_out(int out_dtype, const TableArgs& a, const void* d_table, int count, int blocks,
                      const uint32_t* skip, hipStream_t s, Stamps ev) {
   switch (out_dtype) {
-    case MORPH_DTYPE_NONE: return launch_table<GT, NoOut>(a, d_table, count, blocks, skip, s, ev);
-    case MORPH_DTYPE_F32: return launch_table<GT, F32>(a, d_table, count, blocks, skip, s, ev);
-    case MORPH_DTYPE_F16: return launch_table<GT, F16>(a, d_table, count, blocks, skip, s, ev);
-    case MORPH_DTYPE_BF16: return launch_table<GT, BF16>(a, d_table, count, blocks, skip, s, ev);
+    case MORPH_DTYPE_NONE: return launch_table<GT, NoOut, kBits>(a, d_table, count, blocks, skip, s, ev);
+    case MORPH_DTYPE_F32: return launch_table<GT, F32, kBits>(a, d_table, count, blocks, skip, s, ev);
+    case MORPH_DTYPE_F16: return launch_table<GT, F16, kBits>(a, d_table, count, blocks, skip, s, ev);
+    case MORPH_DTYPE_BF16: return launch_table<GT, BF16, kBits>(a, d_table, count, blocks, skip, s, ev);
     default: return MORPH_EDTYPE;
   }
 }
@@ -578,12 +722,13 @@ extern "C" int morph_adamw_table_fill(const morph_adamw_tensor* tensors, int cou
   return MORPH_OK;
 }
 
-extern "C" int morph_adamw_table_dev(const void* d_table, const morph_adamw_tensor* tensors,
-                                     int count, int grad_dtype, int out_dtype,
-                                     const morph_adamw_hp* hps, const morph_adamw_sched* scheds,
-                                     int n_hp, const int64_t* d_clocks,
-                                     const morph_step_state* d_state, int slot, void* start_event,
-                                     void* stop_event, void* stream) {
+namespace {
+
+template <int kBits>
+int enqueue_table(const void* d_table, const morph_adamw_tensor* tensors, int count, int grad_dtype,
+                  int out_dtype, const morph_adamw_hp* hps, const morph_adamw_sched* scheds, int n_hp,
+                  const int64_t* d_clocks, const morph_step_state* d_state, int slot,
+                  void* start_event, void* stop_event, void* stream) {
   TableShape shape;
   int rc = table_shape(tensors, count, grad_dtype, &shape);
   if (rc != MORPH_OK) return rc;
@@ -604,7 +749,8 @@ extern "C" int morph_adamw_table_dev(const void* d_table, const morph_adamw_tens
   }
   for (int i = 0; i < count; ++i)
     if (tensors[i].hp_index < 0 || tensors[i].hp_index >= n_hp ||
-        (tensors[i].numel > 0 && tensors[i].grad == nullptr))
+        (tensors[i].numel > 0 && tensors[i].grad == nullptr) ||
+        (kBits == 8 && (!aligned(tensors[i].exp_avg, 4) || !aligned(tensors[i].exp_avg_sq, 4))))
       return MORPH_EINVAL;
   a.clocks = d_clocks;
   a.state = d_state;
@@ -634,13 +780,35 @@ extern "C" int morph_adamw_table_dev(const void* d_table, const morph_adamw_tens
     first_launch = false;
     const uint32_t* skip = &d_state->found_inf[slot];
     switch (grad_dtype) {
-      case MORPH_DTYPE_F32: rc = launch_table_out<F32>(out_dtype, a, d_table, count, (int)blocks, skip, s, ev); break;
-      case MORPH_DTYPE_F16: rc = launch_table_out<F16>(out_dtype, a, d_table, count, (int)blocks, skip, s, ev); break;
-      default: rc = launch_table_out<BF16>(out_dtype, a, d_table, count, (int)blocks, skip, s, ev); break;
+      case MORPH_DTYPE_F32: rc = launch_table_out<F32, kBits>(out_dtype, a, d_table, count, (int)blocks, skip, s, ev); break;
+      case MORPH_DTYPE_F16: rc = launch_table_out<F16, kBits>(out_dtype, a, d_table, count, (int)blocks, skip, s, ev); break;
+      default: rc = launch_table_out<BF16, kBits>(out_dtype, a, d_table, count, (int)blocks, skip, s, ev); break;
     }
     if (rc != MORPH_OK) return rc;
   }
   return MORPH_OK;
+}
+
+}  // namespace
+
+extern "C" int morph_adamw_table_dev(const void* d_table, const morph_adamw_tensor* tensors,
+                                     int count, int grad_dtype, int out_dtype,
+                                     const morph_adamw_hp* hps, const morph_adamw_sched* scheds,
+                                     int n_hp, const int64_t* d_clocks,
+                                     const morph_step_state* d_state, int slot, void* start_event,
+                                     void* stop_event, void* stream) {
+  return enqueue_table<32>(d_table, tensors, count, grad_dtype, out_dtype, hps, scheds, n_hp, d_clocks,
+                           d_state, slot, start_event, stop_event, stream);
+}
+
+extern "C" int morph_adamw8_table_dev(const void* d_table, const morph_adamw_tensor* tensors,
+                                      int count, int grad_dtype, int out_dtype,
+                                      const morph_adamw_hp* hps, const morph_adamw_sched* scheds,
+                                      int n_hp, const int64_t* d_clocks,
+                                      const morph_step_state* d_state, int slot, void* start_event,
+                                      void* stop_event, void* stream) {
+  return enqueue_table<8>(d_table, tensors, count, grad_dtype, out_dtype, hps, scheds, n_hp, d_clocks,
+                          d_state, slot, start_event, stop_event, stream);
 }
 
 extern "C" int morph_adamw_multi(const morph_adamw_tensor* tensors, int count, int grad_dtype,
@@ -662,6 +830,109 @@ extern "C" int morph_adamw_multi_dev(const morph_adamw_tensor* tensors, int coun
   return enqueue(tensors, count, grad_dtype, out_dtype, hps, scheds, n_hp, d_clocks, d_state,
                  &d_state->found_inf[slot], stream,
                  Stamps{static_cast<hipEvent_t>(start_event), static_cast<hipEvent_t>(stop_event)});
+}
+
+extern "C" int morph_adamw8_multi_dev(const morph_adamw_tensor* tensors, int count, int grad_dtype,
+                                      int out_dtype, const morph_adamw_hp* hps,
+                                      const morph_adamw_sched* scheds, int n_hp,
+                                      const int64_t* d_clocks, const morph_step_state* d_state,
+                                      int slot, void* start_event, void* stop_event,
+                                      void* stream) {
+  if (d_state == nullptr || (slot != 0 && slot != 1)) return MORPH_EINVAL;
+  return enqueue(tensors, count, grad_dtype, out_dtype, hps, scheds, n_hp, d_clocks, d_state,
+                 &d_state->found_inf[slot], stream,
+                 Stamps{static_cast<hipEvent_t>(start_event), static_cast<hipEvent_t>(stop_event)}, 8);
+}
+
+// ---- what the moments' codes stand for -------------------------------------------
+namespace {
+
+constexpr int kValueTensors = 64;
+constexpr int kValuesPerBlock = 1024;  // 256 lanes, a word of each moment's codes
+
+struct ValueArgs {
+  morph_moment_values t[kValueTensors];
+  int32_t first_block[kValueTensors];
+  int32_t count;
+};
+static_assert(sizeof(ValueArgs) + 64 <= kMaxKernargBytes, "launch table fits the kernel arguments");
+
+template <typename T>
+__global__ __launch_bounds__(256) void moment_values_kernel(const ValueArgs a) {
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.first_block[mid] <= (int)blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const morph_moment_values& t = a.t[lo];
+  const int64_t e = (int64_t)((int)blockIdx.x - a.first_block[lo]) * kValuesPerBlock + threadIdx.x * 4;
+  if (e >= t.numel) return;
+  const int64_t codes = (t.numel + kGroup - 1) / kGroup * kGroup;
+  const uint8_t* first = static_cast<const uint8_t*>(t.exp_avg);
+  const uint8_t* second = static_cast<const uint8_t*>(t.exp_avg_sq);
+  float m[4], v[4];
+  act_decode4(*reinterpret_cast<const uint32_t*>(first + e), act_scale(first[codes + e / kGroup]), m);
+  decode_second4(*reinterpret_cast<const uint32_t*>(second + e), second[codes + e / kGroup], v);
+  const f32x4 M{m[0], m[1], m[2], m[3]}, V{v[0], v[1], v[2], v[3]};
+  constexpr int kBytes = 4 * Fmt<T>::bytes;
+  const bool wide = ((reinterpret_cast<uintptr_t>(t.exp_avg_out) | reinterpret_cast<uintptr_t>(t.exp_avg_sq_out)) %
+                     kBytes) == 0;
+  if (wide && e + 4 <= t.numel) {
+    store_out4<T>(t.exp_avg_out, e, M);
+    store_out4<T>(t.exp_avg_sq_out, e, V);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (e + k < t.numel) {
+      store_out1<T>(t.exp_avg_out, e + k, M[k]);
+      store_out1<T>(t.exp_avg_sq_out, e + k, V[k]);
+    }
+}
+
+}  // namespace
+
+extern "C" int morph_moment_decode(const morph_moment_values* tensors, int count, int dtype, void* stream) {
+  if (count < 0 || (count > 0 && tensors == nullptr)) return MORPH_EINVAL;
+  if (dtype_bytes(dtype) == 0) return MORPH_EDTYPE;
+  for (int i = 0; i < count; ++i) {
+    const morph_moment_values& t = tensors[i];
+    if (t.numel < 0 || (t.numel > 0 && (t.exp_avg == nullptr || t.exp_avg_sq == nullptr ||
+                                        t.exp_avg_out == nullptr || t.exp_avg_sq_out == nullptr ||
+                                        !aligned(t.exp_avg, 4) || !aligned(t.exp_avg_sq, 4))))
+      return MORPH_EINVAL;
+    if (t.numel > kMaxSegment) return MORPH_ERANGE;
+  }
+  hipStream_t s = as_stream(stream);
+  ValueArgs a;
+  a.count = 0;
+  int64_t blocks = 0;
+  auto flush = [&]() -> int {
+    if (a.count == 0) return MORPH_OK;
+    if (dtype == MORPH_DTYPE_F32)
+      hipLaunchKernelGGL(moment_values_kernel<F32>, dim3((int)blocks), dim3(256), 0, s, a);
+    else if (dtype == MORPH_DTYPE_F16)
+      hipLaunchKernelGGL(moment_values_kernel<F16>, dim3((int)blocks), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL(moment_values_kernel<BF16>, dim3((int)blocks), dim3(256), 0, s, a);
+    a.count = 0;
+    blocks = 0;
+    return launch_status();
+  };
+  for (int i = 0; i < count; ++i) {
+    const int64_t need = (tensors[i].numel + kValuesPerBlock - 1) / kValuesPerBlock;
+    if (need == 0) continue;
+    // a launch has fewer than 2^32 threads: 2^24 - 1 workgroups of 256
+    if (a.count == kValueTensors || blocks + need > (1 << 24) - 1) {
+      const int rc = flush();
+      if (rc != MORPH_OK) return rc;
+    }
+    a.t[a.count] = tensors[i];
+    a.first_block[a.count++] = (int32_t)blocks;
+    blocks += need;
+  }
+  return flush();
 }
 
 extern "C" int morph_adamw_fused(const void* grad, int grad_dtype, float* param, float* exp_avg,

@@ -1,0 +1,332 @@
+// Short causal convolution along the steps with silu (morph_state_space.h), and its backward pass.
+//
+// A lane has a few neighbouring channels and walks a run of steps, the last taps - 1 inputs in registers: a row of x
+// is read once by its run and once more by the next one's start.  The backward walks the same way taps - 1 steps
+// further: p and so dp of a step come from the window of x again, the gradient of x from a window of dp, and the
+// weights' gradients stay in registers over the run.  Workgroups take runs of several sequences so that at most
+// kParts rows of partial sums are left for a second launch.  HBM bounds both.
+#include "stage.h"
+
+namespace morph {
+namespace {
+
+constexpr int kRun = 16;      // steps of a wave, forward
+constexpr int kBackRun = 32;  // and backward
+constexpr int kAhead = 4;     // steps whose loads are issued together
+constexpr int kParts = 512;
+
+// kCount neighbouring channels.
+template <typename T, int kCount>
+struct Lanes {
+  static __device__ __forceinline__ void load(const void* p, int64_t at, int64_t n, float (&x)[kCount]) {
+    if constexpr (kCount == Wide<T>::kCount) {
+      Wide<T>::unpack(Wide<T>::load(p, at, n), x);
+    } else {
+      static_assert(Fmt<T>::bytes == 2 && kCount == 4, "half of an access");
+      const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+      typedef uint32_t pair __attribute__((ext_vector_type(2), aligned(2)));
+      u32x2 w = 0;
+      if (n >= 4) {
+        w = *reinterpret_cast<const pair*>(q);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < n) w[k / 2] |= (uint32_t)q[k] << (16 * (k % 2));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = to_float<T>(k % 2 ? w[k / 2] >> 16 : w[k / 2] & 0xFFFFu);
+    }
+  }
+  static __device__ __forceinline__ void store(void* p, int64_t at, int64_t n, const float (&x)[kCount]) {
+    if constexpr (kCount == Wide<T>::kCount) {
+      Wide<T>::store(p, at, Wide<T>::pack(x), n);
+    } else {
+      uint16_t* q = static_cast<uint16_t*>(p) + at;
+      typedef uint32_t pair __attribute__((ext_vector_type(2), aligned(2)));
+      const u32x2 w{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+      if (n >= 4) {
+        *reinterpret_cast<pair*>(q) = w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < n) q[k] = (uint16_t)(w[k / 2] >> (16 * (k % 2)));
+      }
+    }
+  }
+};
+
+template <typename W, int kTaps, int kCount>
+__device__ __forceinline__ void load_taps(const morph_conv& a, int64_t c, int64_t n, float (&w)[kTaps][kCount],
+                                          float (&bias)[kCount]) {
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) {
+    bias[i] = a.bias && i < n ? load_one<W>(a.bias, c + i) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < kTaps; ++k) w[k][i] = i < n ? load_one<W>(a.weight, (c + i) * kTaps + k) : 0.0f;
+  }
+}
+
+// x of step t of sequence b, where t may lie before the first step; 0 behind the last one.
+template <typename T, int kCount>
+__device__ __forceinline__ void load_input(const morph_conv& a, int64_t b, int64_t t, int64_t c, int64_t n,
+                                           float (&x)[kCount]) {
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) x[i] = 0.0f;
+  if (t >= 0) {
+    if (t < a.steps) Lanes<T, kCount>::load(a.x, b * a.x_batch + t * a.x_step + c, n, x);
+  } else if (a.before) {
+    Lanes<T, kCount>::load(a.before, (b * (a.taps - 1) + t + a.taps - 1) * a.dim + c, n, x);
+  }
+}
+
+struct ConvGrid {
+  int64_t channel_blocks, time_blocks;
+};
+
+template <typename T, typename W, int kTaps>
+__global__ __launch_bounds__(256) void conv_kernel(const morph_conv a, const ConvGrid g, void* __restrict__ y,
+                                                   void* __restrict__ after) {
+  constexpr int V = Wide<T>::kCount;
+  const int64_t block = blockIdx.x, cb = block % g.channel_blocks, rest = block / g.channel_blocks;
+  const int64_t tb = rest % g.time_blocks, b = rest / g.time_blocks;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t c = (cb * 64 + (threadIdx.x & 63)) * V, n = a.dim - c;
+  if (n <= 0) return;
+  const int64_t t0 = (tb * 4 + wave) * kRun;
+  if (t0 < a.steps) {
+    float w[kTaps][V], bias[V], x[kTaps - 1 + kAhead][V];
+    load_taps<W, kTaps, V>(a, c, n, w, bias);
+#pragma unroll
+    for (int k = 0; k < kTaps - 1; ++k) load_input<T, V>(a, b, t0 - (kTaps - 1) + k, c, n, x[k]);
+    for (int64_t t = t0; t < t0 + kRun && t < a.steps; t += kAhead) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) load_input<T, V>(a, b, t + i, c, n, x[kTaps - 1 + i]);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (t + i >= a.steps) break;
+        float out[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float p = bias[j];
+#pragma unroll
+          for (int k = 0; k < kTaps; ++k) p = __fmaf_rn(w[k][j], x[i + k][j], p);
+          out[j] = p * gate_sigmoid(p);
+        }
+        Lanes<T, V>::store(y, (b * a.steps + t + i) * a.dim + c, n, out);
+      }
+#pragma unroll
+      for (int k = 0; k < kTaps - 1; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[k][j] = x[kAhead + k][j];
+    }
+  }
+  if (tb == g.time_blocks - 1 && wave == 0) {  // a copy: the conversion to FP32 and back changes nothing
+#pragma unroll
+    for (int k = 0; k < kTaps - 1; ++k) {
+      float x[V];
+      load_input<T, V>(a, b, a.steps - (kTaps - 1) + k, c, n, x);
+      Lanes<T, V>::store(after, (b * (kTaps - 1) + k) * a.dim + c, n, x);
+    }
+  }
+}
+
+// run: steps of a wave.  parts: [gridDim.y][taps + 1][dim].
+template <typename T, typename W, int kTaps>
+__global__ __launch_bounds__(256) void conv_back_kernel(const morph_conv a, const ConvGrid g, int run,
+                                                        const void* __restrict__ dy, int64_t dy_batch, int64_t dy_step,
+                                                        const void* __restrict__ dafter, void* __restrict__ dx,
+                                                        void* __restrict__ dbefore, float* __restrict__ parts) {
+  constexpr int V = 4;
+  __shared__ float join[kTaps + 1][V][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * V, n = a.dim - c;
+  float w[kTaps][V], bias[V], dw[kTaps + 1][V];
+  load_taps<W, kTaps, V>(a, c, n, w, bias);
+#pragma unroll
+  for (int k = 0; k <= kTaps; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[k][j] = 0.0f;
+  for (int64_t unit = blockIdx.y; unit < a.batch * g.time_blocks; unit += gridDim.y) {
+    const int64_t b = unit / g.time_blocks, t0 = ((unit % g.time_blocks) * 4 + wave) * run;
+    if (n <= 0 || (t0 >= a.steps && t0 > 0)) continue;
+    // x[k], d[k]: of step t - (kTaps - 1) + k; d is dp
+    float x[kTaps - 1 + kAhead][V], d[kTaps - 1 + kAhead][V];
+#pragma unroll
+    for (int k = 0; k < kTaps - 1; ++k) {
+      load_input<T, V>(a, b, t0 - (kTaps - 1) + k, c, n, x[k]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[k][j] = 0.0f;  // earlier runs' shares of dx of steps that are theirs
+    }
+    const int64_t end = t0 + run + kTaps - 1;
+    for (int64_t t = t0; t < end && t < a.steps + kTaps - 1; t += kAhead) {
+      float dys[kAhead][V];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        load_input<T, V>(a, b, t + i, c, n, x[kTaps - 1 + i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) dys[i][j] = 0.0f;
+        if (t + i < a.steps && t + i < end) Lanes<T, V>::load(dy, b * dy_batch + (t + i) * dy_step + c, n, dys[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const bool mine = t + i < t0 + run;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float p = bias[j];
+#pragma unroll
+          for (int k = 0; k < kTaps; ++k) p = __fmaf_rn(w[k][j], x[i + k][j], p);
+          const float e = dys[i][j] * silu(p).slope;
+          d[kTaps - 1 + i][j] = e;
+          if (mine) {
+#pragma unroll
+            for (int k = 0; k < kTaps; ++k) dw[k][j] = __fmaf_rn(e, x[i + k][j], dw[k][j]);
+            dw[kTaps][j] += e;
+          }
+        }
+        // the step whose last share this was
+        const int64_t at = t + i - (kTaps - 1);
+        if (at >= a.steps || at >= t0 + run || (at < t0 && t0 > 0)) continue;
+        float out[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          out[j] = 0.0f;
+#pragma unroll
+          for (int k = 0; k < kTaps; ++k) out[j] = __fmaf_rn(w[k][j], d[kTaps - 1 + i - k][j], out[j]);
+        }
+        if (dafter && at + kTaps - 1 >= a.steps) {
+          float more[V];
+          Lanes<T, V>::load(dafter, (b * (kTaps - 1) + at + kTaps - 1 - a.steps) * a.dim + c, n, more);
+#pragma unroll
+          for (int j = 0; j < V; ++j) out[j] += j < n ? more[j] : 0.0f;
+        }
+        if (at >= 0) Lanes<T, V>::store(dx, (b * a.steps + at) * a.dim + c, n, out);
+        else if (dbefore) Lanes<T, V>::store(dbefore, (b * (kTaps - 1) + at + kTaps - 1) * a.dim + c, n, out);
+      }
+#pragma unroll
+      for (int k = 0; k < kTaps - 1; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[k][j] = x[kAhead + k][j], d[k][j] = d[kAhead + k][j];
+    }
+  }
+  for (int i = 0; i < 4; ++i) {  // in the waves' order
+    if (wave == i) {
+#pragma unroll
+      for (int k = 0; k <= kTaps; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) join[k][j][lane] = dw[k][j] += i ? join[k][j][lane] : 0.0f;
+    }
+    __syncthreads();
+  }
+  if (wave != 3 || n <= 0) return;
+#pragma unroll
+  for (int k = 0; k <= kTaps; ++k)
+    Lanes<F32, V>::store(parts, ((int64_t)blockIdx.y * (kTaps + 1) + k) * a.dim + c, n, dw[k]);
+}
+
+template <typename W>
+__global__ __launch_bounds__(1024) void conv_sum_kernel(const float* __restrict__ parts, int count, int64_t dim, int taps,
+                                                        void* __restrict__ dweight, void* __restrict__ dbias) {
+  __shared__ float join[16][64];
+  const int lane = threadIdx.x & 63, stretch = threadIdx.x >> 6, k = blockIdx.y;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  void* out = k < taps ? dweight : dbias;
+  if (!out) return;
+  float sum = 0.0f;
+  if (c < dim) {
+    const int each = (count + 15) / 16, from = stretch * each, to = from + each < count ? from + each : count;
+    const float* p = parts + (int64_t)k * dim + c;
+#pragma unroll 8
+    for (int i = from; i < to; ++i) sum += p[(int64_t)i * (taps + 1) * dim];
+  }
+  join[stretch][lane] = sum;
+  __syncthreads();
+  if (stretch != 0 || c >= dim) return;
+  sum = join[0][lane];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) sum += join[i][lane];
+  store_one<W>(out, k < taps ? c * taps + k : c, sum);
+}
+
+template <typename F>
+int by_taps(int taps, F&& f) {
+  switch (taps) {
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    default: return f(std::integral_constant<int, 4>{});
+  }
+}
+
+int check(const morph_conv* a, int dtype) {
+  if (!a || a->batch < 0 || a->steps < 0 || a->dim < 0) return MORPH_EINVAL;
+  if (a->taps < 2 || a->taps > MORPH_CONV_MAX_TAPS) return MORPH_ERANGE;
+  if (!known_dtype(dtype) || (a->weight_dtype != MORPH_DTYPE_F32 && a->weight_dtype != dtype)) return MORPH_EDTYPE;
+  if (a->batch > 0 && a->dim > 0 && ((a->steps > 0 && !a->x) || !a->weight)) return MORPH_EINVAL;
+  return MORPH_OK;
+}
+
+int64_t over(int64_t n, int64_t by) { return (n + by - 1) / by; }
+
+int64_t back_parts(int64_t batch, int64_t steps) {
+  const int64_t units = batch * (steps > 0 ? over(steps, 4 * kBackRun) : 1);
+  return units < kParts ? units : kParts;
+}
+
+}  // namespace
+}  // namespace morph
+
+using namespace morph;
+
+extern "C" int morph_conv_forward(const morph_conv* a, int dtype, void* y, void* after, void* stream) {
+  if (const int rc = check(a, dtype)) return rc;
+  if (a->batch == 0 || a->dim == 0) return MORPH_OK;
+  if ((a->steps > 0 && !y) || !after) return MORPH_EINVAL;
+  return by_dtypes(dtype, a->weight_dtype, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    const ConvGrid g{over(a->dim, 64 * Wide<T>::kCount), a->steps > 0 ? over(a->steps, 4 * kRun) : 1};
+    if (g.time_blocks > (INT64_MAX >> 16) / g.channel_blocks / a->batch ||
+        !launchable(g.channel_blocks * g.time_blocks * a->batch, 256))
+      return (int)MORPH_ERANGE;
+    return by_taps(a->taps, [&](auto k) {
+      hipLaunchKernelGGL((conv_kernel<T, W, decltype(k)::value>),
+                         dim3((unsigned)(g.channel_blocks * g.time_blocks * a->batch)), dim3(256), 0, as_stream(stream), *a,
+                         g, y, after);
+      return launch_status();
+    });
+  });
+}
+
+extern "C" size_t morph_conv_workspace_bytes(int64_t batch, int64_t steps, int64_t dim, int taps) {
+  if (batch < 0 || steps < 0 || dim < 0 || taps < 0) return 0;
+  return (size_t)back_parts(batch, steps) * (size_t)(taps + 1) * (size_t)dim * sizeof(float);
+}
+
+extern "C" int morph_conv_backward(const morph_conv* a, int dtype, const void* dy, int64_t dy_batch, int64_t dy_step,
+                                   const void* dafter, void* dx, void* dweight, void* dbias, void* dbefore,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check(a, dtype)) return rc;
+  if (a->dim == 0) return MORPH_OK;
+  if (!dweight || (a->batch > 0 && a->steps > 0 && (!dy || !dx))) return MORPH_EINVAL;
+  const size_t need = morph_conv_workspace_bytes(a->batch, a->steps, a->dim, a->taps);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return MORPH_EWORKSPACE;
+  const int64_t blocks = over(a->dim, 256), sum_blocks = over(a->dim, 64);
+  if (!launchable(blocks, 256) || !launchable(sum_blocks, 1024)) return MORPH_ERANGE;
+  const ConvGrid g{blocks, a->steps > 0 ? over(a->steps, 4 * kBackRun) : 1};
+  const int parts = (int)back_parts(a->batch, a->steps);
+  return by_dtypes(dtype, a->weight_dtype, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    if (parts > 0) {
+      const int rc = by_taps(a->taps, [&](auto k) {
+        hipLaunchKernelGGL((conv_back_kernel<T, W, decltype(k)::value>), dim3((unsigned)blocks, parts), dim3(256), 0,
+                           as_stream(stream), *a, g, kBackRun, dy, dy_batch, dy_step, dafter, dx, dbefore,
+                           static_cast<float*>(workspace));
+        return launch_status();
+      });
+      if (rc != MORPH_OK) return rc;
+    }
+    hipLaunchKernelGGL(conv_sum_kernel<W>, dim3((unsigned)sum_blocks, a->taps + 1), dim3(1024), 0, as_stream(stream),
+                       static_cast<const float*>(workspace), parts, a->dim, a->taps, dweight, dbias);
+    return launch_status();
+  });
+}

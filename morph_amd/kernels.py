@@ -64,8 +64,9 @@ class AdamwBatch:
     """
 
     def __init__(self, params, exp_avgs, exp_avg_sqs, grads, outs=None, hp_index=None,
-                 clock_index=None):
+                 clock_index=None, state_bits=32):
         n = len(params)
+        self.state_bits = state_bits
         if not (len(exp_avgs) == len(exp_avg_sqs) == len(grads) == n):
             raise ValueError("params, exp_avgs, exp_avg_sqs and grads must have equal length")
         outs = list(outs) if outs is not None else [None] * n
@@ -87,10 +88,13 @@ class AdamwBatch:
             p, m, v, g, o = params[i], exp_avgs[i], exp_avg_sqs[i], grads[i], outs[i]
             for name, t in (("param", p), ("exp_avg", m), ("exp_avg_sq", v), ("grad", g)):
                 require_device_tensor(t, f"{name}[{i}]")
-            for name, t in (("param", p), ("exp_avg", m), ("exp_avg_sq", v)):
-                if t.dtype != torch.float32:
-                    raise TypeError(f"{name}[{i}] must be float32, got {t.dtype}")
-            if not (m.numel() == v.numel() == g.numel() == p.numel()):
+            moment = torch.uint8 if state_bits == 8 else torch.float32
+            for name, t, dtype in (("param", p, torch.float32), ("exp_avg", m, moment),
+                                   ("exp_avg_sq", v, moment)):
+                if t.dtype != dtype:
+                    raise TypeError(f"{name}[{i}] must be {str(dtype)[6:]}, got {t.dtype}")
+            held = moment8_bytes(p.numel()) if state_bits == 8 else p.numel()
+            if not (m.numel() == v.numel() == held and g.numel() == p.numel()):
                 raise ValueError(f"tensor {i}: param/exp_avg/exp_avg_sq/grad sizes differ")
             if not (p.device == m.device == v.device == g.device):
                 raise ValueError(f"tensor {i}: tensors on different devices")
@@ -204,8 +208,11 @@ class AdamwBatch:
             self.out_dtype, self._table.data_ptr() if self._table is not None else 0,
             clocks.data_ptr(), state.data_ptr(),
             [_lib.entry_address(name) for name in (
-                "morph_nonfinite_or_multi", "morph_nonfinite_or_close", "morph_adamw_multi_dev",
-                "morph_nonfinite_table", "morph_adamw_table_dev")])
+                "morph_nonfinite_or_multi", "morph_nonfinite_or_close", self._entry("multi"),
+                "morph_nonfinite_table", self._entry("table"))])
+
+    def _entry(self, form):
+        return f"morph_adamw{'8' if self.state_bits == 8 else ''}_{form}_dev"
 
     def used_on(self, stream):
         """Keep the batch's masters, moments and exports for the work queued on `stream`."""
@@ -257,14 +264,37 @@ class AdamwBatch:
         sarr = (_lib.AdamwSched * len(scheds))(*scheds)
         e0, e1 = _event_handles(events)
         if self._table is not None and len(hps) <= _lib.ADAMW_TABLE_SETS:
-            check(lib().morph_adamw_table_dev(self._use_table(stream), self.array, self.count,
-                                              self.grad_dtype, self.out_dtype, harr, sarr,
-                                              len(hps), _ptr(clocks), _ptr(state), slot, e0, e1,
-                                              stream_handle(stream)))
+            check(getattr(lib(), self._entry("table"))(
+                self._use_table(stream), self.array, self.count, self.grad_dtype, self.out_dtype,
+                harr, sarr, len(hps), _ptr(clocks), _ptr(state), slot, e0, e1,
+                stream_handle(stream)))
             return
-        check(lib().morph_adamw_multi_dev(self.array, self.count, self.grad_dtype,
-                                          self.out_dtype, harr, sarr, len(hps), _ptr(clocks),
-                                          _ptr(state), slot, e0, e1, stream_handle(stream)))
+        check(getattr(lib(), self._entry("multi"))(
+            self.array, self.count, self.grad_dtype, self.out_dtype, harr, sarr, len(hps),
+            _ptr(clocks), _ptr(state), slot, e0, e1, stream_handle(stream)))
+
+
+def moment8_bytes(numel):
+    """Bytes of a moment in 8 bits: the codes of whole groups, and an exponent for each."""
+    return -(-numel // _lib.MOMENT_GROUP) * (_lib.MOMENT_GROUP + 1)
+
+
+def moment_decode(states, outs, numels, dtype, stream=None):
+    """The values of moments in 8 bits: (exp_avg, exp_avg_sq) pairs into pairs of `dtype` tensors."""
+    array = (_lib.MomentValues * max(len(states), 1))()
+    for i, ((m, v), (om, ov), n) in enumerate(zip(states, outs, numels)):
+        for name, t in (("exp_avg", m), ("exp_avg_sq", v)):
+            require_device_tensor(t, f"{name}[{i}]")
+            if t.dtype != torch.uint8 or t.numel() != moment8_bytes(n):
+                raise ValueError(f"{name}[{i}] is not a moment of {n} values in 8 bits")
+        for t in (om, ov):
+            require_device_tensor(t, f"out[{i}]")
+            if t.dtype != dtype or t.numel() != n or t.device != m.device:
+                raise ValueError(f"out[{i}] must hold {n} values of {dtype} on {m.device}")
+        a = array[i]
+        a.exp_avg, a.exp_avg_sq, a.exp_avg_out, a.exp_avg_sq_out, a.numel = (
+            m.data_ptr(), v.data_ptr(), om.data_ptr(), ov.data_ptr(), n)
+    check(lib().morph_moment_decode(array, len(states), dtype_code(dtype), stream_handle(stream)))
 
 
 class DispatchTimer:

@@ -28,6 +28,7 @@ import torch
 from . import _lib, kernels
 from .control import BiasTables, StepControl
 from .hyper import adamw_constants
+from .layers import running_on
 from .precision import DynamicLossScale
 
 _OVERFLOW_POLICIES = ("skip", "raise")
@@ -80,11 +81,24 @@ class FusedAdamW:
       Writes the counter cannot see -- through `p.data`, a NumPy view or raw
       memory -- must be followed by invalidate_masters().  Each step then moves
       the masters one way (down) instead of both.
+    state_bits: 8 keeps both moments in 8 bits (morph_optim.h has the form): 16 bytes a
+      parameter cross HBM in a step instead of 28, and 2 stay there instead of 8.  The update
+      is the same, from the FP32 moments of the step; only what is kept of them is rounded, without
+      bias, by bits that follow from `rounding_seed` (32 bits), the parameter's index, its step and
+      the element's place, so that a run gives the same bits again.  state[p]["exp_avg"] and
+      "exp_avg_sq" are then the codes and exponents as uint8; moments() gives their values.
+      Masters on the GPU only, at most 2^30 elements each, and no arena.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
                  loss_scale=None, export_dtype=None, on_overflow="skip", sync=False,
-                 arena=False, resident_masters=False):
+                 arena=False, resident_masters=False, state_bits=32, rounding_seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not 0 <= rounding_seed < 1 << 32:
+            raise ValueError("rounding_seed must fit 32 bits")
+        if state_bits == 8 and arena:
+            raise ValueError("arena=True lays out moments of 32 bits; state_bits is 8")
         if on_overflow not in _OVERFLOW_POLICIES:
             raise ValueError(f"on_overflow must be one of {_OVERFLOW_POLICIES}")
         if not 0.0 <= lr:
@@ -96,6 +110,7 @@ class FusedAdamW:
         self.on_overflow = on_overflow
         self.sync = sync or on_overflow == "raise"
         self.export_dtype = export_dtype
+        self.state_bits, self.rounding_seed = state_bits, int(rounding_seed)
         self.state = {}
         self.exports = []
         flat = self._flat()
@@ -109,7 +124,11 @@ class FusedAdamW:
                 raise TypeError("FusedAdamW keeps FP32 masters; got " + str(p.dtype))
             if device is not None and p.device != device:
                 raise ValueError("all parameters must be on one device")
+            if state_bits == 8 and p.numel() > _lib.MOMENT_NUMEL:
+                raise ValueError(f"state_bits=8 takes at most {_lib.MOMENT_NUMEL} elements a parameter")
             device = p.device
+        if state_bits == 8 and device.type == "cpu":
+            raise ValueError("state_bits=8 needs masters on the GPU; these are on the CPU")
         self._staging = None   # HostStaging of CPU masters (None: masters on the GPU)
         self._grad_staging = None
         self.resident_masters = bool(resident_masters)
@@ -137,8 +156,8 @@ class FusedAdamW:
             self._dev = [p for _, p in flat]
         else:
             for (_, p), d in zip(flat, self._dev):
-                self.state[p] = {"step": 0, "exp_avg": torch.zeros_like(d),
-                                 "exp_avg_sq": torch.zeros_like(d)}
+                self.state[p] = {"step": 0, "exp_avg": self._new_moment(d),
+                                 "exp_avg_sq": self._new_moment(d)}
                 if export_dtype is not None:
                     self.exports.append(d.detach().to(export_dtype))
         self.device = device
@@ -162,6 +181,40 @@ class FusedAdamW:
         self.dispatch_timer = None  # optional kernels.DispatchTimer: stamps each AdamW launch
         self.skipped_steps = 0
         self.applied_steps = 0
+
+    def _new_moment(self, p):
+        if self.state_bits == 8:
+            return torch.zeros(kernels.moment8_bytes(p.numel()), dtype=torch.uint8, device=p.device)
+        return torch.zeros_like(p)
+
+    @torch.no_grad()
+    def moments(self, dtype=None, out=None, stream=None):
+        """(exp_avg, exp_avg_sq) of every parameter as values, in the parameters' shapes, behind the
+        steps that are queued on the current stream (or `stream`).  dtype: FP32 (the default), FP16
+        or BF16, which holds what 8 bits stand for exactly.  out: pairs of contiguous tensors of one
+        dtype to write instead of new ones.  With 32-bit moments: copies of them."""
+        flat = [p for _, p in self._flat()]
+        if out is not None:
+            out = [tuple(pair) for pair in out]
+            if len(out) != len(flat) or any(len(pair) != 2 for pair in out):
+                raise ValueError("one pair of output tensors per parameter")
+            dtypes = {t.dtype for pair in out for t in pair}
+            if len(dtypes) != 1 or (dtype is not None and dtypes != {dtype}):
+                raise ValueError("the output tensors must share one dtype")
+            dtype = dtypes.pop()
+        dtype = torch.float32 if dtype is None else dtype
+        _lib.dtype_code(dtype)
+        with running_on(self.device, stream):
+            if out is None:
+                out = [tuple(torch.empty(p.shape, dtype=dtype, device=self.device) for _ in range(2)) for p in flat]
+            held = [(self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"]) for p in flat]
+            if self.state_bits == 8:
+                kernels.moment_decode(held, out, [p.numel() for p in flat], dtype)
+            else:
+                for pair, given in zip(out, held):
+                    for o, t in zip(pair, given):
+                        o.copy_(t.view(o.shape))
+        return out
 
     @property
     def loss_scale(self):
@@ -282,7 +335,8 @@ class FusedAdamW:
                 [self._dev[i] for i in present], [self.state[p]["exp_avg"] for p in ps],
                 [self.state[p]["exp_avg_sq"] for p in ps], [grads[i] for i in present],
                 [self.exports[i] for i in present] if self.exports else None,
-                hp_index=[hp_of[flat[i][0]] for i in present], clock_index=list(present))
+                hp_index=[hp_of[flat[i][0]] for i in present], clock_index=list(present),
+                state_bits=self.state_bits)
             batch.make_table(kept=False)
             clock_list = torch.tensor(present, dtype=torch.int32).to(self.device)
             self._cache = [batch, clock_list, ptrs, groups]
@@ -321,6 +375,8 @@ class FusedAdamW:
             beta1, beta2 = group["betas"]
             hps.append(adamw_constants(lr=group["lr"], beta1=beta1, beta2=beta2, eps=group["eps"],
                                        weight_decay=group["weight_decay"], step=1))
+            if self.state_bits == 8:
+                hps[-1].reserved = self.rounding_seed
             table = self._table(group["betas"])
             if need > table.length:
                 table.ensure(need)
@@ -627,6 +683,11 @@ class FusedAdamW:
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             if len(saved["params"]) != len(group["params"]):
                 raise ValueError("loaded state dict contains a group of a different size")
+        for i, p in enumerate(flat):
+            for name in ("exp_avg", "exp_avg_sq") if self.state_bits == 8 and i in state_dict["state"] else ():
+                saved = state_dict["state"][i][name]
+                if saved.dtype != torch.uint8 or saved.numel() != self.state[p][name].numel():
+                    raise ValueError(f"loaded {name} of parameter {i} is not in 8 bits of its size")
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for k, v in saved.items():
                 if k != "params":
