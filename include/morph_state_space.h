@@ -90,8 +90,9 @@ int morph_conv_backward(const morph_conv* conv, int dtype, const void* dy, int64
  * kept: float [batch, ceil(steps / MORPH_SSM_SPAN), dim, states], the state that each span of steps begins
  * with; written by the forward (NULL: not), read by the backward.
  */
-#define MORPH_SSM_SPAN 64
+#define MORPH_SSM_SPAN 32
 #define MORPH_SSM_MAX_STATES 64
+#define MORPH_SSM_MAX_STEP (1 << 25) /* of dim and of the step strides, in elements */
 
 typedef struct morph_ssm {
   const void* x;
@@ -109,9 +110,11 @@ typedef struct morph_ssm {
   int32_t reserved;     /* 0 */
 } morph_ssm;
 
+/* Bytes of the workspace (16-byte aligned, any contents) of a forward (backward = 0) or backward; may be 0. */
+size_t morph_ssm_workspace_bytes(int64_t batch, int64_t steps, int64_t dim, int states, int backward);
 /* y: [batch, steps, dim] contiguous; last: [batch, dim, states]. */
-int morph_ssm_forward(const morph_ssm* ssm, int dtype, void* y, float* last, float* kept, void* stream);
-size_t morph_ssm_workspace_bytes(int64_t batch, int64_t steps, int64_t dim, int states);
+int morph_ssm_forward(const morph_ssm* ssm, int dtype, void* y, float* last, float* kept, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* What a backward writes, all contiguous; NULL only where the forward had none of it (dz, dskip,
  * ddt_bias) and for dfirst. */

@@ -47,7 +47,7 @@ EXPORTS = (
 )
 SCAN_SPAN = 64  # MORPH_SCAN_SPAN
 CONV_MAX_TAPS = 4  # MORPH_CONV_MAX_TAPS
-SSM_SPAN, SSM_MAX_STATES = 64, 64  # MORPH_SSM_SPAN, MORPH_SSM_MAX_STATES
+SSM_SPAN, SSM_MAX_STATES, SSM_MAX_STEP = 32, 64, 1 << 25  # MORPH_SSM_*
 MOMENT_GROUP = 32  # MORPH_MOMENT_GROUP
 MOMENT_NUMEL = 1 << 30  # elements of a tensor with moments in 8 bits
 ACT_SATURATE = 0x100  # MORPH_ACT_SATURATE
@@ -274,8 +274,8 @@ def _load():
         "morph_conv_forward": ([vp, i32, vp, vp, vp], i32),
         "morph_conv_backward": ([vp, i32, vp, i64, i64, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp],
                                 i32),
-        "morph_ssm_workspace_bytes": ([i64, i64, i64, i32], ctypes.c_size_t),
-        "morph_ssm_forward": ([vp, i32, vp, vp, vp, vp], i32),
+        "morph_ssm_workspace_bytes": ([i64, i64, i64, i32, i32], ctypes.c_size_t),
+        "morph_ssm_forward": ([vp, i32, vp, vp, vp, vp, ctypes.c_size_t, vp], i32),
         "morph_ssm_backward": ([vp, i32, vp, vp, i64, i64, vp, ctypes.POINTER(SsmGrads), vp,
                                 ctypes.c_size_t, vp], i32),
     }

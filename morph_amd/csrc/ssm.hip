@@ -19,17 +19,20 @@
 // lane swaps, stay in registers over the workgroup's channel groups, and are added up over the workgroups by a
 // second launch; the sums over steps (dA, dskip, ddt_bias) stay with the lane and are joined at the end.
 // No atomics: a call gives the same bits each time.
+#include <initializer_list>
+
 #include "stage.h"
 
 namespace morph {
 namespace {
 
 constexpr int kT = 8;  // steps of a wave
-constexpr int kW = 8;  // waves
+constexpr int kW = 4;  // waves
 static_assert(kT * kW == MORPH_SSM_SPAN, "a backward tile begins with a kept state");
-constexpr float kLog2e = 1.44269504088896341f;
-constexpr int kMostGroups = 4;     // channel groups of a backward workgroup
-constexpr int kBackBlocks = 512;   // workgroups from which on they get more than one
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr int kMostGroups = 2;     // channel groups of a backward workgroup
+constexpr int kBusy = 512;         // workgroups that keep the chip busy, so that sequences stay whole
+constexpr int kFull = 768;         // workgroups that it holds at a time
 
 typedef float Four[4];
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -77,6 +80,30 @@ __device__ __forceinline__ float channel_sum(float x) {
   return x;
 }
 
+// The sums over a channel's lanes of kT values, each to the lane whose step it is.  With four lanes a channel four
+// steps are summed together: each pair takes one addition and two selections between lanes that differ in
+// one bit, and half as many pairs are left for the other.
+template <int L>
+struct Sums {
+  float held[4], out[L <= kT ? kT / L : 1];
+  // The value of step t, all of them in descending order.
+  template <int t>
+  __device__ __forceinline__ void take(float x, int own) {
+    if constexpr (L == 4) {
+      held[t % 4] = x;
+      if constexpr (t % 4 == 0) {
+        const bool odd = own & 1, high = own & 2;
+        const float a = (odd ? held[1] : held[0]) + dpp<0xB1>(odd ? held[0] : held[1]);  // quad_perm [1,0,3,2]
+        const float b = (odd ? held[3] : held[2]) + dpp<0xB1>(odd ? held[2] : held[3]);
+        out[t / 4] = (high ? b : a) + dpp<0x4E>(high ? a : b);  // quad_perm [2,3,0,1]
+      }
+    } else {
+      const float s = channel_sum<L>(x);
+      if (own == t % L) out[t / L] = s;
+    }
+  }
+};
+
 __device__ __forceinline__ void swap32(float& a, float& b) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
   a = __builtin_bit_cast(float, (uint32_t)r[0]), b = __builtin_bit_cast(float, (uint32_t)r[1]);
@@ -122,52 +149,125 @@ template <typename T>
 struct Bits {
   typedef std::conditional_t<std::is_same_v<T, F32>, uint32_t, uint16_t> type;
 };
-// A value as loaded, 0 where there is none.
-template <typename T>
-__device__ __forceinline__ uint32_t load_bits(const void* p, int64_t at, bool there) {
-  return there ? (uint32_t)static_cast<const typename Bits<T>::type*>(p)[at] : 0u;
-}
 template <typename T>
 __device__ __forceinline__ float bits_value(uint32_t w) {
   if constexpr (std::is_same_v<T, F32>) return __builtin_bit_cast(float, w);
   else return to_float<T>(w);
 }
+// A value of T at a wave-uniform address and a lane's offset in bytes.
+template <typename T>
+__device__ __forceinline__ uint32_t load_bits(const void* base, uint32_t offset) {
+  return *reinterpret_cast<const typename Bits<T>::type*>(static_cast<const char*>(base) + offset);
+}
+template <typename T>
+__device__ __forceinline__ void store_at(void* base, uint32_t offset, float x) {
+  char* to = static_cast<char*>(base) + offset;
+  if constexpr (std::is_same_v<T, F32>) *reinterpret_cast<float*>(to) = x;
+  else *reinterpret_cast<uint16_t*>(to) = (uint16_t)pack2<T>(x, x);
+}
 
-// A lane's place: its channel, states and, of a wave's kT steps, those whose per-channel work it does.
+// A tensor's rows: where the first step of a sequence begins, and strides in bytes.
+struct View {
+  const char* at;
+  int64_t batch;
+  int32_t step;
+};
+
+// What the kernels walk.  A sequence is cut into `segments` of `per` tiles each.
+struct Scan {
+  View x, dt, z, B, C, dy;
+  const float* A;
+  const float* skip;
+  const float* dt_bias;
+  int32_t batch, steps, dim, states, tiles, groups, segments, per;
+};
+
+// A lane's place: its channel, four of its states and, of a wave's kT steps, those whose per-channel work it does.
+// Lanes past the last channel repeat it and store nothing.
 template <int L>
 struct Lane {
   static constexpr int kR = L <= kT ? kT / L : 1;  // steps of each lane: own + i L
-  int64_t b, ch;
-  int own, first, wave;
+  static constexpr int kC = 64 / L;                // channels of a wave
+  int group0, ch, own, first, inside;              // group0: the group's first channel, inside: of the group
   bool active;
-  __device__ __forceinline__ Lane(int64_t sequence, int64_t group, int64_t dim) {
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __device__ __forceinline__ Lane(int group, int dim) {
     const int lane = threadIdx.x & 63;
     own = lane % L, first = own * 4;
-    b = sequence, ch = group * (64 / L) + lane / L;
-    active = ch < dim;
+    group0 = group * kC;
+    const int left = dim - group0 < kC ? dim - group0 : kC;
+    active = lane / L < left;
+    inside = active ? lane / L : left - 1;
+    ch = group0 + inside;
   }
-  __device__ __forceinline__ int64_t step(int64_t t0, int i) const { return t0 + own + i * L; }
-  __device__ __forceinline__ bool has(int64_t t, int64_t steps) const { return active && t < steps && own < kT; }
+  // Whether all lanes have all of their steps, of which `left` are there.
+  __device__ __forceinline__ bool whole(int dim, int left) const { return left >= kT && dim - group0 >= kC && L <= kT; }
+  __device__ __forceinline__ bool has(int i, int left) const { return active && own + i * L < left && own < kT; }
+  // The offset in bytes of the lane's first step in a tensor of this step stride.
+  template <typename T>
+  __device__ __forceinline__ uint32_t offset(int step) const {
+    return (uint32_t)(own < kT ? own : kT - 1) * (uint32_t)step + (uint32_t)inside * Fmt<T>::bytes;
+  }
+  // That of its i-th, the last of the `left` steps that are there in place of those behind it.
+  template <typename T>
+  __device__ __forceinline__ uint32_t offset_of(int i, int step, int left) const {
+    const int t = own + i * L;
+    return (uint32_t)(t < left ? t : left - 1) * (uint32_t)step + (uint32_t)inside * Fmt<T>::bytes;
+  }
 };
 
-// B and C of a wave's steps on their way from memory to its part of LDS, [2][kT][4 L] floats.
+// A channel and step tensor's values of a wave's steps, at the lane's offset.
+template <typename T, int L>
+struct Rows {
+  uint32_t w[Lane<L>::kR];
+  // The steps from t0 on; in place of those behind the sequence's last, that one.  (Loads under a condition would be
+  // waited for where its branches meet, so only the offsets are.)
+  __device__ __forceinline__ void fetch(const Lane<L>& p, const View& v, int b, int t0, int steps) {
+    t0 = t0 < steps ? t0 : steps - 1;
+    const char* row = v.at + b * v.batch + (int64_t)t0 * v.step + p.group0 * Fmt<T>::bytes;
+    uint32_t at[Lane<L>::kR];
+    if (steps - t0 >= kT) {
+#pragma unroll
+      for (int i = 0; i < Lane<L>::kR; ++i) at[i] = p.template offset<T>(v.step) + (uint32_t)(i * L) * (uint32_t)v.step;
+    } else {
+#pragma unroll
+      for (int i = 0; i < Lane<L>::kR; ++i) at[i] = p.template offset_of<T>(i, v.step, steps - t0);
+    }
+#pragma unroll
+    for (int i = 0; i < Lane<L>::kR; ++i) w[i] = load_bits<T>(row, at[i]);
+  }
+  __device__ __forceinline__ float operator[](int i) const { return bits_value<T>(w[i]); }
+};
+
+// B or C of a wave's steps on its way from memory to the wave's part of LDS, [kT][4 L] floats; 0 for states
+// and steps that are not there.
 template <typename T, int L>
 struct Inputs {
-  uint32_t w[L];
-  __device__ __forceinline__ void fetch(const morph_ssm& a, int64_t b, int64_t t0) {
+  static constexpr int kCount = L > 1 ? L / 2 : 1, kAll = kT * 4 * L;
+  uint32_t w[kCount];
+  __device__ __forceinline__ void fetch(const View& r, int b, int t0, int steps, int states) {
+    t0 = t0 < steps ? t0 : steps - 1;
+    const char* row = r.at + b * r.batch + (int64_t)t0 * r.step;
+    const int left = steps - t0;
+    uint32_t at[kCount];
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int v = i * 64 + (threadIdx.x & 63), n = v % (4 * L);
-      const int64_t t = t0 + v / (4 * L) % kT;
-      const bool there = n < a.states && t < a.steps, second = v >= kT * 4 * L;
-      w[i] = second ? load_bits<T>(a.C, b * a.C_batch + t * a.C_step + n, there)
-                    : load_bits<T>(a.B, b * a.B_batch + t * a.B_step + n, there);
+    for (int i = 0; i < kCount; ++i) {
+      const int v = (i * 64 + (threadIdx.x & 63)) % kAll;
+      int t = v / (4 * L), n = v % (4 * L);
+      n = n < states ? n : states - 1;
+      if (left < kT) t = t < left ? t : left - 1;
+      at[i] = (uint32_t)t * (uint32_t)r.step + (uint32_t)n * Fmt<T>::bytes;
     }
-  }
-  __device__ __forceinline__ void put(float* to) const {
 #pragma unroll
-    for (int i = 0; i < L; ++i) to[i * 64 + (threadIdx.x & 63)] = bits_value<T>(w[i]);
+    for (int i = 0; i < kCount; ++i) w[i] = load_bits<T>(row, at[i]);
+  }
+  // (What is not there is told apart here: looked at in fetch, the loads would be waited for there.)
+  __device__ __forceinline__ void put(float* to, int left, int states) const {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int v = (i * 64 + (threadIdx.x & 63)) % kAll;
+      const bool there = v % (4 * L) < states && v / (4 * L) < left;
+      to[v] = there ? bits_value<T>(w[i]) : 0.0f;
+    }
   }
 };
 
@@ -192,67 +292,81 @@ __device__ __forceinline__ void walk(const float (&d)[Lane<L>::kR], const float 
   });
 }
 
-template <typename T, int L>
-__global__ __launch_bounds__(64 * kW) void ssm_kernel(const morph_ssm a, int64_t groups, void* __restrict__ y,
-                                                      float* __restrict__ last, float* __restrict__ kept) {
-  constexpr int kR = Lane<L>::kR;
-  __shared__ float bc[kW][2 * kT * 4 * L];
-  __shared__ f32x4 ends[2][kW][2][64];
-  const Lane<L> p(blockIdx.x / groups, blockIdx.x % groups, a.dim);
-  const int lane = threadIdx.x & 63;
-  const int64_t tiles = (a.steps + kT * kW - 1) / (kT * kW), row = p.b * a.dim + p.ch;
-  Four A2 = {}, carry = {};
-  float skip = 0.0f, bias = 0.0f;
-  if (p.active) {
-    load_states(a.A + p.ch * a.states, p.first, a.states, A2);
-    if (a.first) load_states(a.first + row * a.states, p.first, a.states, carry);
-    if (a.skip) skip = a.skip[p.ch];
-    if (a.dt_bias) bias = a.dt_bias[p.ch];
-  }
+// What a lane needs of its channel throughout.
+struct Channel {
+  Four A2;  // A log2(e)
+  float skip, bias;
+};
+template <int L>
+__device__ __forceinline__ Channel load_channel(const Scan& a, const Lane<L>& p) {
+  Channel c;
+  load_states(a.A + (int64_t)p.ch * a.states, p.first, a.states, c.A2);
+  c.skip = a.skip ? a.skip[p.ch] : 0.0f;
+  c.bias = a.dt_bias ? a.dt_bias[p.ch] : 0.0f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) A2[j] *= kLog2e;
+  for (int j = 0; j < 4; ++j) c.A2[j] *= kLog2e;
+  return c;
+}
+// The states of a channel in a tensor [.., dim, states], `row` its sequence.
+__device__ __forceinline__ int64_t states_at(const Scan& a, int64_t row, int ch) { return (row * a.dim + ch) * a.states; }
 
-  uint32_t rx[kR], rd[kR], rz[kR];
-  Inputs<T, L> in;
-  auto fetch = [&](int64_t tile) {
-    const int64_t t0 = (tile * kW + p.wave) * kT;
-#pragma unroll
-    for (int i = 0; i < kR; ++i) {
-      const int64_t t = p.step(t0, i);
-      const bool there = p.has(t, a.steps);
-      rx[i] = load_bits<T>(a.x, p.b * a.x_batch + t * a.x_step + p.ch, there);
-      rd[i] = load_bits<T>(a.dt, p.b * a.dt_batch + t * a.dt_step + p.ch, there);
-      rz[i] = a.z ? load_bits<T>(a.z, p.b * a.z_batch + t * a.z_step + p.ch, there) : 0u;
-    }
-    in.fetch(a, p.b, t0);
+template <typename T, int L, bool kGated>
+__global__ __launch_bounds__(64 * kW, L < 4 ? 3 : 4) void ssm_kernel(const Scan a, const float* __restrict__ first,
+                                                         const float* __restrict__ entering, char* __restrict__ y,
+                                                         float* __restrict__ last, float* __restrict__ kept) {
+  constexpr int kR = Lane<L>::kR;
+  __shared__ float bc[kW][2][kT * 4 * L];
+  __shared__ f32x4 ends[2][kW][2][64];
+  const int group = (int)blockIdx.x % a.groups, rest = (int)blockIdx.x / a.groups;
+  const int segment = rest % a.segments, b = rest / a.segments;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const Lane<L> p(group, a.dim);
+  const Channel c = load_channel(a, p);
+  Four carry = {};
+  if (segment > 0) load_states(entering + states_at(a, (int64_t)segment * a.batch + b, p.ch), p.first, a.states, carry);
+  else if (first) load_states(first + states_at(a, b, p.ch), p.first, a.states, carry);
+  const int begin = segment * a.per, end = begin + a.per < a.tiles ? begin + a.per : a.tiles;
+
+  Rows<T, L> rx, rd, rz;
+  Inputs<T, L> inB, inC;
+  auto fetch = [&](int tile) {
+    const int t0 = (tile * kW + wave) * kT;
+    rx.fetch(p, a.x, b, t0, a.steps);
+    rd.fetch(p, a.dt, b, t0, a.steps);
+    if constexpr (kGated) rz.fetch(p, a.z, b, t0, a.steps);
+    inB.fetch(a.B, b, t0, a.steps, a.states);
+    inC.fetch(a.C, b, t0, a.steps, a.states);
   };
-  if (tiles > 0) fetch(0);
-  for (int64_t tile = 0; tile < tiles; ++tile) {
-    const int64_t t0 = (tile * kW + p.wave) * kT;
+  if (begin < end) fetch(begin);
+  for (int tile = begin; tile < end; ++tile) {
+    const int t0 = (tile * kW + wave) * kT, left = a.steps - t0;
+    const bool whole = p.whole(a.dim, left);
     float x[kR], d[kR], u[kR], z[kR];
+    float* B = bc[wave][0];
+    float* C = bc[wave][1];
+    inB.put(B, left, a.states), inC.put(C, left, a.states);
+    wave_order();
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
-      x[i] = bits_value<T>(rx[i]);
-      z[i] = bits_value<T>(rz[i]);
-      d[i] = p.has(p.step(t0, i), a.steps) ? softplus(bits_value<T>(rd[i]) + bias) : 0.0f;
+      x[i] = rx[i];
+      if constexpr (kGated) z[i] = rz[i];
+      d[i] = softplus(rd[i] + c.bias);
+      if (!whole && !p.has(i, left)) d[i] = x[i] = 0.0f;
       u[i] = d[i] * x[i];
     }
-    float* mine = bc[p.wave];
-    in.put(mine);
-    wave_order();
-    if (tile + 1 < tiles) fetch(tile + 1);
-    if (kept && p.wave == 0 && p.active)
-      store_states(kept + ((p.b * tiles + tile) * a.dim + p.ch) * a.states, p.first, a.states, carry);
+    if (tile + 1 < end) fetch(tile + 1);
+    if (kept && wave == 0 && p.active)
+      store_states(kept + states_at(a, (int64_t)b * a.tiles + tile, p.ch), p.first, a.states, carry);
     Four P[kT], h[kT];
-    walk<L, true>(d, u, A2, mine, p.first, P, h);
+    walk<L, true>(d, u, c.A2, B, p.first, P, h);
     const int turn = tile & 1;  // every wave has passed the barrier behind the last use of this half
-    ends[turn][p.wave][0][lane] = as_vector(P[kT - 1]);
-    ends[turn][p.wave][1][lane] = as_vector(h[kT - 1]);
+    ends[turn][wave][0][lane] = as_vector(P[kT - 1]);
+    ends[turn][wave][1][lane] = as_vector(h[kT - 1]);
     __syncthreads();
     Four enter;
 #pragma unroll
     for (int w = 0; w < kW; ++w) {
-      if (w == p.wave) {
+      if (w == wave) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) enter[j] = carry[j];
       }
@@ -260,26 +374,127 @@ __global__ __launch_bounds__(64 * kW) void ssm_kernel(const morph_ssm a, int64_t
 #pragma unroll
       for (int j = 0; j < 4; ++j) carry[j] = __fmaf_rn(A[j], carry[j], S[j]);
     }
-    float out[kR] = {};
+    Sums<L> sums = {};
     each_step<kT>([&](auto step) {
-      constexpr int t = decltype(step)::value;
-      const f32x4 c = *reinterpret_cast<const f32x4*>(mine + (kT + t) * 4 * L + p.first);
-      float s = 0.0f;
+      constexpr int t = kT - 1 - decltype(step)::value;
+      const f32x4 ct = *reinterpret_cast<const f32x4*>(C + t * 4 * L + p.first);
+      float s = ct[0] * __fmaf_rn(P[t][0], enter[0], h[t][0]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s = __fmaf_rn(c[j], __fmaf_rn(P[t][j], enter[j], h[t][j]), s);
-      s = channel_sum<L>(s);
-      if (p.own == t % L) out[t / L] = s;
+      for (int j = 1; j < 4; ++j) s = __fmaf_rn(ct[j], __fmaf_rn(P[t][j], enter[j], h[t][j]), s);
+      sums.template take<t>(s, p.own);
     });
     wave_order();
+    if (left <= 0) continue;
+    char* rows = y + (((int64_t)b * a.steps + t0) * a.dim + p.group0) * Fmt<T>::bytes;
+    const uint32_t to = p.template offset<T>(a.dim * Fmt<T>::bytes);
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
-      const int64_t t = p.step(t0, i);
-      float s = __fmaf_rn(skip, x[i], out[i]);
-      if (a.z) s *= z[i] * gate_sigmoid(z[i]);
-      if (p.has(t, a.steps)) store_one<T>(y, (p.b * a.steps + t) * a.dim + p.ch, s);
+      float s = __fmaf_rn(c.skip, x[i], sums.out[i]);
+      if constexpr (kGated) s *= z[i] * gate_sigmoid(z[i]);
+      if (whole || p.has(i, left)) store_at<T>(rows + (int64_t)(i * L) * a.dim * Fmt<T>::bytes, to, s);
     }
   }
-  if (p.wave == 0 && p.active) store_states(last + row * a.states, p.first, a.states, carry);
+  if (segment == a.segments - 1 && wave == 0 && p.active)
+    store_states(last + states_at(a, b, p.ch), p.first, a.states, carry);
+}
+
+// What a segment does to a state that passes through it, for the segments to be walked side by side: the product of its
+// gates is exp(A times the sum of d), and `ends` its result from a zero state (kBack: of the gradients r, from its last
+// step to its first).  Each wave takes a quarter of its steps; no output, so neither skip nor dB and dC.
+// segment s: ends[s + 1], sums[s + 1] (kBack: s - 1), where what enters the next one then is joined.
+template <typename T, int L, bool kBack, bool kGated>
+__global__ __launch_bounds__(64 * kW) void ssm_ends_kernel(const Scan a, float* __restrict__ ends, float* __restrict__ sums) {
+  constexpr int kR = Lane<L>::kR;
+  __shared__ float bc[kW][kT * 4 * L];
+  __shared__ f32x4 join[kW][2][64];
+  __shared__ float whole_sum[kW][64];
+  const int group = (int)blockIdx.x % a.groups, rest = (int)blockIdx.x / a.groups;
+  const int segment = rest % (a.segments - 1) + (kBack ? 1 : 0), b = rest / (a.segments - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const Lane<L> p(group, a.dim);
+  const Channel c = load_channel(a, p);
+  const int stretch = a.per * kT, t_begin = segment * a.per * kW * kT + wave * stretch;
+  Rows<T, L> rd, rx, rz;  // x: kBack: dy
+  Inputs<T, L> in;
+  float* mine = bc[wave];
+  float sum = 0.0f;
+  Four s = {};
+  auto fetch = [&](int i) {
+    const int t0 = t_begin + (kBack ? a.per - 1 - i : i) * kT;
+    rd.fetch(p, a.dt, b, t0, a.steps);
+    rx.fetch(p, kBack ? a.dy : a.x, b, t0, a.steps);
+    if constexpr (kGated) rz.fetch(p, a.z, b, t0, a.steps);
+    in.fetch(kBack ? a.C : a.B, b, t0, a.steps, a.states);
+  };
+  fetch(0);
+  for (int i = 0; i < a.per; ++i) {
+    const int t0 = t_begin + (kBack ? a.per - 1 - i : i) * kT, left = a.steps - t0;
+    const bool whole = p.whole(a.dim, left);
+    float d[kR], u[kR];
+    in.put(mine, left, a.states);
+    wave_order();
+#pragma unroll
+    for (int k = 0; k < kR; ++k) {
+      d[k] = softplus(rd[k] + c.bias);
+      u[k] = rx[k];
+      if constexpr (kBack) {
+        if constexpr (kGated) u[k] *= silu(rz[k]).y;
+      } else {
+        u[k] *= d[k];
+      }
+      if (!whole && !p.has(k, left)) d[k] = u[k] = 0.0f;
+      sum += d[k];
+    }
+    if (i + 1 < a.per) fetch(i + 1);
+    each_step<kT>([&](auto step) {
+      constexpr int t = kBack ? kT - 1 - decltype(step)::value : decltype(step)::value;
+      const float dt = spread<L, t % L>(d[t / L]), ut = spread<L, t % L>(u[t / L]);
+      const f32x4 in_t = *reinterpret_cast<const f32x4*>(mine + t * 4 * L + p.first);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float gate = __builtin_amdgcn_exp2f(dt * c.A2[j]);
+        s[j] = kBack ? gate * __fmaf_rn(in_t[j], ut, s[j]) : __fmaf_rn(gate, s[j], in_t[j] * ut);
+      }
+    });
+    wave_order();
+  }
+  sum = channel_sum<L>(sum);
+  Four P;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) P[j] = __builtin_amdgcn_exp2f(sum * c.A2[j]);
+  join[wave][0][lane] = as_vector(P), join[wave][1][lane] = as_vector(s);
+  whole_sum[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0) return;
+  Four out = {};
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kW; ++i) {
+    const int w = kBack ? kW - 1 - i : i;
+    const f32x4 A = join[w][0][lane], S = join[w][1][lane];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = __fmaf_rn(A[j], out[j], S[j]);
+    sum += whole_sum[w][lane];
+  }
+  if (!p.active) return;
+  const int64_t row = (int64_t)(segment + (kBack ? -1 : 1)) * a.batch + b;
+  store_states(ends + states_at(a, row, p.ch), p.first, a.states, out);
+  if (p.own == 0) sums[row * a.dim + p.ch] = sum;
+}
+
+// What enters each segment, in place of `ends`: from `first` through one after the other (kBack: from the last, NULL: zeros).
+template <bool kBack>
+__global__ __launch_bounds__(256) void ssm_join_kernel(const Scan a, const float* __restrict__ first, float* __restrict__ ends,
+                                                       const float* __restrict__ sums) {
+  const int64_t size = (int64_t)a.batch * a.dim * a.states, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= size) return;
+  const float A2 = a.A[i % ((int64_t)a.dim * a.states)] * kLog2e;
+  float s = first ? first[i] : 0.0f;
+  for (int k = 1; k < a.segments; ++k) {
+    const int64_t row = kBack ? a.segments - 1 - k : k;
+    s = __fmaf_rn(__builtin_amdgcn_exp2f(sums[row * a.batch * a.dim + i / a.states] * A2), s, ends[row * size + i]);
+    ends[row * size + i] = s;
+  }
 }
 
 // One step: the state crosses once in and once out, and HBM bounds it.
@@ -297,8 +512,8 @@ __global__ __launch_bounds__(256) void ssm_one_kernel(const morph_ssm a, int64_t
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const bool there = first + j < a.states;
-    B[j] = bits_value<T>(load_bits<T>(a.B, b * a.B_batch + first + j, there));
-    C[j] = bits_value<T>(load_bits<T>(a.C, b * a.C_batch + first + j, there));
+    B[j] = there ? load_one<T>(a.B, b * a.B_batch + first + j) : 0.0f;
+    C[j] = there ? load_one<T>(a.C, b * a.C_batch + first + j) : 0.0f;
   }
   const float x = load_one<T>(a.x, b * a.x_batch + ch), z = a.z ? load_one<T>(a.z, b * a.z_batch + ch) : 0.0f;
   const float d = softplus(load_one<T>(a.dt, b * a.dt_batch + ch) + (a.dt_bias ? a.dt_bias[ch] : 0.0f));
@@ -321,73 +536,80 @@ __global__ __launch_bounds__(256) void ssm_one_kernel(const morph_ssm a, int64_t
 // Where a backward's sums lie in its workspace.
 struct SsmParts {
   float* bc;       // [blocks of channel groups][batch][steps][2][4 L]: dB, dC
-  float* A;        // [batch][dim][states]
-  float* skip;     // [batch][dim]
-  float* dt_bias;  // [batch][dim]
+  float* A;        // [segments][batch][dim][states]
+  float* skip;     // [segments][batch][dim]
+  float* dt_bias;  // [segments][batch][dim]
+  float* late;     // [segments][batch][dim][states]: r behind each segment, times its gate
+  float* sums;     // [segments][batch][dim]
 };
 
-template <typename T, int L>
-__global__ __launch_bounds__(64 * kW) void ssm_back_kernel(const morph_ssm a, int64_t blocks, int per,
-                                                           const float* __restrict__ kept, const void* __restrict__ dy,
-                                                           int64_t dy_batch, int64_t dy_step,
-                                                           const float* __restrict__ dlast, const morph_ssm_grads g,
-                                                           const SsmParts parts) {
+// A sequence's channel groups go to `blocks` workgroups, to the first ones one more where they do not come out even.
+template <typename T, int L, bool kGated>
+__global__ __launch_bounds__(64 * kW, L < 16 ? 3 : 2) void ssm_back_kernel(const Scan a, int blocks,
+                                                                           const float* __restrict__ kept,
+                                                                           const float* __restrict__ dlast,
+                                                                           const morph_ssm_grads g, const SsmParts parts) {
   constexpr int kR = Lane<L>::kR, kRep = 16 / L, kSlots = kRep < kT ? kT / kRep : 1;
-  __shared__ float bc[kW][2 * kT * 4 * L];
-  __shared__ f32x4 ends[kW][3][64];
+  __shared__ float bc[kW][2][kT * 4 * L];
+  __shared__ f32x4 ends[2][kW][3][64];
   __shared__ f32x4 late[2][kMostGroups][64];           // r behind the tile, times its gate
   __shared__ f32x4 sum_A[kMostGroups][kW][64];         // dA of each wave's steps
   __shared__ float sum_own[kMostGroups][kW][2][64];    // dskip, ddt_bias
-  const int64_t b = blockIdx.x / blocks, block = blockIdx.x % blocks, channels = (a.dim + 64 / L - 1) / (64 / L);
-  const int count = (int)(channels - block * per < per ? channels - block * per : per);
+  // the larger workgroups of all sequences first
+  const int rows = a.segments * a.batch, block = (int)blockIdx.x / rows, rest = (int)blockIdx.x % rows;
+  const int segment = rest % a.segments, b = rest / a.segments;
+  const int per = a.groups / blocks, more = a.groups % blocks;
+  const int group0 = block * per + (block < more ? block : more), count = per + (block < more ? 1 : 0);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tiles = (a.steps + kT * kW - 1) / (kT * kW);
+  const int begin = segment * a.per, end = begin + a.per < a.tiles ? begin + a.per : a.tiles;
   for (int i = 0; i < count; ++i) {
-    const Lane<L> p(b, block * per + i, a.dim);
+    const Lane<L> p(group0 + i, a.dim);
     sum_A[i][wave][lane] = f32x4{0, 0, 0, 0};
     sum_own[i][wave][0][lane] = sum_own[i][wave][1][lane] = 0.0f;
     if (wave == 0) {
       Four r = {};
-      if (dlast && p.active) load_states(dlast + (b * a.dim + p.ch) * a.states, p.first, a.states, r);
+      if (segment < a.segments - 1)
+        load_states(parts.late + states_at(a, (int64_t)segment * a.batch + b, p.ch), p.first, a.states, r);
+      else if (dlast) load_states(dlast + states_at(a, b, p.ch), p.first, a.states, r);
       late[0][i][lane] = as_vector(r);
     }
   }
-  Inputs<T, L> in;
-  for (int64_t tile = tiles - 1; tile >= 0; --tile) {
-    const int64_t t0 = (tile * kW + wave) * kT;
-    const int turn = (int)((tiles - 1 - tile) & 1);
-    float* mine = bc[wave];
-    in.fetch(a, b, t0);
-    in.put(mine);
+  Inputs<T, L> inB, inC;
+  float* B = bc[wave][0];
+  float* C = bc[wave][1];
+  int half = 0, turn = 0;
+  for (int tile = end - 1; tile >= begin; --tile, turn ^= 1) {
+    const int t0 = (tile * kW + wave) * kT, left = a.steps - t0;
+    inB.fetch(a.B, b, t0, a.steps, a.states);
+    inC.fetch(a.C, b, t0, a.steps, a.states);
+    inB.put(B, left, a.states), inC.put(C, left, a.states);
     wave_order();
     float acc[kSlots][2] = {};
-    for (int i = 0; i < count; ++i) {
-      const Lane<L> p(b, block * per + i, a.dim);
-      float x[kR], d[kR], u[kR], z[kR], e[kR], raw[kR], ds[kR];
-      Four A = {}, A2, enter = {};
-      float skip = 0.0f, bias = 0.0f;
-      if (p.active) {
-        load_states(a.A + p.ch * a.states, p.first, a.states, A);
-        load_states(kept + ((b * tiles + tile) * a.dim + p.ch) * a.states, p.first, a.states, enter);
-        if (a.skip) skip = a.skip[p.ch];
-        if (a.dt_bias) bias = a.dt_bias[p.ch];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) A2[j] = A[j] * kLog2e;
+    for (int i = 0; i < count; ++i, half ^= 1) {
+      const Lane<L> p(group0 + i, a.dim);
+      const bool whole = p.whole(a.dim, left);
+      Rows<T, L> rx, rd, rz, re;
+      rx.fetch(p, a.x, b, t0, a.steps);
+      rd.fetch(p, a.dt, b, t0, a.steps);
+      re.fetch(p, a.dy, b, t0, a.steps);
+      if constexpr (kGated) rz.fetch(p, a.z, b, t0, a.steps);
+      const Channel c = load_channel(a, p);
+      Four enter;
+      load_states(kept + states_at(a, (int64_t)b * a.tiles + tile, p.ch), p.first, a.states, enter);
+      float x[kR], d[kR], u[kR], raw[kR], ds[kR], slope[kR];  // slope: of silu(z), times dy
 #pragma unroll
       for (int k = 0; k < kR; ++k) {
-        const int64_t t = p.step(t0, k);
-        const bool there = p.has(t, a.steps);
-        x[k] = bits_value<T>(load_bits<T>(a.x, b * a.x_batch + t * a.x_step + p.ch, there));
-        raw[k] = bits_value<T>(load_bits<T>(a.dt, b * a.dt_batch + t * a.dt_step + p.ch, there)) + bias;
-        e[k] = bits_value<T>(load_bits<T>(dy, b * dy_batch + t * dy_step + p.ch, there));
-        z[k] = a.z ? bits_value<T>(load_bits<T>(a.z, b * a.z_batch + t * a.z_step + p.ch, there)) : 0.0f;
-        d[k] = there ? softplus(raw[k]) : 0.0f;
+        x[k] = rx[k], raw[k] = rd[k] + c.bias, ds[k] = re[k];
+        d[k] = softplus(raw[k]);
+        if constexpr (kGated) {
+          const Silu q = silu(rz[k]);
+          slope[k] = ds[k] * q.slope, ds[k] *= q.y;
+        }
+        if (!whole && !p.has(k, left)) d[k] = x[k] = ds[k] = 0.0f;
         u[k] = d[k] * x[k];
-        ds[k] = a.z ? e[k] * silu(z[k]).y : e[k];
       }
       Four gate[kT], h[kT];
-      walk<L, false>(d, u, A2, mine, p.first, gate, h);
+      walk<L, false>(d, u, c.A2, B, p.first, gate, h);
       Four P, Q = {};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -398,64 +620,61 @@ __global__ __launch_bounds__(64 * kW) void ssm_back_kernel(const morph_ssm a, in
       each_step<kT>([&](auto step) {
         constexpr int t = kT - 1 - decltype(step)::value;
         const float dst = spread<L, t % L>(ds[t / L]);
-        const f32x4 c = *reinterpret_cast<const f32x4*>(mine + (kT + t) * 4 * L + p.first);
+        const f32x4 ct = *reinterpret_cast<const f32x4*>(C + t * 4 * L + p.first);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) Q[j] = gate[t][j] * __fmaf_rn(c[j], dst, Q[j]);
+        for (int j = 0; j < 4; ++j) Q[j] = gate[t][j] * __fmaf_rn(ct[j], dst, Q[j]);
       });
-      ends[wave][0][lane] = as_vector(P);
-      ends[wave][1][lane] = as_vector(h[kT - 1]);
-      ends[wave][2][lane] = as_vector(Q);
-      __syncthreads();
+      ends[half][wave][0][lane] = as_vector(P);
+      ends[half][wave][1][lane] = as_vector(h[kT - 1]);
+      ends[half][wave][2][lane] = as_vector(Q);
+      __syncthreads();  // every wave has passed it behind its last use of this half
       for (int w = 0; w < wave; ++w) {
-        const f32x4 Pw = ends[w][0][lane], S = ends[w][1][lane];
+        const f32x4 Pw = ends[half][w][0][lane], S = ends[half][w][1][lane];
 #pragma unroll
         for (int j = 0; j < 4; ++j) enter[j] = __fmaf_rn(Pw[j], enter[j], S[j]);
       }
       const f32x4 after = late[turn][i][lane];
       Four r = {after.x, after.y, after.z, after.w};
       for (int w = kW - 1; w > wave; --w) {
-        const f32x4 Pw = ends[w][0][lane], Qw = ends[w][2][lane];
+        const f32x4 Pw = ends[half][w][0][lane], Qw = ends[half][w][2][lane];
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[j] = __fmaf_rn(Pw[j], r[j], Qw[j]);
       }
-      __syncthreads();
       // the states again, from the true one
       each_step<kT>([&](auto step) {
         constexpr int t = decltype(step)::value;
         const float ut = spread<L, t % L>(u[t / L]);
-        const f32x4 B = *reinterpret_cast<const f32x4*>(mine + t * 4 * L + p.first);
+        const f32x4 Bt = *reinterpret_cast<const f32x4*>(B + t * 4 * L + p.first);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[t][j] = __fmaf_rn(gate[t][j], t ? h[t ? t - 1 : 0][j] : enter[j], ut * B[j]);
+        for (int j = 0; j < 4; ++j) h[t][j] = __fmaf_rn(gate[t][j], t ? h[t ? t - 1 : 0][j] : enter[j], ut * Bt[j]);
       });
-      float rB[kR] = {}, wA[kR] = {}, Ch[kR] = {};
+      Sums<L> rB = {}, wA = {}, Ch = {};
+      float pair[4][2];
       const f32x4 before = sum_A[i][wave][lane];
       Four dA = {before.x, before.y, before.z, before.w};
       each_step<kT>([&](auto step) {
         constexpr int t = kT - 1 - decltype(step)::value;
         const float dst = spread<L, t % L>(ds[t / L]), dt = spread<L, t % L>(d[t / L]), ut = spread<L, t % L>(u[t / L]);
-        const f32x4 B = *reinterpret_cast<const f32x4*>(mine + t * 4 * L + p.first);
-        const f32x4 c = *reinterpret_cast<const f32x4*>(mine + (kT + t) * 4 * L + p.first);
-        float sB = 0.0f, sA = 0.0f, sC = 0.0f, v[8];
+        const f32x4 Bt = *reinterpret_cast<const f32x4*>(B + t * 4 * L + p.first);
+        const f32x4 ct = *reinterpret_cast<const f32x4*>(C + t * 4 * L + p.first);
+        float v[8], sB = 0.0f, sA = 0.0f, sC = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float q = __fmaf_rn(c[j], dst, r[j]);
-          sB = __fmaf_rn(q, B[j], sB);
-          sC = __fmaf_rn(c[j], h[t][j], sC);
+          const float q = __fmaf_rn(ct[j], dst, r[j]);
+          sB = j ? __fmaf_rn(q, Bt[j], sB) : q * Bt[j];
+          if constexpr (kGated) sC = j ? __fmaf_rn(ct[j], h[t][j], sC) : ct[j] * h[t][j];
           v[j] = q * ut;
           v[4 + j] = h[t][j] * dst;
           r[j] = gate[t][j] * q;
           const float w = r[j] * (t ? h[t ? t - 1 : 0][j] : enter[j]);
-          sA = __fmaf_rn(w, A[j], sA);
+          sA = j ? __fmaf_rn(w, c.A2[j], sA) : w * c.A2[j];
           dA[j] = __fmaf_rn(w, dt, dA[j]);
         }
-        sB = channel_sum<L>(sB), sA = channel_sum<L>(sA);
-        if (p.own == t % L) rB[t / L] = sB, wA[t / L] = sA;
-        if (a.z) {
-          sC = channel_sum<L>(sC);
-          if (p.own == t % L) Ch[t / L] = sC;
-        }
+        rB.template take<t>(sB, p.own);
+        wA.template take<t>(sA, p.own);
+        if constexpr (kGated) Ch.template take<t>(sC, p.own);
         // over the wave's channels: dB to the lower 32 lanes, dC to the upper; states 0 and 1 to even rows of 16
-        // lanes, 2 and 3 to odd ones; then within the rows
+        // lanes, 2 and 3 to odd ones; then within the rows, with L = 4 four steps together
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           swap32(v[j], v[4 + j]);
@@ -465,25 +684,46 @@ __global__ __launch_bounds__(64 * kW) void ssm_back_kernel(const morph_ssm a, in
         for (int j = 0; j < 2; ++j) {
           swap16(v[j], v[2 + j]);
           v[j] += v[2 + j];
-          if constexpr (L <= 8) v[j] += dpp<kRotate8>(v[j]);
-          if constexpr (L <= 4) v[j] += dpp<kRotate4>(v[j]);
-          if constexpr (L <= 2) v[j] += dpp<kRotate2>(v[j]);
-          if constexpr (L <= 1) v[j] += dpp<kRotate1>(v[j]);
-          if ((lane & 15) / L == t % kRep) acc[t / kRep][j] += v[j];
+          if constexpr (L == 4) {
+            pair[t % 4][j] = v[j];
+          } else {
+            if constexpr (L <= 8) v[j] += dpp<kRotate8>(v[j]);
+            if constexpr (L <= 2) v[j] += dpp<kRotate4>(v[j]);
+            if constexpr (L <= 2) v[j] += dpp<kRotate2>(v[j]);
+            if constexpr (L <= 1) v[j] += dpp<kRotate1>(v[j]);
+            acc[t / kRep][j] += (lane & 15) / L == t % kRep ? v[j] : 0.0f;
+          }
         }
+        if constexpr (L == 4 && t % 4 == 0) {
+          const bool odd = lane & 4, high = lane & 8;  // step t + (lane >> 2) % 4 stays
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float x = (high ? pair[2][j] : pair[0][j]) + dpp<kRotate8>(high ? pair[0][j] : pair[2][j]);
+            const float y = (high ? pair[3][j] : pair[1][j]) + dpp<kRotate8>(high ? pair[1][j] : pair[3][j]);
+            // from 4 lanes before, or for the even ones behind; both by all lanes, since a lane reads active ones only
+            const float give = odd ? x : y, before4 = dpp<kRotate4>(give), behind4 = dpp<kRotate12>(give);
+            acc[t / 4][j] += (odd ? y : x) + (odd ? before4 : behind4);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // steps mixed by the scheduler take more registers than there are
       });
       sum_A[i][wave][lane] = as_vector(dA);
       if (wave == 0) late[turn ^ 1][i][lane] = as_vector(r);
+      if (left <= 0) continue;
       float dskip = 0.0f, dbias = 0.0f;
+      const uint32_t to = p.template offset<T>(a.dim * Fmt<T>::bytes);
+      const int64_t at = (((int64_t)b * a.steps + t0) * a.dim + p.group0) * Fmt<T>::bytes;
 #pragma unroll
       for (int k = 0; k < kR; ++k) {
-        const int64_t t = p.step(t0, k);
-        if (!p.has(t, a.steps)) continue;
-        const int64_t at = (b * a.steps + t) * a.dim + p.ch;
-        const float ddt = __fmaf_rn(x[k], rB[k], wA[k]) * sigmoid(raw[k]).a;
-        store_one<T>(g.dx, at, __fmaf_rn(d[k], rB[k], skip * ds[k]));
-        store_one<T>(g.ddt, at, ddt);
-        if (a.z) store_one<T>(g.dz, at, e[k] * __fmaf_rn(skip, x[k], Ch[k]) * silu(z[k]).slope);
+        const int64_t row = at + (int64_t)(k * L) * a.dim * Fmt<T>::bytes;
+        float ddt = __fmaf_rn(x[k], rB.out[k], wA.out[k] * kLn2) * sigmoid(raw[k]).a;
+        if (whole || p.has(k, left)) {
+          store_at<T>(static_cast<char*>(g.dx) + row, to, __fmaf_rn(d[k], rB.out[k], c.skip * ds[k]));
+          store_at<T>(static_cast<char*>(g.ddt) + row, to, ddt);
+          if constexpr (kGated) store_at<T>(static_cast<char*>(g.dz) + row, to, __fmaf_rn(c.skip, x[k], Ch.out[k]) * slope[k]);
+        } else {
+          ddt = 0.0f;
+        }
         dskip = __fmaf_rn(ds[k], x[k], dskip);
         dbias += ddt;
       }
@@ -494,8 +734,8 @@ __global__ __launch_bounds__(64 * kW) void ssm_back_kernel(const morph_ssm a, in
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       const int t = s * kRep + (lane & 15) / L;
-      if (t < kT && t0 + t < a.steps) {
-        float* to = parts.bc + (((block * a.batch + b) * a.steps + t0 + t) * 2 + (lane >> 5)) * 4 * L +
+      if (t < kT && t < left) {
+        float* to = parts.bc + ((((int64_t)block * a.batch + b) * a.steps + t0 + t) * 2 + (lane >> 5)) * 4 * L +
                     (lane & (L - 1)) * 4 + ((lane >> 4) & 1) * 2;
         *reinterpret_cast<f32x2*>(to) = f32x2{acc[s][0], acc[s][1]};
       }
@@ -503,7 +743,7 @@ __global__ __launch_bounds__(64 * kW) void ssm_back_kernel(const morph_ssm a, in
   }
   __syncthreads();
   for (int i = wave; i < count; i += kW) {  // a wave a channel group
-    const Lane<L> p(b, block * per + i, a.dim);
+    const Lane<L> p(group0 + i, a.dim);
     f32x4 dA = sum_A[i][0][lane];
     float own[2] = {sum_own[i][0][0][lane], sum_own[i][0][1][lane]};
 #pragma unroll
@@ -513,14 +753,14 @@ __global__ __launch_bounds__(64 * kW) void ssm_back_kernel(const morph_ssm a, in
     }
     own[0] = channel_sum<L>(own[0]), own[1] = channel_sum<L>(own[1]);
     if (!p.active) continue;
-    const int64_t row = b * a.dim + p.ch;
+    const int64_t row = (int64_t)segment * a.batch + b;
     const Four sum = {dA.x, dA.y, dA.z, dA.w};
-    store_states(parts.A + row * a.states, p.first, a.states, sum);
-    if (p.own == 0) parts.skip[row] = own[0], parts.dt_bias[row] = own[1];
-    if (g.dfirst) {
-      const f32x4 r = late[tiles & 1][i][lane];
+    store_states(parts.A + states_at(a, row, p.ch), p.first, a.states, sum);
+    if (p.own == 0) parts.skip[row * a.dim + p.ch] = own[0], parts.dt_bias[row * a.dim + p.ch] = own[1];
+    if (segment == 0 && g.dfirst) {
+      const f32x4 r = late[turn][i][lane];
       const Four first = {r.x, r.y, r.z, r.w};
-      store_states(g.dfirst + row * a.states, p.first, a.states, first);
+      store_states(g.dfirst + states_at(a, b, p.ch), p.first, a.states, first);
     }
   }
 }
@@ -539,7 +779,7 @@ __global__ __launch_bounds__(256) void ssm_sum_kernel(const float* __restrict__ 
   store_one<T>(i / wide % 2 ? dC : dB, i / (2 * wide) * states + n, sum);
 }
 
-// dA, dskip and ddt_bias: the sums over the sequences.
+// dA, dskip and ddt_bias: the sums over the sequences and their segments.
 __global__ __launch_bounds__(256) void ssm_batch_kernel(const SsmParts parts, int64_t batch, int64_t dim, int states,
                                                         float* __restrict__ dA, float* __restrict__ dskip,
                                                         float* __restrict__ ddt_bias) {
@@ -564,16 +804,17 @@ int lanes_of(int states) {
   return l;
 }
 
-// f(T{}, lanes) for the activations' dtype and the lanes that a channel's states take.
+// f(T{}, lanes, gated) for the activations' dtype and the lanes that a channel's states take.
 template <typename F>
-int by_form(int dtype, int states, F&& f) {
+int by_form(int dtype, int states, bool gated, F&& f) {
+  auto gate = [&](auto t, auto lanes) { return gated ? f(t, lanes, std::true_type{}) : f(t, lanes, std::false_type{}); };
   auto lanes = [&](auto t) {
     switch (lanes_of(states)) {
-      case 1: return f(t, std::integral_constant<int, 1>{});
-      case 2: return f(t, std::integral_constant<int, 2>{});
-      case 4: return f(t, std::integral_constant<int, 4>{});
-      case 8: return f(t, std::integral_constant<int, 8>{});
-      default: return f(t, std::integral_constant<int, 16>{});
+      case 1: return gate(t, std::integral_constant<int, 1>{});
+      case 2: return gate(t, std::integral_constant<int, 2>{});
+      case 4: return gate(t, std::integral_constant<int, 4>{});
+      case 8: return gate(t, std::integral_constant<int, 8>{});
+      default: return gate(t, std::integral_constant<int, 16>{});
     }
   };
   switch (dtype) {
@@ -584,27 +825,84 @@ int by_form(int dtype, int states, F&& f) {
   }
 }
 
-// Channel groups of a backward workgroup: as many as leave kBackBlocks workgroups, since each
-// workgroup's sums over its channels cross HBM twice.
-int groups_per_block(int64_t batch, int64_t dim, int lanes) {
-  const int64_t groups = over(dim, 64 / lanes) * batch / kBackBlocks;
-  return groups < 1 ? 1 : groups > kMostGroups ? kMostGroups : (int)groups;
+int64_t tiles_of(int64_t steps) { return over(steps, kT * kW); }
+
+// Tiles of a segment.  A scan whose channel groups leave CUs idle is cut into segments that are walked side by side,
+// after a launch that finds what each does to a state: two thirds of the scan's own arithmetic, so not where there
+// are kBusy workgroups without it.
+int64_t tiles_per_segment(int64_t batch, int64_t steps, int64_t groups) {
+  const int64_t tiles = tiles_of(steps), blocks = groups * batch;
+  if (tiles < 4 || blocks >= kBusy) return tiles > 0 ? tiles : 1;
+  int64_t segments = over(kFull, blocks > 0 ? blocks : 1);
+  if (segments > tiles / 2) segments = tiles / 2;
+  return over(tiles, segments);
 }
+
+// Workgroups of a backward per sequence and segment: as many as the chip holds at a time, and a channel group for
+// each of them at least and kMostGroups at most.  (Each workgroup's sums over its channels cross HBM twice.)
+int64_t back_blocks(int64_t batch, int64_t segments, int64_t groups) {
+  int64_t n = kFull / (batch * segments > 0 ? batch * segments : 1);
+  if (n * kMostGroups < groups) n = over(groups, kMostGroups);
+  return n < 1 ? 1 : n > groups ? groups : n;
+}
+
+// A call's sizes, within what the kernels count in 32 bits, and where its workspace's parts lie.
+struct Plan {
+  int64_t groups, tiles, per, segments, blocks;
+  size_t bc, states, channels;  // floats: dB and dC; a state tensor of all segments; a channel tensor
+  Plan(int64_t batch, int64_t steps, int64_t dim, int n) {
+    const int lanes = lanes_of(n);
+    groups = over(dim, 64 / lanes), tiles = tiles_of(steps), per = tiles_per_segment(batch, steps, groups);
+    segments = tiles > 0 ? over(tiles, per) : 1;
+    blocks = back_blocks(batch, segments, groups);
+    bc = (size_t)(blocks * batch * steps) * 8 * (size_t)lanes;
+    channels = (size_t)(segments * batch * dim), states = channels * (size_t)n;
+  }
+  size_t bytes(bool backward) const {
+    const size_t joined = segments > 1 ? states + channels : 0;
+    return (backward ? bc + states + 2 * channels + joined : joined) * sizeof(float);
+  }
+};
 
 int check(const morph_ssm* a, int dtype) {
   if (!a || a->batch < 0 || a->steps < 0 || a->dim < 0 || a->reserved != 0) return MORPH_EINVAL;
   if (a->states < 1 || a->states > MORPH_SSM_MAX_STATES) return MORPH_ERANGE;
   if (!known_dtype(dtype)) return MORPH_EDTYPE;
   if (a->batch > 0 && a->dim > 0 && (!a->A || (a->steps > 0 && (!a->x || !a->dt || !a->B || !a->C)))) return MORPH_EINVAL;
-  const int64_t most = INT64_MAX >> 12;
-  if (a->batch > 0 && a->dim > 0 && (a->dim > most / a->batch || a->steps > most / a->batch / a->dim)) return MORPH_ERANGE;
+  const int64_t most = MORPH_SSM_MAX_STEP;
+  if (a->batch > INT32_MAX || a->steps > INT32_MAX - kT * kW || a->dim > most) return MORPH_ERANGE;
+  for (int64_t step : {a->x_step, a->dt_step, a->z ? a->z_step : 0, a->B_step, a->C_step})
+    if (step < 0 || step > most) return MORPH_ERANGE;
+  const int64_t all = INT64_MAX >> 12;
+  if (a->batch > 0 && a->dim > 0 && (a->dim > all / a->batch || a->steps > all / a->batch / a->dim)) return MORPH_ERANGE;
   return MORPH_OK;
 }
 
-size_t part_floats(int64_t batch, int64_t steps, int64_t dim, int states) {
-  const int lanes = lanes_of(states);
-  const int64_t blocks = over(over(dim, 64 / lanes), groups_per_block(batch, dim, lanes));
-  return (size_t)(blocks * batch * steps) * 8 * (size_t)lanes;
+Scan scan_of(const morph_ssm* a, const Plan& plan, int bytes) {
+  auto view = [&](const void* p, int64_t batch, int64_t step) {
+    return View{static_cast<const char*>(p), batch * bytes, (int32_t)(step * bytes)};
+  };
+  Scan s{};
+  s.x = view(a->x, a->x_batch, a->x_step), s.dt = view(a->dt, a->dt_batch, a->dt_step);
+  s.B = view(a->B, a->B_batch, a->B_step), s.C = view(a->C, a->C_batch, a->C_step);
+  if (a->z) s.z = view(a->z, a->z_batch, a->z_step);
+  s.A = a->A, s.skip = a->skip, s.dt_bias = a->dt_bias;
+  s.batch = (int32_t)a->batch, s.steps = (int32_t)a->steps, s.dim = (int32_t)a->dim, s.states = a->states;
+  s.tiles = (int32_t)plan.tiles, s.groups = (int32_t)plan.groups, s.segments = (int32_t)plan.segments;
+  s.per = (int32_t)plan.per;
+  return s;
+}
+
+// What enters each segment, into ends [segments][batch][dim][states].
+template <typename T, int L, bool kBack, bool kGated>
+int join_segments(const Scan& a, const float* first, float* ends, float* sums, hipStream_t s) {
+  if (a.segments < 2) return MORPH_OK;
+  const int64_t blocks = (int64_t)a.groups * a.batch * (a.segments - 1);
+  hipLaunchKernelGGL((ssm_ends_kernel<T, L, kBack, kGated && kBack>), dim3((unsigned)blocks), dim3(64 * kW), 0, s, a, ends, sums);
+  if (const int rc = launch_status()) return rc;
+  hipLaunchKernelGGL(ssm_join_kernel<kBack>, dim3((unsigned)over((int64_t)a.batch * a.dim * a.states, 256)), dim3(256), 0, s, a,
+                     first, ends, sums);
+  return launch_status();
 }
 
 }  // namespace
@@ -612,31 +910,39 @@ size_t part_floats(int64_t batch, int64_t steps, int64_t dim, int states) {
 
 using namespace morph;
 
-extern "C" int morph_ssm_forward(const morph_ssm* a, int dtype, void* y, float* last, float* kept, void* stream) {
+extern "C" size_t morph_ssm_workspace_bytes(int64_t batch, int64_t steps, int64_t dim, int states, int backward) {
+  if (batch < 1 || steps < 0 || dim < 1 || states < 1 || states > MORPH_SSM_MAX_STATES) return 0;
+  return Plan(batch, steps, dim, states).bytes(backward != 0);
+}
+
+extern "C" int morph_ssm_forward(const morph_ssm* a, int dtype, void* y, float* last, float* kept, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
   if (const int rc = check(a, dtype)) return rc;
   if (a->batch == 0 || a->dim == 0) return MORPH_OK;
   if ((a->steps > 0 && !y) || !last) return MORPH_EINVAL;
-  return by_form(dtype, a->states, [&](auto t, auto lanes) {
+  const Plan plan(a->batch, a->steps, a->dim, a->states);
+  if (a->steps != 1 && plan.bytes(false) > 0 && (!workspace || workspace_bytes < plan.bytes(false))) return MORPH_EWORKSPACE;
+  if (!launchable(plan.groups * plan.segments * a->batch, 64 * kW) ||
+      !launchable(over(a->batch * a->dim * a->states, 256), 256))
+    return MORPH_ERANGE;
+  hipStream_t s = as_stream(stream);
+  return by_form(dtype, a->states, a->z != nullptr, [&](auto t, auto lanes, auto gated) {
     using T = decltype(t);
     constexpr int L = decltype(lanes)::value;
+    constexpr bool kGated = decltype(gated)::value;
     if (a->steps == 1) {
       const int64_t groups = over(a->dim, 256 / L);
-      if (!launchable(groups * a->batch, 256)) return (int)MORPH_ERANGE;
-      hipLaunchKernelGGL((ssm_one_kernel<T, L>), dim3((unsigned)(groups * a->batch)), dim3(256), 0, as_stream(stream), *a,
-                         groups, y, last, kept);
+      hipLaunchKernelGGL((ssm_one_kernel<T, L>), dim3((unsigned)(groups * a->batch)), dim3(256), 0, s, *a, groups, y, last,
+                         kept);
       return launch_status();
     }
-    const int64_t groups = over(a->dim, 64 / L);
-    if (!launchable(groups * a->batch, 64 * kW)) return (int)MORPH_ERANGE;
-    hipLaunchKernelGGL((ssm_kernel<T, L>), dim3((unsigned)(groups * a->batch)), dim3(64 * kW), 0, as_stream(stream), *a,
-                       groups, y, last, kept);
+    const Scan scan = scan_of(a, plan, Fmt<T>::bytes);
+    float* ends = static_cast<float*>(workspace);
+    if (const int rc = join_segments<T, L, false, kGated>(scan, a->first, ends, ends + plan.states, s)) return rc;
+    hipLaunchKernelGGL((ssm_kernel<T, L, kGated>), dim3((unsigned)(plan.groups * plan.segments * a->batch)), dim3(64 * kW), 0,
+                       s, scan, a->first, ends, static_cast<char*>(y), last, kept);
     return launch_status();
   });
-}
-
-extern "C" size_t morph_ssm_workspace_bytes(int64_t batch, int64_t steps, int64_t dim, int states) {
-  if (batch < 0 || steps < 0 || dim < 0 || states < 1 || states > MORPH_SSM_MAX_STATES) return 0;
-  return (part_floats(batch, steps, dim, states) + (size_t)(batch * dim) * (size_t)(states + 2)) * sizeof(float);
 }
 
 extern "C" int morph_ssm_backward(const morph_ssm* a, int dtype, const float* kept, const void* dy, int64_t dy_batch,
@@ -648,34 +954,41 @@ extern "C" int morph_ssm_backward(const morph_ssm* a, int dtype, const float* ke
   if (!g->dA || (a->skip && !g->dskip) || (a->dt_bias && !g->ddt_bias)) return MORPH_EINVAL;
   if (a->batch > 0 && a->steps > 0 && (!kept || !dy || !g->dx || !g->ddt || !g->dB || !g->dC || (a->z && !g->dz)))
     return MORPH_EINVAL;
-  const size_t need = morph_ssm_workspace_bytes(a->batch, a->steps, a->dim, a->states);
+  if (dy_step < 0 || dy_step > MORPH_SSM_MAX_STEP) return MORPH_ERANGE;
+  const Plan plan(a->batch, a->steps, a->dim, a->states);
+  const size_t need = a->batch > 0 ? plan.bytes(true) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need)) return MORPH_EWORKSPACE;
-  SsmParts parts;
-  parts.bc = static_cast<float*>(workspace);
-  parts.A = parts.bc + part_floats(a->batch, a->steps, a->dim, a->states);
-  parts.skip = parts.A + a->batch * a->dim * a->states;
-  parts.dt_bias = parts.skip + a->batch * a->dim;
-  hipStream_t s = as_stream(stream);
   const int64_t rows = a->batch * a->steps, sums = over(rows * 8 * lanes_of(a->states), 256);
   const int64_t ends = over(a->dim * a->states, 256);
-  if (!launchable(sums, 256) || !launchable(ends, 256)) return MORPH_ERANGE;
-  const int rc = by_form(dtype, a->states, [&](auto t, auto lanes) {
+  if (!launchable(sums, 256) || !launchable(ends, 256) || !launchable(over(a->batch * a->dim * a->states, 256), 256) ||
+      !launchable(plan.groups * plan.segments * a->batch, 64 * kW))
+    return MORPH_ERANGE;
+  SsmParts parts;
+  parts.bc = static_cast<float*>(workspace);
+  parts.A = parts.bc + plan.bc;
+  parts.skip = parts.A + plan.states;
+  parts.dt_bias = parts.skip + plan.channels;
+  parts.late = parts.dt_bias + plan.channels;
+  parts.sums = parts.late + plan.states;
+  hipStream_t s = as_stream(stream);
+  const int rc = by_form(dtype, a->states, a->z != nullptr, [&](auto t, auto lanes, auto gated) {
     using T = decltype(t);
     constexpr int L = decltype(lanes)::value;
+    constexpr bool kGated = decltype(gated)::value;
     if (a->batch == 0) return (int)MORPH_OK;
-    const int per = groups_per_block(a->batch, a->dim, L);
-    const int64_t blocks = over(over(a->dim, 64 / L), per);
-    if (!launchable(blocks * a->batch, 64 * kW)) return (int)MORPH_ERANGE;
-    hipLaunchKernelGGL((ssm_back_kernel<T, L>), dim3((unsigned)(blocks * a->batch)), dim3(64 * kW), 0, s, *a, blocks, per,
-                       kept, dy, dy_batch, dy_step, dlast, *g, parts);
+    Scan scan = scan_of(a, plan, Fmt<T>::bytes);
+    scan.dy = View{static_cast<const char*>(dy), dy_batch * Fmt<T>::bytes, (int32_t)(dy_step * Fmt<T>::bytes)};
+    if (const int status = join_segments<T, L, true, kGated>(scan, dlast, parts.late, parts.sums, s)) return status;
+    hipLaunchKernelGGL((ssm_back_kernel<T, L, kGated>), dim3((unsigned)(plan.blocks * plan.segments * a->batch)),
+                       dim3(64 * kW), 0, s, scan, (int)plan.blocks, kept, dlast, *g, parts);
     if (const int status = launch_status()) return status;
     if (rows == 0) return (int)MORPH_OK;
-    hipLaunchKernelGGL(ssm_sum_kernel<T>, dim3((unsigned)sums), dim3(256), 0, s, parts.bc, blocks, rows, 4 * L, a->states,
-                       g->dB, g->dC);
+    hipLaunchKernelGGL(ssm_sum_kernel<T>, dim3((unsigned)sums), dim3(256), 0, s, parts.bc, plan.blocks, rows, 4 * L,
+                       a->states, g->dB, g->dC);
     return launch_status();
   });
   if (rc != MORPH_OK) return rc;
-  hipLaunchKernelGGL(ssm_batch_kernel, dim3((unsigned)ends), dim3(256), 0, s, parts, a->batch, a->dim, a->states, g->dA,
-                     g->dskip, g->ddt_bias);
+  hipLaunchKernelGGL(ssm_batch_kernel, dim3((unsigned)ends), dim3(256), 0, s, parts, plan.segments * a->batch, a->dim,
+                     a->states, g->dA, g->dskip, g->ddt_bias);
   return launch_status();
 }

@@ -66,15 +66,15 @@ __device__ __forceinline__ float load_one(const void* p, int64_t i) {
 template <typename T>
 __device__ __forceinline__ void store_one(void* p, int64_t i, float x) {
   if constexpr (std::is_same_v<T, F32>) static_cast<float*>(p)[i] = x;
-  else static_cast<uint16_t*>(p)[i] = (uint16_t)from_float<T>(x);
+  else static_cast<uint16_t*>(p)[i] = (uint16_t)pack2<T>(x, x);
 }
 
 // x from the lane that a DPP control names, within its row of 16 lanes.
 template <int kControl>
 __device__ __forceinline__ float dpp(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kControl, 0xF, 0xF, false));
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kControl, 0xF, 0xF, true));
 }
-constexpr int kRotate1 = 0x121, kRotate2 = 0x122, kRotate4 = 0x124, kRotate8 = 0x128;
+constexpr int kRotate1 = 0x121, kRotate2 = 0x122, kRotate4 = 0x124, kRotate8 = 0x128, kRotate12 = 0x12C;
 
 // The sum over the wave, in every lane: rotations sum a row of 16 lanes, the swaps the four rows.
 __device__ __forceinline__ float wave_sum(float x) {

@@ -23,7 +23,7 @@ import ctypes
 
 import torch
 
-from ._lib import (CONV_MAX_TAPS, SSM_MAX_STATES, SSM_SPAN, ConvArgs, SsmArgs, SsmGrads, check, lib)
+from ._lib import (CONV_MAX_TAPS, SSM_MAX_STATES, SSM_MAX_STEP, SSM_SPAN, ConvArgs, SsmArgs, SsmGrads, check, lib)
 from .layers import address, current_stream, dtype_code, first_order, require_gpu, requires_grad, running_on
 from .norm import FLOATS, whole
 
@@ -173,19 +173,31 @@ def _scan_args(x, dt, A, B, C, skip, z, dt_bias, state):
     return SsmArgs(*(address(t) for t in (x, dt, z, B, C, A, skip, dt_bias, state)), *x.shape, *strides, A.shape[1], 0)
 
 
+def _workspace(x, A, backward):
+    size = lib().morph_ssm_workspace_bytes(*x.shape, A.shape[1], backward)
+    return (_empty(size, torch.uint8, x.device) if size else None), size
+
+
+def _rows_of(t):
+    """_channels_last, with steps as near to each other as the kernels count (a copy if they are not)."""
+    t = _channels_last(t)
+    return t if t is None or t.stride(1) <= SSM_MAX_STEP else t.contiguous()
+
+
 def _scan(inputs, train, stream):
     x, dt, A, B, C, skip, z, dt_bias, state = inputs
     _check_scan(*inputs)
     with running_on(x.device, stream, inputs):
-        x, dt, B, C, z = (_channels_last(t) for t in (x, dt, B, C, z))
+        x, dt, B, C, z = (_rows_of(t) for t in (x, dt, B, C, z))
         A, skip, dt_bias, state = (whole(t) for t in (A, skip, dt_bias, state))
         batch, steps, dim = x.shape
         y = _empty(x.shape, x.dtype, x.device)
         last = _empty((batch, dim, A.shape[1]), torch.float32, x.device)
         states = _empty((batch, -(-steps // SSM_SPAN), dim, A.shape[1]), torch.float32, x.device) if train else None
         inputs = x, dt, A, B, C, skip, z, dt_bias, state
+        workspace, size = _workspace(x, A, 0)
         check(lib().morph_ssm_forward(ctypes.byref(_scan_args(*inputs)), dtype_code(x.dtype), address(y), address(last),
-                                      address(states), current_stream()))
+                                      address(states), address(workspace), size, current_stream()))
         return y, last, SavedSelective(*inputs, states)
 
 
@@ -212,7 +224,7 @@ def selective_scan_backward(dy, saved, dlast=None, stream=None):
     if dlast is not None:
         require_gpu(dlast, "dlast", (torch.float32,), (batch, dim, A.shape[1]), x.device)
     with running_on(x.device, stream, (dy, *inputs, saved.states, dlast)):
-        dy, dlast = _channels_last(dy), whole(dlast)
+        dy, dlast = _rows_of(dy), whole(dlast)
 
         def like(t):
             return _empty(t.shape, t.dtype, t.device) if t is not None else None
@@ -220,8 +232,7 @@ def selective_scan_backward(dy, saved, dlast=None, stream=None):
         dx, ddt, dA, dB, dC, dskip, dz, ddt_bias = (like(t) for t in inputs[:-1])
         dstate = _empty((batch, dim, A.shape[1]), torch.float32, x.device)
         grads = SsmGrads(*(address(t) for t in (dx, ddt, dz, dB, dC, dA, dskip, ddt_bias, dstate)))
-        size = lib().morph_ssm_workspace_bytes(batch, steps, dim, A.shape[1])
-        workspace = _empty(size, torch.uint8, x.device)
+        workspace, size = _workspace(x, A, 1)
         check(lib().morph_ssm_backward(ctypes.byref(_scan_args(*inputs)), dtype_code(x.dtype), address(saved.states),
                                        address(dy), dy.stride(0), dy.stride(1), address(dlast), ctypes.byref(grads),
                                        address(workspace), size, current_stream()))

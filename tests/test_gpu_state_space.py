@@ -265,7 +265,12 @@ def test_scan_passes_padding_on():
     dlast = normal(gen, 2, 20, 16).to(DEV)
     (y, last), back = check_scan([x, dt, A, B, C, skip, z, bias, first], normal(gen, 2, 150, 20, dtype=BF16).to(DEV), dlast)
     short = selective_scan(x[:1, :100], dt[:1, :100], A, B[:1, :100], C[:1, :100], skip, z[:1, :100], bias, first[:1])
-    assert torch.equal(last[:1], short[1])
+    # the two are joined at other places, as in test_scan_in_pieces_is_the_whole
+    R.assert_scan(last[:1], short[1].cpu(), F32, "last")
+    for steps in (1, 40, 150):  # gates of 1 and inputs of 0, however they are joined
+        nothing = torch.full_like(dt[:, :steps], -math.inf)
+        _, same_state = selective_scan(x[:, :steps], nothing, A, B[:, :steps], C[:, :steps], skip, None, bias, first)
+        assert torch.equal(same_state, first)
     assert not back[1][0, 100:].any() and not back[3][0, 100:].any()
 
 
@@ -342,8 +347,9 @@ def test_calls_repeat_their_bits_on_any_stream_and_in_a_graph(kind):
     assert same(call(), first)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
-    assert same(call(stream=side), first)
+    there = call(stream=side)
     side.synchronize()
+    assert same(there, first)
     with torch.cuda.stream(side):
         call()
         graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()

@@ -99,8 +99,8 @@ def test_scan_refuses_before_any_launch():
                                          *[steps * n, n] * 2, n, reserved))
     full = [P] * 9
 
-    def forward(a, dtype=1, y=p, last=p):
-        return lib.morph_ssm_forward(a, dtype, y, last, p, None)
+    def forward(a, dtype=1, y=p, last=p, ws=p, size=1 << 60):
+        return lib.morph_ssm_forward(a, dtype, y, last, p, ws, size, None)
 
     def backward(a, dtype=1, kept=p, dy=p, grads=full, ws=p, size=1 << 60):
         grads = ctypes.byref(_lib.SsmGrads(*grads)) if grads else None
@@ -116,7 +116,11 @@ def test_scan_refuses_before_any_launch():
     assert backward(args(), grads=None) == EINVAL
     for k in range(8):  # all but dfirst
         assert backward(args(), grads=[None if i == k else P for i in range(9)]) == EINVAL, k
-    assert backward(args(), size=lib.morph_ssm_workspace_bytes(2, 5, 8, 16) - 1) == EWORKSPACE
+    assert backward(args(), size=lib.morph_ssm_workspace_bytes(2, 5, 8, 16, 1) - 1) == EWORKSPACE
+    assert lib.morph_ssm_workspace_bytes(2, 5, 8, 16, 0) == 0 < lib.morph_ssm_workspace_bytes(1, 1000, 64, 16, 0)
+    assert forward(args(1, 1000, 64), size=lib.morph_ssm_workspace_bytes(1, 1000, 64, 16, 0) - 1) == EWORKSPACE
+    assert forward(args(1, 1000, 64), ws=None) == EWORKSPACE
+    assert forward(args(dim=(1 << 25) + 1)) == ERANGE and forward(args(steps=(1 << 31) - 1, dim=1)) == ERANGE
     assert backward(args(), ws=None) == EWORKSPACE
 
 
