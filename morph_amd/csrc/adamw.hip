@@ -38,7 +38,7 @@
 
 #include "adamw_table.h"
 #include "common.h"
-#include "layers.h"
+#include "stage.h"
 
 #ifndef MORPH_ADAMW_UNROLL
 #define MORPH_ADAMW_UNROLL 1
@@ -53,6 +53,9 @@
 #endif
 #ifndef MORPH_ADAMW_BLOCK
 #define MORPH_ADAMW_BLOCK 64
+#endif
+#ifndef MORPH_ADAMW8_CHUNKS
+#define MORPH_ADAMW8_CHUNKS 4
 #endif
 #ifndef MORPH_ADAMW_NT
 #define MORPH_ADAMW_NT 1
@@ -228,6 +231,32 @@ __device__ __forceinline__ float saturated(float x) {
 
 static_assert(kPerBlock == 4 * kBlock && kPerBlock % kGroup == 0, "a lane has one word of codes");
 
+// Chunks of kPerBlock elements of a wave, whose loads are all issued first.
+constexpr int kChunks8 = MORPH_ADAMW8_CHUNKS;
+
+// adamw_update for a step's constants, with the hardware's square root and reciprocal (each within 1 unit of 2^-23, so the master's change is
+// within 2^-20 of itself): the correctly rounded ones are 45 of 64 instructions an element, and the
+// kernel is bound by instructions with them (75 million parameters: 312 us, of which 180 are HBM's).
+// Constants that a call does without are ones here, which change no bit.
+struct Update8 {
+  float scale, inv_scale, clip, decay, lerp, beta2, one_minus_beta2, inverse_bias2, neg_step_size, eps;
+  bool divide, lerp_large;
+  __device__ __forceinline__ explicit Update8(const morph_adamw_hp& hp)
+      : scale(hp.scale), inv_scale(hp.inv_scale), clip(hp.flags & MORPH_HP_APPLY_CLIP ? hp.clip : 1.0f),
+        decay(hp.flags & MORPH_HP_APPLY_DECAY ? hp.decay : 1.0f),
+        lerp(hp.flags & MORPH_HP_LERP_LARGE ? hp.lerp_weight - 1.0f : hp.lerp_weight), beta2(hp.beta2),
+        one_minus_beta2(hp.one_minus_beta2), inverse_bias2(1.0f / hp.bias_correction2_sqrt),
+        neg_step_size(hp.neg_step_size), eps(hp.eps), divide(hp.flags & MORPH_HP_DIVIDE_SCALE),
+        lerp_large(hp.flags & MORPH_HP_LERP_LARGE) {}
+  __device__ __forceinline__ void operator()(float g, float& p, float& m, float& v) const {
+    g = (divide ? g / scale : g * inv_scale) * clip;
+    m = __fmaf_rn(lerp, g - m, lerp_large ? g : m);
+    v = __fmaf_rn(one_minus_beta2 * g, g, v * beta2);
+    const float d = __fmaf_rn(__builtin_amdgcn_sqrtf(v), inverse_bias2, eps);
+    p = __fmaf_rn(neg_step_size * m, __builtin_amdgcn_rcpf(d), p * decay);
+  }
+};
+
 struct VecRegs8 {
   f32x4 P;
   uint32_t M, V;
@@ -236,20 +265,10 @@ struct VecRegs8 {
 };
 
 template <typename GT>
-__device__ __forceinline__ void load_vector8(const TensorArg& T, int64_t base, VecRegs8& r) {
-  const int64_t e = base + threadIdx.x * 4, codes = (T.n + kGroup - 1) / kGroup * kGroup;
+__device__ __forceinline__ void load_vector8(const TensorArg& T, int64_t codes, int64_t base, VecRegs8& r) {
+  const int64_t e = base + threadIdx.x * 4;
   const uint8_t* m = reinterpret_cast<const uint8_t*>(T.m);
   const uint8_t* v = reinterpret_cast<const uint8_t*>(T.v);
-  if (T.vector_ok && base + kPerBlock <= T.n) {
-    load_grad4<GT>(T.grad, e, r.G);
-    r.P = load_stream<kNT>(reinterpret_cast<const f32x4*>(T.p + e));
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      r.G[k] = e + k < T.n ? load_grad1<GT>(T.grad, e + k) : 0.0f;
-      r.P[k] = e + k < T.n ? T.p[e + k] : 0.0f;
-    }
-  }
   r.M = r.V = 0, r.em = r.ev = 1;
   if (e < codes) {
     r.M = load_stream<kNT>(reinterpret_cast<const uint32_t*>(m + e));
@@ -257,12 +276,25 @@ __device__ __forceinline__ void load_vector8(const TensorArg& T, int64_t base, V
     r.em = m[codes + e / kGroup];
     r.ev = v[codes + e / kGroup];
   }
+  if (T.vector_ok && base + kPerBlock <= T.n) {
+    load_grad4<GT>(T.grad, e, r.G);
+    r.P = load_stream<kNT>(reinterpret_cast<const f32x4*>(T.p + e));
+  } else {  // behind the last element: zeros, whose moments stay zeros
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool there = e + k < T.n;
+      r.G[k] = there ? load_grad1<GT>(T.grad, e + k) : 0.0f;
+      r.P[k] = there ? T.p[e + k] : 0.0f;
+      if (!there) r.M &= ~(0xFFu << (8 * k)), r.V &= ~(0xFFu << (8 * k));
+    }
+  }
 }
 
 template <typename OT>
-__device__ __forceinline__ void update_vector8(const TensorArg& T, const morph_adamw_hp& hp, uint32_t key,
+__device__ __forceinline__ void update_vector8(const TensorArg& T, const Update8& update, uint32_t key, int64_t codes,
                                                int64_t base, VecRegs8& r) {
-  const int64_t e = base + threadIdx.x * 4, codes = (T.n + kGroup - 1) / kGroup * kGroup;
+  const int64_t e = base + threadIdx.x * 4;
+  const bool whole = base + kPerBlock <= T.n;
   float m[4], v[4];
   uint32_t most_m = 0, most_v = 0;
   act_decode4(r.M, act_scale(r.em), m);
@@ -270,10 +302,9 @@ __device__ __forceinline__ void update_vector8(const TensorArg& T, const morph_a
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     float p = r.P[k];
-    adamw_update(r.G[k], p, m[k], v[k], hp);
+    update(r.G[k], p, m[k], v[k]);
     r.P[k] = p;
-    m[k] = e + k < T.n ? saturated(m[k]) : 0.0f;
-    v[k] = e + k < T.n ? saturated(v[k]) : 0.0f;
+    m[k] = saturated(m[k]), v[k] = saturated(v[k]);
     most_m = max(most_m, magnitude(m[k]));
     most_v = max(most_v, magnitude(v[k]));
   }
@@ -292,7 +323,7 @@ __device__ __forceinline__ void update_vector8(const TensorArg& T, const morph_a
     r.M |= first << (8 * k);
     r.V |= second << (8 * k);
   }
-  if (T.vector_ok && base + kPerBlock <= T.n) {
+  if (T.vector_ok && whole) {
     store_stream<kNT>(reinterpret_cast<f32x4*>(T.p + e), r.P);
     if (T.out != nullptr) store_out4<OT>(T.out, e, r.P);
   } else {
@@ -402,17 +433,24 @@ __device__ __forceinline__ uint32_t rounding_key(const Args& a, const TensorArg&
   return mix32(mix32(hp.reserved + (uint32_t)(T.clock + 1) * 0x9E3779B9u) ^ (uint32_t)(a.clocks[T.clock] + 1));
 }
 
-// Block b of tensor T.
-template <typename GT, typename OT, bool kDev, int kBits, typename Args>
+// Block b of tensor T; with moments in 8 bits of kChunks times as many elements.
+template <typename GT, typename OT, bool kDev, int kBits, int kChunks = 1, typename Args>
 __device__ __forceinline__ void run_block(const Args& a, const TensorArg& T, int b,
                                           const uint32_t* skip) {
   const int64_t base = (int64_t)(b - T.first_block) * kPerBlock;
   morph_adamw_hp hp;
   if constexpr (kBits == 8) {
-    VecRegs8 r;
-    load_vector8<GT>(T, base, r);
+    const int64_t codes = (T.n + kGroup - 1) / kGroup * kGroup;
+    VecRegs8 r[kChunks];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) load_vector8<GT>(T, codes, base * kChunks + i * kPerBlock, r[i]);
     if (!control<kDev>(a, T, skip, hp)) return;
-    update_vector8<OT>(T, hp, rounding_key(a, T, hp), base, r);
+    const uint32_t key = rounding_key(a, T, hp);
+    const Update8 update(hp);
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+      if (i == 0 || base * kChunks + i * kPerBlock < T.n)
+        update_vector8<OT>(T, update, key, codes, base * kChunks + i * kPerBlock, r[i]);
   } else if (T.vector_ok && base + kPerBlock <= T.n) {
     // The streams are requested before the control words, so their latency
     // overlaps; a skipped step (control false) still writes nothing.
@@ -430,7 +468,7 @@ template <typename GT, typename OT, bool kDev, int kBits>
 __global__ __launch_bounds__(kBlock) void adamw_multi_kernel(const LaunchArgs a,
                                                              const uint32_t* __restrict__ skip) {
   const int b = a.reverse ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
-  run_block<GT, OT, kDev, kBits>(a, a.t[segment_of(a.t, a.count, b)], b, skip);
+  run_block<GT, OT, kDev, kBits, kBits == 8 ? kChunks8 : 1>(a, a.t[segment_of(a.t, a.count, b)], b, skip);
 }
 
 // Many tensors in one launch (adamw_table.h): the descriptors lie in device memory, the
@@ -619,7 +657,8 @@ int enqueue(const morph_adamw_tensor* tensors, int count, int grad_dtype, int ou
       d.first_block = blocks;
       d.vector_ok = vector_ok(d.p, d.m, d.v, d.grad, gb, d.out, ob);
       d.clock = dev ? t.clock_index : 0;
-      blocks += (int)((n + kPerBlock - 1) / kPerBlock);
+      const int64_t each = kPerBlock * (bits == 8 ? kChunks8 : 1);
+      blocks += (int)((n + each - 1) / each);
       grad_bytes += n * gb;
     }
   }
@@ -848,7 +887,7 @@ extern "C" int morph_adamw8_multi_dev(const morph_adamw_tensor* tensors, int cou
 namespace {
 
 constexpr int kValueTensors = 64;
-constexpr int kValuesPerBlock = 1024;  // 256 lanes, a word of each moment's codes
+constexpr int kValuesPerBlock = 2048;  // 256 lanes, two words of each moment's codes
 
 struct ValueArgs {
   morph_moment_values t[kValueTensors];
@@ -856,6 +895,18 @@ struct ValueArgs {
   int32_t count;
 };
 static_assert(sizeof(ValueArgs) + 64 <= kMaxKernargBytes, "launch table fits the kernel arguments");
+
+template <typename T>
+__device__ __forceinline__ void store_values(void* out, int64_t e, int64_t n, const float (&x)[8]) {
+  constexpr int V = Wide<T>::kCount;
+#pragma unroll
+  for (int k = 0; k < 8; k += V) {
+    float part[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[j] = x[k + j];
+    Wide<T>::store(out, e + k, Wide<T>::pack(part), n - k);
+  }
+}
 
 template <typename T>
 __global__ __launch_bounds__(256) void moment_values_kernel(const ValueArgs a) {
@@ -866,29 +917,30 @@ __global__ __launch_bounds__(256) void moment_values_kernel(const ValueArgs a) {
     else hi = mid - 1;
   }
   const morph_moment_values& t = a.t[lo];
-  const int64_t e = (int64_t)((int)blockIdx.x - a.first_block[lo]) * kValuesPerBlock + threadIdx.x * 4;
+  const int64_t e = (int64_t)((int)blockIdx.x - a.first_block[lo]) * kValuesPerBlock + threadIdx.x * 8;
   if (e >= t.numel) return;
   const int64_t codes = (t.numel + kGroup - 1) / kGroup * kGroup;
   const uint8_t* first = static_cast<const uint8_t*>(t.exp_avg);
   const uint8_t* second = static_cast<const uint8_t*>(t.exp_avg_sq);
-  float m[4], v[4];
-  act_decode4(*reinterpret_cast<const uint32_t*>(first + e), act_scale(first[codes + e / kGroup]), m);
-  decode_second4(*reinterpret_cast<const uint32_t*>(second + e), second[codes + e / kGroup], v);
-  const f32x4 M{m[0], m[1], m[2], m[3]}, V{v[0], v[1], v[2], v[3]};
-  constexpr int kBytes = 4 * Fmt<T>::bytes;
-  const bool wide = ((reinterpret_cast<uintptr_t>(t.exp_avg_out) | reinterpret_cast<uintptr_t>(t.exp_avg_sq_out)) %
-                     kBytes) == 0;
-  if (wide && e + 4 <= t.numel) {
-    store_out4<T>(t.exp_avg_out, e, M);
-    store_out4<T>(t.exp_avg_sq_out, e, V);
-    return;
-  }
+  typedef uint32_t pair __attribute__((ext_vector_type(2), aligned(4)));
+  const u32x2 m = *reinterpret_cast<const pair*>(first + e), v = *reinterpret_cast<const pair*>(second + e);
+  const float scale = act_scale(first[codes + e / kGroup]);
+  const int shift = second[codes + e / kGroup];
+  float x[8], four[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (e + k < t.numel) {
-      store_out1<T>(t.exp_avg_out, e + k, M[k]);
-      store_out1<T>(t.exp_avg_sq_out, e + k, V[k]);
-    }
+  for (int w = 0; w < 2; ++w) {
+    act_decode4(m[w], scale, four);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[4 * w + k] = four[k];
+  }
+  store_values<T>(t.exp_avg_out, e, t.numel - e, x);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    decode_second4(v[w], shift, four);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[4 * w + k] = four[k];
+  }
+  store_values<T>(t.exp_avg_sq_out, e, t.numel - e, x);
 }
 
 }  // namespace
