@@ -55,7 +55,7 @@
 #define MORPH_ADAMW_BLOCK 64
 #endif
 #ifndef MORPH_ADAMW8_CHUNKS
-#define MORPH_ADAMW8_CHUNKS 4
+#define MORPH_ADAMW8_CHUNKS 2
 #endif
 #ifndef MORPH_ADAMW_NT
 #define MORPH_ADAMW_NT 1
@@ -231,12 +231,14 @@ __device__ __forceinline__ float saturated(float x) {
 
 static_assert(kPerBlock == 4 * kBlock && kPerBlock % kGroup == 0, "a lane has one word of codes");
 
-// Chunks of kPerBlock elements of a wave, whose loads are all issued first.
+// Chunks of kPerBlock elements of a wave, whose loads are all issued first.  75 million parameters, FP16 gradients and
+// copies: 203 us with two, 206 with four, and no fewer waves on a CU than fit (the 16 of kOccupancyLds: 251
+// and 233; with one chunk 284, with eight 256), of which HBM's are 181.
 constexpr int kChunks8 = MORPH_ADAMW8_CHUNKS;
 
 // adamw_update for a step's constants, with the hardware's square root and reciprocal (each within 1 unit of 2^-23, so the master's change is
 // within 2^-20 of itself): the correctly rounded ones are 45 of 64 instructions an element, and the
-// kernel is bound by instructions with them (75 million parameters: 312 us, of which 180 are HBM's).
+// kernel is bound by instructions with them (75 million parameters: 333 us).
 // Constants that a call does without are ones here, which change no bit.
 struct Update8 {
   float scale, inv_scale, clip, decay, lerp, beta2, one_minus_beta2, inverse_bias2, neg_step_size, eps;
@@ -508,12 +510,11 @@ struct Stamps {
 
 template <typename K>
 void launch_kernel(K kernel, int blocks, const LaunchArgs& a, const uint32_t* skip, hipStream_t s,
-                   Stamps ev) {
+                   Stamps ev, unsigned lds = kOccupancyLds) {
   if (ev.e0 == nullptr && ev.e1 == nullptr)
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBlock), kOccupancyLds, s, a, skip);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBlock), lds, s, a, skip);
   else
-    hipExtLaunchKernelGGL(kernel, dim3(blocks), dim3(kBlock), kOccupancyLds, s, ev.e0, ev.e1, 0u,
-                          a, skip);
+    hipExtLaunchKernelGGL(kernel, dim3(blocks), dim3(kBlock), lds, s, ev.e0, ev.e1, 0u, a, skip);
 }
 
 // How a call's launches run: constants from the host, or from the device with moments in 32 or 8 bits.
@@ -523,7 +524,7 @@ template <typename GT, typename OT>
 int launch(Form form, const LaunchArgs& a, int blocks, const uint32_t* skip, hipStream_t s,
            Stamps ev) {
   if (form == Form::kDev8)
-    launch_kernel(adamw_multi_kernel<GT, OT, true, 8>, blocks, a, skip, s, ev);
+    launch_kernel(adamw_multi_kernel<GT, OT, true, 8>, blocks, a, skip, s, ev, 0u);
   else if (form == Form::kDev)
     launch_kernel(adamw_multi_kernel<GT, OT, true, 32>, blocks, a, skip, s, ev);
   else
@@ -704,12 +705,13 @@ int launch_table(const TableArgs& a, const void* d_table, int count, int blocks,
                  const uint32_t* skip, hipStream_t s, Stamps ev) {
   const TableRow* rows = static_cast<const TableRow*>(d_table);
   const int32_t* map = reinterpret_cast<const int32_t*>(rows + count);
+  const unsigned lds = kBits == 8 ? 0u : kOccupancyLds;
   if (ev.e0 == nullptr && ev.e1 == nullptr)
-    hipLaunchKernelGGL((adamw_table_kernel<GT, OT, kBits>), dim3(blocks), dim3(kBlock), kOccupancyLds,
-                       s, a, rows, map, skip);
+    hipLaunchKernelGGL((adamw_table_kernel<GT, OT, kBits>), dim3(blocks), dim3(kBlock), lds, s, a,
+                       rows, map, skip);
   else
-    hipExtLaunchKernelGGL((adamw_table_kernel<GT, OT, kBits>), dim3(blocks), dim3(kBlock),
-                          kOccupancyLds, s, ev.e0, ev.e1, 0u, a, rows, map, skip);
+    hipExtLaunchKernelGGL((adamw_table_kernel<GT, OT, kBits>), dim3(blocks), dim3(kBlock), lds, s,
+                          ev.e0, ev.e1, 0u, a, rows, map, skip);
   return launch_status();
 }
 

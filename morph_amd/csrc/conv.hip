@@ -12,54 +12,63 @@ namespace {
 
 constexpr int kRun = 16;      // steps of a wave, forward
 constexpr int kBackRun = 32;  // and backward
-constexpr int kAhead = 4;     // steps whose loads are issued together
+constexpr int kAhead = 8;     // steps whose loads are issued together, backward
 constexpr int kParts = 512;
 
-// kCount neighbouring channels.
-template <typename T, int kCount>
-struct Lanes {
-  static __device__ __forceinline__ void load(const void* p, int64_t at, int64_t n, float (&x)[kCount]) {
-    if constexpr (kCount == Wide<T>::kCount) {
-      Wide<T>::unpack(Wide<T>::load(p, at, n), x);
-    } else {
-      static_assert(Fmt<T>::bytes == 2 && kCount == 4, "half of an access");
-      const uint16_t* q = static_cast<const uint16_t*>(p) + at;
-      typedef uint32_t pair __attribute__((ext_vector_type(2), aligned(2)));
-      u32x2 w = 0;
-      if (n >= 4) {
-        w = *reinterpret_cast<const pair*>(q);
-      } else {
+// Four neighbouring channels at any element's address, as loaded (16 bits: two words).
+constexpr int V = 4;
+template <typename T>
+struct Four {
+  typedef std::conditional_t<Fmt<T>::bytes == 4, u32x4, u32x2> raw;
+  typedef uint32_t pair __attribute__((ext_vector_type(2), aligned(2)));
+  typedef std::conditional_t<Fmt<T>::bytes == 4, u32x4_any, pair> at_any;
+  // The first n of them, the others 0.
+  static __device__ __forceinline__ raw load(const void* p, int64_t at, int64_t n) {
+    const char* q = static_cast<const char*>(p) + at * Fmt<T>::bytes;
+    if (n >= V) return *reinterpret_cast<const at_any*>(q);
+    raw w = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < n) w[k / 2] |= (uint32_t)q[k] << (16 * (k % 2));
+    for (int k = 0; k < V; ++k)
+      if (k < n) {
+        if constexpr (Fmt<T>::bytes == 4) w[k] = reinterpret_cast<const uint32_t*>(q)[k];
+        else w[k / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[k] << (16 * (k % 2));
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = to_float<T>(k % 2 ? w[k / 2] >> 16 : w[k / 2] & 0xFFFFu);
-    }
+    return w;
   }
-  static __device__ __forceinline__ void store(void* p, int64_t at, int64_t n, const float (&x)[kCount]) {
-    if constexpr (kCount == Wide<T>::kCount) {
-      Wide<T>::store(p, at, Wide<T>::pack(x), n);
-    } else {
-      uint16_t* q = static_cast<uint16_t*>(p) + at;
-      typedef uint32_t pair __attribute__((ext_vector_type(2), aligned(2)));
-      const u32x2 w{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-      if (n >= 4) {
-        *reinterpret_cast<pair*>(q) = w;
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < n) q[k] = (uint16_t)(w[k / 2] >> (16 * (k % 2)));
-      }
+  static __device__ __forceinline__ float value(const raw& w, int k) {
+    if constexpr (Fmt<T>::bytes == 4) return __builtin_bit_cast(float, (uint32_t)w[k]);
+    else return to_float<T>(k % 2 ? w[k / 2] >> 16 : w[k / 2] & 0xFFFFu);
+  }
+  static __device__ __forceinline__ void store(void* p, int64_t at, int64_t n, const raw& w) {
+    char* q = static_cast<char*>(p) + at * Fmt<T>::bytes;
+    if (n >= V) {
+      *reinterpret_cast<at_any*>(q) = w;
+      return;
     }
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < n) {
+        if constexpr (Fmt<T>::bytes == 4) reinterpret_cast<uint32_t*>(q)[k] = w[k];
+        else reinterpret_cast<uint16_t*>(q)[k] = (uint16_t)(w[k / 2] >> (16 * (k % 2)));
+      }
+  }
+  static __device__ __forceinline__ void store(void* p, int64_t at, int64_t n, const float (&x)[V]) {
+    raw w;
+    if constexpr (Fmt<T>::bytes == 4) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) w[k] = __builtin_bit_cast(uint32_t, x[k]);
+    } else {
+      w = raw{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+    }
+    store(p, at, n, w);
   }
 };
 
-template <typename W, int kTaps, int kCount>
-__device__ __forceinline__ void load_taps(const morph_conv& a, int64_t c, int64_t n, float (&w)[kTaps][kCount],
-                                          float (&bias)[kCount]) {
+template <typename W, int kTaps>
+__device__ __forceinline__ void load_taps(const morph_conv& a, int64_t c, int64_t n, float (&w)[kTaps][V],
+                                          float (&bias)[V]) {
 #pragma unroll
-  for (int i = 0; i < kCount; ++i) {
+  for (int i = 0; i < V; ++i) {
     bias[i] = a.bias && i < n ? load_one<W>(a.bias, c + i) : 0.0f;
 #pragma unroll
     for (int k = 0; k < kTaps; ++k) w[k][i] = i < n ? load_one<W>(a.weight, (c + i) * kTaps + k) : 0.0f;
@@ -67,16 +76,10 @@ __device__ __forceinline__ void load_taps(const morph_conv& a, int64_t c, int64_
 }
 
 // x of step t of sequence b, where t may lie before the first step; 0 behind the last one.
-template <typename T, int kCount>
-__device__ __forceinline__ void load_input(const morph_conv& a, int64_t b, int64_t t, int64_t c, int64_t n,
-                                           float (&x)[kCount]) {
-#pragma unroll
-  for (int i = 0; i < kCount; ++i) x[i] = 0.0f;
-  if (t >= 0) {
-    if (t < a.steps) Lanes<T, kCount>::load(a.x, b * a.x_batch + t * a.x_step + c, n, x);
-  } else if (a.before) {
-    Lanes<T, kCount>::load(a.before, (b * (a.taps - 1) + t + a.taps - 1) * a.dim + c, n, x);
-  }
+template <typename T>
+__device__ __forceinline__ typename Four<T>::raw load_input(const morph_conv& a, int64_t b, int64_t t, int64_t c, int64_t n) {
+  if (t >= 0) return t < a.steps ? Four<T>::load(a.x, b * a.x_batch + t * a.x_step + c, n) : typename Four<T>::raw(0);
+  return a.before ? Four<T>::load(a.before, (b * (a.taps - 1) + t + a.taps - 1) * a.dim + c, n) : typename Four<T>::raw(0);
 }
 
 struct ConvGrid {
@@ -86,126 +89,140 @@ struct ConvGrid {
 template <typename T, typename W, int kTaps>
 __global__ __launch_bounds__(256) void conv_kernel(const morph_conv a, const ConvGrid g, void* __restrict__ y,
                                                    void* __restrict__ after) {
-  constexpr int V = Wide<T>::kCount;
   const int64_t block = blockIdx.x, cb = block % g.channel_blocks, rest = block / g.channel_blocks;
   const int64_t tb = rest % g.time_blocks, b = rest / g.time_blocks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t c = (cb * 64 + (threadIdx.x & 63)) * V, n = a.dim - c;
   if (n <= 0) return;
   const int64_t t0 = (tb * 4 + wave) * kRun;
+  typedef typename Four<T>::raw raw;
   if (t0 < a.steps) {
-    float w[kTaps][V], bias[V], x[kTaps - 1 + kAhead][V];
-    load_taps<W, kTaps, V>(a, c, n, w, bias);
+    raw x[kTaps - 1 + kRun];  // all of the run's loads first
+    float w[kTaps][V], bias[V], in[kTaps][V];
+    if (t0 + kRun <= a.steps) {
+      const int64_t at = b * a.x_batch + t0 * a.x_step + c;
 #pragma unroll
-    for (int k = 0; k < kTaps - 1; ++k) load_input<T, V>(a, b, t0 - (kTaps - 1) + k, c, n, x[k]);
-    for (int64_t t = t0; t < t0 + kRun && t < a.steps; t += kAhead) {
+      for (int i = 0; i < kRun; ++i) x[kTaps - 1 + i] = Four<T>::load(a.x, at + i * a.x_step, n);
+    } else {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) load_input<T, V>(a, b, t + i, c, n, x[kTaps - 1 + i]);
+      for (int i = 0; i < kRun; ++i) x[kTaps - 1 + i] = load_input<T>(a, b, t0 + i, c, n);
+    }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (t + i >= a.steps) break;
-        float out[V];
+    for (int k = 0; k < kTaps - 1; ++k) x[k] = load_input<T>(a, b, t0 - (kTaps - 1) + k, c, n);
+    load_taps<W, kTaps>(a, c, n, w, bias);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float p = bias[j];
+    for (int k = 0; k < kTaps - 1; ++k)
 #pragma unroll
-          for (int k = 0; k < kTaps; ++k) p = __fmaf_rn(w[k][j], x[i + k][j], p);
-          out[j] = p * gate_sigmoid(p);
-        }
-        Lanes<T, V>::store(y, (b * a.steps + t + i) * a.dim + c, n, out);
+      for (int j = 0; j < V; ++j) in[k + 1][j] = Four<T>::value(x[k], j);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      if (t0 + i >= a.steps) break;
+      float out[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+#pragma unroll
+        for (int k = 0; k < kTaps - 1; ++k) in[k][j] = in[k + 1][j];
+        in[kTaps - 1][j] = Four<T>::value(x[kTaps - 1 + i], j);
+        float p = bias[j];
+#pragma unroll
+        for (int k = 0; k < kTaps; ++k) p = __fmaf_rn(w[k][j], in[k][j], p);
+        out[j] = p * gate_sigmoid(p);
       }
-#pragma unroll
-      for (int k = 0; k < kTaps - 1; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[k][j] = x[kAhead + k][j];
+      Four<T>::store(y, (b * a.steps + t0 + i) * a.dim + c, n, out);
     }
   }
-  if (tb == g.time_blocks - 1 && wave == 0) {  // a copy: the conversion to FP32 and back changes nothing
+  if (tb == g.time_blocks - 1 && wave == 0) {
 #pragma unroll
-    for (int k = 0; k < kTaps - 1; ++k) {
-      float x[V];
-      load_input<T, V>(a, b, a.steps - (kTaps - 1) + k, c, n, x);
-      Lanes<T, V>::store(after, (b * (kTaps - 1) + k) * a.dim + c, n, x);
-    }
+    for (int k = 0; k < kTaps - 1; ++k)
+      Four<T>::store(after, (b * (kTaps - 1) + k) * a.dim + c, n, load_input<T>(a, b, a.steps - (kTaps - 1) + k, c, n));
   }
 }
 
-// run: steps of a wave.  parts: [gridDim.y][taps + 1][dim].
+// parts: [gridDim.y][taps + 1][dim].
 template <typename T, typename W, int kTaps>
-__global__ __launch_bounds__(256) void conv_back_kernel(const morph_conv a, const ConvGrid g, int run,
-                                                        const void* __restrict__ dy, int64_t dy_batch, int64_t dy_step,
+__global__ __launch_bounds__(256) void conv_back_kernel(const morph_conv a, const ConvGrid g, const void* __restrict__ dy, int64_t dy_batch, int64_t dy_step,
                                                         const void* __restrict__ dafter, void* __restrict__ dx,
                                                         void* __restrict__ dbefore, float* __restrict__ parts) {
-  constexpr int V = 4;
+  typedef typename Four<T>::raw raw;
   __shared__ float join[kTaps + 1][V][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * V, n = a.dim - c;
   float w[kTaps][V], bias[V], dw[kTaps + 1][V];
-  load_taps<W, kTaps, V>(a, c, n, w, bias);
+  load_taps<W, kTaps>(a, c, n, w, bias);
 #pragma unroll
   for (int k = 0; k <= kTaps; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[k][j] = 0.0f;
   for (int64_t unit = blockIdx.y; unit < a.batch * g.time_blocks; unit += gridDim.y) {
-    const int64_t b = unit / g.time_blocks, t0 = ((unit % g.time_blocks) * 4 + wave) * run;
+    const int64_t b = unit / g.time_blocks, t0 = ((unit % g.time_blocks) * 4 + wave) * kBackRun;
     if (n <= 0 || (t0 >= a.steps && t0 > 0)) continue;
-    // x[k], d[k]: of step t - (kTaps - 1) + k; d is dp
-    float x[kTaps - 1 + kAhead][V], d[kTaps - 1 + kAhead][V];
+    const int64_t end = t0 + kBackRun + kTaps - 1;
+    raw nx[kAhead], ny[kAhead];  // x and dy of the next steps
+    auto fetch = [&](int64_t t) {
+      if (t + kAhead <= a.steps && t + kAhead <= end) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          nx[i] = Four<T>::load(a.x, b * a.x_batch + (t + i) * a.x_step + c, n);
+          ny[i] = Four<T>::load(dy, b * dy_batch + (t + i) * dy_step + c, n);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          nx[i] = load_input<T>(a, b, t + i, c, n);
+          ny[i] = t + i < a.steps && t + i < end ? Four<T>::load(dy, b * dy_batch + (t + i) * dy_step + c, n) : raw(0);
+        }
+      }
+    };
+    float x[kTaps][V], d[kTaps][V];  // of the last kTaps steps; d is dp
+    fetch(t0);
 #pragma unroll
     for (int k = 0; k < kTaps - 1; ++k) {
-      load_input<T, V>(a, b, t0 - (kTaps - 1) + k, c, n, x[k]);
+      const raw in = load_input<T>(a, b, t0 - (kTaps - 1) + k, c, n);
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[k][j] = 0.0f;  // earlier runs' shares of dx of steps that are theirs
+      for (int j = 0; j < V; ++j) x[k + 1][j] = Four<T>::value(in, j), d[k + 1][j] = 0.0f;
     }
-    const int64_t end = t0 + run + kTaps - 1;
     for (int64_t t = t0; t < end && t < a.steps + kTaps - 1; t += kAhead) {
-      float dys[kAhead][V];
+      raw rx[kAhead], ry[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) rx[i] = nx[i], ry[i] = ny[i];
+      if (t + kAhead < end && t + kAhead < a.steps + kTaps - 1) fetch(t + kAhead);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        load_input<T, V>(a, b, t + i, c, n, x[kTaps - 1 + i]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) dys[i][j] = 0.0f;
-        if (t + i < a.steps && t + i < end) Lanes<T, V>::load(dy, b * dy_batch + (t + i) * dy_step + c, n, dys[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const bool mine = t + i < t0 + run;
+        const bool mine = t + i < t0 + kBackRun;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+#pragma unroll
+          for (int k = 0; k < kTaps - 1; ++k) x[k][j] = x[k + 1][j], d[k][j] = d[k + 1][j];
+          x[kTaps - 1][j] = Four<T>::value(rx[i], j);
           float p = bias[j];
 #pragma unroll
-          for (int k = 0; k < kTaps; ++k) p = __fmaf_rn(w[k][j], x[i + k][j], p);
-          const float e = dys[i][j] * silu(p).slope;
-          d[kTaps - 1 + i][j] = e;
+          for (int k = 0; k < kTaps; ++k) p = __fmaf_rn(w[k][j], x[k][j], p);
+          const float e = Four<T>::value(ry[i], j) * silu(p).slope;
+          d[kTaps - 1][j] = e;
           if (mine) {
 #pragma unroll
-            for (int k = 0; k < kTaps; ++k) dw[k][j] = __fmaf_rn(e, x[i + k][j], dw[k][j]);
+            for (int k = 0; k < kTaps; ++k) dw[k][j] = __fmaf_rn(e, x[k][j], dw[k][j]);
             dw[kTaps][j] += e;
           }
         }
         // the step whose last share this was
         const int64_t at = t + i - (kTaps - 1);
-        if (at >= a.steps || at >= t0 + run || (at < t0 && t0 > 0)) continue;
+        if (at >= a.steps || at >= t0 + kBackRun || (at < t0 && t0 > 0)) continue;
         float out[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           out[j] = 0.0f;
 #pragma unroll
-          for (int k = 0; k < kTaps; ++k) out[j] = __fmaf_rn(w[k][j], d[kTaps - 1 + i - k][j], out[j]);
+          for (int k = 0; k < kTaps; ++k) out[j] = __fmaf_rn(w[k][j], d[kTaps - 1 - k][j], out[j]);
         }
         if (dafter && at + kTaps - 1 >= a.steps) {
-          float more[V];
-          Lanes<T, V>::load(dafter, (b * (kTaps - 1) + at + kTaps - 1 - a.steps) * a.dim + c, n, more);
+          const raw more = Four<T>::load(dafter, (b * (kTaps - 1) + at + kTaps - 1 - a.steps) * a.dim + c, n);
 #pragma unroll
-          for (int j = 0; j < V; ++j) out[j] += j < n ? more[j] : 0.0f;
+          for (int j = 0; j < V; ++j) out[j] += Four<T>::value(more, j);
         }
-        if (at >= 0) Lanes<T, V>::store(dx, (b * a.steps + at) * a.dim + c, n, out);
-        else if (dbefore) Lanes<T, V>::store(dbefore, (b * (kTaps - 1) + at + kTaps - 1) * a.dim + c, n, out);
+        if (at >= 0) Four<T>::store(dx, (b * a.steps + at) * a.dim + c, n, out);
+        else if (dbefore) Four<T>::store(dbefore, (b * (kTaps - 1) + at + kTaps - 1) * a.dim + c, n, out);
       }
-#pragma unroll
-      for (int k = 0; k < kTaps - 1; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[k][j] = x[kAhead + k][j], d[k][j] = d[kAhead + k][j];
     }
   }
   for (int i = 0; i < 4; ++i) {  // in the waves' order
@@ -220,7 +237,7 @@ __global__ __launch_bounds__(256) void conv_back_kernel(const morph_conv a, cons
   if (wave != 3 || n <= 0) return;
 #pragma unroll
   for (int k = 0; k <= kTaps; ++k)
-    Lanes<F32, V>::store(parts, ((int64_t)blockIdx.y * (kTaps + 1) + k) * a.dim + c, n, dw[k]);
+    Four<F32>::store(parts, ((int64_t)blockIdx.y * (kTaps + 1) + k) * a.dim + c, n, dw[k]);
 }
 
 template <typename W>
@@ -283,7 +300,7 @@ extern "C" int morph_conv_forward(const morph_conv* a, int dtype, void* y, void*
   return by_dtypes(dtype, a->weight_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    const ConvGrid g{over(a->dim, 64 * Wide<T>::kCount), a->steps > 0 ? over(a->steps, 4 * kRun) : 1};
+    const ConvGrid g{over(a->dim, 64 * V), a->steps > 0 ? over(a->steps, 4 * kRun) : 1};
     if (g.time_blocks > (INT64_MAX >> 16) / g.channel_blocks / a->batch ||
         !launchable(g.channel_blocks * g.time_blocks * a->batch, 256))
       return (int)MORPH_ERANGE;
@@ -319,7 +336,7 @@ extern "C" int morph_conv_backward(const morph_conv* a, int dtype, const void* d
     if (parts > 0) {
       const int rc = by_taps(a->taps, [&](auto k) {
         hipLaunchKernelGGL((conv_back_kernel<T, W, decltype(k)::value>), dim3((unsigned)blocks, parts), dim3(256), 0,
-                           as_stream(stream), *a, g, kBackRun, dy, dy_batch, dy_step, dafter, dx, dbefore,
+                           as_stream(stream), *a, g, dy, dy_batch, dy_step, dafter, dx, dbefore,
                            static_cast<float*>(workspace));
         return launch_status();
       });

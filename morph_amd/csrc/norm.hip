@@ -10,7 +10,11 @@
 namespace morph {
 namespace {
 
-constexpr int kBackGroups = 512;  // of a backward launch: rows of partial sums
+// Workgroups of a launch, each of which loads its next row before it sums the present one and its weights once.
+// 16384 rows of 4096 in BF16, forward: 46.5 us with six on a CU (1024: 47.6, 2048: 49.7, one a row 60), backward 80.5
+// with two (384: 85, 768: 83, 1024: 92; each leaves a row of partial sums).
+constexpr int kForwardGroups = 1536;
+constexpr int kBackGroups = 512;
 constexpr int64_t kMostRowBlocks = int64_t(1) << 20;
 
 // Sums of two values over the kThreads lanes that share a row (a wave, or the workgroup).
@@ -67,19 +71,40 @@ __global__ __launch_bounds__(kThreads == 64 ? 256 : kThreads) void norm_kernel(c
   RowSums<kThreads> sums{slots};
   const int t = kThreads == 64 ? threadIdx.x & 63 : threadIdx.x;
   const float inverse = 1.0f / (float)a.cols;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + (kThreads == 64 ? threadIdx.x >> 6 : 0); row < a.rows;
-       row += (int64_t)gridDim.x * kRows) {
+  // In a workgroup of 1024 lanes the weights are read again for each row: see norm_back_kernel.
+  constexpr bool kKeep = kThreads < 1024;
+  float w[kKeep ? kIters : 1][V], b[kKeep ? kIters : 1][V];
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) {
+      const int64_t c = (int64_t)(i * kThreads + t) * V;
+      if (c >= a.cols) continue;
+      load_weights<W, V>(a.weight, c, kWhole ? V : a.cols - c, 1.0f, w[i]);
+      load_weights<W, V>(a.bias, c, kWhole ? V : a.cols - c, 0.0f, b[i]);
+    }
+  }
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + (kThreads == 64 ? threadIdx.x >> 6 : 0);
+  u32x4 raw[kIters];
+  auto fetch = [&](int64_t at) {
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) {
+      const int64_t c = (int64_t)(i * kThreads + t) * V;
+      raw[i] = 0;
+      if (c < a.cols) raw[i] = Wide<T>::load(a.x, at * a.x_ld + c, kWhole ? V : a.cols - c);
+    }
+  };
+  if (row < a.rows) fetch(row);
+  for (; row < a.rows; row += step) {
     float x[kIters][V];
     float sum = 0.0f, none = 0.0f, squares = 0.0f;
 #pragma unroll
     for (int i = 0; i < kIters; ++i) {
-      const int64_t c = (int64_t)(i * kThreads + t) * V;
-      u32x4 raw = 0;
-      if (c < a.cols) raw = Wide<T>::load(a.x, row * a.x_ld + c, kWhole ? V : a.cols - c);
-      Wide<T>::unpack(raw, x[i]);
+      Wide<T>::unpack(raw[i], x[i]);
 #pragma unroll
       for (int k = 0; k < V; ++k) sum += x[i][k];
     }
+    if (row + step < a.rows) fetch(row + step);
     sums(sum, none);
     const float mean = sum * inverse;
 #pragma unroll
@@ -98,11 +123,15 @@ __global__ __launch_bounds__(kThreads == 64 ? 256 : kThreads) void norm_kernel(c
     for (int i = 0; i < kIters; ++i) {
       const int64_t c = (int64_t)(i * kThreads + t) * V;
       if (c >= a.cols) continue;
-      float w[V], b[V];
-      load_weights<W, V>(a.weight, c, kWhole ? V : a.cols - c, 1.0f, w);
-      load_weights<W, V>(a.bias, c, kWhole ? V : a.cols - c, 0.0f, b);
+      float wi[V], bi[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) x[i][k] = __fmaf_rn(x[i][k] * r, w[k], b[k]);
+      for (int k = 0; k < V; ++k) wi[k] = w[kKeep ? i : 0][k], bi[k] = b[kKeep ? i : 0][k];
+      if constexpr (!kKeep) {
+        load_weights<W, V>(a.weight, c, kWhole ? V : a.cols - c, 1.0f, wi);
+        load_weights<W, V>(a.bias, c, kWhole ? V : a.cols - c, 0.0f, bi);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[i][k] = __fmaf_rn(x[i][k] * r, wi[k], bi[k]);
       Wide<T>::store(y, row * a.cols + c, Wide<T>::pack(x[i]), kWhole ? V : a.cols - c);
     }
   }
@@ -357,7 +386,7 @@ extern "C" int morph_norm_forward(const morph_norm* a, int dtype, void* y, float
       } else {
         constexpr int kRows = kThreads == 64 ? 4 : 1;
         int64_t blocks = (a->rows + kRows - 1) / kRows;
-        if (blocks > kMostRowBlocks) blocks = kMostRowBlocks;
+        if (blocks > kForwardGroups) blocks = kForwardGroups;
         hipLaunchKernelGGL((norm_kernel<T, W, kThreads, kIters, kWhole>), dim3((unsigned)blocks),
                            dim3(kThreads == 64 ? 256 : kThreads), 0, s, *a, y, stats);
       }
