@@ -292,8 +292,11 @@ int morph_nonfinite_table(const void* d_table, const morph_adamw_tensor* tensors
  * (bias 31) over 3 mantissa bits, times the scale, e the least of 11 .. 254 with every value at most
  * 1.75 scales: from 2^-33 to 1.75 scales, whose root has the first moment's range.
  *
- * A step decodes both, updates them in FP32 as morph_adamw_multi_dev does, updates the master from those FP32
- * values, and rounds them to codes: a value between two codes goes up with the probability of its
+ * A step decodes both and updates them in FP32, each operation rounded to nearest (no fused ones):
+ *   m = m + lerp_weight * (g - m)   (MORPH_HP_LERP_LARGE: m = g + (lerp_weight - 1) * (g - m))
+ *   v = v * beta2 + (one_minus_beta2 * g) * g
+ * with g as for morph_adamw_hp, updates the master from those FP32 values (to within 2^-20 of its change and
+ * a unit of its last place of morph_adamw_hp's p) and rounds them to codes: a value between two codes goes up with the probability of its
  * place between them (16 bits of it), so that changes of less than a code's step, a thousandth a step with
  * beta2 = 0.999, are not lost but happen as often as they add up to one.  A second moment that is not
  * 0 keeps the least code at least, so that no first moment is divided by eps alone.  The 16 bits

@@ -321,6 +321,20 @@ def layer_calls():
     return _layer_calls
 
 
+_stage_calls = None
+
+
+def stage_calls():
+    """The native path of the state space operators and of the moments' values (hoststage.cpp)."""
+    global _stage_calls
+    if _stage_calls is None:
+        _stage_calls = hostpath().StageCalls([entry_address(name) for name in (
+            "morph_norm_forward", "morph_norm_workspace_bytes", "morph_norm_backward", "morph_conv_forward",
+            "morph_conv_workspace_bytes", "morph_conv_backward", "morph_ssm_forward",
+            "morph_ssm_workspace_bytes", "morph_ssm_backward", "morph_moment_decode")])
+    return _stage_calls
+
+
 def entry_address(name):
     """The address of one of the library's entry points."""
     return ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value

@@ -23,7 +23,7 @@ SOURCES = ["abi.hip", "adamw.hip", "nonfinite.hip", "step.hip", "grads.hip", "co
            "ffn_tiles_rows.hip", "ffn_tiles_weights.hip", "scan.hip", "norm.hip", "conv.hip", "ssm.hip"]
 OUTPUT = PKG / "lib" / "libmorph_optim.so"
 HOSTPATH = PKG / "lib" / "_hostpath.so"  # Python extension over torch's C++ tensors
-HOST_SOURCES = ["hostpath.cpp", "hostlayers.cpp"]
+HOST_SOURCES = ["hostpath.cpp", "hostlayers.cpp", "hoststage.cpp"]
 ARCH = os.environ.get("MORPH_OFFLOAD_ARCH", "gfx950")
 
 FLAGS = [

@@ -236,7 +236,8 @@ static_assert(kPerBlock == 4 * kBlock && kPerBlock % kGroup == 0, "a lane has on
 // and 233; with one chunk 284, with eight 256), of which HBM's are 181.
 constexpr int kChunks8 = MORPH_ADAMW8_CHUNKS;
 
-// adamw_update for a step's constants, with the hardware's square root and reciprocal (each within 1 unit of 2^-23, so the master's change is
+// The update for a step's constants.  The moments' operations are rounded one by one, so that any implementation of the
+// definition comes to the same codes; the master takes the hardware's square root and reciprocal (each within 1 unit of 2^-23, so the master's change is
 // within 2^-20 of itself): the correctly rounded ones are 45 of 64 instructions an element, and the
 // kernel is bound by instructions with them (75 million parameters: 333 us).
 // Constants that a call does without are ones here, which change no bit.
@@ -252,8 +253,8 @@ struct Update8 {
         lerp_large(hp.flags & MORPH_HP_LERP_LARGE) {}
   __device__ __forceinline__ void operator()(float g, float& p, float& m, float& v) const {
     g = (divide ? g / scale : g * inv_scale) * clip;
-    m = __fmaf_rn(lerp, g - m, lerp_large ? g : m);
-    v = __fmaf_rn(one_minus_beta2 * g, g, v * beta2);
+    m = (lerp_large ? g : m) + lerp * (g - m);
+    v = v * beta2 + (one_minus_beta2 * g) * g;
     const float d = __fmaf_rn(__builtin_amdgcn_sqrtf(v), inverse_bias2, eps);
     p = __fmaf_rn(neg_step_size * m, __builtin_amdgcn_rcpf(d), p * decay);
   }
@@ -888,7 +889,7 @@ extern "C" int morph_adamw8_multi_dev(const morph_adamw_tensor* tensors, int cou
 // ---- what the moments' codes stand for -------------------------------------------
 namespace {
 
-constexpr int kValueTensors = 64;
+constexpr int kValueTensors = 88;
 constexpr int kValuesPerBlock = 2048;  // 256 lanes, two words of each moment's codes
 
 struct ValueArgs {

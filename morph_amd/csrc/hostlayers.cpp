@@ -8,13 +8,7 @@
 // current device, another type, a layout that needs a copy, shapes that do not fit); the
 // caller then takes the Python path, which prepares it or raises.  A status of the library
 // comes back as an int.
-#include "hostpath.h"
-
-#include <ATen/ATen.h>
-#include <c10/hip/HIPFunctions.h>
-#include <c10/hip/HIPStream.h>
-
-#include "../../include/morph_layers.h"
+#include "hostcalls.h"
 
 namespace {
 
@@ -29,42 +23,8 @@ struct Calls {  // of the library, by address
   decltype(&morph_scan_backward) scan_backward;
 };
 
-int code(at::ScalarType t) {
-  return t == at::kFloat      ? MORPH_DTYPE_F32
-         : t == at::kHalf     ? MORPH_DTYPE_F16
-         : t == at::kBFloat16 ? MORPH_DTYPE_BF16
-                              : MORPH_DTYPE_NONE;
-}
 bool half(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 int64_t groups_of(int64_t n) { return (n + MORPH_ACT_GROUP - 1) / MORPH_ACT_GROUP; }
-
-// The current device and its stream, and outputs there; asked for a call whose first tensor
-// is on a GPU.
-struct Here {
-  c10::Device device{c10::DeviceType::CPU};
-  explicit Here(py::handle first) {
-    const at::Tensor* t = plain_tensor(first.ptr());
-    if (t != nullptr && t->is_cuda()) device = c10::Device(c10::DeviceType::CUDA, c10::hip::current_device());
-  }
-  void* stream() const { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
-  at::Tensor empty(at::IntArrayRef shape, at::ScalarType type) const {
-    return at::empty(shape, at::TensorOptions().device(device).dtype(type));
-  }
-  // o as a plain tensor on this device, or null.
-  const at::Tensor* tensor(py::handle o) const {
-    const at::Tensor* t = plain_tensor(o.ptr());
-    return t != nullptr && t->is_cuda() && t->layout() == at::kStrided && t->device() == device ? t : nullptr;
-  }
-};
-
-// A 2-D tensor of this shape with contiguous rows: its row stride, or 0.
-int64_t rows_of(const at::Tensor& t, at::ScalarType type, int64_t rows, int64_t cols) {
-  if (t.dim() != 2 || t.scalar_type() != type || t.size(0) != rows || t.size(1) != cols) return 0;
-  if (t.is_contiguous()) return cols;
-  return t.stride(1) == 1 && t.stride(0) >= cols ? t.stride(0) : 0;
-}
-
-py::object wrap(at::Tensor t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(t))); }
 
 class LayerCalls {
  public:
@@ -284,13 +244,6 @@ class LayerCalls {
   Calls c_;
 
   static uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
-
-  // The GIL is released around the library: a launch waits when the queue is full.
-  template <typename F>
-  static int released(F&& f) {
-    const py::gil_scoped_release nogil;
-    return f();
-  }
 
   // The weights of a block for x (or dy) of [.., d], into `block`.
   static bool weights(const at::Tensor& x, const at::Tensor* gate, const at::Tensor* up, const at::Tensor* down,

@@ -262,6 +262,7 @@ py::bytes places(const py::list& tensors) {
 
 PYBIND11_MODULE(_hostpath, m) {
   bind_layers(m);
+  bind_stage(m);
   m.def("places", &places);
   py::class_<StepPlan>(m, "StepPlan")
       .def(py::init<py::list, std::vector<int64_t>, uint64_t, int, int, uint64_t, uint64_t, uint64_t,

@@ -25,3 +25,4 @@ inline bool holds(const at::Tensor& t, at::ScalarType type, int64_t n) {
 }
 
 void bind_layers(py::module_& m);  // hostlayers.cpp
+void bind_stage(py::module_& m);   // hoststage.cpp

@@ -33,7 +33,9 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kMostGroups = 2;     // channel groups of a backward workgroup
 constexpr int kSequences = 4;      // of a lane in a single step: 13.0 us for 64 x 5120 x 16, 13.8 with one, 17.0 with eight
 constexpr int kBusy = 512;         // workgroups that keep the chip busy, so that sequences stay whole
-constexpr int kFull = 768;         // workgroups that it holds at a time
+constexpr int kFull = 1024;        // workgroups that it holds at a time
+constexpr int kBackFull = 768;     // and of the backward
+constexpr int kJoined = 16;        // segments up to which those that need a segment's first state join it themselves
 
 typedef float Four[4];
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -290,6 +292,33 @@ struct Inputs {
   }
 };
 
+// The states of a channel in a tensor [.., dim, states], `row` its sequence.
+__device__ __forceinline__ int64_t states_at(const Scan& a, int64_t row, int ch) { return (row * a.dim + ch) * a.states; }
+
+// What enters a segment, four states of a channel: behind few segments joined here, from `start` on through one after the
+// other, what more than kJoined leave is there (ssm_join_kernel).  kBack: from the last segment on.
+template <bool kBack>
+__device__ __forceinline__ void entering_states(const Scan& a, int segment, int b, int ch, int first, const Four& A2,
+                                                const float* start, const float* ends, const float* sums, Four& s) {
+  const int last = kBack ? a.segments - 1 : 0;
+  if (segment != last && a.segments > kJoined) {
+    load_states(ends + states_at(a, (int64_t)segment * a.batch + b, ch), first, a.states, s);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j] = 0.0f;
+  if (start) load_states(start + states_at(a, b, ch), first, a.states, s);
+  for (int k = last; k != segment;) {
+    k += kBack ? -1 : 1;
+    const int64_t row = (int64_t)k * a.batch + b;
+    Four S;
+    load_states(ends + states_at(a, row, ch), first, a.states, S);
+    const float d = sums[row * a.dim + ch];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = __fmaf_rn(__builtin_amdgcn_exp2f(d * A2[j]), s[j], S[j]);
+  }
+}
+
 // Steps of a wave from a zero state: gates a (or their products up to each step), and the states.
 template <int L, bool kProducts>
 __device__ __forceinline__ void walk(const float (&d)[Lane<L>::kR], const float (&u)[Lane<L>::kR], const Four& A2,
@@ -326,13 +355,13 @@ __device__ __forceinline__ Channel load_channel(const Scan& a, const Lane<L>& p)
   for (int j = 0; j < 4; ++j) c.A2[j] *= kLog2e;
   return c;
 }
-// The states of a channel in a tensor [.., dim, states], `row` its sequence.
-__device__ __forceinline__ int64_t states_at(const Scan& a, int64_t row, int ch) { return (row * a.dim + ch) * a.states; }
 
 template <typename T, int L, bool kGated>
 __global__ __launch_bounds__(64 * kW, L < 4 ? 3 : 4) void ssm_kernel(const Scan a, const float* __restrict__ first,
-                                                         const float* __restrict__ entering, char* __restrict__ y,
-                                                         float* __restrict__ last, float* __restrict__ kept) {
+                                                                        const float* __restrict__ from,
+                                                                        const float* __restrict__ sums,
+                                                                        char* __restrict__ y, float* __restrict__ last,
+                                                                        float* __restrict__ kept) {
   constexpr int kR = Lane<L>::kR;
   __shared__ float bc[kW][2][kT * 4 * L];
   __shared__ f32x4 ends[2][kW][2][64];
@@ -341,9 +370,8 @@ __global__ __launch_bounds__(64 * kW, L < 4 ? 3 : 4) void ssm_kernel(const Scan 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const Lane<L> p(group, a.dim);
   const Channel c = load_channel(a, p);
-  Four carry = {};
-  if (segment > 0) load_states(entering + states_at(a, (int64_t)segment * a.batch + b, p.ch), p.first, a.states, carry);
-  else if (first) load_states(first + states_at(a, b, p.ch), p.first, a.states, carry);
+  Four carry;
+  entering_states<false>(a, segment, b, p.ch, p.first, c.A2, first, from, sums, carry);
   const int begin = segment * a.per, end = begin + a.per < a.tiles ? begin + a.per : a.tiles;
 
   Rows<T, L> rx, rd, rz;
@@ -598,10 +626,8 @@ __global__ __launch_bounds__(64 * kW, L < 16 ? 3 : 2) void ssm_back_kernel(const
     sum_A[i][wave][lane] = f32x4{0, 0, 0, 0};
     sum_own[i][wave][0][lane] = sum_own[i][wave][1][lane] = 0.0f;
     if (wave == 0) {
-      Four r = {};
-      if (segment < a.segments - 1)
-        load_states(parts.late + states_at(a, (int64_t)segment * a.batch + b, p.ch), p.first, a.states, r);
-      else if (dlast) load_states(dlast + states_at(a, b, p.ch), p.first, a.states, r);
+      Four r;
+      entering_states<true>(a, segment, b, p.ch, p.first, load_channel(a, p).A2, dlast, parts.late, parts.sums, r);
       late[0][i][lane] = as_vector(r);
     }
   }
@@ -796,35 +822,36 @@ __global__ __launch_bounds__(64 * kW, L < 16 ? 3 : 2) void ssm_back_kernel(const
   }
 }
 
-// dB and dC: the sums over `count` blocks of channel groups.
+// dB and dC, the sums over `count` blocks of channel groups, by the first workgroups; dA, dskip and ddt_bias, the sums
+// over the sequences and their segments, by the others, from workgroup `ends` on.
 template <typename T>
-__global__ __launch_bounds__(256) void ssm_sum_kernel(const float* __restrict__ parts, int64_t count, int64_t rows,
-                                                      int wide, int states, void* __restrict__ dB, void* __restrict__ dC) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, size = rows * 2 * wide;
-  if (i >= size) return;
-  const int n = (int)(i % wide);
-  if (n >= states) return;
-  float sum = 0.0f;
+__global__ __launch_bounds__(256) void ssm_sum_kernel(const SsmParts parts, int64_t count, int64_t rows, int wide,
+                                                      int64_t sequences, int64_t dim, int states, int ends,
+                                                      const morph_ssm_grads g) {
+  if ((int)blockIdx.x < ends) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, size = rows * 2 * wide;
+    if (i >= size) return;
+    const int n = (int)(i % wide);
+    if (n >= states) return;
+    float sum = 0.0f;
 #pragma unroll 8
-  for (int64_t k = 0; k < count; ++k) sum += parts[k * size + i];
-  store_one<T>(i / wide % 2 ? dC : dB, i / (2 * wide) * states + n, sum);
-}
-
-// dA, dskip and ddt_bias: the sums over the sequences and their segments.
-__global__ __launch_bounds__(256) void ssm_batch_kernel(const SsmParts parts, int64_t batch, int64_t dim, int states,
-                                                        float* __restrict__ dA, float* __restrict__ dskip,
-                                                        float* __restrict__ ddt_bias) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = dim * states;
+    for (int64_t k = 0; k < count; ++k) sum += parts.bc[k * size + i];
+    store_one<T>(i / wide % 2 ? g.dC : g.dB, i / (2 * wide) * states + n, sum);
+    return;
+  }
+  const int64_t i = (int64_t)((int)blockIdx.x - ends) * 256 + threadIdx.x, n = dim * states;
   if (i < n) {
     float sum = 0.0f;
-    for (int64_t b = 0; b < batch; ++b) sum += parts.A[b * n + i];
-    dA[i] = sum;
+#pragma unroll 4
+    for (int64_t b = 0; b < sequences; ++b) sum += parts.A[b * n + i];
+    g.dA[i] = sum;
   }
   if (i < dim) {
     float s = 0.0f, t = 0.0f;
-    for (int64_t b = 0; b < batch; ++b) s += parts.skip[b * dim + i], t += parts.dt_bias[b * dim + i];
-    if (dskip) dskip[i] = s;
-    if (ddt_bias) ddt_bias[i] = t;
+#pragma unroll 4
+    for (int64_t b = 0; b < sequences; ++b) s += parts.skip[b * dim + i], t += parts.dt_bias[b * dim + i];
+    if (g.dskip) g.dskip[i] = s;
+    if (g.ddt_bias) g.ddt_bias[i] = t;
   }
 }
 
@@ -863,16 +890,16 @@ int64_t tiles_of(int64_t steps) { return over(steps, kT * kW); }
 // are kBusy workgroups without it.
 int64_t tiles_per_segment(int64_t batch, int64_t steps, int64_t groups) {
   const int64_t tiles = tiles_of(steps), blocks = groups * batch;
-  if (tiles < 4 || blocks >= kBusy) return tiles > 0 ? tiles : 1;
-  int64_t segments = over(kFull, blocks > 0 ? blocks : 1);
-  if (segments > tiles / 2) segments = tiles / 2;
+  if (tiles < 2 || blocks >= kBusy) return tiles > 0 ? tiles : 1;
+  int64_t segments = kFull / (blocks > 0 ? blocks : 1);
+  if (segments > tiles) segments = tiles;
   return over(tiles, segments);
 }
 
 // Workgroups of a backward per sequence and segment: as many as the chip holds at a time, and a channel group for
 // each of them at least and kMostGroups at most.  (Each workgroup's sums over its channels cross HBM twice.)
 int64_t back_blocks(int64_t batch, int64_t segments, int64_t groups) {
-  int64_t n = kFull / (batch * segments > 0 ? batch * segments : 1);
+  int64_t n = kBackFull / (batch * segments > 0 ? batch * segments : 1);
   if (n * kMostGroups < groups) n = over(groups, kMostGroups);
   return n < 1 ? 1 : n > groups ? groups : n;
 }
@@ -930,7 +957,8 @@ int join_segments(const Scan& a, const float* first, float* ends, float* sums, h
   if (a.segments < 2) return MORPH_OK;
   const int64_t blocks = (int64_t)a.groups * a.batch * (a.segments - 1);
   hipLaunchKernelGGL((ssm_ends_kernel<T, L, kBack, kGated && kBack>), dim3((unsigned)blocks), dim3(64 * kW), 0, s, a, ends, sums);
-  if (const int rc = launch_status()) return rc;
+  const int rc = launch_status();
+  if (rc != MORPH_OK || a.segments <= kJoined) return rc;
   hipLaunchKernelGGL(ssm_join_kernel<kBack>, dim3((unsigned)over((int64_t)a.batch * a.dim * a.states, 256)), dim3(256), 0, s, a,
                      first, ends, sums);
   return launch_status();
@@ -971,7 +999,7 @@ extern "C" int morph_ssm_forward(const morph_ssm* a, int dtype, void* y, float* 
     float* ends = static_cast<float*>(workspace);
     if (const int rc = join_segments<T, L, false, kGated>(scan, a->first, ends, ends + plan.states, s)) return rc;
     hipLaunchKernelGGL((ssm_kernel<T, L, kGated>), dim3((unsigned)(plan.groups * plan.segments * a->batch)), dim3(64 * kW), 0,
-                       s, scan, a->first, ends, static_cast<char*>(y), last, kept);
+                       s, scan, a->first, ends, ends + plan.states, static_cast<char*>(y), last, kept);
     return launch_status();
   });
 }
@@ -991,7 +1019,7 @@ extern "C" int morph_ssm_backward(const morph_ssm* a, int dtype, const float* ke
   if (need > 0 && (!workspace || workspace_bytes < need)) return MORPH_EWORKSPACE;
   const int64_t rows = a->batch * a->steps, sums = over(rows * 8 * lanes_of(a->states), 256);
   const int64_t ends = over(a->dim * a->states, 256);
-  if (!launchable(sums, 256) || !launchable(ends, 256) || !launchable(over(a->batch * a->dim * a->states, 256), 256) ||
+  if (!launchable(sums, 256) || !launchable(sums + ends, 256) || !launchable(over(a->batch * a->dim * a->states, 256), 256) ||
       !launchable(plan.groups * plan.segments * a->batch, 64 * kW))
     return MORPH_ERANGE;
   SsmParts parts;
@@ -1012,14 +1040,14 @@ extern "C" int morph_ssm_backward(const morph_ssm* a, int dtype, const float* ke
     if (const int status = join_segments<T, L, true, kGated>(scan, dlast, parts.late, parts.sums, s)) return status;
     hipLaunchKernelGGL((ssm_back_kernel<T, L, kGated>), dim3((unsigned)(plan.blocks * plan.segments * a->batch)),
                        dim3(64 * kW), 0, s, scan, (int)plan.blocks, kept, dlast, *g, parts);
-    if (const int status = launch_status()) return status;
-    if (rows == 0) return (int)MORPH_OK;
-    hipLaunchKernelGGL(ssm_sum_kernel<T>, dim3((unsigned)sums), dim3(256), 0, s, parts.bc, plan.blocks, rows, 4 * L,
-                       a->states, g->dB, g->dC);
     return launch_status();
   });
   if (rc != MORPH_OK) return rc;
-  hipLaunchKernelGGL(ssm_batch_kernel, dim3((unsigned)ends), dim3(256), 0, s, parts, plan.segments * a->batch, a->dim,
-                     a->states, g->dA, g->dskip, g->ddt_bias);
-  return launch_status();
+  const int wide = 4 * lanes_of(a->states);
+  auto sum = [&](auto t) {
+    hipLaunchKernelGGL(ssm_sum_kernel<decltype(t)>, dim3((unsigned)(sums + ends)), dim3(256), 0, s, parts, plan.blocks, rows,
+                       wide, plan.segments * a->batch, a->dim, a->states, (int)sums, *g);
+    return launch_status();
+  };
+  return dtype == MORPH_DTYPE_F32 ? sum(F32{}) : dtype == MORPH_DTYPE_F16 ? sum(F16{}) : sum(BF16{});
 }

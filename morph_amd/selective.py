@@ -23,8 +23,9 @@ import ctypes
 
 import torch
 
-from ._lib import (CONV_MAX_TAPS, SSM_MAX_STATES, SSM_MAX_STEP, SSM_SPAN, ConvArgs, SsmArgs, SsmGrads, check, lib)
-from .layers import address, current_stream, dtype_code, first_order, require_gpu, requires_grad, running_on
+from ._lib import (CONV_MAX_TAPS, SSM_MAX_STATES, SSM_MAX_STEP, SSM_SPAN, ConvArgs, SsmArgs, SsmGrads, check, lib,
+                   stage_calls)
+from .layers import address, current_stream, dtype_code, first_order, native, require_gpu, requires_grad, running_on
 from .norm import FLOATS, whole
 
 
@@ -73,8 +74,16 @@ def _conv_args(x, weight, bias, state):
                     weight.shape[1], dtype_code(weight.dtype))
 
 
-def causal_conv_forward(x, weight, bias=None, state=None, stream=None):
-    """(u, inputs, saved): causal_conv, with what the backward needs."""
+def _bare(*tensors):
+    return (t.detach() if t is not None else None for t in tensors)
+
+
+def _conv(x, weight, bias, state, train, stream):
+    if stream is None:
+        made = stage_calls().conv_forward(x, weight, bias, state)
+        if made is not None:
+            u, last = native(made)
+            return u, last, SavedConv(*_bare(x, weight, bias, state)) if train else None
     _check_conv(x, weight, bias, state)
     with running_on(x.device, stream, (x, weight, bias, state)):
         x, weight, bias, state = _channels_last(x), whole(weight), whole(bias), whole(state)
@@ -87,7 +96,12 @@ def causal_conv_forward(x, weight, bias=None, state=None, stream=None):
 
 def causal_conv(x, weight, bias=None, state=None, stream=None):
     """(u, the last taps - 1 inputs); state: those before the first step (None: zeros)."""
-    return causal_conv_forward(x, weight, bias, state, stream)[:2]
+    return _conv(x, weight, bias, state, False, stream)[:2]
+
+
+def causal_conv_forward(x, weight, bias=None, state=None, stream=None):
+    """(u, inputs, saved): causal_conv, with what the backward needs."""
+    return _conv(x, weight, bias, state, True, stream)
 
 
 def causal_conv_backward(du, saved, dlast=None, stream=None):
@@ -96,6 +110,10 @@ def causal_conv_backward(du, saved, dlast=None, stream=None):
     if not isinstance(saved, SavedConv):
         raise TypeError("saved must come from causal_conv_forward")
     x, weight, bias, state = saved.x, saved.weight, saved.bias, saved.state
+    if stream is None:
+        made = stage_calls().conv_backward(du, x, weight, bias, state, dlast)
+        if made is not None:
+            return native(made)
     require_gpu(du, "du", (x.dtype,), x.shape, x.device)
     batch, steps, dim, taps = *x.shape, weight.shape[1]
     if dlast is not None:
@@ -185,6 +203,13 @@ def _rows_of(t):
 
 
 def _scan(inputs, train, stream):
+    if stream is None:
+        made = stage_calls().ssm_forward(inputs, train)
+        if made is not None:
+            if not train:
+                return native(made)
+            y, last, states = native(made)
+            return y, last, SavedSelective(*_bare(*inputs), states)
     x, dt, A, B, C, skip, z, dt_bias, state = inputs
     _check_scan(*inputs)
     with running_on(x.device, stream, inputs):
@@ -217,7 +242,11 @@ def selective_scan_backward(dy, saved, dlast=None, stream=None):
     zeros)."""
     if not isinstance(saved, SavedSelective):
         raise TypeError("saved must come from selective_scan_forward")
-    inputs = [getattr(saved, name) for name in SavedSelective.__slots__[:-1]]
+    inputs = tuple(getattr(saved, name) for name in SavedSelective.__slots__[:-1])
+    if stream is None:
+        made = stage_calls().ssm_backward(dy, inputs, saved.states, dlast)
+        if made is not None:
+            return native(made)
     x, dt, A, B, C, skip, z, dt_bias, state = inputs
     require_gpu(dy, "dy", (x.dtype,), x.shape, x.device)
     batch, steps, dim = x.shape

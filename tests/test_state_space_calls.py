@@ -11,7 +11,7 @@ import torch
 
 from morph_amd import _lib, norm, selective
 from test_abi import no_gpu_visible
-from test_layer_calls import _Copies, _Library
+from test_layer_calls import _Copies, _Library, _NoNativePath
 
 ROOT = Path(__file__).resolve().parents[1]
 P = 0x10000  # never allocated: only where no GPU is visible, and nothing is launched
@@ -187,8 +187,7 @@ def wrappers(monkeypatch):
         monkeypatch.setattr(module, "require_gpu", require)
         monkeypatch.setattr(module, "lib", _Library)
         monkeypatch.setattr(module, "current_stream", lambda: None)
-        if hasattr(module, "layer_calls"):
-            monkeypatch.setattr(module, "layer_calls", lambda: type("No", (), {"__getattr__": lambda s, n: lambda *a: None})())
+        monkeypatch.setattr(module, "stage_calls", _NoNativePath)
     return place
 
 
