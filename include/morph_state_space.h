@@ -79,7 +79,8 @@ int morph_conv_backward(const morph_conv* conv, int dtype, const void* dy, int64
  *   y_t = (sum over n of C_t h_t + skip x_t) silu(z_t)
  * for x, dt, z [batch, steps, dim], B and C [batch, steps, states], A [dim, states], states h [batch, dim,
  * states] in FP32.  Without z, skip, dt_bias, first state: 1, 0, 0, 0.  dt = -inf passes a state on unchanged
- * (padding).
+ * (padding, with x, B and C finite).  A positive A is taken while exp(A times the sum of d over the steps) stays
+ * finite: products of gates over many steps are formed.
  *
  * Backward, with ds = dy silu(z): r_t = ds_t C_t + exp(d_(t+1) A) r_(t+1), with dlast added to the last;
  *   dx = d sum_n(r B) + skip ds, dB = sum over channels of r d x, dC = sum over channels of h ds,
@@ -92,7 +93,7 @@ int morph_conv_backward(const morph_conv* conv, int dtype, const void* dy, int64
  */
 #define MORPH_SSM_SPAN 32
 #define MORPH_SSM_MAX_STATES 64
-#define MORPH_SSM_MAX_STEP (1 << 25) /* of dim and of the step strides, in elements */
+#define MORPH_SSM_MAX_STEP (1 << 25) /* of dim, and of the step strides in elements */
 
 typedef struct morph_ssm {
   const void* x;

@@ -140,7 +140,8 @@ __global__ __launch_bounds__(256) void conv_kernel(const morph_conv a, const Con
 
 // parts: [gridDim.y][taps + 1][dim].
 template <typename T, typename W, int kTaps>
-__global__ __launch_bounds__(256) void conv_back_kernel(const morph_conv a, const ConvGrid g, const void* __restrict__ dy, int64_t dy_batch, int64_t dy_step,
+__global__ __launch_bounds__(256) void conv_back_kernel(const morph_conv a, const ConvGrid g, const void* __restrict__ dy,
+                                                        int64_t dy_batch, int64_t dy_step,
                                                         const void* __restrict__ dafter, void* __restrict__ dx,
                                                         void* __restrict__ dbefore, float* __restrict__ parts) {
   typedef typename Four<T>::raw raw;
@@ -278,6 +279,8 @@ int check(const morph_conv* a, int dtype) {
   if (a->taps < 2 || a->taps > MORPH_CONV_MAX_TAPS) return MORPH_ERANGE;
   if (!known_dtype(dtype) || (a->weight_dtype != MORPH_DTYPE_F32 && a->weight_dtype != dtype)) return MORPH_EDTYPE;
   if (a->batch > 0 && a->dim > 0 && ((a->steps > 0 && !a->x) || !a->weight)) return MORPH_EINVAL;
+  const int64_t all = INT64_MAX >> 12;
+  if (a->batch > 0 && a->dim > 0 && (a->dim > all / a->batch || a->steps > all / a->batch / a->dim)) return MORPH_ERANGE;
   return MORPH_OK;
 }
 
@@ -301,9 +304,7 @@ extern "C" int morph_conv_forward(const morph_conv* a, int dtype, void* y, void*
     using T = decltype(t);
     using W = decltype(w);
     const ConvGrid g{over(a->dim, 64 * V), a->steps > 0 ? over(a->steps, 4 * kRun) : 1};
-    if (g.time_blocks > (INT64_MAX >> 16) / g.channel_blocks / a->batch ||
-        !launchable(g.channel_blocks * g.time_blocks * a->batch, 256))
-      return (int)MORPH_ERANGE;
+    if (!launchable(g.channel_blocks * g.time_blocks * a->batch, 256)) return (int)MORPH_ERANGE;
     return by_taps(a->taps, [&](auto k) {
       hipLaunchKernelGGL((conv_kernel<T, W, decltype(k)::value>),
                          dim3((unsigned)(g.channel_blocks * g.time_blocks * a->batch)), dim3(256), 0, as_stream(stream), *a,

@@ -8,8 +8,8 @@ single steps.
 x, dt, z [batch, steps, dim] and B, C [batch, steps, states] are FP32, FP16 or BF16; A [dim, states] (negative, so
 that states fade), skip and dt_bias [dim] and the states [batch, dim, states] are FP32, up to 64 states a
 channel.  weight [dim, taps] and bias [dim] have x's type or FP32, taps 2 to 4; the convolution's state is its
-last inputs, [batch, taps - 1, dim].  dt = -inf passes a state on unchanged (padding).  Kernels: csrc/conv.hip,
-csrc/ssm.hip.
+last inputs, [batch, taps - 1, dim].  dt = -inf passes a state on unchanged (padding, with x, B and C finite).  A
+positive A is taken while exp(A times the sum of d over the steps) stays finite.  Kernels: csrc/conv.hip, csrc/ssm.hip.
 
     u, inputs = causal_conv(x, weight, bias, inputs)                       # a prompt, then token by token
     y, state = selective_scan(u, dt, A, B, C, skip, z, dt_bias, state)
@@ -186,8 +186,13 @@ def _check_scan(x, dt, A, B, C, skip, z, dt_bias, state):
         require_gpu(state, "state", (torch.float32,), (batch, dim, A.shape[1]), x.device)
 
 
+def _step(t):
+    """From step to step; of one step it does not matter."""
+    return t.stride(1) if t.shape[1] > 1 else 0
+
+
 def _scan_args(x, dt, A, B, C, skip, z, dt_bias, state):
-    strides = [s for t in (x, dt, z, B, C) for s in ((t.stride(0), t.stride(1)) if t is not None else (0, 0))]
+    strides = [s for t in (x, dt, z, B, C) for s in ((t.stride(0), _step(t)) if t is not None else (0, 0))]
     return SsmArgs(*(address(t) for t in (x, dt, z, B, C, A, skip, dt_bias, state)), *x.shape, *strides, A.shape[1], 0)
 
 
@@ -199,7 +204,7 @@ def _workspace(x, A, backward):
 def _rows_of(t):
     """_channels_last, with steps as near to each other as the kernels count (a copy if they are not)."""
     t = _channels_last(t)
-    return t if t is None or t.stride(1) <= SSM_MAX_STEP else t.contiguous()
+    return t if t is None or _step(t) <= SSM_MAX_STEP else t.contiguous()
 
 
 def _scan(inputs, train, stream):
@@ -263,7 +268,7 @@ def selective_scan_backward(dy, saved, dlast=None, stream=None):
         grads = SsmGrads(*(address(t) for t in (dx, ddt, dz, dB, dC, dA, dskip, ddt_bias, dstate)))
         workspace, size = _workspace(x, A, 1)
         check(lib().morph_ssm_backward(ctypes.byref(_scan_args(*inputs)), dtype_code(x.dtype), address(saved.states),
-                                       address(dy), dy.stride(0), dy.stride(1), address(dlast), ctypes.byref(grads),
+                                       address(dy), dy.stride(0), _step(dy), address(dlast), ctypes.byref(grads),
                                        address(workspace), size, current_stream()))
         return dx, ddt, dA, dB, dC, dskip, dz, ddt_bias, dstate
 

@@ -465,3 +465,105 @@ def plain_scan(x, dt, A, B, C, skip, z, bias, first):
         s.append((h * C[:, t, None]).sum(2))
     s = torch.stack(s, 1) + skip * x
     return s * z * torch.sigmoid(z), h
+
+
+# ---- forms that sizes alone choose -----------------------------------------------------------
+@pytest.mark.parametrize("rows,cols", [(3300, 1100), (1700, 2100), (1600, 8200)])
+def test_norm_of_more_rows_than_workgroups(rows, cols):
+    gen = torch.Generator().manual_seed(20)
+    check_norm(*on_gpu(normal(gen, rows, cols, dtype=BF16), normal(gen, cols, mean=1), normal(gen, cols),
+                       normal(gen, rows, cols, dtype=BF16)), 1e-5)
+
+
+@pytest.mark.parametrize("batch,steps,dim,n", [
+    (1, 700, 16, 16), (2, 600, 7, 5),     # more segments than are joined where they are needed
+    (400, 140, 16, 16),                   # segments of several tiles
+    (520, 70, 10, 8),                     # sequences enough to stay whole
+    (800, 3, 32, 16), (300, 34, 40, 16),  # two channel groups a workgroup backward; two and one
+    (130, 40, 100, 64)])
+def test_scan_forms(batch, steps, dim, n):
+    gen = torch.Generator().manual_seed(21)
+    inputs = scan_inputs(gen, batch, steps, dim, n, F32)
+    check_scan(inputs, *on_gpu(normal(gen, batch, steps, dim), normal(gen, batch, dim, n)))
+
+
+@pytest.mark.parametrize("batch,steps", [(1, 1), (1, 3), (2, 1), (2, 3)])
+def test_scan_of_steps_that_lie_far_apart(batch, steps):
+    """Steps farther apart than the kernels count: copies of them, and of one step its stride does not matter."""
+    gen = torch.Generator().manual_seed(22)
+    inputs = scan_inputs(gen, batch, steps, 21, 16, BF16)
+    dy = normal(gen, batch, steps, 21, dtype=BF16).to(DEV)
+    y, last, saved = selective_scan_forward(*inputs)
+    far = torch.empty(batch, steps, (1 << 25) + 8, dtype=BF16, device=DEV)
+    views = [inputs[0], inputs[1], inputs[3], inputs[4], inputs[6], dy]
+    places, at = [], 0
+    for t in views:
+        far[..., at:at + t.shape[2]] = t
+        places.append(far[..., at:at + t.shape[2]])
+        at += t.shape[2]
+    x2, dt2, B2, C2, z2, dy2 = places
+    for stream in (None, torch.cuda.current_stream()):
+        y2, last2, saved2 = selective_scan_forward(x2, dt2, inputs[2], B2, C2, inputs[5], z2, *inputs[7:], stream=stream)
+        assert same((y, last), (y2, last2))
+        assert same(selective_scan_backward(dy, saved), selective_scan_backward(dy2, saved2, stream=stream))
+
+
+def test_scan_of_inputs_that_are_shared():
+    """One state, one B and C for all sequences, one step length for all steps: expanded views, and their gradients."""
+    gen = torch.Generator().manual_seed(23)
+    x, dt, A, B, C, skip, z, bias, first = scan_inputs(gen, 3, 50, 20, 16, F32)
+    shared = [x, dt[:, :1], A, B[:1], C[:1], skip, z, bias, first[:1]]
+    sizes = [None, (3, 50, 20), None, (3, 50, 16), (3, 50, 16), None, None, None, (3, 20, 16)]
+    end = normal(gen, 3, 50, 20)
+
+    def run(leaves, f, end):
+        wide = [t if size is None else t.expand(size) for t, size in zip(leaves, sizes)]
+        return torch.autograd.grad(f(*wide)[0], leaves, end)
+    refs = run([t.cpu().double().requires_grad_() for t in shared], plain_scan, end.double())
+    for k, (g, r) in enumerate(zip(run([t.clone().requires_grad_() for t in shared], selective_state_space, end.to(DEV)), refs)):
+        R.assert_scan(g, r, F32, f"gradient {k}")
+
+
+@pytest.mark.parametrize("kind", ["norm", "conv", "scan"])
+def test_autograd_in_a_graph(kind):
+    """Forward and backward of leaves of the capture's own, replayed between eager work."""
+    gen = torch.Generator().manual_seed(24)
+    f, tensors, _, _ = autograd_cases(gen)[kind]
+    ends = [normal(gen, *o.shape, dtype=o.dtype).to(DEV) for o in f(*tensors)]
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in tensors]
+        outs = f(*leaves)
+        return [o.detach() for o in outs] + list(torch.autograd.grad(outs, leaves, ends))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = run()
+    side.synchronize()
+    for k in range(3):
+        for t in tensors[:2]:
+            t.copy_(t.roll(1, 0))
+        expected = run()
+        torch.cuda.synchronize()
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, expected), k
+
+
+@pytest.mark.parametrize("kind", ["norm", "conv", "scan"])
+def test_two_streams_at_once(kind):
+    call, _ = operators(torch.Generator().manual_seed(25))[kind]
+    first = call()
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(call())
+    torch.cuda.synchronize()
+    assert all(same(r, first) for r in results)
