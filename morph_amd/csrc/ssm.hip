@@ -35,6 +35,9 @@ constexpr int kSequences = 4;      // of a lane in a single step: 13.0 us for 64
 constexpr int kBusy = 512;         // workgroups that keep the chip busy, so that sequences stay whole
 constexpr int kFull = 1024;        // workgroups that it holds at a time
 constexpr int kBackFull = 768;     // and of the backward
+// Tiles of a segment from which 16 waves take its steps in the launch that finds its ends, otherwise 4: 32768 steps of 2048 channels in
+// segments of 128 tiles 227 us (4 waves: 257), 3 x 777 of 1100 in segments of 3 tiles 14.3 (13.4).
+constexpr int kManyTiles = 16;
 constexpr int kJoined = 16;        // segments up to which those that need a segment's first state join it themselves
 
 typedef float Four[4];
@@ -447,35 +450,38 @@ __global__ __launch_bounds__(64 * kW, L < 4 ? 3 : 4) void ssm_kernel(const Scan 
 
 // What a segment does to a state that passes through it, for the segments to be walked side by side: the product of its
 // gates is exp(A times the sum of d), and `ends` its result from a zero state (kBack: of the gradients r, from its last
-// step to its first).  Each wave takes a quarter of its steps; no output, so neither skip nor dB and dC.
+// step to its first).  Each wave takes its part of the segment's steps; no output, so neither skip nor dB and dC.
 // segment s: ends[s + 1], sums[s + 1] (kBack: s - 1), where what enters the next one then is joined.
-template <typename T, int L, bool kBack, bool kGated>
-__global__ __launch_bounds__(64 * kW) void ssm_ends_kernel(const Scan a, float* __restrict__ ends, float* __restrict__ sums) {
+template <typename T, int L, bool kBack, bool kGated, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void ssm_ends_kernel(const Scan a, float* __restrict__ ends, float* __restrict__ sums) {
   constexpr int kR = Lane<L>::kR;
-  __shared__ float bc[kW][kT * 4 * L];
-  __shared__ f32x4 join[kW][2][64];
-  __shared__ float whole_sum[kW][64];
+  __shared__ float bc[kWaves][kT * 4 * L];
+  __shared__ f32x4 join[kWaves][2][64];
+  __shared__ float whole_sum[kWaves][64];
   const int group = (int)blockIdx.x % a.groups, rest = (int)blockIdx.x / a.groups;
   const int segment = rest % (a.segments - 1) + (kBack ? 1 : 0), b = rest / (a.segments - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const Lane<L> p(group, a.dim);
   const Channel c = load_channel(a, p);
-  const int stretch = a.per * kT, t_begin = segment * a.per * kW * kT + wave * stretch;
+  // runs of kT steps: all of the segment's, and from the wave's first on (kBack: its last, downwards) how many it takes
+  const int all = a.per * kW, each = (all + kWaves - 1) / kWaves, before = wave * each;
+  const int count = before >= all ? 0 : all - before < each ? all - before : each;
+  const int run0 = segment * all + (kBack ? before + count - 1 : before);
   Rows<T, L> rd, rx, rz;  // x: kBack: dy
   Inputs<T, L> in;
   float* mine = bc[wave];
   float sum = 0.0f;
   Four s = {};
   auto fetch = [&](int i) {
-    const int t0 = t_begin + (kBack ? a.per - 1 - i : i) * kT;
+    const int t0 = (run0 + (kBack ? -i : i)) * kT;
     rd.fetch(p, a.dt, b, t0, a.steps);
     rx.fetch(p, kBack ? a.dy : a.x, b, t0, a.steps);
     if constexpr (kGated) rz.fetch(p, a.z, b, t0, a.steps);
     in.fetch(kBack ? a.C : a.B, b, t0, a.steps, a.states);
   };
-  fetch(0);
-  for (int i = 0; i < a.per; ++i) {
-    const int t0 = t_begin + (kBack ? a.per - 1 - i : i) * kT, left = a.steps - t0;
+  if (count > 0) fetch(0);
+  for (int i = 0; i < count; ++i) {
+    const int t0 = (run0 + (kBack ? -i : i)) * kT, left = a.steps - t0;
     const bool whole = p.whole(a.dim, left);
     float d[kR], u[kR];
     in.put(mine, left, a.states);
@@ -492,7 +498,7 @@ __global__ __launch_bounds__(64 * kW) void ssm_ends_kernel(const Scan a, float* 
       if (!whole && !p.has(k, left)) d[k] = u[k] = 0.0f;
       sum += d[k];
     }
-    if (i + 1 < a.per) fetch(i + 1);
+    if (i + 1 < count) fetch(i + 1);
     each_step<kT>([&](auto step) {
       constexpr int t = kBack ? kT - 1 - decltype(step)::value : decltype(step)::value;
       const float dt = spread<L, t % L>(d[t / L]), ut = spread<L, t % L>(u[t / L]);
@@ -516,8 +522,8 @@ __global__ __launch_bounds__(64 * kW) void ssm_ends_kernel(const Scan a, float* 
   Four out = {};
   sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kW; ++i) {
-    const int w = kBack ? kW - 1 - i : i;
+  for (int i = 0; i < kWaves; ++i) {
+    const int w = kBack ? kWaves - 1 - i : i;
     const f32x4 A = join[w][0][lane], S = join[w][1][lane];
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = __fmaf_rn(A[j], out[j], S[j]);
@@ -956,7 +962,13 @@ template <typename T, int L, bool kBack, bool kGated>
 int join_segments(const Scan& a, const float* first, float* ends, float* sums, hipStream_t s) {
   if (a.segments < 2) return MORPH_OK;
   const int64_t blocks = (int64_t)a.groups * a.batch * (a.segments - 1);
-  hipLaunchKernelGGL((ssm_ends_kernel<T, L, kBack, kGated && kBack>), dim3((unsigned)blocks), dim3(64 * kW), 0, s, a, ends, sums);
+  auto find = [&](auto waves) {
+    constexpr int kWaves = decltype(waves)::value;
+    hipLaunchKernelGGL((ssm_ends_kernel<T, L, kBack, kGated && kBack, kWaves>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, s, a,
+                       ends, sums);
+  };
+  if (a.per >= kManyTiles) find(std::integral_constant<int, 16>{});
+  else find(std::integral_constant<int, 4>{});
   const int rc = launch_status();
   if (rc != MORPH_OK || a.segments <= kJoined) return rc;
   hipLaunchKernelGGL(ssm_join_kernel<kBack>, dim3((unsigned)over((int64_t)a.batch * a.dim * a.states, 256)), dim3(256), 0, s, a,

@@ -478,6 +478,7 @@ def test_norm_of_more_rows_than_workgroups(rows, cols):
 @pytest.mark.parametrize("batch,steps,dim,n", [
     (1, 700, 16, 16), (2, 600, 7, 5),     # more segments than are joined where they are needed
     (400, 140, 16, 16),                   # segments of several tiles
+    (300, 1600, 5, 4), (100, 6000, 3, 17),  # of many, and not a multiple of the waves
     (520, 70, 10, 8),                     # sequences enough to stay whole
     (800, 3, 32, 16), (300, 34, 40, 16),  # two channel groups a workgroup backward; two and one
     (130, 40, 100, 64)])
