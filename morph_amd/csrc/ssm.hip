@@ -1,9 +1,10 @@
 // Selective state space scan (morph_state_space.h) and its backward pass: h_t = exp(d_t A) h_(t-1) + d_t x_t B_t for
 // every state of every channel, y = C_t . h_t + skip x, along the steps.
 //
-// A step costs each state an exponential (a quarter-rate instruction, as long as four others) and four to seven more
-// instructions, so with 16 states a channel arithmetic bounds the scan, three times above what HBM does; the layout
-// is for that.  A lane has four states of a channel, kLanes neighbouring lanes the channel, a wave 64 / kLanes
+// A step costs each state an exponential (which issues for as long as two other instructions) and four to seven more
+// instructions, so with 16 states a channel arithmetic bounds the scan, more than twice above what HBM does; the layout
+// is for that.  4 x 1024 steps of 5120 channels of 16 states in BF16: forward 160 us, of which vector instructions' issue takes
+// 108, backward 383, of which it takes 302, and 20 for the sums.  A lane has four states of a channel, kLanes neighbouring lanes the channel, a wave 64 / kLanes
 // channels and kT consecutive steps.  What belongs to a channel and step alone (softplus, the gate, conversions) is
 // done once, by one of its lanes, and spread by DPP; what belongs to a state and step alone (B and C) lies
 // converted in LDS.
@@ -70,8 +71,7 @@ __device__ __forceinline__ float softplus(float x) {
 // The value of lane K of this lane's channel, L lanes a channel.
 template <int L, int K>
 __device__ __forceinline__ float spread(float x) {
-  if constexpr (L == 1) return x;
-  else if constexpr (L == 2) return dpp<K | K << 2 | (2 + K) << 4 | (2 + K) << 6>(x);
+  if constexpr (L == 2) return dpp<K | K << 2 | (2 + K) << 4 | (2 + K) << 6>(x);
   else if constexpr (L == 4) return dpp<K * 0x55>(x);
   else  // lane (l & ~(L - 1)) | K of 32
     return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, x), (0x1F & ~(L - 1)) | K << 5));
@@ -79,7 +79,7 @@ __device__ __forceinline__ float spread(float x) {
 // The sum over a channel's lanes, in each.
 template <int L>
 __device__ __forceinline__ float channel_sum(float x) {
-  if constexpr (L >= 2) x += dpp<0xB1>(x);    // quad_perm [1,0,3,2]
+  x += dpp<0xB1>(x);                          // quad_perm [1,0,3,2]
   if constexpr (L >= 4) x += dpp<0x4E>(x);    // quad_perm [2,3,0,1]
   if constexpr (L >= 8) x += dpp<0x141>(x);   // row_half_mirror
   if constexpr (L >= 16) x += dpp<0x140>(x);  // row_mirror
@@ -226,35 +226,53 @@ struct Lane {
   // Whether all lanes have all of their steps, of which `left` are there.
   __device__ __forceinline__ bool whole(int dim, int left) const { return left >= kT && dim - group0 >= kC && L <= kT; }
   __device__ __forceinline__ bool has(int i, int left) const { return active && own + i * L < left && own < kT; }
-  // The offset in bytes of the lane's first step in a tensor of this step stride.
-  template <typename T>
-  __device__ __forceinline__ uint32_t offset(int step) const {
-    return (uint32_t)(own < kT ? own : kT - 1) * (uint32_t)step + (uint32_t)inside * Fmt<T>::bytes;
-  }
-  // That of its i-th, the last of the `left` steps that are there in place of those behind it.
-  template <typename T>
-  __device__ __forceinline__ uint32_t offset_of(int i, int step, int left) const {
-    const int t = own + i * L;
-    return (uint32_t)(t < left ? t : left - 1) * (uint32_t)step + (uint32_t)inside * Fmt<T>::bytes;
-  }
 };
 
-// A channel and step tensor's values of a wave's steps, at the lane's offset.
+// A wave's kT steps from t0 on; in place of those behind the sequence's last, that one.  (Loads under a condition
+// would be waited for where its branches meet, and so would those of one tensor before the condition for the next: a
+// kernel that loads ahead finds all of its offsets first, then loads.  4 x 1024 steps of 2560 channels of 16 states in
+// BF16, forward: 78 us, tensor by tensor 83.)
+struct Span {
+  int t0, left;
+  __device__ __forceinline__ Span(int t, int steps) : t0(t < steps ? t : steps - 1), left(steps - t0) {}
+  __device__ __forceinline__ bool whole() const { return left >= kT; }
+  // The first step's row of a sequence, a wave-uniform address.
+  __device__ __forceinline__ const char* row(const View& v, int b) const { return v.at + b * v.batch + (int64_t)t0 * v.step; }
+};
+
+// A channel and step tensor's values of a wave's steps.
 template <typename T, int L>
 struct Rows {
-  uint32_t w[Lane<L>::kR];
-  // The steps from t0 on; in place of those behind the sequence's last, that one.  (Loads under a condition would be
-  // waited for where its branches meet, so only the offsets are.)
-  __device__ __forceinline__ void fetch(const Lane<L>& p, const View& v, int b, int t0, int steps) {
-    t0 = t0 < steps ? t0 : steps - 1;
-    const char* row = v.at + b * v.batch + (int64_t)t0 * v.step + p.group0 * Fmt<T>::bytes;
-    uint32_t at[Lane<L>::kR];
-    if (steps - t0 >= kT) {
+  uint32_t w[Lane<L>::kR], at[Lane<L>::kR];
+  // The lane's first step's offset in bytes; its others' are added to the address.
+  static __device__ __forceinline__ uint32_t offset(const Lane<L>& p, int step) {
+    return (uint32_t)(p.own < kT ? p.own : kT - 1) * (uint32_t)step + (uint32_t)p.inside * Fmt<T>::bytes;
+  }
+  __device__ __forceinline__ void place_whole(const Lane<L>& p, const View& v) {
 #pragma unroll
-      for (int i = 0; i < Lane<L>::kR; ++i) at[i] = p.template offset<T>(v.step) + (uint32_t)(i * L) * (uint32_t)v.step;
+    for (int i = 0; i < Lane<L>::kR; ++i) at[i] = offset(p, v.step);
+  }
+  __device__ __forceinline__ void place_part(const Lane<L>& p, const View& v, const Span& s) {
+#pragma unroll
+    for (int i = 0; i < Lane<L>::kR; ++i) {
+      const int t = p.own + i * L;
+      at[i] = (uint32_t)(t < s.left ? t : s.left - 1) * (uint32_t)v.step + (uint32_t)p.inside * Fmt<T>::bytes;
+    }
+  }
+  __device__ __forceinline__ void load(const Lane<L>& p, const View& v, int b, const Span& s) {
+    const char* row = s.row(v, b) + p.group0 * Fmt<T>::bytes;
+    const int64_t next = s.whole() ? (int64_t)L * v.step : 0;
+#pragma unroll
+    for (int i = 0; i < Lane<L>::kR; ++i) w[i] = load_bits<T>(row + i * next, at[i]);
+  }
+  // Both, where nothing is computed between loads and use: with all offsets in vector registers.
+  __device__ __forceinline__ void fetch(const Lane<L>& p, const View& v, int b, const Span& s) {
+    const char* row = s.row(v, b) + p.group0 * Fmt<T>::bytes;
+    if (s.whole()) {
+#pragma unroll
+      for (int i = 0; i < Lane<L>::kR; ++i) at[i] = offset(p, v.step) + (uint32_t)(i * L) * (uint32_t)v.step;
     } else {
-#pragma unroll
-      for (int i = 0; i < Lane<L>::kR; ++i) at[i] = p.template offset_of<T>(i, v.step, steps - t0);
+      place_part(p, v, s);
     }
 #pragma unroll
     for (int i = 0; i < Lane<L>::kR; ++i) w[i] = load_bits<T>(row, at[i]);
@@ -266,30 +284,47 @@ struct Rows {
 // and steps that are not there.
 template <typename T, int L>
 struct Inputs {
-  static constexpr int kCount = L > 1 ? L / 2 : 1, kAll = kT * 4 * L;
-  uint32_t w[kCount];
-  __device__ __forceinline__ void fetch(const View& r, int b, int t0, int steps, int states) {
-    t0 = t0 < steps ? t0 : steps - 1;
-    const char* row = r.at + b * r.batch + (int64_t)t0 * r.step;
-    const int left = steps - t0;
-    uint32_t at[kCount];
+  static constexpr int kCount = L / 2;
+  uint32_t w[kCount], at[kCount];
+  static __device__ __forceinline__ int step_of(int i) { return (i * 64 + (int)(threadIdx.x & 63)) / (4 * L); }
+  static __device__ __forceinline__ int state_of(int i) { return (i * 64 + (int)(threadIdx.x & 63)) % (4 * L); }
+  static __device__ __forceinline__ uint32_t offset(int i, int t, int step, int states) {
+    const int n = state_of(i);
+    return (uint32_t)t * (uint32_t)step + (uint32_t)(n < states ? n : states - 1) * Fmt<T>::bytes;
+  }
+  __device__ __forceinline__ void place_whole(const View& v, int states) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) at[i] = offset(i, step_of(i), v.step, states);
+  }
+  __device__ __forceinline__ void place_part(const View& v, const Span& s, int states) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      const int v = (i * 64 + (threadIdx.x & 63)) % kAll;
-      int t = v / (4 * L), n = v % (4 * L);
-      n = n < states ? n : states - 1;
-      if (left < kT) t = t < left ? t : left - 1;
-      at[i] = (uint32_t)t * (uint32_t)r.step + (uint32_t)n * Fmt<T>::bytes;
+      const int t = step_of(i);
+      at[i] = offset(i, t < s.left ? t : s.left - 1, v.step, states);
+    }
+  }
+  __device__ __forceinline__ void load(const View& v, int b, const Span& s) {
+    const char* row = s.row(v, b);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) w[i] = load_bits<T>(row, at[i]);
+  }
+  __device__ __forceinline__ void fetch(const View& v, int b, const Span& s, int states) {
+    const char* row = s.row(v, b);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      int t = step_of(i);
+      if (!s.whole()) t = t < s.left ? t : s.left - 1;
+      at[i] = offset(i, t, v.step, states);
     }
 #pragma unroll
     for (int i = 0; i < kCount; ++i) w[i] = load_bits<T>(row, at[i]);
   }
-  // (What is not there is told apart here: looked at in fetch, the loads would be waited for there.)
+  // (What is not there is told apart here: looked at in load, the loads would be waited for there.)
   __device__ __forceinline__ void put(float* to, int left, int states) const {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      const int v = (i * 64 + (threadIdx.x & 63)) % kAll;
-      const bool there = v % (4 * L) < states && v / (4 * L) < left;
+      const int v = i * 64 + (threadIdx.x & 63);
+      const bool there = state_of(i) < states && step_of(i) < left;
       to[v] = there ? bits_value<T>(w[i]) : 0.0f;
     }
   }
@@ -380,12 +415,24 @@ __global__ __launch_bounds__(64 * kW, L < 4 ? 3 : 4) void ssm_kernel(const Scan 
   Rows<T, L> rx, rd, rz;
   Inputs<T, L> inB, inC;
   auto fetch = [&](int tile) {
-    const int t0 = (tile * kW + wave) * kT;
-    rx.fetch(p, a.x, b, t0, a.steps);
-    rd.fetch(p, a.dt, b, t0, a.steps);
-    if constexpr (kGated) rz.fetch(p, a.z, b, t0, a.steps);
-    inB.fetch(a.B, b, t0, a.steps, a.states);
-    inC.fetch(a.C, b, t0, a.steps, a.states);
+    const Span s((tile * kW + wave) * kT, a.steps);
+    if constexpr (L > 4) {  // the registers that all offsets take are not there: 64 states 234 us, with them 244 to 252
+      rx.fetch(p, a.x, b, s), rd.fetch(p, a.dt, b, s);
+      if constexpr (kGated) rz.fetch(p, a.z, b, s);
+      inB.fetch(a.B, b, s, a.states), inC.fetch(a.C, b, s, a.states);
+      return;
+    }
+    rx.place_whole(p, a.x), rd.place_whole(p, a.dt);
+    if constexpr (kGated) rz.place_whole(p, a.z);
+    inB.place_whole(a.B, a.states), inC.place_whole(a.C, a.states);
+    if (!s.whole()) {
+      rx.place_part(p, a.x, s), rd.place_part(p, a.dt, s);
+      if constexpr (kGated) rz.place_part(p, a.z, s);
+      inB.place_part(a.B, s, a.states), inC.place_part(a.C, s, a.states);
+    }
+    rx.load(p, a.x, b, s), rd.load(p, a.dt, b, s);
+    if constexpr (kGated) rz.load(p, a.z, b, s);
+    inB.load(a.B, b, s), inC.load(a.C, b, s);
   };
   if (begin < end) fetch(begin);
   for (int tile = begin; tile < end; ++tile) {
@@ -436,7 +483,7 @@ __global__ __launch_bounds__(64 * kW, L < 4 ? 3 : 4) void ssm_kernel(const Scan 
     wave_order();
     if (left <= 0) continue;
     char* rows = y + (((int64_t)b * a.steps + t0) * a.dim + p.group0) * Fmt<T>::bytes;
-    const uint32_t to = p.template offset<T>(a.dim * Fmt<T>::bytes);
+    const uint32_t to = Rows<T, L>::offset(p, a.dim * Fmt<T>::bytes);
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
       float s = __fmaf_rn(c.skip, x[i], sums.out[i]);
@@ -473,11 +520,19 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_ends_kernel(const Scan a, flo
   float sum = 0.0f;
   Four s = {};
   auto fetch = [&](int i) {
-    const int t0 = (run0 + (kBack ? -i : i)) * kT;
-    rd.fetch(p, a.dt, b, t0, a.steps);
-    rx.fetch(p, kBack ? a.dy : a.x, b, t0, a.steps);
-    if constexpr (kGated) rz.fetch(p, a.z, b, t0, a.steps);
-    in.fetch(kBack ? a.C : a.B, b, t0, a.steps, a.states);
+    const Span s((run0 + (kBack ? -i : i)) * kT, a.steps);
+    const View &x = kBack ? a.dy : a.x, &v = kBack ? a.C : a.B;
+    rd.place_whole(p, a.dt), rx.place_whole(p, x);
+    if constexpr (kGated) rz.place_whole(p, a.z);
+    in.place_whole(v, a.states);
+    if (!s.whole()) {
+      rd.place_part(p, a.dt, s), rx.place_part(p, x, s);
+      if constexpr (kGated) rz.place_part(p, a.z, s);
+      in.place_part(v, s, a.states);
+    }
+    rd.load(p, a.dt, b, s), rx.load(p, x, b, s);
+    if constexpr (kGated) rz.load(p, a.z, b, s);
+    in.load(v, b, s);
   };
   if (count > 0) fetch(0);
   for (int i = 0; i < count; ++i) {
@@ -643,8 +698,8 @@ __global__ __launch_bounds__(64 * kW, L < 16 ? 3 : 2) void ssm_back_kernel(const
   int half = 0, turn = 0;
   for (int tile = end - 1; tile >= begin; --tile, turn ^= 1) {
     const int t0 = (tile * kW + wave) * kT, left = a.steps - t0;
-    inB.fetch(a.B, b, t0, a.steps, a.states);
-    inC.fetch(a.C, b, t0, a.steps, a.states);
+    const Span span(t0, a.steps);
+    inB.fetch(a.B, b, span, a.states), inC.fetch(a.C, b, span, a.states);
     inB.put(B, left, a.states), inC.put(C, left, a.states);
     wave_order();
     float acc[kSlots][2] = {};
@@ -652,10 +707,8 @@ __global__ __launch_bounds__(64 * kW, L < 16 ? 3 : 2) void ssm_back_kernel(const
       const Lane<L> p(group0 + i, a.dim);
       const bool whole = p.whole(a.dim, left);
       Rows<T, L> rx, rd, rz, re;
-      rx.fetch(p, a.x, b, t0, a.steps);
-      rd.fetch(p, a.dt, b, t0, a.steps);
-      re.fetch(p, a.dy, b, t0, a.steps);
-      if constexpr (kGated) rz.fetch(p, a.z, b, t0, a.steps);
+      rx.fetch(p, a.x, b, span), rd.fetch(p, a.dt, b, span), re.fetch(p, a.dy, b, span);
+      if constexpr (kGated) rz.fetch(p, a.z, b, span);
       const Channel c = load_channel(a, p);
       Four enter;
       load_states(kept + states_at(a, (int64_t)b * a.tiles + tile, p.ch), p.first, a.states, enter);
@@ -753,7 +806,6 @@ __global__ __launch_bounds__(64 * kW, L < 16 ? 3 : 2) void ssm_back_kernel(const
             if constexpr (L <= 8) v[j] += dpp<kRotate8>(v[j]);
             if constexpr (L <= 2) v[j] += dpp<kRotate4>(v[j]);
             if constexpr (L <= 2) v[j] += dpp<kRotate2>(v[j]);
-            if constexpr (L <= 1) v[j] += dpp<kRotate1>(v[j]);
             acc[t / kRep][j] += (lane & 15) / L == t % kRep ? v[j] : 0.0f;
           }
         }
@@ -774,7 +826,7 @@ __global__ __launch_bounds__(64 * kW, L < 16 ? 3 : 2) void ssm_back_kernel(const
       if (wave == 0) late[turn ^ 1][i][lane] = as_vector(r);
       if (left <= 0) continue;
       float dskip = 0.0f, dbias = 0.0f;
-      const uint32_t to = p.template offset<T>(a.dim * Fmt<T>::bytes);
+      const uint32_t to = Rows<T, L>::offset(p, a.dim * Fmt<T>::bytes);
       const int64_t at = (((int64_t)b * a.steps + t0) * a.dim + p.group0) * Fmt<T>::bytes;
 #pragma unroll
       for (int k = 0; k < kR; ++k) {
@@ -862,8 +914,10 @@ __global__ __launch_bounds__(256) void ssm_sum_kernel(const SsmParts parts, int6
 }
 
 int64_t over(int64_t n, int64_t by) { return (n + by - 1) / by; }
+// Of a channel, four states each; two at least: 4 states take 170 us backward (4 x 1024 steps of 2560 channels in BF16) with two
+// lanes, one of them idle, and 287 with one, whose steps' own values do not fit its registers; forward 70 and 67.
 int lanes_of(int states) {
-  int l = 1;
+  int l = 2;
   while (4 * l < states) l *= 2;
   return l;
 }
@@ -874,7 +928,6 @@ int by_form(int dtype, int states, bool gated, F&& f) {
   auto gate = [&](auto t, auto lanes) { return gated ? f(t, lanes, std::true_type{}) : f(t, lanes, std::false_type{}); };
   auto lanes = [&](auto t) {
     switch (lanes_of(states)) {
-      case 1: return gate(t, std::integral_constant<int, 1>{});
       case 2: return gate(t, std::integral_constant<int, 2>{});
       case 4: return gate(t, std::integral_constant<int, 4>{});
       case 8: return gate(t, std::integral_constant<int, 8>{});
